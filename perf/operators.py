@@ -148,7 +148,7 @@ def _codes(x, fmt):
     """Rows of `x` (32 bits) as codes with one scale a row."""
     top = x.abs().amax(-1)
     scale = torch.where(top >= TINY, top / TOP[fmt], 0.0)
-    inv = torch.where(top >= TINY, TOP[fmt] / top, 0.0)
+    inv = torch.where(top >= TINY, torch.full_like(top, TOP[fmt]) / top, 0.0)  # one rounding: a number / tensor takes two
     v = x * inv[..., None]
     return (v.round().to(torch.int8) if fmt == "i8" else v.to(F8)), scale
 
