@@ -41,6 +41,7 @@ EXPORTED = [  # every symbol include/checkers_amd.h declares
     "ckr_arena_create", "ckr_arena_alloc", "ckr_arena_used", "ckr_arena_reset", "ckr_arena_destroy",
     "ckr_stats_slab_bytes", "ckr_carve_stats_slab", "ckr_analyze_device_records",
     "ckr_analyze_device_records_workspace_bytes", "ckr_make_contiguous",
+    "ckr_kv_write", "ckr_kv_read", "ckr_kv_attention_workspace_bytes", "ckr_kv_attention", "ckr_add_rms_norm",
 ]
 
 
@@ -129,6 +130,7 @@ def lib():
         raise ImportError(f"checkers_amd: {LIB_PATH} not built; run `python -m checkers_amd.build`")
     L_ = ctypes.CDLL(LIB_PATH)
     u64, i32, vp = ctypes.c_uint64, ctypes.c_int, ctypes.c_void_p
+    i64, u32, f32 = ctypes.c_int64, ctypes.c_uint32, ctypes.c_float
     sig = {
         "ckr_last_error": (ctypes.c_char_p, []),
         "ckr_version": (ctypes.c_char_p, []),
@@ -186,6 +188,11 @@ def lib():
         "ckr_analyze_device_records": (i32, [vp, u64, vp, u64, vp]),
         "ckr_analyze_device_records_workspace_bytes": (u64, [vp, u64]),
         "ckr_make_contiguous": (i32, [vp, i32, vp, vp, i32, vp, vp]),
+        "ckr_kv_write": (i32, [vp, vp, vp, i64, i64, vp, i64, i64, i32, vp]),
+        "ckr_kv_read": (i32, [vp, vp, vp, i64, i64, vp, i64, i64, i32, vp]),
+        "ckr_kv_attention_workspace_bytes": (u64, [u32] * 7),
+        "ckr_kv_attention": (i32, [vp, vp, vp, i64, i64, i32, u32, f32, u32, vp, i64, i64, vp, vp, u64, vp]),
+        "ckr_add_rms_norm": (i32, [vp, i64, vp, i64, vp, i32, u64, u32, i32, f32, i32, u32, vp, i64, vp, vp, i64, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L_, name)
@@ -799,3 +806,7 @@ class Checkpoint:
             self.close()
         except Exception:
             pass
+
+
+# ---- operators around an 8-bit key/value cache (checkers_amd/kv.py)
+from .kv import F8, KvAttention, KvBatch, KvCache, add_rms_norm, kv_read, kv_write  # noqa: E402,F401

@@ -17,7 +17,7 @@ LIB = os.path.join(HERE, "libcheckers_amd.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["ckr_kernels.hip", "ckr_repair.hip", "ckr_api.cpp", "ckr_checkpoint.cpp", "ckr_context.hip",
-           "ckr_container.hip", "ckr_analyzer.hip"]
+           "ckr_container.hip", "ckr_analyzer.hip", "ckr_kv.hip", "ckr_attention.hip"]
 
 # -packed-fp32-ops: no v_pk_*_f32 generated anywhere (wrong results seen with
 # some of their forms on these machines).
@@ -73,7 +73,7 @@ def _stale(src, obj):
     if not os.path.exists(obj):
         return True
     deps = [src, os.path.join(ROOT, "include", "checkers_amd.h"), os.path.join(CSRC, "ckr_internal.h"),
-            os.path.join(CSRC, "ckr_table.h"),
+            os.path.join(CSRC, "ckr_table.h"), os.path.join(CSRC, "ckr_kv.h"),
             os.path.join(CSRC, "ckr_container.h")]
     return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps)
 

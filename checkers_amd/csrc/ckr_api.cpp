@@ -93,6 +93,12 @@ int check_buffer(const void* p, uint64_t bytes, const char* what) {
     return CKR_OK;
 }
 
+}  // namespace
+
+int ckr::check_range(const void* p, uint64_t bytes, const char* what) { return check_buffer(p, bytes, what); }
+
+namespace {
+
 // A source the kernels can read with 32-bit loads at its 4-byte columns.  A
 // tensor that is only element-aligned (a 16-bit or 8-bit tensor starting at an
 // address that is not a multiple of 4, e.g. a slice at an odd element offset

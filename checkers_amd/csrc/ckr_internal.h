@@ -50,6 +50,9 @@ uint64_t* prof_phase_buffer(uint64_t n, hipStream_t s);
     } while (0)
 // Sets the calling thread's last error (ckr_last_error) and returns code.
 int set_error(int code, const std::string& msg);
+// Whether [p, p + bytes) is memory the device can reach, inside one allocation
+// (CKR_OK, or CKR_E_INVALID with the message naming `what`); 0 bytes pass.
+int check_range(const void* p, uint64_t bytes, const char* what);
 
 // ckr_encode_planes for a slice of a tensor whose own plane histograms are
 // h_planes: every symbol of the slice is then known to have a slot, so the

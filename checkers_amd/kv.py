@@ -1,0 +1,254 @@
+"""The operators around an 8-bit key/value cache: kv_write, kv_read, KvAttention
+and add_rms_norm over the C ABI (include/checkers_amd.h).
+
+A KvCache names the cache's tensors, a KvBatch the tokens a call is about; both
+are descriptors made once and passed to every call (the page table, starts and
+offsets may change in place between calls: the kernels read them on the
+device).  Nothing here copies or synchronises.
+"""
+import ctypes
+
+from . import CKR_E_INVALID, BF16, F16, F32, I8, CkrError, _check, _stream, _torch, lib
+
+F8 = 16  # 8-bit floating point (e4m3, largest value 448), a type of these operators only
+
+_i64x3, _i64x2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("d_k", ctypes.c_void_p), ("d_v", ctypes.c_void_p), ("d_k_scale", ctypes.c_void_p),
+                ("d_v_scale", ctypes.c_void_p), ("k_stride", _i64x3), ("v_stride", _i64x3),
+                ("k_scale_stride", _i64x2), ("v_scale_stride", _i64x2), ("n_pages", ctypes.c_uint32),
+                ("page_size", ctypes.c_uint32), ("n_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("dtype", ctypes.c_int32), ("pad", ctypes.c_int32)]
+
+
+class _Batch(ctypes.Structure):
+    _fields_ = [("d_page_table", ctypes.c_void_p), ("d_starts", ctypes.c_void_p), ("d_offsets", ctypes.c_void_p),
+                ("table_stride", ctypes.c_uint64), ("table_width", ctypes.c_uint32), ("n_seqs", ctypes.c_uint32),
+                ("n_tokens", ctypes.c_uint32), ("max_chunk", ctypes.c_uint32), ("max_context", ctypes.c_uint32),
+                ("pad", ctypes.c_uint32)]
+
+
+_TAGS = {}   # torch dtype -> tag
+
+
+def _tag(dtype):
+    """C tag of a torch dtype of these operators (8-bit floats among them)."""
+    if not _TAGS:
+        torch = _torch()
+        _TAGS.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int8: I8,
+                      torch.float8_e4m3fn: F8})
+    tag = _TAGS.get(dtype)
+    if tag is None:
+        raise CkrError(CKR_E_INVALID, f"[ckr] {dtype} is not a type of the cache and norm operators")
+    return tag
+
+
+def _torch_dtype(tag):
+    _tag(_torch().int8)
+    for d, t in _TAGS.items():
+        if t == tag:
+            return d
+    raise CkrError(CKR_E_INVALID, f"[ckr] tag {tag} is not a type of the cache and norm operators")
+
+
+def _need(ok, msg):
+    if not ok:
+        raise CkrError(CKR_E_INVALID, "[ckr] " + msg)
+
+
+def _on_gpu(t, what):
+    _need(t.is_cuda, f"{what} must be on a GPU")
+
+
+class KvCache:
+    """A paged cache over the caller's tensors: k and v [pages, heads, page_size,
+    head_dim] with any strides of the first three axes, for 8-bit types k_scale
+    and v_scale [pages, heads, page_size] in float32 (slots contiguous)."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype, "k and v must be alike, [pages, heads, page_size, head_dim]")
+        _need(k.stride(3) == 1 and v.stride(3) == 1, "the last axis of k and v must be contiguous")
+        self.dtype = _tag(k.dtype)
+        coded = self.dtype in (F8, I8)
+        _need(coded == (k_scale is not None) == (v_scale is not None), "scales belong to 8-bit caches, and to both k and v")
+        for t, what in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t is not None:
+                _on_gpu(t, what)
+                _need(t.device == k.device, "the cache's tensors must be on one GPU")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.n_heads, self.page_size, self.head_dim = k.shape
+        c = _Cache(k.data_ptr(), v.data_ptr(), None, None, _i64x3(*k.stride()[:3]), _i64x3(*v.stride()[:3]),
+                   _i64x2(0, 0), _i64x2(0, 0), *(int(n) for n in (k.shape[0], k.shape[2], k.shape[1], k.shape[3])),
+                   self.dtype, 0)
+        if coded:
+            for t in (k_scale, v_scale):
+                _need(t.shape == k.shape[:3] and t.dtype == _torch().float32 and t.stride(2) == 1,
+                      "scales must be float32 [pages, heads, page_size], slots contiguous")
+            c.d_k_scale, c.d_v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+            c.k_scale_stride, c.v_scale_stride = _i64x2(*k_scale.stride()[:2]), _i64x2(*v_scale.stride()[:2])
+        self._c = c
+        self._p = ctypes.byref(c)
+
+    @classmethod
+    def empty(cls, n_pages, page_size, n_heads, head_dim, dtype, device="cuda"):
+        """A cache of new tensors (dtype: F8, I8, BF16 or F16), zeroed."""
+        torch = _torch()
+        t = _torch_dtype(dtype)
+        kv = [torch.zeros((n_pages, n_heads, page_size, head_dim), dtype=torch.uint8 if dtype == F8 else t, device=device)
+              for _ in range(2)]
+        if dtype == F8:
+            kv = [x.view(t) for x in kv]
+        sc = [torch.zeros((n_pages, n_heads, page_size), dtype=torch.float32, device=device) if dtype in (F8, I8) else None
+              for _ in range(2)]
+        return cls(kv[0], kv[1], sc[0], sc[1])
+
+    def tensors(self):
+        """The cache's tensors (k, v and, in 8 bits, their scales)."""
+        return [t for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None]
+
+
+class KvBatch:
+    """The tokens of a call: sequence s has starts[s] tokens before its chunk,
+    rows offsets[s]:offsets[s + 1] of the packed tensors, in the cache pages that
+    page_table[s] lists (negative: unmapped).  All int32 on the GPU; n_tokens is
+    offsets[-1], max_chunk and max_context (the longest chunk, the largest
+    context with its chunk) choose launches and need not be exact."""
+
+    def __init__(self, page_table, starts, offsets, n_tokens, max_chunk=None, max_context=None):
+        torch = _torch()
+        _need(page_table.dim() == 2 and page_table.stride(1) == 1, "page_table must be [sequences, pages], its rows contiguous")
+        n = page_table.shape[0]
+        _need(tuple(starts.shape) == (n,) and tuple(offsets.shape) == (n + 1,), "starts and offsets must hold n and n + 1 entries")
+        for t, what in ((page_table, "page_table"), (starts, "starts"), (offsets, "offsets")):
+            _need(t.dtype == torch.int32 and (t.dim() == 2 or t.is_contiguous()), f"{what} must be int32, contiguous")
+            _on_gpu(t, what)
+        _need(0 <= n_tokens < 1 << 31, "n_tokens out of range")
+        self.page_table, self.starts, self.offsets, self.n_seqs, self.n_tokens = page_table, starts, offsets, n, int(n_tokens)
+        self.max_chunk = int(n_tokens if max_chunk is None else max_chunk)
+        self.max_context = max_context
+        width = page_table.shape[1]
+        self._c = _Batch(page_table.data_ptr(), starts.data_ptr(), offsets.data_ptr(), max(page_table.stride(0), width),
+                         width, n, self.n_tokens, min(self.max_chunk, 0xffffffff),
+                         0xffffffff if max_context is None else min(int(max_context), 0xffffffff), 0)
+        self._p = ctypes.byref(self._c)
+
+
+def _rows(t, batch, heads, dim, what):
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != batch.n_tokens or shape[1] != heads or shape[2] != dim:
+        raise CkrError(CKR_E_INVALID, f"[ckr] {what} must be [{batch.n_tokens}, {heads}, {dim}], not {list(shape)}")
+    a, b, c = t.stride()
+    _need(c == 1 or dim == 1, f"the last axis of {what} must be contiguous")
+    _on_gpu(t, what)
+    return a, b
+
+
+def _used_on(stream, *tensors):
+    """Tensors this module allocated, used on a stream other than the current one."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
+def kv_write(cache, batch, k, v, stream=None):
+    """Quantise the batch's keys and values [tokens, heads, head_dim] into the cache."""
+    _need(k.dtype == v.dtype, "k and v must be of one type")
+    kt, kh = _rows(k, batch, cache.n_heads, cache.head_dim, "k")
+    vt, vh = _rows(v, batch, cache.n_heads, cache.head_dim, "v")
+    _check(lib().ckr_kv_write(cache._p, batch._p, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _tag(k.dtype), _stream(stream)))
+
+
+def kv_read(cache, batch, dtype=BF16, out=None, stream=None):
+    """(k, v) of the batch's tokens as the cache holds them, [tokens, heads,
+    head_dim] of dtype (a tag), into out (a pair of tensors) when given."""
+    if out is None:
+        torch = _torch()
+        shape = (batch.n_tokens, cache.n_heads, cache.head_dim)
+        out = tuple(torch.empty(shape, dtype=_torch_dtype(dtype), device=cache.k.device) for _ in range(2))
+        _used_on(stream, *out)
+    k, v = out
+    _need(_tag(k.dtype) == dtype and _tag(v.dtype) == dtype, "out must be of the type asked for")
+    kt, kh = _rows(k, batch, cache.n_heads, cache.head_dim, "out[0]")
+    vt, vh = _rows(v, batch, cache.n_heads, cache.head_dim, "out[1]")
+    _check(lib().ckr_kv_read(cache._p, batch._p, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, dtype, _stream(stream)))
+    return k, v
+
+
+class KvAttention:
+    """Attention over a paged cache, with the workspace it needs for batches of at
+    most these sizes (n_heads query heads over n_kv_heads; max_context None: any)."""
+
+    def __init__(self, n_heads, n_kv_heads, head_dim, n_seqs, n_tokens, max_chunk=None, max_context=None, device="cuda"):
+        torch = _torch()
+        self.n_heads, self.n_kv_heads, self.head_dim = int(n_heads), int(n_kv_heads), int(head_dim)
+        self.ws_bytes = int(lib().ckr_kv_attention_workspace_bytes(
+            self.n_heads, self.n_kv_heads, self.head_dim, n_seqs, n_tokens,
+            n_tokens if max_chunk is None else max_chunk, 0xffffffff if max_context is None else max_context))
+        self.ws = torch.zeros(max(self.ws_bytes, 1), dtype=torch.uint8, device=device)
+
+    def run(self, cache, batch, q, scale=None, window=0, out=None, lse=None, stream=None):
+        """Attention of the batch's tokens, whose keys and values the cache already
+        holds: q [tokens, n_heads, head_dim] -> out (of q's type, new when None).
+        scale: head_dim ** -0.5 when None.  lse: a contiguous float32 [tokens,
+        n_heads] that receives the logarithm of each row's sum of exponentials."""
+        qt, qh = _rows(q, batch, self.n_heads, cache.head_dim, "q")
+        if out is None:
+            out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+            _used_on(stream, out)
+        _need(out.dtype == q.dtype, "out must be of q's type")
+        ot, oh = _rows(out, batch, self.n_heads, cache.head_dim, "out")
+        if lse is not None:
+            _need(tuple(lse.shape) == (batch.n_tokens, self.n_heads) and lse.dtype == _torch().float32 and lse.is_contiguous()
+                  and lse.is_cuda, "lse must be a contiguous float32 [tokens, n_heads] on the GPU")
+        _check(lib().ckr_kv_attention(
+            cache._p, batch._p, q.data_ptr(), qt, qh, _tag(q.dtype), self.n_heads,
+            cache.head_dim ** -0.5 if scale is None else scale, int(window), out.data_ptr(), ot, oh,
+            None if lse is None else lse.data_ptr(), self.ws.data_ptr(), self.ws_bytes, _stream(stream)))
+        return out
+
+
+def add_rms_norm(x, residual, weight, eps=1e-5, dtype=None, group=0, out=None, scales=None, total=None, stream=None):
+    """h = x + residual (None: x alone), y = h / sqrt(mean(h^2) + eps) * weight over
+    the last axis of x [rows, n].  Returns (out, scales, h): y of dtype (a tag; x's
+    type when None, F8 or I8 with float32 scales per row, or per group of the
+    row), scales None for 16 and 32 bits, h rounded to x's type.  out, scales and
+    total (may be x or residual) are written in place when given."""
+    torch = _torch()
+    _need(x.dim() == 2, "x must be [rows, n]")
+    rows, n = x.shape
+    xt = _tag(x.dtype)
+    tag = xt if dtype is None else dtype
+    coded = tag in (F8, I8)
+    if out is None:
+        out = torch.empty((rows, n), dtype=_torch_dtype(tag), device=x.device)
+        _used_on(stream, out)
+    if total is None:
+        total = torch.empty((rows, n), dtype=x.dtype, device=x.device)
+        _used_on(stream, total)
+    if coded:
+        _need(group >= 0 and (group == 0 or n % group == 0), "group must divide the row length")
+        shape = (rows, n // group) if group else (rows,)
+        if scales is None:
+            scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+            _used_on(stream, scales)
+        _need(tuple(scales.shape) == shape and scales.dtype == torch.float32 and scales.is_contiguous() and scales.is_cuda,
+              f"scales must be contiguous float32 {list(shape)} on the GPU")
+    else:
+        _need(scales is None, "scales belong to 8-bit outputs")
+    for t, what in ((x, "x"), (residual, "residual"), (out, "out"), (total, "total")):
+        if t is not None:
+            _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == n and (t.stride(1) == 1 or n == 1) and t.is_cuda,
+                  f"{what} must be [{rows}, {n}] on the GPU, its last axis contiguous")
+    _need(_tag(out.dtype) == tag and total.dtype == x.dtype and (residual is None or residual.dtype == x.dtype),
+          "residual and total must be of x's type, out of the type asked for")
+    _need(weight.dim() == 1 and weight.shape[0] == n and (weight.stride(0) == 1 or n == 1) and weight.is_cuda,
+          f"weight must be [{n}] on the GPU")
+    _check(lib().ckr_add_rms_norm(
+        x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(),
+        0 if residual is None else residual.stride(0), weight.data_ptr(), _tag(weight.dtype), rows, n, xt, eps, tag, group,
+        out.data_ptr(), out.stride(0), scales.data_ptr() if coded else None, total.data_ptr(), total.stride(0),
+        _stream(stream)))
+    return out, scales, total

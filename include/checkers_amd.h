@@ -56,6 +56,10 @@ extern "C" {
 #define CKR_I8       3
 #define CKR_I32      4
 #define CKR_UNKNOWN  255
+/* 8-bit floating point (OCP e4m3: 4 exponent bits, 3 fraction bits, largest
+ * value 448): a type of the cache and norm operators only, not of tensors (the
+ * codec takes such bytes as CKR_I8). */
+#define CKR_F8       16
 
 /* rANS constants: include/checkers/ANSCompressor.hpp:51-55 */
 #define CKR_SCALE_BITS 12u
@@ -531,6 +535,105 @@ CKR_API int ckr_analyze_device_records(const ckr_device_tensor_record* h_recs, u
  * gather follows every stride, which is the same copy wherever that holds. */
 CKR_API int ckr_make_contiguous(const void* d_src, int ndim, const int64_t* shape, const int64_t* strides,
                                 int elem_size, void* d_dst, void* stream);
+
+/* ---- operators around an 8-bit key/value cache, no counterpart in the
+ * reference.  A program that serves a model holds its cache in pages; in 8 bits
+ * the pages are byte tensors that ckr_compress / ckr_decode park and restore
+ * like any other.
+ *
+ * Quantised rows: n values x share one fp32 scale.  With a = max |x| and T the
+ * type's largest value (CKR_F8 448, CKR_I8 127):
+ *   scale = a / T,  code = round(x * (T / a)) (ties to even),  value = code * scale
+ * in fp32; a < 2^-100 gives scale 0 and codes 0, and a row that holds an
+ * infinity or NaN gives scale NaN and codes 0, so that it reads back as NaN. ---- */
+
+/* A paged cache: keys and values [n_pages][n_heads][page_size][head_dim] in any
+ * order of the first three axes (strides in elements, >= 0; the last axis is
+ * contiguous).  dtype CKR_F8 or CKR_I8, with a scale per (page, head, slot) whose
+ * slots are contiguous, or CKR_BF16 / CKR_F16 without scales.  page_size is a
+ * power of two from 16 on, head_dim a multiple of 16 up to 256; every row must
+ * start on a 16-byte boundary, every page's scales of a head too. */
+typedef struct {
+    void* d_k;
+    void* d_v;
+    float* d_k_scale;           /* NULL without scales                          */
+    float* d_v_scale;
+    int64_t k_stride[3];        /* page, head, slot                             */
+    int64_t v_stride[3];
+    int64_t k_scale_stride[2];  /* page, head                                   */
+    int64_t v_scale_stride[2];
+    uint32_t n_pages, page_size, n_heads, head_dim;
+    int32_t dtype;
+    int32_t pad;
+} ckr_kv_cache;
+
+/* Which tokens of which sequences a call is about.  Sequence s has d_starts[s]
+ * tokens before its chunk; its chunk's tokens are rows d_offsets[s] to
+ * d_offsets[s + 1] of the packed tensors (d_offsets[0] == 0, d_offsets[n_seqs]
+ * == n_tokens), token i at position d_starts[s] + i, which lies in page
+ * d_page_table[s * table_stride + position / page_size].  The arrays are on the
+ * device and read when the call's kernels run.  A table entry outside
+ * [0, n_pages), or a position beyond table_width pages, is an unmapped page:
+ * it is not written, reads as zeros and is not attended to.  max_chunk and
+ * max_context (the longest chunk, the largest d_starts[s] + chunk) choose the
+ * attention's kernel and how it splits the keys; the result is right whatever
+ * they are. */
+typedef struct {
+    const int32_t* d_page_table;
+    const int32_t* d_starts;
+    const int32_t* d_offsets;
+    uint64_t table_stride;
+    uint32_t table_width;
+    uint32_t n_seqs, n_tokens, max_chunk, max_context;
+    uint32_t pad;
+} ckr_kv_batch;
+
+/* Keys and values of the batch's tokens into the cache, quantised per (token,
+ * head) row.  d_k, d_v: [n_tokens][n_heads][head_dim] of dtype (CKR_F32, BF16 or
+ * F16) with token and head strides in elements, rows on 16-byte boundaries.
+ * Only queues work. */
+CKR_API int ckr_kv_write(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const void* d_k, int64_t k_token_stride,
+                         int64_t k_head_stride, const void* d_v, int64_t v_token_stride, int64_t v_head_stride,
+                         int dtype, void* stream);
+/* The values of the batch's tokens back from the cache, laid out as
+ * ckr_kv_write's inputs, each rounded once to dtype.  Only queues work. */
+CKR_API int ckr_kv_read(const ckr_kv_cache* cache, const ckr_kv_batch* batch, void* d_k, int64_t k_token_stride,
+                        int64_t k_head_stride, void* d_v, int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                        void* stream);
+
+/* Attention of the batch's tokens over the cache, which already holds them
+ * (ckr_kv_write): token at position p of sequence s attends to the positions j
+ * of s with p - window < j <= p (window 0: all j <= p) on mapped pages.  Query
+ * head h uses key/value head h / (n_heads / cache->n_heads).  d_q and d_out:
+ * [n_tokens][n_heads][head_dim] of dtype (CKR_BF16 or CKR_F16; a 16-bit cache
+ * must be of the same type) with token and head strides in elements, rows on
+ * 16-byte boundaries.  d_lse (may be NULL): [n_tokens][n_heads] fp32, the
+ * logarithm of the sum of exp(scale * q.k).  A token that attends to nothing
+ * gives zeros and -infinity.  The workspace (256-byte aligned) must be all
+ * zeros when it is first used and is left fit for the next call; calls that share one
+ * must follow each other in stream order.  One sized for the largest n_seqs,
+ * n_tokens, max_chunk and max_context serves smaller ones.  Only queues work. */
+CKR_API uint64_t ckr_kv_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                                  uint32_t n_seqs, uint32_t n_tokens, uint32_t max_chunk,
+                                                  uint32_t max_context);
+CKR_API int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const void* d_q,
+                             int64_t q_token_stride, int64_t q_head_stride, int dtype, uint32_t n_heads, float scale,
+                             uint32_t window, void* d_out, int64_t out_token_stride, int64_t out_head_stride,
+                             float* d_lse, void* d_workspace, uint64_t workspace_bytes, void* stream);
+
+/* Residual sum and root-mean-square norm of each row:
+ *   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight
+ * in fp32.  d_x, d_residual (NULL: none), d_total (h rounded to dtype; NULL: not
+ * stored) and d_out: [rows][n] with row strides in elements, the last axis
+ * contiguous; dtype CKR_F32, BF16 or F16; d_weight [n] of w_dtype (dtype or
+ * CKR_F32).  out_dtype: dtype (y rounded once), or CKR_F8 / CKR_I8 (y quantised;
+ * d_scales [rows] with group 0, or [rows][n / group] with group 32, 64, 128 or
+ * 256 dividing n).  d_total may be d_x or d_residual; d_out overlaps nothing.
+ * n is at most 65536.  Only queues work. */
+CKR_API int ckr_add_rms_norm(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride,
+                             const void* d_weight, int w_dtype, uint64_t rows, uint32_t n, int dtype, float eps,
+                             int out_dtype, uint32_t group, void* d_out, int64_t out_stride, float* d_scales,
+                             void* d_total, int64_t total_stride, void* stream);
 
 /* ---- path selection, no counterpart in the reference.  mode 1 (default):
  * fast kernels — lanes of masked planes coded once per lane count (their

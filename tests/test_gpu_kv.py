@@ -1,0 +1,378 @@
+"""kv_write, kv_read and KvAttention against plain forms: codes and scales bit for
+bit, attention within bounds derived from its arithmetic."""
+import numpy as np
+import pytest
+import torch
+
+import checkers_amd as ck
+from tests import kv_oracle as ko
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+TAGS = {"bf16": ck.BF16, "f16": ck.F16, "f32": ck.F32, "f8": ck.F8, "i8": ck.I8}
+
+
+def _batch(sq, gpu, hints=True):
+    i32 = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device=gpu)  # noqa: E731
+    return ck.KvBatch(i32(sq.table), i32(sq.starts), i32(sq.offsets), sq.tokens, max(sq.lens) if hints else None,
+                      max(o + n for o, n in zip(sq.starts, sq.lens)) if hints else None)
+
+
+def _cache(sq, heads, dim, fmt, gpu, order="phsd", fill=None):
+    """A cache whose storage has the given axis order, filled with garbage that a
+    call must not use: NaN scales and codes."""
+    shape = dict(p=sq.n_pages, h=heads, s=sq.page, d=dim)
+    back = [order.index(c) for c in "phsd"]
+    def make(t):
+        x = torch.full([shape[c] for c in order], 0x7f, dtype=torch.uint8, device=gpu).view(t) if t.itemsize == 1 else \
+            torch.full([shape[c] for c in order], float("nan"), dtype=t, device=gpu)
+        return x.permute(back)
+    t = {"f8": torch.float8_e4m3fn, "i8": torch.int8}.get(fmt) or TYPES[fmt]
+    sc = [torch.full((sq.n_pages, heads, sq.page), float("nan"), device=gpu) if fmt in ko.TOP else None for _ in range(2)]
+    return ck.KvCache(make(t), make(t), *sc)
+
+
+def _values(cache, name, fmt):
+    x = getattr(cache, name).cpu().to(torch.float64 if fmt in TYPES else torch.float32)
+    if fmt in ko.TOP:
+        return (x.double() * getattr(cache, name + "_scale").cpu().double()[..., None]).numpy()
+    return x.numpy()
+
+
+def _fill(sq, cache, batch, heads, dim, typ, gpu, seed):
+    """Every token of the sequences (old and new) written; returns nothing."""
+    whole = ko.Seqs([0] * len(sq.starts), [o + n for o, n in zip(sq.starts, sq.lens)], sq.page)
+    whole.table = sq.table
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    kv = [(torch.randn(whole.tokens, heads, dim, generator=g, device=gpu) * s).to(TYPES[typ]) for s in (1.3, 0.7)]
+    i32 = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device=gpu)  # noqa: E731
+    ck.kv_write(cache, ck.KvBatch(batch.page_table, i32(whole.starts), i32(whole.offsets), whole.tokens), *kv)
+
+
+@pytest.mark.parametrize("fmt", ["f8", "i8", "bf16", "f16"])
+@pytest.mark.parametrize("typ,heads,dim,page,order", [
+    ("bf16", 8, 128, 64, "phsd"), ("f16", 3, 80, 16, "pshd"), ("f32", 1, 16, 32, "hpsd"), ("bf16", 5, 256, 16, "phsd"),
+    ("f32", 2, 208, 128, "pshd"), ("f16", 7, 64, 256, "sphd")])
+def test_write_and_read(gpu, fmt, typ, heads, dim, page, order):
+    print(f"[case] write/read {fmt} {typ} heads={heads} dim={dim} page={page} {order}", flush=True)
+    sq = ko.Seqs([5, 0, 130, 17, 0], [1, 33, 0, 100, 257], page, seed=dim)
+    sq.table[3, 0] = -1 if page > 16 else sq.table[3, 0]     # an unmapped page (its tokens are not stored)
+    sq.table[4, 1 if page <= 128 else 0] = sq.n_pages + 5 if page != 256 else sq.table[4, 0]
+    cache = _cache(sq, heads, dim, fmt, gpu, order)
+    before = [t.clone() for t in cache.tensors()]
+    b = _batch(sq, gpu)
+    g = torch.Generator().manual_seed(dim)
+    x = [torch.randn(sq.tokens, heads, dim, generator=g) * torch.exp(3 * torch.randn(sq.tokens, heads, 1, generator=g)) for _ in range(2)]
+    x[0][7] = 0                       # an empty row, a tiny one, an infinite one, one with NaN
+    x[0][8] *= 0 if typ == "f16" else 1e-36
+    x[1][9, 0, 3] = float("inf")
+    x[1][10, heads - 1, dim - 1] = float("nan")
+    x = [t.to(TYPES[typ]) for t in x]
+    ck.kv_write(cache, b, *(t.to(gpu) for t in x))
+    out = tuple(torch.full((sq.tokens, heads, dim), 7.0, dtype=TYPES[typ], device=gpu) for _ in range(2))
+    ck.kv_read(cache, b, TAGS[typ], out=out)
+    torch.cuda.synchronize()
+    touched = torch.zeros(sq.n_pages, sq.page, dtype=torch.bool)
+    for which, name in enumerate(("k", "v")):
+        got, new = getattr(cache, name).cpu(), x[which]
+        if fmt in ko.TOP:
+            codes, scales = ko.quantise(new.float(), fmt)
+            got_s = getattr(cache, name + "_scale").cpu()
+            want_back = (codes * scales[..., None]).to(TYPES[typ])
+        else:
+            codes, scales, want_back = new.float().to(TYPES[fmt]), None, new.float().to(TYPES[fmt]).float().to(TYPES[typ])
+        t = 0
+        for s in range(len(sq.lens)):
+            for i in range(sq.lens[s]):
+                p, slot = sq.place(s, sq.starts[s] + i)
+                if p < 0:
+                    assert (out[which][t] == 0).all(), (s, i)
+                    t += 1
+                    continue
+                touched[p, slot] = True
+                have = got[p, :, slot]
+                assert torch.equal(torch.nan_to_num(have.float(), nan=5e4), torch.nan_to_num(codes[t].float(), nan=5e4)), (s, i)
+                if scales is not None:
+                    assert torch.equal(torch.nan_to_num(got_s[p, :, slot], nan=-1.0), torch.nan_to_num(scales[t], nan=-1.0))
+                back = out[which][t].cpu()
+                assert torch.equal(torch.nan_to_num(back.float(), nan=5e4), torch.nan_to_num(want_back[t].float(), nan=5e4)), (s, i)
+                t += 1
+    for old, new in zip(before, cache.tensors()):   # nothing else was written
+        keep = ~touched.to(gpu)
+        a, c = (z.view(torch.uint8) if z.element_size() == 1 else z.view(torch.int16 if z.element_size() == 2 else torch.int32) for z in (old, new))
+        a, c = a.transpose(1, 2)[keep], c.transpose(1, 2)[keep]
+        assert torch.equal(a, c)
+
+
+ATTEND = [
+    # q type, cache, kv heads, group, dim, page, starts, lens, window
+    ("bf16", "f8", 8, 4, 128, 64, [1000], [1], 0),
+    ("bf16", "f8", 2, 4, 128, 16, [0, 5, 63, 64, 700], [1, 1, 1, 1, 1], 0),
+    ("f16", "i8", 1, 8, 64, 32, [31, 32, 200], [1, 2, 1], 0),
+    ("bf16", "bf16", 2, 1, 128, 128, [100, 0], [1, 1], 50),
+    ("f16", "f16", 3, 2, 80, 16, [250, 0, 9], [1, 1, 5], 0),
+    ("bf16", "i8", 1, 16, 256, 64, [129], [1], 0),
+    ("bf16", "f8", 1, 20, 96, 16, [77, 300], [1, 1], 0),
+    ("bf16", "f8", 2, 4, 128, 64, [0], [300], 0),
+    ("bf16", "f8", 1, 4, 128, 32, [190, 0, 64], [70, 130, 1], 0),
+    ("f16", "f16", 1, 8, 128, 16, [0, 33], [150, 64], 0),
+    ("bf16", "bf16", 2, 2, 64, 256, [500], [65], 0),
+    ("f16", "i8", 2, 3, 112, 64, [40, 0], [129, 31], 33),
+    ("bf16", "i8", 1, 2, 256, 16, [90], [100], 0),
+    ("f16", "f8", 1, 1, 16, 16, [10, 0], [40, 200], 64),
+    ("bf16", "f8", 1, 7, 48, 16, [3, 0, 0, 400], [17, 0, 1, 9], 10),
+    ("f16", "f16", 1, 4, 256, 32, [70, 0], [40, 90], 0),
+    ("bf16", "bf16", 1, 5, 176, 16, [2000], [3], 0),
+]
+
+
+def _attend(gpu, typ, fmt, heads, group, dim, page, starts, lens, window, sq=None, scale=None, order="phsd", loud=1.0):
+    sq = sq or ko.Seqs(starts, lens, page, seed=len(starts))
+    cache = _cache(sq, heads, dim, fmt, gpu, order)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, heads, dim, typ, gpu, 3)
+    g = torch.Generator(device=gpu).manual_seed(4)
+    q = (torch.randn(sq.tokens, heads * group, dim, generator=g, device=gpu) * loud).to(TYPES[typ])
+    plan = ck.KvAttention(heads * group, heads, dim, len(starts), sq.tokens, max(lens), max(o + n for o, n in zip(starts, lens)))
+    out = torch.full_like(q, 9.0)
+    lse = torch.full((sq.tokens, heads * group), 9.0, device=gpu)
+    plan.run(cache, b, q, scale=scale, window=window, out=out, lse=lse)
+    torch.cuda.synchronize()
+    return sq, cache, b, q, plan, out, lse
+
+
+def _check(sq, cache, q, out, lse, fmt, group, window, scale=None):
+    D = q.shape[2]
+    k, v = (np.nan_to_num(_values(cache, n, fmt), nan=0.0) for n in ("k", "v"))
+    ref = ko.attention(sq, k, v, q.cpu().double().numpy(), group, scale or D ** -0.5, window)
+    p_unit = ko.UNIT[torch.float16 if fmt == "f16" else torch.bfloat16]   # weights of 8-bit values are bfloat16
+    bound, lbound = ko.attention_bounds(*ref, D, p_unit, q.dtype, np.abs(v).max())
+    err = np.abs(out.cpu().double().numpy() - ref[0])
+    print(f"  largest error / bound: {(err / bound).max():.3f}", flush=True)
+    assert (err <= bound).all()
+    got, none = lse.cpu().double().numpy(), ~np.isfinite(ref[1])
+    assert (got[none] == -np.inf).all()
+    assert (np.abs(got[~none] - ref[1][~none]) <= np.broadcast_to(lbound, got.shape)[~none]).all()
+
+
+@pytest.mark.parametrize("case", ATTEND, ids=lambda c: "-".join(map(str, c[:6])))
+def test_attention(gpu, case):
+    print(f"[case] attend {case}", flush=True)
+    typ, fmt, heads, group, dim, page, starts, lens, window = case
+    sq, cache, b, q, plan, out, lse = _attend(gpu, *case)
+    _check(sq, cache, q, out, lse, fmt, group, window)
+    # the same call again on the same workspace, and without hints or lse
+    again = torch.full_like(q, 5.0)
+    plan.run(cache, b, q, window=window, out=again)
+    torch.cuda.synchronize()
+    assert torch.equal(again, out)
+    plan2 = ck.KvAttention(heads * group, heads, dim, len(starts), sq.tokens)
+    loose = plan2.run(cache, _batch(sq, gpu, hints=False), q, window=window)
+    _check(sq, cache, q, loose, lse, fmt, group, window)
+
+
+@pytest.mark.parametrize("fmt", ["f8", "f16"])
+@pytest.mark.parametrize("lens", [[1, 1, 1], [40, 90, 2]])
+def test_attention_unmapped_pages_and_rows_without_keys(gpu, fmt, lens):
+    """Evicted pages (negative or out of range ids) are not attended to; rows whose
+    window holds only such pages, or whose table is too short, give zeros and
+    -inf; what lies in masked places (NaN everywhere here) never shows."""
+    print(f"[case] unmapped {fmt} {lens}", flush=True)
+    starts = [100, 20, 300]
+    sq = ko.Seqs(starts, lens, 16, seed=8)
+    full = sq.table.copy()
+    cache = _cache(sq, 2, 64, fmt, gpu)
+    _fill(sq, cache, _batch(sq, gpu), 2, 64, "f16", gpu, 3)
+    sq.table[0, :4] = [-1, -7, sq.n_pages, 2**31 - 1]
+    sq.table[1, :] = -1                      # nothing left of sequence 1
+    sq.table[2, 3:17] = -1
+    for s, c in ((0, 0), (0, 1), (2, 5)):    # poison the pages that went away
+        cache.k[int(full[s, c])] = float("nan")
+        cache.v[int(full[s, c])] = float("nan")
+    g = torch.Generator(device=gpu).manual_seed(4)
+    q = torch.randn(sq.tokens, 8, 64, generator=g, device=gpu).half()
+    plan = ck.KvAttention(8, 2, 64, 3, sq.tokens, max(lens), 400)
+    for window in (0, 30):
+        lse = torch.full((sq.tokens, 8), 9.0, device=gpu)
+        out = plan.run(cache, _batch(sq, gpu), q, window=window, lse=lse)
+        torch.cuda.synchronize()
+        assert (out[lens[0]:lens[0] + lens[1]] == 0).all()
+        _check(sq, cache, q, out, lse, fmt, 4, window)
+    sq.table = sq.table[:, :2].copy()        # a table narrower than the contexts
+    lse = torch.full((sq.tokens, 8), 9.0, device=gpu)
+    out = plan.run(cache, _batch(sq, gpu), q, lse=lse)
+    torch.cuda.synchronize()
+    _check(sq, cache, q, out, lse, fmt, 4, 0)
+
+
+@pytest.mark.parametrize("lens", [[1], [50]])
+def test_attention_poisoned_rows_show(gpu, lens):
+    """A cached row that held an infinity reads as NaN: every token that sees it
+    gives NaN, a token whose window ends after it does not."""
+    sq = ko.Seqs([200], lens, 16, seed=1)
+    cache = _cache(sq, 1, 64, "f8", gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 1, 64, "bf16", gpu, 3)
+    p, slot = sq.place(0, 100)
+    cache.k_scale[p, 0, slot] = float("nan")
+    q = torch.randn(sq.tokens, 4, 64, device=gpu).to(torch.bfloat16)
+    plan = ck.KvAttention(4, 1, 64, 1, sq.tokens, max(lens), 300)
+    assert torch.isnan(plan.run(cache, b, q)).all()
+    assert torch.isfinite(plan.run(cache, b, q, window=100)).all()
+    cache.k_scale[p, 0, slot] = 1.0
+    cache.v_scale[p, 0, slot] = float("nan")
+    assert torch.isnan(plan.run(cache, b, q)).all()
+    assert torch.isfinite(plan.run(cache, b, q, window=100)).all()
+
+
+@pytest.mark.parametrize("lens", [[1, 1], [60, 33]])
+@pytest.mark.parametrize("loud,scale", [(30.0, None), (0.0, None), (1.0, -0.2), (1.0, 4.0)])
+def test_attention_of_peaked_and_flat_scores(gpu, lens, loud, scale):
+    print(f"[case] peaks {lens} {loud} {scale}", flush=True)
+    for fmt in ("f8", "f16"):
+        sq, cache, b, q, plan, out, lse = _attend(gpu, "f16", fmt, 2, 4, 128, 32, [500, 0], lens, 0, scale=scale, loud=loud)
+        _check(sq, cache, q, out, lse, fmt, 4, 0, scale)
+
+
+@pytest.mark.parametrize("n", [1, 70])
+def test_attention_strides_and_orders(gpu, n):
+    """q and out as slices of a packed projection, the cache's storage in another order."""
+    sq = ko.Seqs([90, 0], [n, n], 32, seed=2)
+    cache = _cache(sq, 2, 64, "i8", gpu, order="pshd")
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 64, "bf16", gpu, 3)
+    big = torch.randn(sq.tokens, 3 * 8 + 5, 64, device=gpu).to(torch.bfloat16)
+    q = big[:, 4:12]
+    hold = torch.zeros(8, sq.tokens, 64, dtype=torch.bfloat16, device=gpu)
+    lse = torch.empty(sq.tokens, 8, device=gpu)
+    plan = ck.KvAttention(8, 2, 64, 2, sq.tokens)
+    plan.run(cache, b, q, out=hold.transpose(0, 1), lse=lse)
+    torch.cuda.synchronize()
+    _check(sq, cache, q, hold.transpose(0, 1), lse, "i8", 4, 0)
+
+
+def test_offsets_past_32_bits(gpu):
+    """Pages whose elements lie beyond 2^32 bytes of the cache's start."""
+    n_pages, page, heads, dim = 70_000, 16, 8, 512 // 4
+    k = torch.zeros(n_pages, heads, page, 4 * dim, dtype=torch.int8, device=gpu)   # 4.6 GB
+    cache = ck.KvCache(k[..., :dim], k[..., dim:2 * dim], *(torch.zeros(n_pages, heads, page, device=gpu) for _ in range(2)))
+    sq = ko.Seqs([0], [50], page)
+    sq.n_pages = n_pages
+    sq.table = np.array([[n_pages - 1, n_pages - 2, 66_000, 69_000]], np.int32)
+    b = _batch(sq, gpu)
+    x = [torch.randn(50, heads, dim, device=gpu).half() for _ in range(2)]
+    ck.kv_write(cache, b, *x)
+    back = ck.kv_read(cache, b, ck.F16)
+    for a, c in zip(x, back):
+        codes, scales = ko.quantise(a.cpu().float(), "i8")
+        assert torch.equal((codes * scales[..., None]).half(), c.cpu())
+    q = torch.randn(50, heads, dim, device=gpu).half()
+    lse = torch.empty(50, heads, device=gpu)
+    out = ck.KvAttention(heads, heads, dim, 1, 50).run(cache, b, q, lse=lse)
+    near = ko.Seqs([0], [50], page)
+    near.table, near.n_pages = np.array([[3, 2, 0, 1]], np.int32), 4
+    pick = torch.tensor([66_000, 69_000, n_pages - 2, n_pages - 1], device=gpu)
+    small = ck.KvCache(cache.k[pick].contiguous(), cache.v[pick].contiguous(), cache.k_scale[pick].contiguous(), cache.v_scale[pick].contiguous())
+    _check(near, small, q, out, lse, "i8", 1, 0)
+
+
+def test_calls_on_another_stream_and_in_a_graph(gpu):
+    """Write, read and attention on a side stream, then captured: every replay
+    (with eager work and synchronisation between) equals the eager result, and
+    follows a page table, starts and offsets changed in place."""
+    sq = ko.Seqs([300, 40], [1, 1], 16, seed=5)
+    cache = _cache(sq, 2, 128, "f8", gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 128, "bf16", gpu, 3)
+    plan = ck.KvAttention(8, 2, 128, 2, 2, 1, 400)
+    kv = [torch.randn(2, 2, 128, device=gpu).to(torch.bfloat16) for _ in range(2)]
+    q, out = torch.randn(2, 8, 128, device=gpu).to(torch.bfloat16), torch.zeros(2, 8, 128, dtype=torch.bfloat16, device=gpu)
+    back = tuple(torch.zeros(2, 2, 128, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+
+    def step(stream=None):
+        ck.kv_write(cache, b, *kv, stream=stream)
+        ck.kv_read(cache, b, ck.BF16, out=back, stream=stream)
+        plan.run(cache, b, q, out=out, stream=stream)
+
+    step()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (*back, out)]
+    side = torch.cuda.Stream()
+    for t in (*back, out):
+        t.zero_()
+    torch.cuda.synchronize()
+    step(side)
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip((*back, out), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):
+        for t in (*back, out):
+            t.zero_()
+        kv[0].copy_(torch.randn(2, 2, 128, device=gpu))
+        b.starts.copy_(torch.tensor([300 - 7 * i, 40 + i], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (*back, out)]
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip((*back, out), got)), i
+
+
+def test_empty_batches(gpu):
+    sq = ko.Seqs([10], [2], 16)
+    cache = _cache(sq, 1, 64, "f8", gpu)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=gpu)  # noqa: E731
+    for table, starts, offsets in ((torch.zeros(0, 1, dtype=torch.int32, device=gpu), i32([]), i32([0])),
+                                   (i32([[0], [1]]), i32([3, 4]), i32([0, 0, 0]))):
+        b = ck.KvBatch(table, starts, offsets, 0)
+        e = torch.empty(0, 1, 64, dtype=torch.bfloat16, device=gpu)
+        ck.kv_write(cache, b, e, e)
+        assert ck.kv_read(cache, b)[0].shape == (0, 1, 64)
+        assert ck.KvAttention(4, 1, 64, 2, 0).run(cache, b, torch.empty(0, 4, 64, dtype=torch.bfloat16, device=gpu)).shape == (0, 4, 64)
+
+
+def test_refusals(gpu):
+    sq = ko.Seqs([10], [2], 16)
+    cache = _cache(sq, 2, 64, "f8", gpu)
+    b = _batch(sq, gpu)
+    plan = ck.KvAttention(4, 2, 64, 1, 2)
+    kv = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=gpu)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=gpu)
+
+    def bad(part, f, *a, **kw):
+        with pytest.raises(ck.CkrError) as e:
+            f(*a, **kw)
+        assert e.value.code in (ck.CKR_E_INVALID, ck.CKR_E_CAPACITY) and part in str(e.value), str(e.value)
+
+    bad("[2, 2, 64]", ck.kv_write, cache, b, kv[:1], kv)
+    bad("one type", ck.kv_write, cache, b, kv, kv.half())
+    bad("type", ck.kv_write, cache, b, kv.int(), kv.int())
+    bad("contiguous", ck.kv_write, cache, b, kv.transpose(1, 2).contiguous().transpose(1, 2), kv)
+    odd = torch.zeros(2 * 2 * 64 + 1, dtype=torch.bfloat16, device=gpu)[1:].view(2, 2, 64)
+    bad("16-byte", ck.kv_write, cache, b, odd, kv)
+    bad("16-byte", plan.run, cache, b, torch.zeros(2 * 4 * 64 + 4, dtype=torch.bfloat16, device=gpu)[4:].view(2, 4, 64))
+    bad("float32, bfloat16", ck.kv_read, cache, b, ck.I8)
+    bad("type", ck.kv_read, cache, b, ck.F16, out=(kv, kv))
+    bad("bfloat16 or float16", plan.run, cache, b, q.float())
+    bad("GPU", ck.kv_write, cache, b, kv.cpu(), kv.cpu())
+    bad("lse", plan.run, cache, b, q, lse=torch.zeros(2, 4, dtype=torch.float16, device=gpu))
+    bad("scale", plan.run, cache, b, q, scale=float("nan"))
+    bad("multiple", ck.KvAttention(3, 2, 64, 1, 2).run, cache, b, torch.zeros(2, 3, 64, dtype=torch.bfloat16, device=gpu))
+    wide = _cache(sq, 2, 64, "f16", gpu)
+    bad("queries' type", plan.run, wide, b, q)
+    bad("scales", ck.KvCache, cache.k, cache.v)
+    bad("scales", ck.KvCache, wide.k, wide.v, cache.k_scale, cache.v_scale)
+    bad("scales", ck.KvCache, cache.k, cache.v, cache.k_scale, None)
+    bad("alike", ck.KvCache, cache.k, cache.v[:1], cache.k_scale, cache.v_scale)
+    for shape, part in (((3, 2, 8, 64), "page size"), ((3, 2, 24, 64), "page size"), ((3, 2, 16, 40), "head size"), ((3, 2, 16, 272), "head size")):
+        c = ck.KvCache(*(torch.zeros(shape, dtype=torch.float16, device=gpu) for _ in range(2)))
+        bad(part, ck.kv_write, c, b, *(torch.zeros(2, 2, shape[3], dtype=torch.float16, device=gpu) for _ in range(2)))
+    bad("int32", ck.KvBatch, b.page_table.long(), b.starts, b.offsets, 2)
+    bad("entries", ck.KvBatch, b.page_table, b.starts, b.offsets[:1], 2)
+    small = ck.KvBatch(b.page_table, b.starts, b.offsets, 2)
+    small._c.d_page_table = 0x1000                     # not device memory
+    bad("page table", ck.kv_write, cache, small, kv, kv)
+    torch.cuda.synchronize()
