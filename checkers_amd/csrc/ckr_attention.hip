@@ -29,107 +29,763 @@ struct AttnArg {
     const uint8_t* cv;
     const float* sk;
     const float* sv;
-    int64_t kst[3], vst[3], skst[2], svst[2];
-    uint32_t n_pages, page_shift, dim, heads, group;  // heads: query heads
+    int64_t kst[3], vst[3], skst[2], svst[2];  // of rows in bytes, of scales in elements
+    uint32_t n_pages, page_shift, dim, heads, group, kv_heads;  // heads: query heads
     uint32_t window;
-    float scale2;  // scale * log2(e): the softmax runs in powers of two
+    float scale2;   // |scale| log2(e): the softmax runs in powers of two
+    uint32_t flip;  // 0x80008000 when scale is negative: the queries' signs are flipped instead
     KvBatch b;
+    uint32_t tiles, splits, split_len;  // row tiles, key ranges of a tile, their length (a multiple of 128)
+    float* part_o;  // [tile][kv head][split][rows of a tile][DP], with splits > 1
+    float* part_m;  // [tile][kv head][split][rows of a tile][2]: maximum (in powers of two), sum
 };
 
-// One wave per (token, query head): 64 keys at a time, a key per lane for the
-// scores, four dimensions per lane for the weighted sum of the values.
-template <typename X, typename C>
-__global__ void __launch_bounds__(64) attend_row_kernel(AttnArg a) {
-    __shared__ float q[256];
-    const uint32_t token = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = threadIdx.x;
-    uint32_t seq = 0;
-    for (uint32_t base = 0; base < a.b.n_seqs; base += 64) {
-        const bool here = base + lane < a.b.n_seqs && a.b.offsets[base + lane + 1] <= (int32_t)token;
-        const int n = __popcll(__ballot(here));
-        seq += n;
-        if (n < 64) break;
+// ---- matrix instructions.  Operands are 8 elements of 16 bits a lane.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <typename E> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (E::tag == CKR_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename E> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (E::tag == CKR_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Four codes of a dword as two dwords of 16-bit values (exact: e4m3 values and
+// int8 fit both 16-bit types).
+template <typename C, typename E> __device__ __forceinline__ u32x2 widen4(uint32_t v) {
+    if constexpr (C::tag == CKR_F8 && E::tag == CKR_BF16)
+        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.f, true))};
+    else if constexpr (C::tag == CKR_F8)
+        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.f, true))};
+    else {
+        const f32x4 f = codes4<C>(v);
+        return u32x2{pack16<E>(f[0], f[1]), pack16<E>(f[2], f[3])};
     }
-    const int64_t kh = head / a.group;
-    for (uint32_t d = lane; d < a.dim; d += 64)
-        q[d] = load_one<X>(a.q + ((int64_t)token * a.q_tok + (int64_t)head * a.q_head) * 2, d) * a.scale2;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// Maximum over the lanes l, l ^ 32 (and l ^ 16).
+__device__ __forceinline__ float max_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
+    return fmaxf(as_f32(r[0]), as_f32(r[1]));
+}
+__device__ __forceinline__ float max_quarters(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
+    return max_half(fmaxf(as_f32(r[0]), as_f32(r[1])));
+}
+__device__ __forceinline__ float sum_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
+    return as_f32(r[0]) + as_f32(r[1]);
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
+    return sum_half(as_f32(r[0]) + as_f32(r[1]));
+}
+
+// The probabilities' type: 8-bit values meet bfloat16 weights, which take the
+// value's scale without a range of their own; float16 values meet float16
+// weights, scaled up by 2^7 (their largest is 1, or 2^8 where a running maximum
+// lags, so at most 2^15) so that small ones keep their bits.
+template <typename C> struct Prob { typedef ElemBF16 E; static constexpr float up = 0.f; };
+template <> struct Prob<ElemF16> { typedef ElemF16 E; static constexpr float up = 7.f; };
+// How far a row's running maximum may lag behind (in powers of two) before the
+// accumulators are scaled: sums and outputs use the same lagging maximum.
+constexpr float kLag = 8.f;
+
+// Which sequence and rows a tile of BM rows is: rows of a sequence are its
+// chunk's tokens times the query heads of a key/value head, in that order.
+// Every thread of the block calls it; s_tmp: 8 words of LDS.
+struct Tile {
+    uint32_t seq, row0, rows, token0;  // rows: of the whole sequence; token0: its first packed row
+    int64_t start, end;                // the position of its first token, and after its last
+};
+template <uint32_t BM>
+__device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint32_t tile, uint32_t* s_tmp, Tile& t) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t done = 0;
+    for (uint32_t base = 0; base < b.n_seqs; base += 256) {
+        const uint32_t i = base + threadIdx.x;
+        uint32_t n = 0;
+        if (i < b.n_seqs) {
+            const int32_t lo = b.offsets[i], hi = min(b.offsets[i + 1], (int32_t)b.n_tokens);
+            n = lo >= 0 && hi > lo ? ((uint32_t)(hi - lo) * group + BM - 1) / BM : 0;
+        }
+        uint32_t sum = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t u = (uint32_t)__shfl_up((int)sum, d);
+            if (lane >= (uint32_t)d) sum += u;
+        }
+        if (lane == 63) s_tmp[wave] = sum;
+        __syncthreads();
+        uint32_t before = done, all = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < 4; w++) {
+            if (w < wave) before += s_tmp[w];
+            all += s_tmp[w];
+        }
+        if (tile < done + all) {
+            const uint32_t first = before + sum - n;
+            if (tile >= first && tile < first + n) s_tmp[4] = i, s_tmp[5] = tile - first;
+            __syncthreads();
+            t.seq = s_tmp[4], t.row0 = s_tmp[5] * BM;
+            const int32_t lo = b.offsets[t.seq], hi = min(b.offsets[t.seq + 1], (int32_t)b.n_tokens);
+            t.token0 = (uint32_t)lo, t.rows = (uint32_t)(hi - lo) * group;
+            t.start = b.starts[t.seq], t.end = t.start + (hi - lo);
+            return true;
+        }
+        done += all;
+        __syncthreads();
+    }
+    return false;
+}
+
+// ------------------------------------------------------------ few rows
+// A wave takes tiles of 32 keys against 16 rows (16x16x32 matrix products):
+//   S^T = K Q^T: operand A holds a key per lane and row, so a lane reads whole
+//   16-byte pieces of its key's row; the order of the contraction is free, and Q
+//   is laid out to match;
+//   O^T = V^T P^T: the lane's 8 keys of P are the rows of S^T it already holds
+//   (keys 4 g + i and 16 + 4 g + i of the tile, g the lane's quarter), so P needs no
+//   exchange between lanes; V's operand holds those keys for one dimension, which
+//   a lane gets by loading NV = DP / 16 dimensions of 8 keys and transposing them in
+//   registers.
+// So nothing goes through LDS but the join of the block's four waves.
+template <typename C, int DP> struct FewRegs {
+    static constexpr int KL = DP * C::bytes / 64;      // 16-byte pieces of a key's row per lane
+    static constexpr int VD = DP / 16 * C::bytes / 4;  // dwords of a key's value row per lane
+    u32x4 k[2][KL];
+    uint32_t v[8][VD];
+    f32x4 sk[2], sv[2];
+};
+
+template <typename X, typename C, int DP>
+__global__ void __launch_bounds__(256, (DP * C::bytes > 256 ? 1 : 2)) attend_few_kernel(AttnArg a) {
+    typedef typename Prob<C>::E P;
+    typedef FewRegs<C, DP> Regs;
+    constexpr int KL = Regs::KL, VD = Regs::VD, NV = DP / 16, KS = DP / 32;
+    __shared__ float s_o[4][16][DP + 4];
+    __shared__ float s_m[4][16][2];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
+    Tile t;
+    if (!find_tile<16>(a.b, a.group, tile, reinterpret_cast<uint32_t*>(s_m), t)) return;
     __syncthreads();
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    if (seq < a.b.n_seqs) {
-        const int64_t pos = (int64_t)a.b.starts[seq] + (int64_t)token - a.b.offsets[seq];
-        const int64_t first = a.window ? max((int64_t)0, pos - (int64_t)a.window + 1) : 0;
-        const int64_t end = min(pos + 1, (int64_t)a.b.width << a.page_shift);
-        for (int64_t base = first & ~63ll; base < end; base += 64) {
-            const int64_t j = base + lane;
-            const int32_t page = j >= first && j < end ? page_of(a.b, seq, j, a.page_shift, a.n_pages) : -1;
-            const int64_t slot = j & ((1ll << a.page_shift) - 1);
-            float s = -INFINITY, vs = 0.f;
-            if (page >= 0) {
-                const uint8_t* k = a.ck + ((int64_t)page * a.kst[0] + kh * a.kst[1] + slot * a.kst[2]) * C::bytes;
-                float dot = 0.f;
-                for (uint32_t d = 0; d < a.dim; d += 16) {
-                    float x[16];
-                    load_vec<C, 16>(k + d * C::bytes, x);
+    // the keys that some row of the tile sees, this split's part of them, this wave's
+    const uint32_t row = t.row0 + col, last_row = min(t.row0 + 15, t.rows - 1);
+    const int64_t pos = t.start + min(row, t.rows - 1) / a.group;
+    const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + last_row / a.group;
+    const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
+    const int64_t first = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) & ~31ll : 0;
+    const int64_t see = a.window ? pos - (int64_t)a.window : -1;  // a row sees keys above this
+    int64_t lo = first + (int64_t)split * a.split_len, hi = split + 1 == a.splits ? limit : min(limit, lo + (int64_t)a.split_len);
+    const int64_t n_tiles = hi > lo ? (hi - lo + 31) / 32 : 0, per = (n_tiles + 3) / 4;
+    const int64_t t0 = lo + 32 * min(n_tiles, per * wave), t1 = lo + 32 * min(n_tiles, per * (wave + 1));
+
+    // queries: the elements of each 32-wide step in the order of the keys' pieces
+    u32x4 q[KS];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) dot = __builtin_fmaf(x[i], q[d + i], dot);
-                }
-                if constexpr (C::bytes == 1) {
-                    dot *= a.sk[(int64_t)page * a.skst[0] + kh * a.skst[1] + slot];
-                    vs = a.sv[(int64_t)page * a.svst[0] + kh * a.svst[1] + slot];
-                } else {
-                    vs = 1.f;
-                }
-                s = dot;
+    for (int ks = 0; ks < KS; ks++) {
+        const uint32_t d = C::bytes == 1 ? (ks / 2) * 64 + g * 16 + (ks % 2) * 8 : ks * 32 + g * 8;
+        q[ks] = u32x4{0, 0, 0, 0};
+        if (row < t.rows && d < a.dim) {
+            q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(t.token0 + row / a.group) * a.q_tok +
+                                                          (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
+            q[ks] ^= a.flip;
+        }
+    }
+    const int64_t k_off = (int64_t)col * a.kst[2] + g * 16, v_off = (int64_t)(4 * g) * a.vst[2] + col * (VD * 4);
+    const bool v_in = col * NV < a.dim;
+    const int32_t* table = a.b.table + (int64_t)t.seq * a.b.table_stride;
+    const auto page_lane = [&](int64_t c0) {  // lane i: the page of table column c0 + i
+        const int64_t c = c0 + lane;
+        const int32_t p = c < (int64_t)a.b.width ? table[c] : -1;
+        return (uint32_t)p < a.n_pages ? p : -1;
+    };
+    const auto load = [&](Regs& r, int64_t base, int32_t p0, int32_t p1) {
+        const uint32_t mask = (1u << a.page_shift) - 1;
+        const bool whole = p0 >= 0 && p1 >= 0 && base + 32 <= limit && DP == a.dim;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int32_t page = h ? p1 : p0;
+            const int64_t slot = ((uint32_t)base + 16 * h) & mask;
+            const uint8_t* kp = a.ck + (int64_t)page * a.kst[0] + (int64_t)kvh * a.kst[1] + slot * a.kst[2] + k_off;
+            const uint8_t* vp = a.cv + (int64_t)page * a.vst[0] + (int64_t)kvh * a.vst[1] + slot * a.vst[2] + v_off;
+#pragma unroll
+            for (int j = 0; j < KL; j++) {
+                r.k[h][j] = u32x4{0, 0, 0, 0};
+                if (whole || (page >= 0 && base + 16 * h + col < limit && (j * 64 + g * 16) / C::bytes < a.dim))
+                    r.k[h][j] = *reinterpret_cast<const u32x4*>(kp + j * 64);
             }
-            // a NaN score must reach the result: fmax alone would pass it over
-            float top = s;
-            for (int d = 32; d; d /= 2) {
-                const float u = __shfl_xor(top, d);
-                top = u != u || top != top ? NAN : fmaxf(top, u);
-            }
-            if (top == -INFINITY) continue;  // no key of these 64
-            const float m2 = m != m || top != top ? NAN : fmaxf(m, top);
-            const float back = m == -INFINITY ? 0.f : exp2f(m - m2);
-            float p = page >= 0 ? exp2f(s - m2) : 0.f, sum = p;
-            for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-            l = l * back + sum;
-            m = m2;
-            p = page >= 0 ? p * vs : 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] *= back;
-            for (int t = 0; t < 64; t++) {
-                const int32_t pg = __shfl(page, t);
-                const float w = __shfl(p, t);
-                if (pg < 0) continue;
-                const uint8_t* v = a.cv + ((int64_t)pg * a.vst[0] + kh * a.vst[1] + ((base + t) & ((1ll << a.page_shift) - 1)) * a.vst[2]) * C::bytes;
-                if (4 * lane < a.dim) {
-                    if constexpr (C::bytes == 1) {
-                        const f32x4 x = codes4<C>(*reinterpret_cast<const uint32_t*>(v + 4 * lane));
+            for (int i = 0; i < 4; i++) {
+                const uint32_t* x = reinterpret_cast<const uint32_t*>(vp + i * a.vst[2]);
+                const bool in = whole || (page >= 0 && base + 16 * h + 4 * g + i < limit && v_in);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(w, x[i], o[i]);
+                for (int j = 0; j < VD; j++) r.v[4 * h + i][j] = 0;
+                if (in) {
+                    if constexpr (VD == 1) r.v[4 * h + i][0] = *x;
+                    else if constexpr (VD == 2) {
+                        const u32x2 y = *reinterpret_cast<const u32x2*>(x);
+                        r.v[4 * h + i][0] = y[0], r.v[4 * h + i][1] = y[1];
                     } else {
-                        const u32x2 x = *reinterpret_cast<const u32x2*>(v + 8 * lane);
-                        o[0] = __builtin_fmaf(w, lo16<C>(x.x), o[0]);
-                        o[1] = __builtin_fmaf(w, hi16<C>(x.x), o[1]);
-                        o[2] = __builtin_fmaf(w, lo16<C>(x.y), o[2]);
-                        o[3] = __builtin_fmaf(w, hi16<C>(x.y), o[3]);
+#pragma unroll
+                        for (int j = 0; j < VD; j += 4) {
+                            const u32x4 y = *reinterpret_cast<const u32x4*>(x + j);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) r.v[4 * h + i][j + k] = y[k];
+                        }
                     }
                 }
             }
+            if constexpr (C::bytes == 1) {
+                r.sk[h] = r.sv[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (page >= 0) {
+                    r.sk[h] = *reinterpret_cast<const f32x4*>(a.sk + (int64_t)page * a.skst[0] + (int64_t)kvh * a.skst[1] + slot + 4 * g);
+                    r.sv[h] = *reinterpret_cast<const f32x4*>(a.sv + (int64_t)page * a.svst[0] + (int64_t)kvh * a.svst[1] + slot + 4 * g);
+                }
+            }
+        }
+    };
+
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[NV];
+#pragma unroll
+    for (int c = 0; c < NV; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto compute = [&](const Regs& r, int64_t base, int32_t p0, int32_t p1) {
+        f32x4 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KL; j++) {
+                if constexpr (C::bytes == 1) {
+                    const u32x4 x = r.k[h][j];
+                    const u32x2 w0 = widen4<C, X>(x[0]), w1 = widen4<C, X>(x[1]), w2 = widen4<C, X>(x[2]), w3 = widen4<C, X>(x[3]);
+                    s[h] = mfma16<X>(u32x4{w0[0], w0[1], w1[0], w1[1]}, q[2 * j], s[h]);
+                    s[h] = mfma16<X>(u32x4{w2[0], w2[1], w3[0], w3[1]}, q[2 * j + 1], s[h]);
+                } else {
+                    s[h] = mfma16<X>(r.k[h][j], q[j], s[h]);
+                }
+            }
+        }
+        // every row sees every key of the tile, or not
+        const bool full = p0 >= 0 && p1 >= 0 && base + 31 <= pos_lo && base + 32 <= limit &&
+                          (!a.window || base > pos_hi - (int64_t)a.window);
+        uint32_t seen = 0xffu;
+        if (!full) {
+            seen = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int64_t j = base + 16 * (i / 4) + 4 * g + i % 4;
+                if ((i < 4 ? p0 : p1) >= 0 && j <= pos && j > see && j < limit) seen |= 1u << i;
+            }
+        }
+        float x[8], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[i] = s[i / 4][i % 4] * a.scale2;
+            if constexpr (C::bytes == 1) x[i] *= r.sk[i / 4][i % 4];
+            if (!full) x[i] = seen >> i & 1 ? x[i] : -INFINITY;
+            top = fmaxf(top, x[i]);
+        }
+        top = max_quarters(top);
+        if (__any(top > m + kLag)) {
+            const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
+            m = m2;
+            l *= back;
+#pragma unroll
+            for (int c = 0; c < NV; c++) o[c] *= back;
+        }
+        const float ref = m == -INFINITY ? 0.f : m - Prob<C>::up;
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i] = exp2_fast(x[i] - ref);
+            l += p[i];
+            if constexpr (C::bytes == 1) p[i] *= r.sv[i / 4][i % 4];
+            if (!full) p[i] = seen >> i & 1 ? p[i] : 0.f;
+        }
+        const u32x4 pf = {pack16<P>(p[0], p[1]), pack16<P>(p[2], p[3]), pack16<P>(p[4], p[5]), pack16<P>(p[6], p[7])};
+        if constexpr (C::bytes == 1) {
+#pragma unroll
+            for (int j = 0; j < VD; j++) {  // four dimensions of eight keys
+                uint32_t w[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t a0 = r.v[4 * h][j], a1 = r.v[4 * h + 1][j], a2 = r.v[4 * h + 2][j], a3 = r.v[4 * h + 3][j];
+                    const uint32_t x0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), x1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
+                    const uint32_t y0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), y1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+                    w[h][0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u);
+                    w[h][1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
+                    w[h][2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u);
+                    w[h][3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const u32x2 w0 = widen4<C, P>(w[0][k]), w1 = widen4<C, P>(w[1][k]);
+                    o[4 * j + k] = mfma16<P>(u32x4{w0[0], w0[1], w1[0], w1[1]}, pf, o[4 * j + k]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VD; j++) {  // two dimensions of eight keys
+                u32x4 w0, w1;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
+                    w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
+                }
+                o[2 * j] = mfma16<P>(w0, pf, o[2 * j]);
+                o[2 * j + 1] = mfma16<P>(w1, pf, o[2 * j + 1]);
+            }
+        }
+    };
+
+    if (t0 < t1) {
+        // table columns c0 .. c0 + 63 in a register of the wave, the next 64 on their way
+        int64_t c0 = t0 >> a.page_shift;
+        int32_t now = page_lane(c0), next = page_lane(c0 + 64);
+        const auto page_at = [&](int64_t base) {
+            int64_t c = base >> a.page_shift;
+            if (c - c0 >= 64) {
+                c0 += 64;
+                now = next;
+                next = page_lane(c0 + 64);
+            }
+            return (int32_t)__builtin_amdgcn_readlane(now, (int)(c - c0));
+        };
+        Regs r[2];
+        int32_t p[2][2];
+        p[0][0] = page_at(t0), p[0][1] = page_at(t0 + 16);
+        load(r[0], t0, p[0][0], p[0][1]);
+        for (int64_t base = t0; base < t1; base += 64) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int64_t at = base + 32 * u;
+                if (at >= t1) break;
+                if (at + 32 < t1) {
+                    p[1 - u][0] = page_at(at + 32), p[1 - u][1] = page_at(at + 48);
+                    load(r[1 - u], at + 32, p[1 - u][0], p[1 - u][1]);
+                }
+                compute(r[u], at, p[u][0], p[u][1]);
+            }
         }
     }
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
-    if (4 * lane < a.dim) {
-        uint8_t* out = a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head + 4 * lane) * 2;
-        *reinterpret_cast<u32x2*>(out) = u32x2{pack16<X>(o[0] * inv, o[1] * inv), pack16<X>(o[2] * inv, o[3] * inv)};
+    // join the four waves: lane (col, g) holds dimensions 4 g NV .. 4 (g + 1) NV of row col
+    l = sum_quarters(l);
+    if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int c = 0; c < NV; c++) s_o[wave][col][(4 * g + i) * NV + c] = o[c][i];
+    if (g == 0) s_m[wave][col][0] = m, s_m[wave][col][1] = l;
+    __syncthreads();
+    const uint64_t part = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * 16;
+    for (uint32_t e = threadIdx.x; e < 16 * (DP / 4); e += 256) {
+        const uint32_t rr = e / (DP / 4), d = e % (DP / 4) * 4, orow = t.row0 + rr;
+        if (orow >= t.rows) continue;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) top = fmaxf(top, s_m[w][rr][0]);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float mw = s_m[w][rr][0], f = mw == -INFINITY ? 0.f : exp2_fast(mw - top);
+            sum += s_m[w][rr][1] * f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] += mw == -INFINITY ? 0.f : s_o[w][rr][d + k] * f;
+        }
+        if (a.splits > 1) {
+            *reinterpret_cast<f32x4*>(a.part_o + (part + rr) * DP + d) = v;
+            if (d == 0) a.part_m[(part + rr) * 2] = top, a.part_m[(part + rr) * 2 + 1] = sum;
+            continue;
+        }
+        const uint32_t token = t.token0 + orow / a.group, head = kvh * a.group + orow % a.group;
+        const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+        if (d < a.dim)
+            *reinterpret_cast<u32x2*>(a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head + d) * 2) =
+                u32x2{pack16<X>(v[0] * inv, v[1] * inv), pack16<X>(v[2] * inv, v[3] * inv)};
+        if (a.lse && d == 0) a.lse[(int64_t)token * a.heads + head] = top == -INFINITY ? -INFINITY : (top - Prob<C>::up + log2f(sum)) * kLn2;
     }
-    if (a.lse && lane == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-template <typename X, typename C>
-hipError_t launch_attend(const AttnArg& a, hipStream_t s) {
-    const uint64_t rows = (uint64_t)a.b.n_tokens * a.heads;
-    CKR_LAUNCH("kv_attention", s, attend_row_kernel<X, C><<<dim3((uint32_t)rows), 64, 0, s>>>(a));
+// ------------------------------------------------------------ many rows
+// A block takes BM = 128 rows, a wave 32 of them (32x32x16 matrix products), against
+// tiles of TK keys staged through LDS in 16 bits, double buffered: while a tile is
+// computed, the next one's bytes are on their way to registers, and the one
+// after's page numbers too; 8-bit codes are widened once, when they are stored to LDS.
+//   S^T = K Q^T: a lane holds one row (its column) and 16 of 32 keys, 8 (i / 4) + 4 h + i % 4
+//   with h its half, so a row's maximum takes one exchange between two lanes;
+//   O^T = V^T P^T: P's operand is again what the lane holds (eight keys of each 16);
+//   V's is read transposed from LDS, four keys of one dimension at a time.
+template <typename C, int DP> struct ManyShape {
+    static constexpr int TK = DP > 128 ? 32 : 64;
+    static constexpr int PITCH = DP * 2 + 32;  // bytes of a row in LDS: rows 8 banks apart (mod 64)
+    static constexpr int LPR = DP * C::bytes / 16, LOADS = TK * LPR / 256;  // lanes of a row, 16-byte loads a thread
+    static constexpr int ROWS = 256 / LPR;                                  // rows a load of the block covers
+};
+
+template <typename X, typename C, int DP>
+__global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(AttnArg a) {
+    typedef typename Prob<C>::E P;
+    typedef ManyShape<C, DP> Sh;
+    constexpr int TK = Sh::TK, PITCH = Sh::PITCH, LPR = Sh::LPR, LOADS = Sh::LOADS, ROWS = Sh::ROWS;
+    constexpr int KS = DP / 16, DT = DP / 32, TT = TK / 32;
+    static_assert(LOADS >= 1 && TK * LPR % 256 == 0, "a tile is whole loads of the block");
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[2][TK * PITCH];
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[2][TK * PITCH];
+    __shared__ __attribute__((aligned(16))) float s_sk[2][TK];
+    __shared__ __attribute__((aligned(16))) float s_sv[2][TK];
+    __shared__ uint64_t s_valid[2];
+    __shared__ uint32_t s_tmp[8];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
+    Tile t;
+    if (!find_tile<128>(a.b, a.group, tile, s_tmp, t)) return;
+    const uint32_t row = t.row0 + wave * 32 + col;
+    const int64_t pos = t.start + min(row, t.rows - 1) / a.group;
+    const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + 127, t.rows - 1) / a.group;
+    // the wave's own range of positions
+    const int64_t wave_lo = t.start + min(t.row0 + wave * 32, t.rows - 1) / a.group;
+    const int64_t wave_hi = t.start + min(t.row0 + wave * 32 + 31, t.rows - 1) / a.group;
+    const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
+    const int64_t first = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) & ~(int64_t)(TK - 1) : 0;
+    const int64_t see = a.window ? pos - (int64_t)a.window : -1;
+    const int64_t lo = first + (int64_t)split * a.split_len;
+    const int64_t hi = split + 1 == a.splits ? limit : min(limit, lo + (int64_t)a.split_len);
+    const int n_tiles = hi > lo ? (int)((hi - lo + TK - 1) / TK) : 0;
+
+    u32x4 q[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        const uint32_t d = ks * 16 + half * 8;
+        q[ks] = u32x4{0, 0, 0, 0};
+        if (row < t.rows && d < a.dim) {
+            q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(t.token0 + row / a.group) * a.q_tok +
+                                                          (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
+            q[ks] ^= a.flip;
+        }
+    }
+    // staging: thread's rows r0 + u ROWS of a tile, 16 bytes at its place in the row
+    const int32_t* table = a.b.table + (int64_t)t.seq * a.b.table_stride;
+    const uint32_t r0 = threadIdx.x / LPR, piece = threadIdx.x % LPR;
+    const bool d_in = piece * 16 / C::bytes < a.dim;
+    const uint32_t slot_mask = (1u << a.page_shift) - 1;
+    const auto page_id = [&](int64_t j) {
+        const int64_t c = j >> a.page_shift;
+        const int32_t p = j < limit && c < (int64_t)a.b.width ? table[c] : -1;
+        return (uint32_t)p < a.n_pages ? p : -1;
+    };
+    int32_t pg[LOADS], pg_s = -1;  // pages of the rows of the tile that is loaded next; of key threadIdx % TK for its scale
+    const auto load_pages = [&](int64_t base) {
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) pg[u] = page_id(base + r0 + u * ROWS);
+        if (threadIdx.x < 2 * TK) pg_s = page_id(base + threadIdx.x % TK);
+    };
+    u32x4 kr[LOADS], vr[LOADS];
+    float sr = 0.f;
+    bool in_s = false;
+    const auto load_tile = [&](int64_t base) {
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) {
+            const int64_t slot = (uint32_t)(base + r0 + u * ROWS) & slot_mask;
+            kr[u] = vr[u] = u32x4{0, 0, 0, 0};
+            if (pg[u] >= 0 && d_in) {
+                kr[u] = *reinterpret_cast<const u32x4*>(a.ck + (int64_t)pg[u] * a.kst[0] + (int64_t)kvh * a.kst[1] + slot * a.kst[2] + piece * 16);
+                vr[u] = *reinterpret_cast<const u32x4*>(a.cv + (int64_t)pg[u] * a.vst[0] + (int64_t)kvh * a.vst[1] + slot * a.vst[2] + piece * 16);
+            }
+        }
+        in_s = pg_s >= 0;
+        if (threadIdx.x < 2 * TK) {
+            sr = 0.f;
+            if (C::bytes == 1 && in_s) {
+                const int64_t slot = (uint32_t)(base + threadIdx.x % TK) & slot_mask;
+                sr = threadIdx.x < TK ? a.sk[(int64_t)pg_s * a.skst[0] + (int64_t)kvh * a.skst[1] + slot] * a.scale2
+                                      : a.sv[(int64_t)pg_s * a.svst[0] + (int64_t)kvh * a.svst[1] + slot];
+            }
+        }
+    };
+    const auto store_tile = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) {
+            uint8_t* k = s_k[buf] + (r0 + u * ROWS) * PITCH;
+            uint8_t* v = s_v[buf] + (r0 + u * ROWS) * PITCH;
+            if constexpr (C::bytes == 2) {
+                *reinterpret_cast<u32x4*>(k + piece * 16) = kr[u];
+                *reinterpret_cast<u32x4*>(v + piece * 16) = vr[u];
+            } else {
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const u32x2 x = widen4<C, X>(kr[u][2 * w]), y = widen4<C, X>(kr[u][2 * w + 1]);
+                    *reinterpret_cast<u32x4*>(k + piece * 32 + w * 16) = u32x4{x[0], x[1], y[0], y[1]};
+                    const u32x2 z = widen4<C, P>(vr[u][2 * w]), zz = widen4<C, P>(vr[u][2 * w + 1]);
+                    *reinterpret_cast<u32x4*>(v + piece * 32 + w * 16) = u32x4{z[0], z[1], zz[0], zz[1]};
+                }
+            }
+        }
+        if constexpr (C::bytes == 1) {
+            if (threadIdx.x < TK) s_sk[buf][threadIdx.x] = sr;
+            else if (threadIdx.x < 2 * TK) s_sv[buf][threadIdx.x - TK] = sr;
+        }
+        if (threadIdx.x < 64) {
+            const uint64_t ok = __ballot(in_s && lane < TK);
+            if (lane == 0) s_valid[buf] = ok;
+        }
+    };
+
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
+    // where this lane reads V: 4 keys x 16 dimensions per group of 16 lanes
+    const uint32_t v_lane = (4 * half + (lane & 15) / 4) * PITCH + (16 * ((lane >> 4) & 1) + (lane & 3) * 4) * 2;
+
+    const auto compute = [&](int buf, int64_t base) {
+        if (base > wave_hi) return;                                             // every key is after every row
+        if (a.window && base + TK - 1 <= wave_lo - (int64_t)a.window) return;   // every key has left every window
+        f32x16 s[TT];
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[tt][i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const u32x4 k = *reinterpret_cast<const u32x4*>(s_k[buf] + (tt * 32 + col) * PITCH + ks * 32 + half * 16);
+                s[tt] = mfma32<X>(k, q[ks], s[tt]);
+            }
+        }
+        const uint64_t valid = s_valid[buf];
+        const bool full = valid == (TK == 64 ? ~0ull : (1ull << TK % 64) - 1) && base + TK - 1 <= wave_lo &&
+                          (!a.window || base > wave_hi - (int64_t)a.window);
+        float top = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                if constexpr (C::bytes == 1) {
+                    const f32x4 sk = *reinterpret_cast<const f32x4*>(&s_sk[buf][tt * 32 + 2 * i + 4 * half]);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) s[tt][i + k] *= sk[k];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) s[tt][i + k] *= a.scale2;
+                }
+            }
+        uint32_t seen[TT];
+        if (!full) {
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) {
+                seen[tt] = 0;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = tt * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                    if ((valid >> key & 1) && base + key <= pos && base + key > see) seen[tt] |= 1u << i;
+                    s[tt][i] = seen[tt] >> i & 1 ? s[tt][i] : -INFINITY;
+                }
+            }
+        }
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[tt][i]);
+        top = max_half(top);
+        if (__any(top > m + kLag)) {
+            const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
+            m = m2;
+            l *= back;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[dt][i] *= back;
+        }
+        const float ref = m == -INFINITY ? 0.f : m - Prob<C>::up;
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) {
+                float p[8];
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        p[i + k] = exp2_fast(s[tt][8 * kb + i + k] - ref);
+                        l += p[i + k];
+                    }
+                    if constexpr (C::bytes == 1) {
+                        const f32x4 sv = *reinterpret_cast<const f32x4*>(&s_sv[buf][tt * 32 + 16 * kb + 2 * i + 4 * half]);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) p[i + k] *= sv[k];
+                    }
+                    if (!full) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) p[i + k] = seen[tt] >> (8 * kb + i + k) & 1 ? p[i + k] : 0.f;
+                    }
+                }
+                const u32x4 pf = {pack16<P>(p[0], p[1]), pack16<P>(p[2], p[3]), pack16<P>(p[4], p[5]), pack16<P>(p[6], p[7])};
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    typedef short s16x4 __attribute__((ext_vector_type(4)));
+                    typedef __attribute__((address_space(3))) s16x4* lds4;
+                    const uint8_t* at = s_v[buf] + (tt * 32 + kb * 16) * PITCH + v_lane + dt * 64;
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at));
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * PITCH));
+                    const u32x2 xa = __builtin_bit_cast(u32x2, x), ya = __builtin_bit_cast(u32x2, y);
+                    o[dt] = mfma32<P>(u32x4{xa[0], xa[1], ya[0], ya[1]}, pf, o[dt]);
+                }
+            }
+    };
+
+    if (n_tiles > 0) {
+        load_pages(lo);
+        load_tile(lo);
+        load_pages(lo + TK);
+        store_tile(0);
+        __syncthreads();
+        for (int i = 0; i < n_tiles; i++) {
+            const int64_t base = lo + (int64_t)i * TK;
+            if (i + 1 < n_tiles) {
+                load_tile(base + TK);
+                load_pages(base + 2 * TK);
+            }
+            compute(i & 1, base);
+            if (i + 1 < n_tiles) store_tile((i + 1) & 1);
+            __syncthreads();
+        }
+    }
+    l = sum_half(l);
+    if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+    if (row >= t.rows) return;
+    if (a.splits > 1) {
+        const uint64_t p = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * 128 + wave * 32 + col;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f32x4*>(a.part_o + p * DP + dt * 32 + 2 * i + 4 * half) = f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+        if (half == 0) a.part_m[p * 2] = m, a.part_m[p * 2 + 1] = l;
+        return;
+    }
+    const uint32_t token = t.token0 + row / a.group, head = kvh * a.group + row % a.group;
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    uint8_t* out = a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head) * 2;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const uint32_t d = dt * 32 + 2 * i + 4 * half;
+            if (d < a.dim)
+                *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[dt][i] * inv, o[dt][i + 1] * inv), pack16<X>(o[dt][i + 2] * inv, o[dt][i + 3] * inv)};
+        }
+    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<C>::up + log2f(l)) * kLn2;
+}
+
+// ------------------------------------------------------------ the splits' join
+// The splits of a row, in their order: 4 dimensions a thread.
+template <typename X, int DP, uint32_t BM>
+__global__ void __launch_bounds__(256) attend_join_kernel(AttnArg a, float up) {
+    __shared__ uint32_t s_tmp[8];
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
+    Tile t;
+    if (!find_tile<BM>(a.b, a.group, tile, s_tmp, t)) return;
+    constexpr uint32_t PER = 256 / (DP / 4);  // rows of a block
+    const uint32_t rr = blockIdx.y * PER + threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4, row = t.row0 + rr;
+    if (rr >= BM || row >= t.rows) return;
+    const uint64_t part = ((uint64_t)tile * a.kv_heads + kvh) * a.splits * BM + rr;
+    float top = -INFINITY, sum = 0.f;
+    for (uint32_t s = 0; s < a.splits; s++) top = fmaxf(top, a.part_m[(part + (uint64_t)s * BM) * 2]);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s = 0; s < a.splits; s++) {
+        const uint64_t p = part + (uint64_t)s * BM;
+        const float ms = a.part_m[p * 2];
+        if (ms == -INFINITY) continue;
+        const float f = exp2_fast(ms - top);
+        sum += a.part_m[p * 2 + 1] * f;
+        v += *reinterpret_cast<const f32x4*>(a.part_o + p * DP + d) * f;
+    }
+    const uint32_t token = t.token0 + row / a.group, head = kvh * a.group + row % a.group;
+    const float inv = top == -INFINITY ? 0.f : 1.f / sum;  // both carry 2^up
+    if (d < a.dim)
+        *reinterpret_cast<u32x2*>(a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head + d) * 2) =
+            u32x2{pack16<X>(v[0] * inv, v[1] * inv), pack16<X>(v[2] * inv, v[3] * inv)};
+    if (a.lse && d == 0) a.lse[(int64_t)token * a.heads + head] = top == -INFINITY ? -INFINITY : (top - up + log2f(sum)) * kLn2;
+}
+// ------------------------------------------------------------ the launch
+// How a batch is cut: rows of a tile, tiles (an upper bound: each sequence's last
+// tile may be short), key ranges of a tile.
+struct Cut {
+    uint32_t bm, dp, tiles, splits, split_len;
+    uint64_t part_m_bytes, bytes;  // of the workspace: the rows' maxima and sums, then their outputs
+};
+constexpr uint32_t kFewRows = 16, kManyRows = 128;
+constexpr uint64_t kSplitMin = 128;                   // keys of a split at least
+uint64_t blocks_wanted(uint32_t bm) { return bm == kFewRows ? 2048 : 512; }
+uint32_t padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+uint64_t most_tiles(uint32_t bm, uint64_t group, uint64_t n_seqs, uint64_t n_tokens) {
+    return std::min(n_tokens * group / bm + std::min(n_seqs, n_tokens), n_tokens * ((group + bm - 1) / bm));
+}
+uint64_t part_bytes(uint64_t rows, uint32_t dp, uint64_t* m_bytes) {
+    *m_bytes = (rows * 8 + 255) / 256 * 256;
+    return *m_bytes + rows * dp * 4;
+}
+Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t n_tokens, uint32_t max_chunk,
+        uint64_t max_context, uint32_t window) {
+    Cut c{};
+    const uint64_t group = n_heads / n_kv;
+    c.dp = padded_dim(dim);
+    c.bm = (uint64_t)max_chunk * group <= kFewRows ? kFewRows : kManyRows;
+    c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
+    // the keys of a tile: a window's, and as many again as the tile has tokens
+    if (window) max_context = std::min<uint64_t>(max_context, (uint64_t)window + c.bm / group + 64);
+    const uint64_t blocks = std::max<uint64_t>((uint64_t)c.tiles * n_kv, 1);
+    const uint64_t most = std::max<uint64_t>((max_context + kSplitMin - 1) / kSplitMin, 1);
+    const uint64_t splits = std::min(std::max<uint64_t>(blocks_wanted(c.bm) / blocks, 1), most);
+    c.split_len = (uint32_t)std::min<uint64_t>((std::max<uint64_t>(max_context, 1) + splits * kSplitMin - 1) / (splits * kSplitMin) * kSplitMin, 1u << 31);
+    c.splits = (uint32_t)std::max<uint64_t>((max_context + c.split_len - 1) / c.split_len, 1);
+    if (c.splits > 1) c.bytes = part_bytes(blocks * c.splits * c.bm, c.dp, &c.part_m_bytes);
+    return c;
+}
+// What cut() asks for at most, for any batch up to these sizes.
+uint64_t most_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t n_tokens, uint64_t max_context) {
+    uint64_t most = 0, m;
+    for (const uint32_t bm : {kFewRows, kManyRows}) {
+        const uint64_t blocks = most_tiles(bm, n_heads / n_kv, n_seqs, n_tokens) * n_kv;
+        const uint64_t parts = std::min(blocks_wanted(bm), blocks * ((max_context + kSplitMin - 1) / kSplitMin));
+        if (max_context > kSplitMin) most = std::max(most, part_bytes(parts * bm, padded_dim(dim), &m));
+    }
+    return most;
+}
+
+template <typename X, typename C, int DP>
+hipError_t launch_attend(const AttnArg& a, const Cut& c, hipStream_t s) {
+    const dim3 grid(a.tiles * a.kv_heads, c.splits);
+    if (c.bm == kFewRows) CKR_LAUNCH("kv_attention_few", s, attend_few_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
+    else CKR_LAUNCH("kv_attention_many", s, attend_many_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
+    if (c.splits > 1) {
+        const uint32_t per = 256 / (DP / 4);
+        const dim3 jgrid(a.tiles * a.kv_heads, (c.bm + per - 1) / per);
+        if (c.bm == kFewRows) CKR_LAUNCH("kv_attention_join", s, attend_join_kernel<X, DP, 16><<<jgrid, 256, 0, s>>>(a, Prob<C>::up));
+        else CKR_LAUNCH("kv_attention_join", s, attend_join_kernel<X, DP, 128><<<jgrid, 256, 0, s>>>(a, Prob<C>::up));
+    }
     return hipGetLastError();
+}
+template <typename X, typename C>
+hipError_t launch_attend_dim(const AttnArg& a, const Cut& c, hipStream_t s) {
+    if (c.dp == 64) return launch_attend<X, C, 64>(a, c, s);
+    if (c.dp == 128) return launch_attend<X, C, 128>(a, c, s);
+    return launch_attend<X, C, 256>(a, c, s);
 }
 
 }  // namespace
@@ -141,7 +797,8 @@ extern "C" {
 
 uint64_t ckr_kv_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_seqs,
                                           uint32_t n_tokens, uint32_t max_chunk, uint32_t max_context) {
-    return 0;
+    if (n_kv_heads == 0 || n_heads == 0 || n_heads % n_kv_heads || head_dim == 0 || head_dim > 256) return 0;
+    return most_bytes(n_heads, n_kv_heads, head_dim, n_seqs, n_tokens, max_context);
 }
 
 int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const void* d_q, int64_t q_token_stride,
@@ -171,24 +828,39 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
     a.q_tok = q_token_stride, a.q_head = q_head_stride, a.o_tok = out_token_stride, a.o_head = out_head_stride;
     a.ck = static_cast<const uint8_t*>(cache->d_k), a.cv = static_cast<const uint8_t*>(cache->d_v);
     a.sk = cache->d_k_scale, a.sv = cache->d_v_scale;
-    std::copy(cache->k_stride, cache->k_stride + 3, a.kst);
-    std::copy(cache->v_stride, cache->v_stride + 3, a.vst);
+    const int ces = cache->dtype == CKR_F8 || cache->dtype == CKR_I8 ? 1 : 2;
+    for (int i = 0; i < 3; i++) a.kst[i] = cache->k_stride[i] * ces, a.vst[i] = cache->v_stride[i] * ces;
     std::copy(cache->k_scale_stride, cache->k_scale_stride + 2, a.skst);
     std::copy(cache->v_scale_stride, cache->v_scale_stride + 2, a.svst);
     a.n_pages = cache->n_pages, a.page_shift = (uint32_t)__builtin_ctz(cache->page_size), a.dim = cache->head_dim;
-    a.heads = n_heads, a.group = n_heads / cache->n_heads, a.window = window, a.scale2 = scale * kLog2e;
+    a.heads = n_heads, a.kv_heads = cache->n_heads, a.group = n_heads / cache->n_heads, a.window = window;
+    // a scale of 0 makes every weight equal, as any scale that leaves no bit of a
+    // score above 1 does; 0 itself would turn masked scores (-inf) into NaN
+    a.scale2 = std::max(std::fabs(scale) * kLog2e, 0x1p-120f), a.flip = scale < 0.f ? 0x80008000u : 0u;
     a.b = {batch->d_page_table, batch->d_starts, batch->d_offsets, (int64_t)batch->table_stride, batch->table_width,
            batch->n_seqs, batch->n_tokens};
+    const Cut c = cut(n_heads, cache->n_heads, cache->head_dim, batch->n_seqs, batch->n_tokens, batch->max_chunk,
+                      std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size), window);
+    if ((uint64_t)c.tiles * cache->n_heads * 256 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
+    a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len;
+    if (c.bytes) {
+        if (workspace_bytes < c.bytes)
+            return err(CKR_E_CAPACITY, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(c.bytes) + " needed");
+        if (reinterpret_cast<uintptr_t>(d_workspace) % 256) return err(CKR_E_INVALID, "workspace must be aligned to 256 bytes");
+        if ((rc = check_range(d_workspace, c.bytes, "workspace"))) return rc;
+        a.part_m = static_cast<float*>(d_workspace);
+        a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) + c.part_m_bytes);
+    }
     const hipStream_t s = (hipStream_t)stream;
     hipError_t e;
     if (dtype == CKR_BF16)
-        e = cache->dtype == CKR_F8   ? launch_attend<ElemBF16, ElemF8>(a, s)
-            : cache->dtype == CKR_I8 ? launch_attend<ElemBF16, ElemI8>(a, s)
-                                     : launch_attend<ElemBF16, ElemBF16>(a, s);
+        e = cache->dtype == CKR_F8   ? launch_attend_dim<ElemBF16, ElemF8>(a, c, s)
+            : cache->dtype == CKR_I8 ? launch_attend_dim<ElemBF16, ElemI8>(a, c, s)
+                                     : launch_attend_dim<ElemBF16, ElemBF16>(a, c, s);
     else
-        e = cache->dtype == CKR_F8   ? launch_attend<ElemF16, ElemF8>(a, s)
-            : cache->dtype == CKR_I8 ? launch_attend<ElemF16, ElemI8>(a, s)
-                                     : launch_attend<ElemF16, ElemF16>(a, s);
+        e = cache->dtype == CKR_F8   ? launch_attend_dim<ElemF16, ElemF8>(a, c, s)
+            : cache->dtype == CKR_I8 ? launch_attend_dim<ElemF16, ElemI8>(a, c, s)
+                                     : launch_attend_dim<ElemF16, ElemF16>(a, c, s);
     return e == hipSuccess ? CKR_OK : err(CKR_E_HIP, std::string("HIP error in kv_attention: ") + hipGetErrorString(e));
 }
 
