@@ -8,7 +8,7 @@ device).  Nothing here copies or synchronises.
 """
 import ctypes
 
-from . import CKR_E_INVALID, BF16, F16, F32, I8, CkrError, _check, _stream, _torch, lib
+from . import CKR_E_INVALID, BF16, F16, F32, I8, CkrError, _check, _torch, lib
 
 F8 = 16  # 8-bit floating point (e4m3, largest value 448), a type of these operators only
 
@@ -135,13 +135,29 @@ class KvBatch:
         self._p = ctypes.byref(self._c)
 
 
-def _rows(t, batch, heads, dim, what):
+def _stream_of(stream, tensor):
+    """The stream's handle; None: the current stream of the tensor's GPU.  (A
+    decoding step's calls last a few microseconds each, so neither this nor the
+    checks below build objects that they do not need.)"""
+    if stream is not None:
+        return stream.cuda_stream
+    return _torch()._C._cuda_getCurrentRawStream(tensor.get_device())
+
+
+def _bad(msg):
+    raise CkrError(CKR_E_INVALID, "[ckr] " + msg)
+
+
+def _rows(t, n_tokens, heads, dim, what):
+    """(token stride, head stride) of a [tokens, heads, dim] tensor on a GPU."""
     shape = t.shape
-    if len(shape) != 3 or shape[0] != batch.n_tokens or shape[1] != heads or shape[2] != dim:
-        raise CkrError(CKR_E_INVALID, f"[ckr] {what} must be [{batch.n_tokens}, {heads}, {dim}], not {list(shape)}")
+    if len(shape) != 3 or shape[0] != n_tokens or shape[1] != heads or shape[2] != dim:
+        _bad(f"{what} must be [{n_tokens}, {heads}, {dim}], not {list(shape)}")
     a, b, c = t.stride()
-    _need(c == 1 or dim == 1, f"the last axis of {what} must be contiguous")
-    _on_gpu(t, what)
+    if c != 1:
+        _bad(f"the last axis of {what} must be contiguous")
+    if not t.is_cuda:
+        _bad(f"{what} must be on a GPU")
     return a, b
 
 
@@ -155,25 +171,32 @@ def _used_on(stream, *tensors):
 
 def kv_write(cache, batch, k, v, stream=None):
     """Quantise the batch's keys and values [tokens, heads, head_dim] into the cache."""
-    _need(k.dtype == v.dtype, "k and v must be of one type")
-    kt, kh = _rows(k, batch, cache.n_heads, cache.head_dim, "k")
-    vt, vh = _rows(v, batch, cache.n_heads, cache.head_dim, "v")
-    _check(lib().ckr_kv_write(cache._p, batch._p, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _tag(k.dtype), _stream(stream)))
+    dtype, n, h, d = k.dtype, batch.n_tokens, cache.n_heads, cache.head_dim
+    if v.dtype != dtype:
+        _bad("k and v must be of one type")
+    kt, kh = _rows(k, n, h, d, "k")
+    vt, vh = _rows(v, n, h, d, "v")
+    rc = lib().ckr_kv_write(cache._p, batch._p, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _tag(dtype), _stream_of(stream, k))
+    if rc:
+        _check(rc)
 
 
 def kv_read(cache, batch, dtype=BF16, out=None, stream=None):
     """(k, v) of the batch's tokens as the cache holds them, [tokens, heads,
     head_dim] of dtype (a tag), into out (a pair of tensors) when given."""
+    n, h, d = batch.n_tokens, cache.n_heads, cache.head_dim
     if out is None:
         torch = _torch()
-        shape = (batch.n_tokens, cache.n_heads, cache.head_dim)
-        out = tuple(torch.empty(shape, dtype=_torch_dtype(dtype), device=cache.k.device) for _ in range(2))
+        out = tuple(torch.empty((n, h, d), dtype=_torch_dtype(dtype), device=cache.k.device) for _ in range(2))
         _used_on(stream, *out)
     k, v = out
-    _need(_tag(k.dtype) == dtype and _tag(v.dtype) == dtype, "out must be of the type asked for")
-    kt, kh = _rows(k, batch, cache.n_heads, cache.head_dim, "out[0]")
-    vt, vh = _rows(v, batch, cache.n_heads, cache.head_dim, "out[1]")
-    _check(lib().ckr_kv_read(cache._p, batch._p, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, dtype, _stream(stream)))
+    if _tag(k.dtype) != dtype or _tag(v.dtype) != dtype:
+        _bad("out must be of the type asked for")
+    kt, kh = _rows(k, n, h, d, "out[0]")
+    vt, vh = _rows(v, n, h, d, "out[1]")
+    rc = lib().ckr_kv_read(cache._p, batch._p, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, dtype, _stream_of(stream, k))
+    if rc:
+        _check(rc)
     return k, v
 
 
@@ -188,25 +211,32 @@ class KvAttention:
             self.n_heads, self.n_kv_heads, self.head_dim, n_seqs, n_tokens,
             n_tokens if max_chunk is None else max_chunk, 0xffffffff if max_context is None else max_context))
         self.ws = torch.zeros(max(self.ws_bytes, 1), dtype=torch.uint8, device=device)
+        self._ws_ptr = self.ws.data_ptr()
 
     def run(self, cache, batch, q, scale=None, window=0, out=None, lse=None, stream=None):
         """Attention of the batch's tokens, whose keys and values the cache already
         holds: q [tokens, n_heads, head_dim] -> out (of q's type, new when None).
         scale: head_dim ** -0.5 when None.  lse: a contiguous float32 [tokens,
         n_heads] that receives the logarithm of each row's sum of exponentials."""
-        qt, qh = _rows(q, batch, self.n_heads, cache.head_dim, "q")
+        n, h, d, dtype = batch.n_tokens, self.n_heads, cache.head_dim, q.dtype
+        qt, qh = _rows(q, n, h, d, "q")
         if out is None:
-            out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+            out = _torch().empty(q.shape, dtype=dtype, device=q.device)
             _used_on(stream, out)
-        _need(out.dtype == q.dtype, "out must be of q's type")
-        ot, oh = _rows(out, batch, self.n_heads, cache.head_dim, "out")
+        if out.dtype != dtype:
+            _bad("out must be of q's type")
+        ot, oh = _rows(out, n, h, d, "out")
+        if window < 0:
+            _bad("window must not be negative")
+        lse_ptr = None
         if lse is not None:
-            _need(tuple(lse.shape) == (batch.n_tokens, self.n_heads) and lse.dtype == _torch().float32 and lse.is_contiguous()
-                  and lse.is_cuda, "lse must be a contiguous float32 [tokens, n_heads] on the GPU")
-        _check(lib().ckr_kv_attention(
-            cache._p, batch._p, q.data_ptr(), qt, qh, _tag(q.dtype), self.n_heads,
-            cache.head_dim ** -0.5 if scale is None else scale, int(window), out.data_ptr(), ot, oh,
-            None if lse is None else lse.data_ptr(), self.ws.data_ptr(), self.ws_bytes, _stream(stream)))
+            if lse.shape != q.shape[:2] or lse.dtype != _torch().float32 or not lse.is_contiguous() or not lse.is_cuda:
+                _bad("lse must be a contiguous float32 [tokens, n_heads] on the GPU")
+            lse_ptr = lse.data_ptr()
+        rc = lib().ckr_kv_attention(cache._p, batch._p, q.data_ptr(), qt, qh, _tag(dtype), h, d ** -0.5 if scale is None else scale,
+                                    window, out.data_ptr(), ot, oh, lse_ptr, self._ws_ptr, self.ws_bytes, _stream_of(stream, q))
+        if rc:
+            _check(rc)
         return out
 
 
@@ -216,39 +246,54 @@ def add_rms_norm(x, residual, weight, eps=1e-5, dtype=None, group=0, out=None, s
     type when None, F8 or I8 with float32 scales per row, or per group of the
     row), scales None for 16 and 32 bits, h rounded to x's type.  out, scales and
     total (may be x or residual) are written in place when given."""
-    torch = _torch()
-    _need(x.dim() == 2, "x must be [rows, n]")
-    rows, n = x.shape
-    xt = _tag(x.dtype)
+    shape, x_dtype = x.shape, x.dtype
+    if len(shape) != 2:
+        _bad("x must be [rows, n]")
+    rows, n = shape
+    xt = _tag(x_dtype)
     tag = xt if dtype is None else dtype
-    coded = tag in (F8, I8)
+    coded = tag == F8 or tag == I8
     if out is None:
-        out = torch.empty((rows, n), dtype=_torch_dtype(tag), device=x.device)
+        out = _torch().empty((rows, n), dtype=_torch_dtype(tag), device=x.device)
         _used_on(stream, out)
     if total is None:
-        total = torch.empty((rows, n), dtype=x.dtype, device=x.device)
+        total = _torch().empty((rows, n), dtype=x_dtype, device=x.device)
         _used_on(stream, total)
+    scales_ptr = None
     if coded:
-        _need(group >= 0 and (group == 0 or n % group == 0), "group must divide the row length")
-        shape = (rows, n // group) if group else (rows,)
+        if group < 0 or group and n % group:
+            _bad("group must divide the row length")
+        want = (rows, n // group) if group else (rows,)
         if scales is None:
-            scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+            scales = _torch().empty(want, dtype=_torch().float32, device=x.device)
             _used_on(stream, scales)
-        _need(tuple(scales.shape) == shape and scales.dtype == torch.float32 and scales.is_contiguous() and scales.is_cuda,
-              f"scales must be contiguous float32 {list(shape)} on the GPU")
-    else:
-        _need(scales is None, "scales belong to 8-bit outputs")
-    for t, what in ((x, "x"), (residual, "residual"), (out, "out"), (total, "total")):
-        if t is not None:
-            _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == n and (t.stride(1) == 1 or n == 1) and t.is_cuda,
-                  f"{what} must be [{rows}, {n}] on the GPU, its last axis contiguous")
-    _need(_tag(out.dtype) == tag and total.dtype == x.dtype and (residual is None or residual.dtype == x.dtype),
-          "residual and total must be of x's type, out of the type asked for")
-    _need(weight.dim() == 1 and weight.shape[0] == n and (weight.stride(0) == 1 or n == 1) and weight.is_cuda,
-          f"weight must be [{n}] on the GPU")
-    _check(lib().ckr_add_rms_norm(
-        x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(),
-        0 if residual is None else residual.stride(0), weight.data_ptr(), _tag(weight.dtype), rows, n, xt, eps, tag, group,
-        out.data_ptr(), out.stride(0), scales.data_ptr() if coded else None, total.data_ptr(), total.stride(0),
-        _stream(stream)))
+        if scales.shape != want or scales.dtype != _torch().float32 or not scales.is_contiguous() or not scales.is_cuda:
+            _bad(f"scales must be contiguous float32 {list(want)} on the GPU")
+        scales_ptr = scales.data_ptr()
+    elif scales is not None:
+        _bad("scales belong to 8-bit outputs")
+    r_ptr, rs = None, 0
+    if residual is not None:
+        if residual.dtype != x_dtype:
+            _bad("residual must be of x's type")
+        r_ptr, rs = residual.data_ptr(), _row_stride(residual, shape, "residual")
+    if total.dtype != x_dtype or _tag(out.dtype) != tag:
+        _bad("total must be of x's type, out of the type asked for")
+    if weight.shape != shape[1:] or not weight.is_cuda or n > 1 and weight.stride(0) != 1:
+        _bad(f"weight must be contiguous [{n}] on the GPU")
+    rc = lib().ckr_add_rms_norm(
+        x.data_ptr(), _row_stride(x, shape, "x"), r_ptr, rs, weight.data_ptr(), _tag(weight.dtype), rows, n, xt, eps, tag, group,
+        out.data_ptr(), _row_stride(out, shape, "out"), scales_ptr, total.data_ptr(), _row_stride(total, shape, "total"),
+        _stream_of(stream, x))
+    if rc:
+        _check(rc)
     return out, scales, total
+
+
+def _row_stride(t, shape, what):
+    if t.shape != shape or not t.is_cuda:
+        _bad(f"{what} must be {list(shape)} on the GPU")
+    a, b = t.stride()
+    if b != 1 and shape[1] > 1:
+        _bad(f"the last axis of {what} must be contiguous, {what} {list(shape)}")
+    return a

@@ -360,6 +360,7 @@ def test_refusals(gpu):
     bad("GPU", ck.kv_write, cache, b, kv.cpu(), kv.cpu())
     bad("lse", plan.run, cache, b, q, lse=torch.zeros(2, 4, dtype=torch.float16, device=gpu))
     bad("scale", plan.run, cache, b, q, scale=float("nan"))
+    bad("window", plan.run, cache, b, q, window=-1)
     bad("multiple", ck.KvAttention(3, 2, 64, 1, 2).run, cache, b, torch.zeros(2, 3, 64, dtype=torch.bfloat16, device=gpu))
     wide = _cache(sq, 2, 64, "f16", gpu)
     bad("queries' type", plan.run, wide, b, q)
