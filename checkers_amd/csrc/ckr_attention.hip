@@ -454,17 +454,21 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     Tile t;
     if (!find_tile<128>(a.b, a.group, tile, s_tmp, t)) return;
     const uint32_t row = t.row0 + wave * 32 + col;
-    const int64_t pos = t.start + min(row, t.rows - 1) / a.group;
     const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + 127, t.rows - 1) / a.group;
-    // the wave's own range of positions
-    const int64_t wave_lo = t.start + min(t.row0 + wave * 32, t.rows - 1) / a.group;
-    const int64_t wave_hi = t.start + min(t.row0 + wave * 32 + 31, t.rows - 1) / a.group;
     const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
     const int64_t first = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) & ~(int64_t)(TK - 1) : 0;
-    const int64_t see = a.window ? pos - (int64_t)a.window : -1;
     const int64_t lo = first + (int64_t)split * a.split_len;
     const int64_t hi = split + 1 == a.splits ? limit : min(limit, lo + (int64_t)a.split_len);
     const int n_tiles = hi > lo ? (int)((hi - lo + TK - 1) / TK) : 0;
+    // from here on keys are counted from lo, in 32 bits
+    const auto rel = [&](int64_t p) { return (int)max((int64_t)-0x40000000, min(p - lo, (int64_t)0x7fffffff - 2 * TK)); };
+    const uint32_t wave_row = __builtin_amdgcn_readfirstlane(t.row0 + wave * 32);
+    const int end = rel(limit), pos = rel(t.start + min(row, t.rows - 1) / a.group);
+    const int wave_lo = rel(t.start + min(wave_row, t.rows - 1) / a.group), wave_hi = rel(t.start + min(wave_row + 31, t.rows - 1) / a.group);
+    // a row sees the keys above `see`; the wave's first and last row's bounds
+    const int see = a.window ? rel(t.start + min(row, t.rows - 1) / a.group - (int64_t)a.window) : -0x40000000;
+    const int see_lo = a.window ? rel(t.start + min(wave_row, t.rows - 1) / a.group - (int64_t)a.window) : -0x40000000;
+    const int see_hi = a.window ? rel(t.start + min(wave_row + 31, t.rows - 1) / a.group - (int64_t)a.window) : -0x40000000;
 
     u32x4 q[KS];
 #pragma unroll
@@ -482,24 +486,26 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     const uint32_t r0 = threadIdx.x / LPR, piece = threadIdx.x % LPR;
     const bool d_in = piece * 16 / C::bytes < a.dim;
     const uint32_t slot_mask = (1u << a.page_shift) - 1;
-    const auto page_id = [&](int64_t j) {
-        const int64_t c = j >> a.page_shift;
-        const int32_t p = j < limit && c < (int64_t)a.b.width ? table[c] : -1;
+    const int64_t c0 = lo >> a.page_shift;               // table column of lo, and lo's place in its page
+    const uint32_t in0 = (uint32_t)lo & slot_mask;
+    const auto page_id = [&](int j) {
+        const int64_t c = c0 + ((in0 + (uint32_t)j) >> a.page_shift);
+        const int32_t p = j < end && c < (int64_t)a.b.width ? table[c] : -1;
         return (uint32_t)p < a.n_pages ? p : -1;
     };
-    int32_t pg[LOADS], pg_s = -1;  // pages of the rows of the tile that is loaded next; of key threadIdx % TK for its scale
-    const auto load_pages = [&](int64_t base) {
+    int32_t pg[LOADS], pg_s = -1;  // pages of the rows of the tile that is loaded next; of key threadIdx for its scales
+    const auto load_pages = [&](int base) {
 #pragma unroll
-        for (int u = 0; u < LOADS; u++) pg[u] = page_id(base + r0 + u * ROWS);
-        if (threadIdx.x < 2 * TK) pg_s = page_id(base + threadIdx.x % TK);
+        for (int u = 0; u < LOADS; u++) pg[u] = page_id(base + (int)r0 + u * ROWS);
+        if (threadIdx.x < TK) pg_s = page_id(base + (int)threadIdx.x);
     };
     u32x4 kr[LOADS], vr[LOADS];
-    float sr = 0.f;
+    float sk = 0.f, sv = 0.f;
     bool in_s = false;
-    const auto load_tile = [&](int64_t base) {
+    const auto load_tile = [&](int base) {
 #pragma unroll
         for (int u = 0; u < LOADS; u++) {
-            const int64_t slot = (uint32_t)(base + r0 + u * ROWS) & slot_mask;
+            const int64_t slot = (in0 + (uint32_t)base + r0 + u * ROWS) & slot_mask;
             kr[u] = vr[u] = u32x4{0, 0, 0, 0};
             if (pg[u] >= 0 && d_in) {
                 kr[u] = *reinterpret_cast<const u32x4*>(a.ck + (int64_t)pg[u] * a.kst[0] + (int64_t)kvh * a.kst[1] + slot * a.kst[2] + piece * 16);
@@ -507,13 +513,10 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
             }
         }
         in_s = pg_s >= 0;
-        if (threadIdx.x < 2 * TK) {
-            sr = 0.f;
-            if (C::bytes == 1 && in_s) {
-                const int64_t slot = (uint32_t)(base + threadIdx.x % TK) & slot_mask;
-                sr = threadIdx.x < TK ? a.sk[(int64_t)pg_s * a.skst[0] + (int64_t)kvh * a.skst[1] + slot] * a.scale2
-                                      : a.sv[(int64_t)pg_s * a.svst[0] + (int64_t)kvh * a.svst[1] + slot];
-            }
+        if (C::bytes == 1 && in_s) {
+            const int64_t slot = (in0 + (uint32_t)base + threadIdx.x) & slot_mask;
+            sk = a.sk[(int64_t)pg_s * a.skst[0] + (int64_t)kvh * a.skst[1] + slot];
+            sv = a.sv[(int64_t)pg_s * a.svst[0] + (int64_t)kvh * a.svst[1] + slot];
         }
     };
     const auto store_tile = [&](int buf) {
@@ -534,9 +537,12 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                 }
             }
         }
-        if constexpr (C::bytes == 1) {
-            if (threadIdx.x < TK) s_sk[buf][threadIdx.x] = sr;
-            else if (threadIdx.x < 2 * TK) s_sv[buf][threadIdx.x - TK] = sr;
+        if (C::bytes == 1 && threadIdx.x < TK) {
+            // a value scale that is not finite shows in the score instead, so that a
+            // weight of 0 (a key that a row does not see) always gives 0
+            const bool fine = abs_bits(sv) < 0x7f800000u;
+            s_sk[buf][threadIdx.x] = !in_s ? 0.f : fine ? sk * a.scale2 : as_f32(0x7fc00000u);
+            s_sv[buf][threadIdx.x] = in_s && fine ? sv : 0.f;
         }
         if (threadIdx.x < 64) {
             const uint64_t ok = __ballot(in_s && lane < TK);
@@ -553,9 +559,8 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     // where this lane reads V: 4 keys x 16 dimensions per group of 16 lanes
     const uint32_t v_lane = (4 * half + (lane & 15) / 4) * PITCH + (16 * ((lane >> 4) & 1) + (lane & 3) * 4) * 2;
 
-    const auto compute = [&](int buf, int64_t base) {
-        if (base > wave_hi) return;                                             // every key is after every row
-        if (a.window && base + TK - 1 <= wave_lo - (int64_t)a.window) return;   // every key has left every window
+    // full: every row of the wave sees every key of the tile
+    const auto compute = [&](bool full, int buf, int base, uint64_t valid) {
         f32x16 s[TT];
 #pragma unroll
         for (int tt = 0; tt < TT; tt++) {
@@ -567,35 +572,30 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                 s[tt] = mfma32<X>(k, q[ks], s[tt]);
             }
         }
-        const uint64_t valid = s_valid[buf];
-        const bool full = valid == (TK == 64 ? ~0ull : (1ull << TK % 64) - 1) && base + TK - 1 <= wave_lo &&
-                          (!a.window || base > wave_hi - (int64_t)a.window);
         float top = -INFINITY;
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 if constexpr (C::bytes == 1) {
-                    const f32x4 sk = *reinterpret_cast<const f32x4*>(&s_sk[buf][tt * 32 + 2 * i + 4 * half]);
+                    const f32x4 f = *reinterpret_cast<const f32x4*>(&s_sk[buf][tt * 32 + 2 * i + 4 * half]);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) s[tt][i + k] *= sk[k];
+                    for (int k = 0; k < 4; k++) s[tt][i + k] *= f[k];
                 } else {
 #pragma unroll
                     for (int k = 0; k < 4; k++) s[tt][i + k] *= a.scale2;
                 }
             }
-        uint32_t seen[TT];
         if (!full) {
+            valid >>= 4 * half;
+            const int k0 = base + 4 * half;
 #pragma unroll
-            for (int tt = 0; tt < TT; tt++) {
-                seen[tt] = 0;
+            for (int tt = 0; tt < TT; tt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int key = tt * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                    if ((valid >> key & 1) && base + key <= pos && base + key > see) seen[tt] |= 1u << i;
-                    s[tt][i] = seen[tt] >> i & 1 ? s[tt][i] : -INFINITY;
+                    const int key = tt * 32 + 8 * (i / 4) + i % 4;
+                    s[tt][i] = (valid >> key & 1) && k0 + key <= pos && k0 + key > see ? s[tt][i] : -INFINITY;
                 }
-            }
         }
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
@@ -625,13 +625,9 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                         l += p[i + k];
                     }
                     if constexpr (C::bytes == 1) {
-                        const f32x4 sv = *reinterpret_cast<const f32x4*>(&s_sv[buf][tt * 32 + 16 * kb + 2 * i + 4 * half]);
+                        const f32x4 f = *reinterpret_cast<const f32x4*>(&s_sv[buf][tt * 32 + 16 * kb + 2 * i + 4 * half]);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) p[i + k] *= sv[k];
-                    }
-                    if (!full) {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) p[i + k] = seen[tt] >> (8 * kb + i + k) & 1 ? p[i + k] : 0.f;
+                        for (int k = 0; k < 4; k++) p[i + k] *= f[k];
                     }
                 }
                 const u32x4 pf = {pack16<P>(p[0], p[1]), pack16<P>(p[2], p[3]), pack16<P>(p[4], p[5]), pack16<P>(p[6], p[7])};
@@ -649,18 +645,22 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     };
 
     if (n_tiles > 0) {
-        load_pages(lo);
-        load_tile(lo);
-        load_pages(lo + TK);
+        load_pages(0);
+        load_tile(0);
+        load_pages(TK);
         store_tile(0);
         __syncthreads();
         for (int i = 0; i < n_tiles; i++) {
-            const int64_t base = lo + (int64_t)i * TK;
+            const int base = i * TK;
             if (i + 1 < n_tiles) {
                 load_tile(base + TK);
                 load_pages(base + 2 * TK);
             }
-            compute(i & 1, base);
+            if (base <= wave_hi && base + TK - 1 > see_lo) {  // some row sees some key
+                const uint64_t valid = s_valid[i & 1];
+                const bool full = valid == (TK == 64 ? ~0ull : (1ull << TK % 64) - 1) && base + TK - 1 <= wave_lo && base > see_hi;
+                compute(__builtin_amdgcn_readfirstlane(full), i & 1, base, valid);
+            }
             if (i + 1 < n_tiles) store_tile((i + 1) & 1);
             __syncthreads();
         }
