@@ -68,6 +68,12 @@ def _run(cmd, verbose):
         raise subprocess.CalledProcessError(r.returncode, cmd)
 
 
+# ckr_attention.hip: matrix products whose result the vector units read next leave
+# it in vector registers (by default a kernel of more than 256 registers keeps all
+# results in accumulation registers and copies them: 1.47 against 1.20 ms)
+SOURCE_FLAGS = {"ckr_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
+
 def _stale(src, obj):
     """An object older than its source or a shared header."""
     if not os.path.exists(obj):
@@ -82,7 +88,7 @@ def build(verbose=True, incremental=False):
     """Compile every source (incremental: only those whose object is stale) and link."""
     os.makedirs(OBJ, exist_ok=True)
     objs = [os.path.join(OBJ, os.path.splitext(s)[0] + ".o") for s in SOURCES]
-    cmds = [[HIPCC] + FLAGS + ["-x", "hip", "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objs)
+    cmds = [[HIPCC] + FLAGS + SOURCE_FLAGS.get(s, []) + ["-x", "hip", "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objs)
             if not incremental or _stale(os.path.join(CSRC, s), o)]
     with ThreadPoolExecutor(max(len(cmds), 1)) as ex:
         for f in [ex.submit(_run, c, verbose) for c in cmds]:

@@ -3,6 +3,8 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
+#include <utility>
 
 #include "ckr_internal.h"
 #include "ckr_kv.h"
@@ -101,6 +103,12 @@ template <> struct Prob<ElemF16> { typedef ElemF16 E; static constexpr float up 
 // How far a row's running maximum may lag behind (in powers of two) before the
 // accumulators are scaled: sums and outputs use the same lagging maximum.
 constexpr float kLag = 8.f;
+
+// f(0) .. f(N - 1) with constants.
+template <typename F, int... I> __device__ __forceinline__ void unroll_list(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F> __device__ __forceinline__ void unroll(F f) { unroll_list(f, std::make_integer_sequence<int, N>{}); }
 
 // Which sequence and rows a tile of BM rows is: rows of a sequence are its
 // chunk's tokens times the query heads of a key/value head, in that order.
@@ -431,7 +439,10 @@ __global__ void __launch_bounds__(256, (DP * C::bytes > 256 ? 1 : 2)) attend_few
 //   V's is read transposed from LDS, four keys of one dimension at a time.
 template <typename C, int DP> struct ManyShape {
     static constexpr int TK = DP > 128 ? 32 : 64;
-    static constexpr int PITCH = DP * 2 + 32;  // bytes of a row in LDS: rows 8 banks apart (mod 64)
+    // bytes of a row in LDS: 16-byte reads of 32 rows run at 206 bytes a cycle with
+    // rows 16 bytes past a multiple of 256 (126 with 32, 16 with none), transposed
+    // reads of 4 rows at 121 with rows 64 past it (114 with 32, 60 with 16)
+    static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 64;
     static constexpr int LPR = DP * C::bytes / 16, LOADS = TK * LPR / 256;  // lanes of a row, 16-byte loads a thread
     static constexpr int ROWS = 256 / LPR;                                  // rows a load of the block covers
 };
@@ -440,11 +451,11 @@ template <typename X, typename C, int DP>
 __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(AttnArg a) {
     typedef typename Prob<C>::E P;
     typedef ManyShape<C, DP> Sh;
-    constexpr int TK = Sh::TK, PITCH = Sh::PITCH, LPR = Sh::LPR, LOADS = Sh::LOADS, ROWS = Sh::ROWS;
+    constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, ROWS = Sh::ROWS;
     constexpr int KS = DP / 16, DT = DP / 32, TT = TK / 32;
     static_assert(LOADS >= 1 && TK * LPR % 256 == 0, "a tile is whole loads of the block");
-    __shared__ __attribute__((aligned(16))) uint8_t s_k[2][TK * PITCH];
-    __shared__ __attribute__((aligned(16))) uint8_t s_v[2][TK * PITCH];
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[2][TK * KP];
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[2][TK * VP];
     __shared__ __attribute__((aligned(16))) float s_sk[2][TK];
     __shared__ __attribute__((aligned(16))) float s_sv[2][TK];
     __shared__ uint64_t s_valid[2];
@@ -522,8 +533,8 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     const auto store_tile = [&](int buf) {
 #pragma unroll
         for (int u = 0; u < LOADS; u++) {
-            uint8_t* k = s_k[buf] + (r0 + u * ROWS) * PITCH;
-            uint8_t* v = s_v[buf] + (r0 + u * ROWS) * PITCH;
+            uint8_t* k = s_k[buf] + (r0 + u * ROWS) * KP;
+            uint8_t* v = s_v[buf] + (r0 + u * ROWS) * VP;
             if constexpr (C::bytes == 2) {
                 *reinterpret_cast<u32x4*>(k + piece * 16) = kr[u];
                 *reinterpret_cast<u32x4*>(v + piece * 16) = vr[u];
@@ -557,7 +568,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 #pragma unroll
         for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
     // where this lane reads V: 4 keys x 16 dimensions per group of 16 lanes
-    const uint32_t v_lane = (4 * half + (lane & 15) / 4) * PITCH + (16 * ((lane >> 4) & 1) + (lane & 3) * 4) * 2;
+    const uint32_t v_lane = (4 * half + (lane & 15) / 4) * VP + (16 * ((lane >> 4) & 1) + (lane & 3) * 4) * 2;
 
     // full: every row of the wave sees every key of the tile
     const auto compute = [&](bool full, int buf, int base, uint64_t valid) {
@@ -568,7 +579,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
             for (int i = 0; i < 16; i++) s[tt][i] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                const u32x4 k = *reinterpret_cast<const u32x4*>(s_k[buf] + (tt * 32 + col) * PITCH + ks * 32 + half * 16);
+                const u32x4 k = *reinterpret_cast<const u32x4*>(s_k[buf] + (tt * 32 + col) * KP + ks * 32 + half * 16);
                 s[tt] = mfma32<X>(k, q[ks], s[tt]);
             }
         }
@@ -635,9 +646,9 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                 for (int dt = 0; dt < DT; dt++) {
                     typedef short s16x4 __attribute__((ext_vector_type(4)));
                     typedef __attribute__((address_space(3))) s16x4* lds4;
-                    const uint8_t* at = s_v[buf] + (tt * 32 + kb * 16) * PITCH + v_lane + dt * 64;
+                    const uint8_t* at = s_v[buf] + (tt * 32 + kb * 16) * VP + v_lane + dt * 64;
                     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at));
-                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * PITCH));
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * VP));
                     const u32x2 xa = __builtin_bit_cast(u32x2, x), ya = __builtin_bit_cast(u32x2, y);
                     o[dt] = mfma32<P>(u32x4{xa[0], xa[1], ya[0], ya[1]}, pf, o[dt]);
                 }
@@ -692,6 +703,384 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<C>::up + log2f(l)) * kLn2;
 }
 
+// ------------------------------------------------------------ very many rows
+// A block takes 256 rows, a wave 64 of them as two halves of 32, one wave a SIMD
+// with all of its registers.  The halves take turns: while the matrix cores work
+// for one half, the vector units run the other's softmax, in one stream of
+// instructions.  With S(i) the scores of the i-th 32 keys, in turn
+//   A(i): O1 += V(i-1) P1(i-1), S0(i+1) = K(i+1) Q0   beside  softmax of S0(i) -> P0(i)
+//   B(i): S1(i+1) = K(i+1) Q1,  O0 += V(i) P0(i)      beside  softmax of S1(i) -> P1(i)
+// so K(i+1) and V(i) are read from LDS once for both halves (half of what a wave of
+// 32 rows reads), each a turn before its second use.  Tiles of 64 keys go through
+// a ring of three in LDS.
+template <typename C, int DP> struct WideShape {
+    static constexpr int TK = 64, BM = 256;
+    static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 64;  // as ManyShape's
+    static constexpr int LPR = DP * C::bytes / 16, LOADS = TK * LPR / 256, ROWS = 256 / LPR;
+};
+
+template <typename X, typename C, int DP>
+__global__ void __launch_bounds__(256, 1) attend_wide_kernel(AttnArg a) {
+    typedef typename Prob<C>::E P;
+    typedef WideShape<C, DP> Sh;
+    constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, ROWS = Sh::ROWS;
+    constexpr int KS = DP / 16, DT = DP / 32;
+    constexpr float kMost = Prob<C>::up == 0.f ? 256.f : 32768.f;  // 2^(kLag + up)
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[3 * TK * KP];
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[3 * TK * VP];
+    __shared__ __attribute__((aligned(16))) float s_sk[4][TK];  // [3]: ones, for scores that carry their scale
+    __shared__ __attribute__((aligned(16))) float s_sv[3][TK];
+    __shared__ uint64_t s_valid[3];
+    __shared__ uint32_t s_tmp[8];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
+    Tile t;
+    if (!find_tile<Sh::BM>(a.b, a.group, tile, s_tmp, t)) return;
+    const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + Sh::BM - 1, t.rows - 1) / a.group;
+    const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
+    const int64_t first = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) & ~(int64_t)(TK - 1) : 0;
+    const int64_t lo = first + (int64_t)split * a.split_len;
+    const int64_t hi = split + 1 == a.splits ? limit : min(limit, lo + (int64_t)a.split_len);
+    const int n_tiles = hi > lo ? (int)((hi - lo + TK - 1) / TK) : 0;
+    const auto rel = [&](int64_t p) { return (int)max((int64_t)-0x40000000, min(p - lo, (int64_t)0x7fffffff - 8 * TK)); };
+    const uint32_t wave_row = __builtin_amdgcn_readfirstlane(t.row0 + wave * 64);
+    const int end = rel(limit);
+    const int wave_lo = rel(t.start + min(wave_row, t.rows - 1) / a.group);
+    const int see_hi = a.window ? rel(t.start + min(wave_row + 63, t.rows - 1) / a.group - (int64_t)a.window) : -0x40000000;
+    int pos[2], see[2];
+    u32x4 q[2][KS];
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+        const uint32_t row = wave_row + n * 32 + col;
+        const int64_t p = t.start + min(row, t.rows - 1) / a.group;
+        pos[n] = rel(p), see[n] = a.window ? rel(p - (int64_t)a.window) : -0x40000000;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const uint32_t d = ks * 16 + half * 8;
+            q[n][ks] = u32x4{0, 0, 0, 0};
+            if (row < t.rows && d < a.dim) {
+                q[n][ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(t.token0 + row / a.group) * a.q_tok +
+                                                                 (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
+                q[n][ks] ^= a.flip;
+            }
+            // the queries stay in accumulation registers, which the products read as well
+            asm volatile("" : "+a"(q[n][ks]));
+        }
+    }
+    // staging, without branches: a key of no mapped page is read from page 0 (its
+    // values are cleared, its scores masked), pieces past the head's size are the
+    // last piece again (they meet queries of zero, and dimensions that are not stored)
+    typedef __attribute__((address_space(1))) const int32_t* global_i32;
+    const global_i32 table = (global_i32)(a.b.table + (int64_t)t.seq * a.b.table_stride);
+    const uint32_t r0 = threadIdx.x / LPR, piece = min(threadIdx.x % LPR, a.dim * C::bytes / 16 - 1), place = threadIdx.x % LPR;
+    const uint32_t slot_mask = (1u << a.page_shift) - 1;
+    const int64_t c0 = lo >> a.page_shift;
+    const uint32_t in0 = (uint32_t)lo & slot_mask, last_col = a.b.width - 1;
+    const u32x4* kp = reinterpret_cast<const u32x4*>(a.ck + (int64_t)kvh * a.kst[1]) + piece;
+    const u32x4* vp = reinterpret_cast<const u32x4*>(a.cv + (int64_t)kvh * a.vst[1]) + piece;
+    const uint32_t ks0 = (uint32_t)(a.kst[0] >> 4), ks2 = (uint32_t)(a.kst[2] >> 4), vs0 = (uint32_t)(a.vst[0] >> 4), vs2 = (uint32_t)(a.vst[2] >> 4);
+    const float* skp = a.sk + (int64_t)kvh * a.skst[1];
+    const float* svp = a.sv + (int64_t)kvh * a.svst[1];
+    const auto page_id = [&](int j) {
+        const uint32_t c = (uint32_t)min((uint64_t)c0 + ((in0 + (uint32_t)j) >> a.page_shift), (uint64_t)last_col);
+        const int32_t p = table[c];
+        return ((j < end) & ((uint32_t)p < a.n_pages)) ? p : -1;  // end lies within the table
+    };
+    int32_t pg[LOADS], pg_s;
+    const auto load_pages = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) pg[u] = page_id(base + (int)r0 + u * ROWS);
+        pg_s = page_id(base + (int)lane);
+    };
+    u32x4 kr[LOADS], vr[LOADS];
+    float sk = 0.f, sv = 0.f;
+    bool in_s = false, in_v[LOADS];
+    const auto load_rows = [&](int u, int base) {
+        const uint32_t slot = (in0 + (uint32_t)base + r0 + u * ROWS) & slot_mask, page = (uint32_t)max(pg[u], 0);
+        in_v[u] = pg[u] >= 0;
+        kr[u] = kp[(uint64_t)page * ks0 + (uint64_t)slot * ks2];
+        vr[u] = vp[(uint64_t)page * vs0 + (uint64_t)slot * vs2];
+    };
+    const auto load_scales = [&](int base) {
+        in_s = pg_s >= 0;
+        if constexpr (C::bytes == 1) {
+            const uint32_t slot = (in0 + (uint32_t)base + lane) & slot_mask;
+            sk = skp[(int64_t)max(pg_s, 0) * a.skst[0] + slot];
+            sv = svp[(int64_t)max(pg_s, 0) * a.svst[0] + slot];
+        }
+    };
+    const auto store_k = [&](int u, int slot) {
+        uint8_t* k = s_k + slot * (TK * KP) + (r0 + u * ROWS) * KP;
+        if constexpr (C::bytes == 2) {
+            *reinterpret_cast<u32x4*>(k + place * 16) = kr[u];
+        } else {
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const u32x2 x = widen4<C, X>(kr[u][2 * w]), y = widen4<C, X>(kr[u][2 * w + 1]);
+                *reinterpret_cast<u32x4*>(k + place * 32 + w * 16) = u32x4{x[0], x[1], y[0], y[1]};
+            }
+        }
+    };
+    const auto store_v = [&](int u, int slot) {
+        uint8_t* v = s_v + slot * (TK * VP) + (r0 + u * ROWS) * VP;
+        const u32x4 vx = in_v[u] ? vr[u] : u32x4{0, 0, 0, 0};
+        if constexpr (C::bytes == 2) {
+            *reinterpret_cast<u32x4*>(v + place * 16) = vx;
+        } else {
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const u32x2 x = widen4<C, P>(vx[2 * w]), y = widen4<C, P>(vx[2 * w + 1]);
+                *reinterpret_cast<u32x4*>(v + place * 32 + w * 16) = u32x4{x[0], x[1], y[0], y[1]};
+            }
+        }
+    };
+    const auto store_scales = [&](int slot) {  // every wave writes the same values
+        if constexpr (C::bytes == 1) {
+            const bool fine = abs_bits(sv) < 0x7f800000u;
+            s_sk[slot][lane] = fine ? sk * a.scale2 : as_f32(0x7fc00000u);
+            s_sv[slot][lane] = in_s && fine ? sv : 0.f;
+        }
+        s_valid[slot] = __ballot(in_s);
+    };
+    const auto load_tile = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) load_rows(u, base);
+        load_scales(base);
+    };
+    const auto store_tile = [&](int slot) {
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) store_k(u, slot), store_v(u, slot);
+        store_scales(slot);
+    };
+
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    f32x16 o[2][DT], s[2];
+    u32x4 pf[2][2], kf[KS], vf[2][DT];
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[n][dt][i] = 0.f;
+            vf[n][dt] = u32x4{0, 0, 0, 0};
+        }
+    pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
+    const uint32_t k_lane = col * KP + half * 16;
+    const uint32_t v_lane = (4 * half + (lane & 15) / 4) * VP + (16 * ((lane >> 4) & 1) + (lane & 3) * 4) * 2;
+    // scores that some row of the wave must not see: scaled here, -inf where hidden
+    const auto mask = [&](int n, int slot, int sub, int base, uint32_t valid) {
+        valid >>= 4 * half;
+        const int k0 = base + 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int key = 8 * (i / 4) + i % 4;
+            const float f = C::bytes == 1 ? s_sk[slot][sub * 32 + key + 4 * half] : a.scale2;
+            s[n][i] = (valid >> key & 1) && k0 + key <= pos[n] && k0 + key > see[n] ? s[n][i] * f : -INFINITY;
+        }
+    };
+    f32x4 fk[4], fv[4];  // the keys' scales, of keys 8 j + 4 half on
+    const auto read_scales = [&](const float* at_fk, const float* at_fv, int j) {
+        if constexpr (C::bytes == 1) {
+            fk[j] = *reinterpret_cast<const f32x4*>(at_fk + 8 * j + 4 * half);
+            fv[j] = *reinterpret_cast<const f32x4*>(at_fv + 8 * j + 4 * half);
+        }
+    };
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* lds4;
+    // the weight of score k, with its share of the sum
+    const auto weight = [&](int n, int k, float f, float ref) {
+        const float p = exp2_fast(__builtin_fmaf(s[n][k], C::bytes == 1 ? fk[k / 4][k % 4] : f, -ref));
+        return p;
+    };
+    float ref[2] = {0.f, 0.f};
+    // One turn: 16 steps, each at most one matrix product and its share of the rest,
+    // kept in this order.  TURN 0 is A, 1 is B; half n = TURN takes its softmax, the
+    // scores of half n for the next keys are made, and half 1 - n (the one whose weights
+    // the last turn made) gathers its values.  The weights are taken against the
+    // maximum so far; only where one comes out above 2^kLag, or a row has no maximum
+    // yet, is the new maximum looked for and the turn's weights made again.
+    const auto turn = [&](auto turn_tag, float f, const uint8_t* at_k, const uint8_t* at_v, const float* at_fk,
+                          const float* at_fv, auto side) {
+        constexpr int n = decltype(turn_tag)::value, NM = KS + 2 * DT;
+        f32x16 z;
+#pragma unroll
+        for (int i = 0; i < 16; i++) z[i] = 0.f;
+        float sum = 0.f, top = 0.f, p_even = 0.f, p_last = 0.f;
+        const auto use = [&](auto k_tag) {
+            constexpr int k = decltype(k_tag)::value;
+            sum += p_last;
+            if constexpr (k % 2 == 0) {
+                p_even = p_last;
+            } else {
+                top = fmaxf(fmaxf(top, p_even), p_last);
+                uint32_t w = C::bytes == 1 ? pack16<P>(p_even * fv[k / 4][k % 4 - 1], p_last * fv[k / 4][k % 4]) : pack16<P>(p_even, p_last);
+                asm volatile("" : "+v"(w));
+                pf[n][k / 8][k % 8 / 2] = w;
+            }
+        };
+        unroll<16>([&](auto step_tag) {
+            constexpr int S = decltype(step_tag)::value;
+            if constexpr (S % (16 / NM) == 0) {
+                constexpr int j = S * NM / 16, first = n == 0 ? 2 * DT : KS;
+                constexpr bool scores = (j >= first) == (n == 0);
+                constexpr int e = j >= first ? j - first : j;
+                if constexpr (scores) z = mfma32<X>(kf[e], q[n][e], z);
+                else o[1 - n][e % DT] = mfma32<P>(vf[e / DT][e % DT], pf[1 - n][e / DT], o[1 - n][e % DT]);
+            }
+            // reads of LDS: keys in A and values in B for the turn's second half; scales
+            if constexpr (n == 0 && S < 4) {
+#pragma unroll
+                for (int ks = S * KS / 4; ks < (S + 1) * KS / 4; ks++) kf[ks] = *reinterpret_cast<const u32x4*>(at_k + ks * 32);
+                if constexpr (S == 0) read_scales(at_fk, at_fv, 3);
+            }
+            if constexpr (n == 1 && S < 2 * DT) {
+                constexpr int kb = S / DT, dt = S % DT;
+                const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at_v + kb * 16 * VP + dt * 64)));
+                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at_v + (kb * 16 + 8) * VP + dt * 64)));
+                vf[kb][dt] = u32x4{u[0], u[1], w[0], w[1]};
+            }
+            // a weight is used a step after its exponential
+            const float p = weight(n, S, f, ref[n]);
+            if constexpr (S > 0) use(std::integral_constant<int, S - 1>{});
+            side(step_tag);
+            p_last = p;
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        use(std::integral_constant<int, 15>{});
+        asm volatile("" : "+v"(sum), "+v"(top));
+        if (__any(top > kMost || m[n] == -INFINITY)) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 16; k++) most = fmaxf(most, s[n][k] * (C::bytes == 1 ? fk[k / 4][k % 4] : f));
+            most = max_half(most);
+            const float m2 = fmaxf(m[n], most), back = m2 == -INFINITY ? 1.f : exp2_fast(m[n] - m2);
+            m[n] = m2;
+            ref[n] = m2 == -INFINITY ? 0.f : m2 - Prob<C>::up;
+            l[n] *= back;
+            sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+                const float p0 = weight(n, k, f, ref[n]), p1 = weight(n, k + 1, f, ref[n]);
+                sum += p0 + p1;
+                pf[n][k / 8][k % 8 / 2] = C::bytes == 1 ? pack16<P>(p0 * fv[k / 4][k % 4], p1 * fv[k / 4][k % 4 + 1]) : pack16<P>(p0, p1);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[n][dt][i] *= back;
+        }
+        l[n] += sum;
+        asm volatile("" : "+v"(l[n]));
+        s[n] = z;
+        // the next keys' scales, where this turn was the last to use these
+        if constexpr (n == 1) {
+#pragma unroll
+            for (int j = 0; j < 3; j++) read_scales(at_fk, at_fv, j);
+        }
+    };
+
+    if (n_tiles > 0) {
+        s_sk[3][lane] = 1.f;
+        load_pages(0);
+        load_tile(0);
+        load_pages(TK);
+        store_tile(0);
+        load_tile(TK);
+        load_pages(2 * TK);
+        store_tile(1);
+        load_tile(2 * TK);
+        load_pages(3 * TK);
+        __syncthreads();
+        const auto full_at = [&](int slot, int base, uint32_t& valid) {
+            valid = __builtin_amdgcn_readfirstlane((uint32_t)(s_valid[slot] >> (base & 32)));
+            return valid == 0xffffffffu && base + 31 <= wave_lo && base > see_hi;
+        };
+        uint32_t valid;
+        bool full = full_at(0, 0, valid);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) kf[ks] = *reinterpret_cast<const u32x4*>(s_k + k_lane + ks * 32);
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[n][i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) s[n] = mfma32<X>(kf[ks], q[n][ks], s[n]);
+        }
+#pragma unroll
+        for (int j = 0; j < 3; j++) read_scales(s_sk[full ? 0 : 3], s_sv[0], j);
+        int cur = 0, next = 1, third = 2;
+        for (int i = 0; i < n_tiles; i++) {
+            unroll<2>([&](auto sub_tag) {
+                constexpr int sub = decltype(sub_tag)::value;
+                const int base = i * TK + sub * 32;
+                if (!full) mask(0, cur, sub, base, valid), mask(1, cur, sub, base, valid);
+                const float f = full ? a.scale2 : 1.f;
+                const bool full2 = full_at(sub ? next : cur, base + 32, valid);
+                const int slot2 = sub ? next : cur;
+                const float* at_fk = s_sk[full ? cur : 3] + sub * 32;
+                turn(std::integral_constant<int, 0>{}, f, s_k + slot2 * (TK * KP) + (1 - sub) * 32 * KP + k_lane, nullptr, at_fk,
+                     s_sv[cur] + sub * 32, [&](auto step_tag) {
+                         constexpr int S = decltype(step_tag)::value;
+                         if constexpr (sub == 0) {  // the third tile into LDS
+                             if constexpr (S >= 4 && S < 4 + 2 * LOADS) {
+                                 if constexpr (S % 2 == 0) store_k((S - 4) / 2, third);
+                                 else store_v((S - 4) / 2, third);
+                             } else if constexpr (S == 15) {
+                                 store_scales(third);
+                             }
+                         }
+                     });
+                turn(std::integral_constant<int, 1>{}, f, nullptr, s_v + cur * (TK * VP) + sub * 32 * VP + v_lane,
+                     s_sk[full2 ? slot2 : 3] + (1 - sub) * 32, s_sv[slot2] + (1 - sub) * 32, [&](auto step_tag) {
+                         constexpr int S = decltype(step_tag)::value;
+                         if constexpr (sub == 0) {  // the fourth on its way, and its successor's pages
+                             if constexpr (S < LOADS) load_rows(S, i * TK + 3 * TK);
+                             else if constexpr (S == LOADS) load_scales(i * TK + 3 * TK);
+                             else if constexpr (S == LOADS + 1) load_pages(i * TK + 4 * TK);
+                         }
+                     });
+                full = full2;
+            });
+            const int was = cur;
+            cur = next, next = third, third = was;
+            __syncthreads();
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * DT; e++) o[1][e % DT] = mfma32<P>(vf[e / DT][e % DT], pf[1][e / DT], o[1][e % DT]);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+        float ln = sum_half(l[n]), mn = m[n];
+        if (ln != ln && mn == -INFINITY) mn = 0.f;  // only NaN scores so far: not a row without keys
+        const uint32_t row = wave_row + n * 32 + col;
+        if (row >= t.rows) continue;
+        if (a.splits > 1) {
+            const uint64_t p = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * Sh::BM + wave * 64 + n * 32 + col;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<f32x4*>(a.part_o + p * DP + dt * 32 + 2 * i + 4 * half) =
+                        f32x4{o[n][dt][i], o[n][dt][i + 1], o[n][dt][i + 2], o[n][dt][i + 3]};
+            if (half == 0) a.part_m[p * 2] = mn, a.part_m[p * 2 + 1] = ln;
+            continue;
+        }
+        const uint32_t token = t.token0 + row / a.group, head = kvh * a.group + row % a.group;
+        const float inv = mn == -INFINITY ? 0.f : 1.f / ln;
+        uint8_t* out = a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head) * 2;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const uint32_t d = dt * 32 + 2 * i + 4 * half;
+                if (d < a.dim)
+                    *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[n][dt][i] * inv, o[n][dt][i + 1] * inv),
+                                                                   pack16<X>(o[n][dt][i + 2] * inv, o[n][dt][i + 3] * inv)};
+            }
+        if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = mn == -INFINITY ? -INFINITY : (mn - Prob<C>::up + log2f(ln)) * kLn2;
+    }
+}
+
 // ------------------------------------------------------------ the splits' join
 // The splits of a row, in their order: 4 dimensions a thread.
 template <typename X, int DP, uint32_t BM>
@@ -729,9 +1118,9 @@ struct Cut {
     uint32_t bm, dp, tiles, splits, split_len;
     uint64_t part_m_bytes, bytes;  // of the workspace: the rows' maxima and sums, then their outputs
 };
-constexpr uint32_t kFewRows = 16, kManyRows = 128;
+constexpr uint32_t kFewRows = 16, kManyRows = 128, kWideRows = 256;
 constexpr uint64_t kSplitMin = 128;                   // keys of a split at least
-uint64_t blocks_wanted(uint32_t bm) { return bm == kFewRows ? 2048 : 512; }
+uint64_t blocks_wanted(uint32_t bm) { return bm == kFewRows ? 2048 : bm == kManyRows ? 512 : 256; }
 uint32_t padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 uint64_t most_tiles(uint32_t bm, uint64_t group, uint64_t n_seqs, uint64_t n_tokens) {
     return std::min(n_tokens * group / bm + std::min(n_seqs, n_tokens), n_tokens * ((group + bm - 1) / bm));
@@ -745,7 +1134,8 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     Cut c{};
     const uint64_t group = n_heads / n_kv;
     c.dp = padded_dim(dim);
-    c.bm = (uint64_t)max_chunk * group <= kFewRows ? kFewRows : kManyRows;
+    const uint64_t rows = (uint64_t)max_chunk * group;
+    c.bm = rows <= kFewRows ? kFewRows : rows <= kManyRows || c.dp == 256 ? kManyRows : kWideRows;
     c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
     // the keys of a tile: a window's, and as many again as the tile has tokens
     if (window) max_context = std::min<uint64_t>(max_context, (uint64_t)window + c.bm / group + 64);
@@ -760,7 +1150,7 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
 // What cut() asks for at most, for any batch up to these sizes.
 uint64_t most_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t n_tokens, uint64_t max_context) {
     uint64_t most = 0, m;
-    for (const uint32_t bm : {kFewRows, kManyRows}) {
+    for (const uint32_t bm : {kFewRows, kManyRows, kWideRows}) {
         const uint64_t blocks = most_tiles(bm, n_heads / n_kv, n_seqs, n_tokens) * n_kv;
         const uint64_t parts = std::min(blocks_wanted(bm), blocks * ((max_context + kSplitMin - 1) / kSplitMin));
         if (max_context > kSplitMin) most = std::max(most, part_bytes(parts * bm, padded_dim(dim), &m));
@@ -771,13 +1161,20 @@ uint64_t most_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_se
 template <typename X, typename C, int DP>
 hipError_t launch_attend(const AttnArg& a, const Cut& c, hipStream_t s) {
     const dim3 grid(a.tiles * a.kv_heads, c.splits);
-    if (c.bm == kFewRows) CKR_LAUNCH("kv_attention_few", s, attend_few_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
-    else CKR_LAUNCH("kv_attention_many", s, attend_many_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
-    if (c.splits > 1) {
+    const auto join = [&](auto kernel) {
+        if (c.splits <= 1) return;
         const uint32_t per = 256 / (DP / 4);
-        const dim3 jgrid(a.tiles * a.kv_heads, (c.bm + per - 1) / per);
-        if (c.bm == kFewRows) CKR_LAUNCH("kv_attention_join", s, attend_join_kernel<X, DP, 16><<<jgrid, 256, 0, s>>>(a, Prob<C>::up));
-        else CKR_LAUNCH("kv_attention_join", s, attend_join_kernel<X, DP, 128><<<jgrid, 256, 0, s>>>(a, Prob<C>::up));
+        CKR_LAUNCH("kv_attention_join", s, kernel<<<dim3(a.tiles * a.kv_heads, (c.bm + per - 1) / per), 256, 0, s>>>(a, Prob<C>::up));
+    };
+    if (c.bm == kFewRows) {
+        CKR_LAUNCH("kv_attention_few", s, attend_few_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
+        join(attend_join_kernel<X, DP, kFewRows>);
+    } else if (c.bm == kManyRows) {
+        CKR_LAUNCH("kv_attention_many", s, attend_many_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
+        join(attend_join_kernel<X, DP, kManyRows>);
+    } else if constexpr (DP <= 128) {
+        CKR_LAUNCH("kv_attention_wide", s, attend_wide_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
+        join(attend_join_kernel<X, DP, kWideRows>);
     }
     return hipGetLastError();
 }
