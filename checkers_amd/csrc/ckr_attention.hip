@@ -112,16 +112,17 @@ template <int N, typename F> __device__ __forceinline__ void unroll(F f) { unrol
 
 // Which sequence and rows a tile of BM rows is: rows of a sequence are its
 // chunk's tokens times the query heads of a key/value head, in that order.
-// Every thread of the block calls it; s_tmp: 8 words of LDS.
+// Every thread of the block calls it; s_tmp: a word of LDS per wave and two more.
 struct Tile {
     uint32_t seq, row0, rows, token0;  // rows: of the whole sequence; token0: its first packed row
     int64_t start, end;                // the position of its first token, and after its last
 };
-template <uint32_t BM>
+template <uint32_t BM, uint32_t THREADS = 256>
 __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint32_t tile, uint32_t* s_tmp, Tile& t) {
+    constexpr uint32_t WAVES = THREADS / 64;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t done = 0;
-    for (uint32_t base = 0; base < b.n_seqs; base += 256) {
+    for (uint32_t base = 0; base < b.n_seqs; base += THREADS) {
         const uint32_t i = base + threadIdx.x;
         uint32_t n = 0;
         if (i < b.n_seqs) {
@@ -138,15 +139,15 @@ __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint
         __syncthreads();
         uint32_t before = done, all = 0;
 #pragma unroll
-        for (uint32_t w = 0; w < 4; w++) {
+        for (uint32_t w = 0; w < WAVES; w++) {
             if (w < wave) before += s_tmp[w];
             all += s_tmp[w];
         }
         if (tile < done + all) {
             const uint32_t first = before + sum - n;
-            if (tile >= first && tile < first + n) s_tmp[4] = i, s_tmp[5] = tile - first;
+            if (tile >= first && tile < first + n) s_tmp[WAVES] = i, s_tmp[WAVES + 1] = tile - first;
             __syncthreads();
-            t.seq = s_tmp[4], t.row0 = s_tmp[5] * BM;
+            t.seq = s_tmp[WAVES], t.row0 = s_tmp[WAVES + 1] * BM;
             const int32_t lo = b.offsets[t.seq], hi = min(b.offsets[t.seq + 1], (int32_t)b.n_tokens);
             t.token0 = (uint32_t)lo, t.rows = (uint32_t)(hi - lo) * group;
             t.start = b.starts[t.seq], t.end = t.start + (hi - lo);
@@ -704,204 +705,199 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 }
 
 // ------------------------------------------------------------ very many rows
-// A block takes 256 rows, a wave 64 of them as two halves of 32, one wave a SIMD
-// with all of its registers.  The halves take turns: while the matrix cores work
-// for one half, the vector units run the other's softmax, in one stream of
-// instructions.  With S(i) the scores of the i-th 32 keys, in turn
-//   A(i): O1 += V(i-1) P1(i-1), S0(i+1) = K(i+1) Q0   beside  softmax of S0(i) -> P0(i)
-//   B(i): S1(i+1) = K(i+1) Q1,  O0 += V(i) P0(i)      beside  softmax of S1(i) -> P1(i)
-// so K(i+1) and V(i) are read from LDS once for both halves (half of what a wave of
-// 32 rows reads), each a turn before its second use.  Tiles of 64 keys go through
-// a ring of three in LDS.
+// A block of eight waves takes 256 rows, a wave 32 of them, two waves a SIMD.  With
+// S(i) the scores of the i-th 32 keys and P(i) their weights, a wave's turn i is
+//   S(i+1) = K(i+1) Q  and  O += V(i-1) P(i-1)  on the matrix cores, beside
+//   P(i) = exp(S(i) - maximum so far)           on the vector units,
+// three things that do not wait for each other, written as 16 steps of a matrix
+// product, the reads of LDS for the products three steps on, and one score's
+// weight, in that order.  What bounds it is the issue of vector instructions (five
+// and a half per score and lane), so the maximum is not looked for at each turn:
+// weights are taken against the maximum so far, and only where one comes out above
+// 2^kLag, or a row has no maximum yet, is the turn's softmax made again.
+// Tiles of 64 keys go through a ring of four in LDS (the turns of a tile still read
+// the last half of the one before and the first half of the one after, while the
+// next but one is stored): waves 0 to 3 stage the keys, 4 to 7 the values.  A wave's
+// rows of a tile lie in one page (16 slots at least), so addresses are the page's,
+// in scalar registers, and an offset that never changes.
 template <typename C, int DP> struct WideShape {
-    static constexpr int TK = 64, BM = 256;
+    static constexpr int TK = 64, BM = 256, RING = 4;
     static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 64;  // as ManyShape's
-    static constexpr int LPR = DP * C::bytes / 16, LOADS = TK * LPR / 256, ROWS = 256 / LPR;
+    static constexpr int LPR = DP * C::bytes / 16, LOADS = TK * LPR / 256;  // lanes of a row, loads of a thread
+    static constexpr int RPW = 64 / LPR, ROWS = 256 / LPR;                  // rows of a wave's load, of four waves'
 };
 
 template <typename X, typename C, int DP>
-__global__ void __launch_bounds__(256, 1) attend_wide_kernel(AttnArg a) {
+__global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     typedef typename Prob<C>::E P;
     typedef WideShape<C, DP> Sh;
-    constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, ROWS = Sh::ROWS;
-    constexpr int KS = DP / 16, DT = DP / 32;
+    constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, RPW = Sh::RPW, ROWS = Sh::ROWS;
+    constexpr int KS = DP / 16, DT = DP / 32, NM = 2 * KS;  // KS products for the scores, as many for the values
+    static_assert(KS == 2 * DT && KS % 4 == 0, "pairs of products, operands in rings of four");
     constexpr float kMost = Prob<C>::up == 0.f ? 256.f : 32768.f;  // 2^(kLag + up)
-    __shared__ __attribute__((aligned(16))) uint8_t s_k[3 * TK * KP];
-    __shared__ __attribute__((aligned(16))) uint8_t s_v[3 * TK * VP];
-    __shared__ __attribute__((aligned(16))) float s_sk[4][TK];  // [3]: ones, for scores that carry their scale
-    __shared__ __attribute__((aligned(16))) float s_sv[3][TK];
-    __shared__ uint64_t s_valid[3];
-    __shared__ uint32_t s_tmp[8];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[Sh::RING * TK * KP];
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[Sh::RING * TK * VP];
+    __shared__ __attribute__((aligned(16))) float s_sk[Sh::RING + 1][TK];  // the last: ones, for scores that carry their scale
+    __shared__ __attribute__((aligned(16))) float s_sv[Sh::RING][TK];
+    __shared__ uint32_t s_tmp[16];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
     Tile t;
-    if (!find_tile<Sh::BM>(a.b, a.group, tile, s_tmp, t)) return;
+    if (!find_tile<Sh::BM, 512>(a.b, a.group, tile, s_tmp, t)) return;
     const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + Sh::BM - 1, t.rows - 1) / a.group;
     const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
     const int64_t first = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) & ~(int64_t)(TK - 1) : 0;
     const int64_t lo = first + (int64_t)split * a.split_len;
     const int64_t hi = split + 1 == a.splits ? limit : min(limit, lo + (int64_t)a.split_len);
-    const int n_tiles = hi > lo ? (int)((hi - lo + TK - 1) / TK) : 0;
+    const int n_tiles = __builtin_amdgcn_readfirstlane(hi > lo ? (int)((hi - lo + TK - 1) / TK) : 0);
+    // from here on keys are counted from lo, in 32 bits
     const auto rel = [&](int64_t p) { return (int)max((int64_t)-0x40000000, min(p - lo, (int64_t)0x7fffffff - 8 * TK)); };
-    const uint32_t wave_row = __builtin_amdgcn_readfirstlane(t.row0 + wave * 64);
-    const int end = rel(limit);
-    const int wave_lo = rel(t.start + min(wave_row, t.rows - 1) / a.group);
-    const int see_hi = a.window ? rel(t.start + min(wave_row + 63, t.rows - 1) / a.group - (int64_t)a.window) : -0x40000000;
-    int pos[2], see[2];
-    u32x4 q[2][KS];
+    const uint32_t wave_row = t.row0 + wave * 32, row = wave_row + col;
+    const int end = __builtin_amdgcn_readfirstlane(rel(limit));
+    const int wave_lo = __builtin_amdgcn_readfirstlane(rel(t.start + min(wave_row, t.rows - 1) / a.group));
+    const int see_hi = __builtin_amdgcn_readfirstlane(
+        a.window ? rel(t.start + min(wave_row + 31, t.rows - 1) / a.group - (int64_t)a.window) : -0x40000000);
+    const int64_t my_pos = t.start + min(row, t.rows - 1) / a.group;
+    const int pos = rel(my_pos), see = a.window ? rel(my_pos - (int64_t)a.window) : -0x40000000;
+    u32x4 q[KS];
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-        const uint32_t row = wave_row + n * 32 + col;
-        const int64_t p = t.start + min(row, t.rows - 1) / a.group;
-        pos[n] = rel(p), see[n] = a.window ? rel(p - (int64_t)a.window) : -0x40000000;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const uint32_t d = ks * 16 + half * 8;
-            q[n][ks] = u32x4{0, 0, 0, 0};
-            if (row < t.rows && d < a.dim) {
-                q[n][ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(t.token0 + row / a.group) * a.q_tok +
-                                                                 (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
-                q[n][ks] ^= a.flip;
-            }
-            // the queries stay in accumulation registers, which the products read as well
-            asm volatile("" : "+a"(q[n][ks]));
+    for (int ks = 0; ks < KS; ks++) {
+        const uint32_t d = ks * 16 + half * 8;
+        q[ks] = u32x4{0, 0, 0, 0};
+        if (row < t.rows && d < a.dim) {
+            q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(t.token0 + row / a.group) * a.q_tok +
+                                                          (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
+            q[ks] ^= a.flip;
         }
     }
-    // staging, without branches: a key of no mapped page is read from page 0 (its
-    // values are cleared, its scores masked), pieces past the head's size are the
-    // last piece again (they meet queries of zero, and dimensions that are not stored)
-    typedef __attribute__((address_space(1))) const int32_t* global_i32;
-    const global_i32 table = (global_i32)(a.b.table + (int64_t)t.seq * a.b.table_stride);
-    const uint32_t r0 = threadIdx.x / LPR, piece = min(threadIdx.x % LPR, a.dim * C::bytes / 16 - 1), place = threadIdx.x % LPR;
+    // staging.  A key of no mapped page is read from page 0 and then cleared (values)
+    // or masked (scores); pieces past the head's size are the last piece again (they
+    // meet queries of zero, and dimensions that are not stored)
+    typedef __attribute__((address_space(4))) const int32_t* const_i32;
+    const const_i32 table = (const_i32)(a.b.table + (int64_t)__builtin_amdgcn_readfirstlane(t.seq) * a.b.table_stride);
+    const bool stage_k = wave < 4;
+    const uint32_t w4 = wave & 3, row_of = w4 * RPW + lane / LPR, place = lane % LPR;
+    const uint32_t piece = min(place, a.dim * C::bytes / 16 - 1);
     const uint32_t slot_mask = (1u << a.page_shift) - 1;
-    const int64_t c0 = lo >> a.page_shift;
-    const uint32_t in0 = (uint32_t)lo & slot_mask, last_col = a.b.width - 1;
-    const u32x4* kp = reinterpret_cast<const u32x4*>(a.ck + (int64_t)kvh * a.kst[1]) + piece;
-    const u32x4* vp = reinterpret_cast<const u32x4*>(a.cv + (int64_t)kvh * a.vst[1]) + piece;
-    const uint32_t ks0 = (uint32_t)(a.kst[0] >> 4), ks2 = (uint32_t)(a.kst[2] >> 4), vs0 = (uint32_t)(a.vst[0] >> 4), vs2 = (uint32_t)(a.vst[2] >> 4);
-    const float* skp = a.sk + (int64_t)kvh * a.skst[1];
-    const float* svp = a.sv + (int64_t)kvh * a.svst[1];
+    const uint32_t st0 = (uint32_t)((stage_k ? a.kst[0] : a.vst[0]) >> 4), st2 = (uint32_t)((stage_k ? a.kst[2] : a.vst[2]) >> 4);
+    const uint8_t* const from = stage_k ? a.ck + (int64_t)kvh * a.kst[1] : a.cv + (int64_t)kvh * a.vst[1];
+    const uint32_t from_lane = ((row_of & 15) * st2 + piece) * 16;
+    uint8_t* const to = (stage_k ? s_k + row_of * KP : s_v + row_of * VP) + place * (C::bytes == 1 ? 32 : 16);
+    const uint32_t to_rows = ROWS * (stage_k ? KP : VP), to_slot = TK * (stage_k ? KP : VP);
+    const uint32_t c0 = (uint32_t)(lo >> a.page_shift), in0 = (uint32_t)lo & slot_mask, last_col = a.b.width - 1;
+    // the page of the 16 keys from j (a multiple of 16) on; -1: none
     const auto page_id = [&](int j) {
-        const uint32_t c = (uint32_t)min((uint64_t)c0 + ((in0 + (uint32_t)j) >> a.page_shift), (uint64_t)last_col);
-        const int32_t p = table[c];
+        const int32_t p = table[min(c0 + ((in0 + (uint32_t)j) >> a.page_shift), last_col)];
         return ((j < end) & ((uint32_t)p < a.n_pages)) ? p : -1;  // end lies within the table
     };
-    int32_t pg[LOADS], pg_s;
+    int32_t pg[4];         // of the tile that is loaded next
+    uint64_t valid[4];     // keys of mapped pages: of this tile, and of the next three
     const auto load_pages = [&](int base) {
 #pragma unroll
-        for (int u = 0; u < LOADS; u++) pg[u] = page_id(base + (int)r0 + u * ROWS);
-        pg_s = page_id(base + (int)lane);
+        for (int g = 0; g < 4; g++) pg[g] = page_id(base + 16 * g);
     };
-    u32x4 kr[LOADS], vr[LOADS];
+    const auto valid_of = [&](int base) {
+        uint64_t v = 0;
+#pragma unroll
+        for (int g = 0; g < 4; g++) v |= pg[g] >= 0 ? 0xffffull << (16 * g) : 0;
+        return end - base >= TK ? v : end - base <= 0 ? 0 : v & ((1ull << (end - base)) - 1);
+    };
+    u32x4 held[LOADS];
     float sk = 0.f, sv = 0.f;
-    bool in_s = false, in_v[LOADS];
+    uint64_t held_valid = 0;
     const auto load_rows = [&](int u, int base) {
-        const uint32_t slot = (in0 + (uint32_t)base + r0 + u * ROWS) & slot_mask, page = (uint32_t)max(pg[u], 0);
-        in_v[u] = pg[u] >= 0;
-        kr[u] = kp[(uint64_t)page * ks0 + (uint64_t)slot * ks2];
-        vr[u] = vp[(uint64_t)page * vs0 + (uint64_t)slot * vs2];
+        const uint32_t g = (w4 * RPW + u * ROWS) / 16;
+        const int32_t p = g == 0 ? pg[0] : g == 1 ? pg[1] : g == 2 ? pg[2] : pg[3];
+        const uint32_t slot = (in0 + (uint32_t)base + 16 * g) & slot_mask;
+        const uint64_t off = (uint64_t)(uint32_t)max(p, 0) * st0 + (uint64_t)slot * st2;
+        held[u] = *reinterpret_cast<const u32x4*>(from + off * 16 + from_lane);
     };
     const auto load_scales = [&](int base) {
-        in_s = pg_s >= 0;
         if constexpr (C::bytes == 1) {
-            const uint32_t slot = (in0 + (uint32_t)base + lane) & slot_mask;
-            sk = skp[(int64_t)max(pg_s, 0) * a.skst[0] + slot];
-            sv = svp[(int64_t)max(pg_s, 0) * a.svst[0] + slot];
+            const int32_t p = max(w4 == 0 ? pg[0] : w4 == 1 ? pg[1] : w4 == 2 ? pg[2] : pg[3], 0);
+            const uint32_t slot = (in0 + (uint32_t)base + 16 * w4) & slot_mask;
+            sk = (a.sk + ((int64_t)p * a.skst[0] + (int64_t)kvh * a.skst[1] + slot))[lane & 15];
+            sv = (a.sv + ((int64_t)p * a.svst[0] + (int64_t)kvh * a.svst[1] + slot))[lane & 15];
         }
+        held_valid = valid_of(base);
     };
-    const auto store_k = [&](int u, int slot) {
-        uint8_t* k = s_k + slot * (TK * KP) + (r0 + u * ROWS) * KP;
+    const auto store_rows = [&](int u, int slot) {
+        u32x4 x = held[u];
+        if (!stage_k && held_valid != ~0ull) {
+            const bool in = held_valid >> (row_of + u * ROWS) & 1;
+            x = in ? x : u32x4{0, 0, 0, 0};
+        }
+        uint8_t* at = to + slot * to_slot + u * to_rows;
         if constexpr (C::bytes == 2) {
-            *reinterpret_cast<u32x4*>(k + place * 16) = kr[u];
+            *reinterpret_cast<u32x4*>(at) = x;
+        } else if (X::tag == P::tag || stage_k) {
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const u32x2 y = widen4<C, X>(x[2 * w]), z = widen4<C, X>(x[2 * w + 1]);
+                *reinterpret_cast<u32x4*>(at + w * 16) = u32x4{y[0], y[1], z[0], z[1]};
+            }
         } else {
 #pragma unroll
             for (int w = 0; w < 2; w++) {
-                const u32x2 x = widen4<C, X>(kr[u][2 * w]), y = widen4<C, X>(kr[u][2 * w + 1]);
-                *reinterpret_cast<u32x4*>(k + place * 32 + w * 16) = u32x4{x[0], x[1], y[0], y[1]};
+                const u32x2 y = widen4<C, P>(x[2 * w]), z = widen4<C, P>(x[2 * w + 1]);
+                *reinterpret_cast<u32x4*>(at + w * 16) = u32x4{y[0], y[1], z[0], z[1]};
             }
         }
     };
-    const auto store_v = [&](int u, int slot) {
-        uint8_t* v = s_v + slot * (TK * VP) + (r0 + u * ROWS) * VP;
-        const u32x4 vx = in_v[u] ? vr[u] : u32x4{0, 0, 0, 0};
-        if constexpr (C::bytes == 2) {
-            *reinterpret_cast<u32x4*>(v + place * 16) = vx;
-        } else {
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-                const u32x2 x = widen4<C, P>(vx[2 * w]), y = widen4<C, P>(vx[2 * w + 1]);
-                *reinterpret_cast<u32x4*>(v + place * 32 + w * 16) = u32x4{x[0], x[1], y[0], y[1]};
-            }
-        }
-    };
-    const auto store_scales = [&](int slot) {  // every wave writes the same values
+    const auto store_scales = [&](int slot) {  // four lanes write the same values
         if constexpr (C::bytes == 1) {
-            const bool fine = abs_bits(sv) < 0x7f800000u;
-            s_sk[slot][lane] = fine ? sk * a.scale2 : as_f32(0x7fc00000u);
-            s_sv[slot][lane] = in_s && fine ? sv : 0.f;
+            // a value scale that is not finite shows in the score instead, so that a
+            // weight of 0 (a key that a row does not see) always gives 0
+            const bool fine = abs_bits(sv) < 0x7f800000u, in = held_valid >> (16 * w4 + (lane & 15)) & 1;
+            if (stage_k) s_sk[slot][16 * w4 + (lane & 15)] = fine ? sk * a.scale2 : as_f32(0x7fc00000u);
+            else s_sv[slot][16 * w4 + (lane & 15)] = in && fine ? sv : 0.f;
         }
-        s_valid[slot] = __ballot(in_s);
-    };
-    const auto load_tile = [&](int base) {
-#pragma unroll
-        for (int u = 0; u < LOADS; u++) load_rows(u, base);
-        load_scales(base);
-    };
-    const auto store_tile = [&](int slot) {
-#pragma unroll
-        for (int u = 0; u < LOADS; u++) store_k(u, slot), store_v(u, slot);
-        store_scales(slot);
     };
 
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    f32x16 o[2][DT], s[2];
-    u32x4 pf[2][2], kf[KS], vf[2][DT];
+    float m = -INFINITY, l = 0.f, ref = 0.f;
+    f32x16 o[DT], s;
+    u32x4 pf[2][2], kf[4], vf[4];  // weights of two turns; operands, read three pairs of steps ahead
+    f32x4 fk[2], fv[2];            // the keys' scales, of keys 8 j + 4 half on
 #pragma unroll
-    for (int n = 0; n < 2; n++)
+    for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[n][dt][i] = 0.f;
-            vf[n][dt] = u32x4{0, 0, 0, 0};
-        }
-    pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
+        for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
     const uint32_t k_lane = col * KP + half * 16;
     const uint32_t v_lane = (4 * half + (lane & 15) / 4) * VP + (16 * ((lane >> 4) & 1) + (lane & 3) * 4) * 2;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* lds4;
+    const auto k_at = [&](int slot, int sub) { return s_k + slot * (TK * KP) + sub * 32 * KP + k_lane; };
+    const auto v_at = [&](int slot, int sub) { return s_v + slot * (TK * VP) + sub * 32 * VP + v_lane; };
+    const auto read_k = [&](int e, const uint8_t* at) { kf[e % 4] = *reinterpret_cast<const u32x4*>(at + e * 32); };
+    const auto read_v = [&](int e, const uint8_t* at) {
+        at += e / DT * 16 * VP + e % DT * 64;
+        const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at)));
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * VP)));
+        vf[e % 4] = u32x4{u[0], u[1], w[0], w[1]};
+    };
+    const auto read_scales = [&](int j, const float* at_fk, const float* at_fv) {
+        if constexpr (C::bytes == 1) {
+            fk[j % 2] = *reinterpret_cast<const f32x4*>(at_fk + 8 * j + 4 * half);
+            fv[j % 2] = *reinterpret_cast<const f32x4*>(at_fv + 8 * j + 4 * half);
+        }
+    };
+    const auto weight = [&](int k, f32x4 g, float f) {
+        return exp2_fast(__builtin_fmaf(s[k], C::bytes == 1 ? g[k % 4] : f, -ref));
+    };
     // scores that some row of the wave must not see: scaled here, -inf where hidden
-    const auto mask = [&](int n, int slot, int sub, int base, uint32_t valid) {
-        valid >>= 4 * half;
+    const auto mask = [&](const float* at_fk, int base, uint32_t seen) {
+        seen >>= 4 * half;
         const int k0 = base + 4 * half;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int key = 8 * (i / 4) + i % 4;
-            const float f = C::bytes == 1 ? s_sk[slot][sub * 32 + key + 4 * half] : a.scale2;
-            s[n][i] = (valid >> key & 1) && k0 + key <= pos[n] && k0 + key > see[n] ? s[n][i] * f : -INFINITY;
+            const float f = C::bytes == 1 ? at_fk[key + 4 * half] : a.scale2;
+            s[i] = (seen >> key & 1) && k0 + key <= pos && k0 + key > see ? s[i] * f : -INFINITY;
         }
     };
-    f32x4 fk[4], fv[4];  // the keys' scales, of keys 8 j + 4 half on
-    const auto read_scales = [&](const float* at_fk, const float* at_fv, int j) {
-        if constexpr (C::bytes == 1) {
-            fk[j] = *reinterpret_cast<const f32x4*>(at_fk + 8 * j + 4 * half);
-            fv[j] = *reinterpret_cast<const f32x4*>(at_fv + 8 * j + 4 * half);
-        }
-    };
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4* lds4;
-    // the weight of score k, with its share of the sum
-    const auto weight = [&](int n, int k, float f, float ref) {
-        const float p = exp2_fast(__builtin_fmaf(s[n][k], C::bytes == 1 ? fk[k / 4][k % 4] : f, -ref));
-        return p;
-    };
-    float ref[2] = {0.f, 0.f};
-    // One turn: 16 steps, each at most one matrix product and its share of the rest,
-    // kept in this order.  TURN 0 is A, 1 is B; half n = TURN takes its softmax, the
-    // scores of half n for the next keys are made, and half 1 - n (the one whose weights
-    // the last turn made) gathers its values.  The weights are taken against the
-    // maximum so far; only where one comes out above 2^kLag, or a row has no maximum
-    // yet, is the new maximum looked for and the turn's weights made again.
-    const auto turn = [&](auto turn_tag, float f, const uint8_t* at_k, const uint8_t* at_v, const float* at_fk,
-                          const float* at_fv, auto side) {
-        constexpr int n = decltype(turn_tag)::value, NM = KS + 2 * DT;
+    struct Where { const uint8_t *k, *v; const float *fk, *fv; };  // what a turn reads: K(i+1), V(i-1), scales(i)
+    const auto turn = [&](auto sub_tag, float f, const Where& now, const Where& after, auto side) {
+        constexpr int sub = decltype(sub_tag)::value;
         f32x16 z;
 #pragma unroll
         for (int i = 0; i < 16; i++) z[i] = 0.f;
@@ -910,175 +906,185 @@ __global__ void __launch_bounds__(256, 1) attend_wide_kernel(AttnArg a) {
             constexpr int k = decltype(k_tag)::value;
             sum += p_last;
             if constexpr (k % 2 == 0) {
-                p_even = p_last;
+                p_even = C::bytes == 1 ? p_last * fv[k / 4 % 2][k % 4] : p_last;
+                top = fmaxf(top, p_last);
             } else {
-                top = fmaxf(fmaxf(top, p_even), p_last);
-                uint32_t w = C::bytes == 1 ? pack16<P>(p_even * fv[k / 4][k % 4 - 1], p_last * fv[k / 4][k % 4]) : pack16<P>(p_even, p_last);
+                top = fmaxf(top, p_last);
+                uint32_t w = pack16<P>(p_even, C::bytes == 1 ? p_last * fv[k / 4 % 2][k % 4] : p_last);
                 asm volatile("" : "+v"(w));
-                pf[n][k / 8][k % 8 / 2] = w;
+                pf[sub][k / 8][k % 8 / 2] = w;
             }
         };
         unroll<16>([&](auto step_tag) {
             constexpr int S = decltype(step_tag)::value;
             if constexpr (S % (16 / NM) == 0) {
-                constexpr int j = S * NM / 16, first = n == 0 ? 2 * DT : KS;
-                constexpr bool scores = (j >= first) == (n == 0);
-                constexpr int e = j >= first ? j - first : j;
-                if constexpr (scores) z = mfma32<X>(kf[e], q[n][e], z);
-                else o[1 - n][e % DT] = mfma32<P>(vf[e / DT][e % DT], pf[1 - n][e / DT], o[1 - n][e % DT]);
-            }
-            // reads of LDS: keys in A and values in B for the turn's second half; scales
-            if constexpr (n == 0 && S < 4) {
-#pragma unroll
-                for (int ks = S * KS / 4; ks < (S + 1) * KS / 4; ks++) kf[ks] = *reinterpret_cast<const u32x4*>(at_k + ks * 32);
-                if constexpr (S == 0) read_scales(at_fk, at_fv, 3);
-            }
-            if constexpr (n == 1 && S < 2 * DT) {
-                constexpr int kb = S / DT, dt = S % DT;
-                const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at_v + kb * 16 * VP + dt * 64)));
-                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at_v + (kb * 16 + 8) * VP + dt * 64)));
-                vf[kb][dt] = u32x4{u[0], u[1], w[0], w[1]};
+                constexpr int j = S * NM / 16, e = j / 2;
+                if constexpr (j % 2 == 0) {
+                    o[e % DT] = mfma32<P>(vf[e % 4], pf[1 - sub][e / DT], o[e % DT]);
+                    if constexpr (e + 3 < KS) read_v(e + 3, now.v);
+                    else read_v(e + 3 - KS, after.v);
+                } else {
+                    z = mfma32<X>(kf[e % 4], q[e], z);
+                    if constexpr (e + 3 < KS) read_k(e + 3, now.k);
+                    else read_k(e + 3 - KS, after.k);
+                }
             }
             // a weight is used a step after its exponential
-            const float p = weight(n, S, f, ref[n]);
+            const float p = weight(S, fk[S / 4 % 2], f);
             if constexpr (S > 0) use(std::integral_constant<int, S - 1>{});
+            if constexpr (S % 4 == 1) {  // the last group's scales have been used
+                if constexpr (S < 12) read_scales(S / 4 + 1, now.fk, now.fv);
+                else read_scales(0, after.fk, after.fv);
+            }
             side(step_tag);
             p_last = p;
             __builtin_amdgcn_sched_barrier(0);
         });
         use(std::integral_constant<int, 15>{});
         asm volatile("" : "+v"(sum), "+v"(top));
-        if (__any(top > kMost || m[n] == -INFINITY)) {
+        if (__any(top > kMost || m == -INFINITY)) {
             float most = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 16; k++) most = fmaxf(most, s[n][k] * (C::bytes == 1 ? fk[k / 4][k % 4] : f));
+            for (int k = 0; k < 16; k += 4) {
+                const f32x4 g = C::bytes == 1 ? *reinterpret_cast<const f32x4*>(now.fk + 2 * k + 4 * half) : f32x4{f, f, f, f};
+#pragma unroll
+                for (int i = 0; i < 4; i++) most = fmaxf(most, s[k + i] * g[i]);
+            }
             most = max_half(most);
-            const float m2 = fmaxf(m[n], most), back = m2 == -INFINITY ? 1.f : exp2_fast(m[n] - m2);
-            m[n] = m2;
-            ref[n] = m2 == -INFINITY ? 0.f : m2 - Prob<C>::up;
-            l[n] *= back;
+            const float m2 = fmaxf(m, most), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
+            m = m2;
+            ref = m2 == -INFINITY ? 0.f : m2 - Prob<C>::up;
+            l *= back;
             sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-                const float p0 = weight(n, k, f, ref[n]), p1 = weight(n, k + 1, f, ref[n]);
-                sum += p0 + p1;
-                pf[n][k / 8][k % 8 / 2] = C::bytes == 1 ? pack16<P>(p0 * fv[k / 4][k % 4], p1 * fv[k / 4][k % 4 + 1]) : pack16<P>(p0, p1);
+            for (int k = 0; k < 16; k += 4) {
+                f32x4 g = {f, f, f, f}, gv = {1.f, 1.f, 1.f, 1.f};
+                if constexpr (C::bytes == 1) {
+                    g = *reinterpret_cast<const f32x4*>(now.fk + 2 * k + 4 * half);
+                    gv = *reinterpret_cast<const f32x4*>(now.fv + 2 * k + 4 * half);
+                }
+                float p[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    p[i] = weight(k + i, g, f);
+                    sum += p[i];
+                }
+                pf[sub][k / 8][k % 8 / 2] = pack16<P>(p[0] * gv[0], p[1] * gv[1]);
+                pf[sub][k / 8][k % 8 / 2 + 1] = pack16<P>(p[2] * gv[2], p[3] * gv[3]);
             }
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[n][dt][i] *= back;
+                for (int i = 0; i < 16; i++) o[dt][i] *= back;
         }
-        l[n] += sum;
-        asm volatile("" : "+v"(l[n]));
-        s[n] = z;
-        // the next keys' scales, where this turn was the last to use these
-        if constexpr (n == 1) {
-#pragma unroll
-            for (int j = 0; j < 3; j++) read_scales(at_fk, at_fv, j);
-        }
+        l += sum;
+        asm volatile("" : "+v"(l));
+        s = z;
     };
 
     if (n_tiles > 0) {
-        s_sk[3][lane] = 1.f;
-        load_pages(0);
-        load_tile(0);
-        load_pages(TK);
-        store_tile(0);
-        load_tile(TK);
-        load_pages(2 * TK);
-        store_tile(1);
-        load_tile(2 * TK);
+        if (wave == 0) s_sk[Sh::RING][lane] = 1.f;
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            load_pages(i * TK);
+            valid[i] = valid_of(i * TK);
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) load_rows(u, i * TK);
+            load_scales(i * TK);
+            if (i < 2) {
+#pragma unroll
+                for (int u = 0; u < LOADS; u++) store_rows(u, i);
+                store_scales(i);
+            }
+        }
         load_pages(3 * TK);
         __syncthreads();
-        const auto full_at = [&](int slot, int base, uint32_t& valid) {
-            valid = __builtin_amdgcn_readfirstlane((uint32_t)(s_valid[slot] >> (base & 32)));
-            return valid == 0xffffffffu && base + 31 <= wave_lo && base > see_hi;
+        const auto full_at = [&](uint64_t v, int base) {
+            return (uint32_t)(v >> (base & 32)) == 0xffffffffu && base + 31 <= wave_lo && base > see_hi;
         };
-        uint32_t valid;
-        bool full = full_at(0, 0, valid);
+        bool full = full_at(valid[0], 0);
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) kf[ks] = *reinterpret_cast<const u32x4*>(s_k + k_lane + ks * 32);
+        for (int i = 0; i < 16; i++) s[i] = 0.f;
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[n][i] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) s[n] = mfma32<X>(kf[ks], q[n][ks], s[n]);
+        for (int e = 0; e < KS; e++) {
+            read_k(e, k_at(0, 0));
+            s = mfma32<X>(kf[e % 4], q[e], s);
         }
+        // turn 0 has no values before it: what it gathers is dropped after it
+        pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
+        Where now = {k_at(0, 1), v_at(0, 0), s_sk[full ? 0 : Sh::RING], s_sv[0]};
 #pragma unroll
-        for (int j = 0; j < 3; j++) read_scales(s_sk[full ? 0 : 3], s_sv[0], j);
-        int cur = 0, next = 1, third = 2;
+        for (int e = 0; e < 3; e++) read_k(e, now.k), read_v(e, now.v);
+        read_scales(0, now.fk, now.fv);
         for (int i = 0; i < n_tiles; i++) {
+            const int cur = i & 3, next = (i + 1) & 3, third = (i + 2) & 3;
             unroll<2>([&](auto sub_tag) {
                 constexpr int sub = decltype(sub_tag)::value;
                 const int base = i * TK + sub * 32;
-                if (!full) mask(0, cur, sub, base, valid), mask(1, cur, sub, base, valid);
+                if (!full) mask(s_sk[cur] + sub * 32, base, (uint32_t)(valid[0] >> (32 * sub)));
                 const float f = full ? a.scale2 : 1.f;
-                const bool full2 = full_at(sub ? next : cur, base + 32, valid);
+                const bool full2 = full_at(valid[sub], base + 32);
                 const int slot2 = sub ? next : cur;
-                const float* at_fk = s_sk[full ? cur : 3] + sub * 32;
-                turn(std::integral_constant<int, 0>{}, f, s_k + slot2 * (TK * KP) + (1 - sub) * 32 * KP + k_lane, nullptr, at_fk,
-                     s_sv[cur] + sub * 32, [&](auto step_tag) {
-                         constexpr int S = decltype(step_tag)::value;
-                         if constexpr (sub == 0) {  // the third tile into LDS
-                             if constexpr (S >= 4 && S < 4 + 2 * LOADS) {
-                                 if constexpr (S % 2 == 0) store_k((S - 4) / 2, third);
-                                 else store_v((S - 4) / 2, third);
-                             } else if constexpr (S == 15) {
-                                 store_scales(third);
-                             }
-                         }
-                     });
-                turn(std::integral_constant<int, 1>{}, f, nullptr, s_v + cur * (TK * VP) + sub * 32 * VP + v_lane,
-                     s_sk[full2 ? slot2 : 3] + (1 - sub) * 32, s_sv[slot2] + (1 - sub) * 32, [&](auto step_tag) {
-                         constexpr int S = decltype(step_tag)::value;
-                         if constexpr (sub == 0) {  // the fourth on its way, and its successor's pages
-                             if constexpr (S < LOADS) load_rows(S, i * TK + 3 * TK);
-                             else if constexpr (S == LOADS) load_scales(i * TK + 3 * TK);
-                             else if constexpr (S == LOADS + 1) load_pages(i * TK + 4 * TK);
-                         }
-                     });
+                const Where after = {k_at(next, sub), v_at(cur, sub), s_sk[full2 ? slot2 : Sh::RING] + (1 - sub) * 32,
+                                     s_sv[slot2] + (1 - sub) * 32};
+                turn(sub_tag, f, now, after, [&](auto step_tag) {
+                    constexpr int S = decltype(step_tag)::value;
+                    if constexpr (sub == 0) {  // the next tile but one into LDS
+                        if constexpr (S % 2 == 0 && S >= 4 && S / 2 - 2 < LOADS) store_rows(S / 2 - 2, third);
+                        else if constexpr (S == 15) store_scales(third);
+                    } else {  // the one after it on its way, and its successor's pages
+                        if constexpr (S % 2 == 0 && S / 2 < LOADS) load_rows(S / 2, i * TK + 3 * TK);
+                        else if constexpr (S == 10) load_scales(i * TK + 3 * TK);
+                        else if constexpr (S == 12) {
+                            valid[3] = held_valid;
+                            load_pages(i * TK + 4 * TK);
+                        }
+                    }
+                });
+                if (sub == 0 && i == 0) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                        for (int k = 0; k < 16; k++) o[dt][k] = 0.f;
+                }
+                now = after;
                 full = full2;
             });
-            const int was = cur;
-            cur = next, next = third, third = was;
+            valid[0] = valid[1], valid[1] = valid[2], valid[2] = valid[3];
             __syncthreads();
         }
+        // the last turn's values: its first three operands have been read
 #pragma unroll
-        for (int e = 0; e < 2 * DT; e++) o[1][e % DT] = mfma32<P>(vf[e / DT][e % DT], pf[1][e / DT], o[1][e % DT]);
-    }
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-        float ln = sum_half(l[n]), mn = m[n];
-        if (ln != ln && mn == -INFINITY) mn = 0.f;  // only NaN scores so far: not a row without keys
-        const uint32_t row = wave_row + n * 32 + col;
-        if (row >= t.rows) continue;
-        if (a.splits > 1) {
-            const uint64_t p = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * Sh::BM + wave * 64 + n * 32 + col;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<f32x4*>(a.part_o + p * DP + dt * 32 + 2 * i + 4 * half) =
-                        f32x4{o[n][dt][i], o[n][dt][i + 1], o[n][dt][i + 2], o[n][dt][i + 3]};
-            if (half == 0) a.part_m[p * 2] = mn, a.part_m[p * 2 + 1] = ln;
-            continue;
+        for (int e = 0; e < KS; e++) {
+            if (e + 3 < KS) read_v(e + 3, now.v);
+            o[e % DT] = mfma32<P>(vf[e % 4], pf[1][e / DT], o[e % DT]);
         }
-        const uint32_t token = t.token0 + row / a.group, head = kvh * a.group + row % a.group;
-        const float inv = mn == -INFINITY ? 0.f : 1.f / ln;
-        uint8_t* out = a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head) * 2;
+    }
+    l = sum_half(l);
+    if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+    if (row >= t.rows) return;
+    if (a.splits > 1) {
+        const uint64_t p = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * Sh::BM + wave * 32 + col;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const uint32_t d = dt * 32 + 2 * i + 4 * half;
-                if (d < a.dim)
-                    *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[n][dt][i] * inv, o[n][dt][i + 1] * inv),
-                                                                   pack16<X>(o[n][dt][i + 2] * inv, o[n][dt][i + 3] * inv)};
-            }
-        if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = mn == -INFINITY ? -INFINITY : (mn - Prob<C>::up + log2f(ln)) * kLn2;
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f32x4*>(a.part_o + p * DP + dt * 32 + 2 * i + 4 * half) = f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+        if (half == 0) a.part_m[p * 2] = m, a.part_m[p * 2 + 1] = l;
+        return;
     }
+    const uint32_t token = t.token0 + row / a.group, head = kvh * a.group + row % a.group;
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    uint8_t* out = a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head) * 2;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const uint32_t d = dt * 32 + 2 * i + 4 * half;
+            if (d < a.dim)
+                *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[dt][i] * inv, o[dt][i + 1] * inv), pack16<X>(o[dt][i + 2] * inv, o[dt][i + 3] * inv)};
+        }
+    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<C>::up + log2f(l)) * kLn2;
 }
 
 // ------------------------------------------------------------ the splits' join
@@ -1130,12 +1136,12 @@ uint64_t part_bytes(uint64_t rows, uint32_t dp, uint64_t* m_bytes) {
     return *m_bytes + rows * dp * 4;
 }
 Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t n_tokens, uint32_t max_chunk,
-        uint64_t max_context, uint32_t window) {
+        uint64_t max_context, uint32_t window, bool near_slots) {
     Cut c{};
     const uint64_t group = n_heads / n_kv;
     c.dp = padded_dim(dim);
     const uint64_t rows = (uint64_t)max_chunk * group;
-    c.bm = rows <= kFewRows ? kFewRows : rows <= kManyRows || c.dp == 256 ? kManyRows : kWideRows;
+    c.bm = rows <= kFewRows ? kFewRows : rows <= kManyRows || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
     c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
     // the keys of a tile: a window's, and as many again as the tile has tokens
     if (window) max_context = std::min<uint64_t>(max_context, (uint64_t)window + c.bm / group + 64);
@@ -1173,7 +1179,7 @@ hipError_t launch_attend(const AttnArg& a, const Cut& c, hipStream_t s) {
         CKR_LAUNCH("kv_attention_many", s, attend_many_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
         join(attend_join_kernel<X, DP, kManyRows>);
     } else if constexpr (DP <= 128) {
-        CKR_LAUNCH("kv_attention_wide", s, attend_wide_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
+        CKR_LAUNCH("kv_attention_wide", s, attend_wide_kernel<X, C, DP><<<grid, 512, 0, s>>>(a));
         join(attend_join_kernel<X, DP, kWideRows>);
     }
     return hipGetLastError();
@@ -1236,9 +1242,12 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
     a.scale2 = std::max(std::fabs(scale) * kLog2e, 0x1p-120f), a.flip = scale < 0.f ? 0x80008000u : 0u;
     a.b = {batch->d_page_table, batch->d_starts, batch->d_offsets, (int64_t)batch->table_stride, batch->table_width,
            batch->n_seqs, batch->n_tokens};
+    // the slots of a page within 32-bit offsets of each other, pages within 2^36 bytes
+    bool near_slots = true;
+    for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 28) - 16 && st[0] < (1ll << 36);
     const Cut c = cut(n_heads, cache->n_heads, cache->head_dim, batch->n_seqs, batch->n_tokens, batch->max_chunk,
-                      std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size), window);
-    if ((uint64_t)c.tiles * cache->n_heads * 256 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
+                      std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size), window, near_slots);
+    if ((uint64_t)c.tiles * cache->n_heads * 512 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
     a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len;
     if (c.bytes) {
         if (workspace_bytes < c.bytes)
