@@ -741,7 +741,8 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     __shared__ __attribute__((aligned(16))) float s_sv[Sh::RING][TK];
     __shared__ uint32_t s_tmp[16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
+    // a sequence's later tiles see more keys: they start first
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = a.tiles - 1 - blockIdx.x / a.kv_heads, split = blockIdx.y;
     Tile t;
     if (!find_tile<Sh::BM, 512>(a.b, a.group, tile, s_tmp, t)) return;
     const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + Sh::BM - 1, t.rows - 1) / a.group;
@@ -767,7 +768,6 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         if (row < t.rows && d < a.dim) {
             q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(t.token0 + row / a.group) * a.q_tok +
                                                           (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
-            q[ks] ^= a.flip;
         }
     }
     // staging.  A key of no mapped page is read from page 0 and then cleared (values)
@@ -781,7 +781,9 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     const uint32_t slot_mask = (1u << a.page_shift) - 1;
     const uint32_t st0 = (uint32_t)((stage_k ? a.kst[0] : a.vst[0]) >> 4), st2 = (uint32_t)((stage_k ? a.kst[2] : a.vst[2]) >> 4);
     const uint8_t* const from = stage_k ? a.ck + (int64_t)kvh * a.kst[1] : a.cv + (int64_t)kvh * a.vst[1];
-    const uint32_t from_lane = ((row_of & 15) * st2 + piece) * 16;
+    const uint32_t from_lane = ((row_of & 15) * st2 + piece) * 16, w4_rows = w4 * RPW / 16 * 16;
+    const float* const scale_k = a.sk + (int64_t)kvh * a.skst[1];
+    const float* const scale_v = a.sv + (int64_t)kvh * a.svst[1];
     uint8_t* const to = (stage_k ? s_k + row_of * KP : s_v + row_of * VP) + place * (C::bytes == 1 ? 32 : 16);
     const uint32_t to_rows = ROWS * (stage_k ? KP : VP), to_slot = TK * (stage_k ? KP : VP);
     const uint32_t c0 = (uint32_t)(lo >> a.page_shift), in0 = (uint32_t)lo & slot_mask, last_col = a.b.width - 1;
@@ -790,34 +792,47 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         const int32_t p = table[min(c0 + ((in0 + (uint32_t)j) >> a.page_shift), last_col)];
         return ((j < end) & ((uint32_t)p < a.n_pages)) ? p : -1;  // end lies within the table
     };
-    int32_t pg[4];         // of the tile that is loaded next
-    uint64_t valid[4];     // keys of mapped pages: of this tile, and of the next three
+    // a tile is part of one page, or of several small ones
+    const bool one_page = a.page_shift >= 6;
+    int32_t pg[4] = {-1, -1, -1, -1};  // of the tile that is loaded next (of all of it in pg[0])
+    uint64_t valid[4];  // keys of mapped pages: of this tile, and of the next three
     const auto load_pages = [&](int base) {
+        pg[0] = page_id(base);
+        if (!one_page) {
 #pragma unroll
-        for (int g = 0; g < 4; g++) pg[g] = page_id(base + 16 * g);
+            for (int g = 1; g < 4; g++) pg[g] = page_id(base + 16 * g);
+        }
     };
     const auto valid_of = [&](int base) {
+        if (one_page && pg[0] >= 0 && base + TK <= end) return ~0ull;
         uint64_t v = 0;
 #pragma unroll
-        for (int g = 0; g < 4; g++) v |= pg[g] >= 0 ? 0xffffull << (16 * g) : 0;
+        for (int g = 0; g < 4; g++) v |= pg[one_page ? 0 : g] >= 0 ? 0xffffull << (16 * g) : 0;
         return end - base >= TK ? v : end - base <= 0 ? 0 : v & ((1ull << (end - base)) - 1);
     };
     u32x4 held[LOADS];
     float sk = 0.f, sv = 0.f;
     uint64_t held_valid = 0;
-    const auto load_rows = [&](int u, int base) {
-        const uint32_t g = (w4 * RPW + u * ROWS) / 16;
-        const int32_t p = g == 0 ? pg[0] : g == 1 ? pg[1] : g == 2 ? pg[2] : pg[3];
-        const uint32_t slot = (in0 + (uint32_t)base + 16 * g) & slot_mask;
-        const uint64_t off = (uint64_t)(uint32_t)max(p, 0) * st0 + (uint64_t)slot * st2;
-        held[u] = *reinterpret_cast<const u32x4*>(from + off * 16 + from_lane);
-    };
-    const auto load_scales = [&](int base) {
+    const auto load_tile = [&](int base) {
+        if (one_page) {
+            const uint32_t p = (uint32_t)max(pg[0], 0), slot = (in0 + (uint32_t)base) & slot_mask;
+            const uint8_t* at = from + ((uint64_t)p * st0 + (uint64_t)slot * st2) * 16;
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) held[u] = *reinterpret_cast<const u32x4*>(at + (from_lane + (w4_rows + u * ROWS) * st2 * 16));
+        } else {
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                const uint32_t g = (w4 * RPW + u * ROWS) / 16;
+                const uint32_t p = (uint32_t)max(g == 0 ? pg[0] : g == 1 ? pg[1] : g == 2 ? pg[2] : pg[3], 0);
+                const uint32_t slot = (in0 + (uint32_t)base + 16 * g) & slot_mask;
+                held[u] = *reinterpret_cast<const u32x4*>(from + ((uint64_t)p * st0 + (uint64_t)slot * st2) * 16 + from_lane);
+            }
+        }
         if constexpr (C::bytes == 1) {
-            const int32_t p = max(w4 == 0 ? pg[0] : w4 == 1 ? pg[1] : w4 == 2 ? pg[2] : pg[3], 0);
+            const int32_t p = max(one_page || w4 == 0 ? pg[0] : w4 == 1 ? pg[1] : w4 == 2 ? pg[2] : pg[3], 0);
             const uint32_t slot = (in0 + (uint32_t)base + 16 * w4) & slot_mask;
-            sk = (a.sk + ((int64_t)p * a.skst[0] + (int64_t)kvh * a.skst[1] + slot))[lane & 15];
-            sv = (a.sv + ((int64_t)p * a.svst[0] + (int64_t)kvh * a.svst[1] + slot))[lane & 15];
+            sk = (scale_k + ((int64_t)p * a.skst[0] + slot))[lane & 15];
+            sv = (scale_v + ((int64_t)p * a.svst[0] + slot))[lane & 15];
         }
         held_valid = valid_of(base);
     };
@@ -984,19 +999,38 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
 
     if (n_tiles > 0) {
         if (wave == 0) s_sk[Sh::RING][lane] = 1.f;
+        // the first three tiles: their pages, then their rows, all on their way at once
+        int32_t pages[3][4];
 #pragma unroll
         for (int i = 0; i < 3; i++) {
             load_pages(i * TK);
-            valid[i] = valid_of(i * TK);
 #pragma unroll
-            for (int u = 0; u < LOADS; u++) load_rows(u, i * TK);
-            load_scales(i * TK);
-            if (i < 2) {
-#pragma unroll
-                for (int u = 0; u < LOADS; u++) store_rows(u, i);
-                store_scales(i);
-            }
+            for (int g = 0; g < 4; g++) pages[i][g] = pg[g];
         }
+        u32x4 rows[3][LOADS];
+        float scales[3][2];
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) pg[g] = pages[i][g];
+            load_tile(i * TK);
+            valid[i] = held_valid;
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) rows[i][u] = held[u];
+            scales[i][0] = sk, scales[i][1] = sv;
+        }
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) held[u] = rows[i][u];
+            sk = scales[i][0], sv = scales[i][1], held_valid = valid[i];
+            if (i == 2) break;
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) store_rows(u, i);
+            store_scales(i);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) q[ks] ^= a.flip;
         load_pages(3 * TK);
         __syncthreads();
         const auto full_at = [&](uint64_t v, int base) {
@@ -1033,9 +1067,8 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                         if constexpr (S % 2 == 0 && S >= 4 && S / 2 - 2 < LOADS) store_rows(S / 2 - 2, third);
                         else if constexpr (S == 15) store_scales(third);
                     } else {  // the one after it on its way, and its successor's pages
-                        if constexpr (S % 2 == 0 && S / 2 < LOADS) load_rows(S / 2, i * TK + 3 * TK);
-                        else if constexpr (S == 10) load_scales(i * TK + 3 * TK);
-                        else if constexpr (S == 12) {
+                        if constexpr (S == 0) load_tile(i * TK + 3 * TK);
+                        else if constexpr (S == 4) {
                             valid[3] = held_valid;
                             load_pages(i * TK + 4 * TK);
                         }
@@ -1244,7 +1277,7 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
            batch->n_seqs, batch->n_tokens};
     // the slots of a page within 32-bit offsets of each other, pages within 2^36 bytes
     bool near_slots = true;
-    for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 28) - 16 && st[0] < (1ll << 36);
+    for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 26) - 16 && st[0] < (1ll << 36);
     const Cut c = cut(n_heads, cache->n_heads, cache->head_dim, batch->n_seqs, batch->n_tokens, batch->max_chunk,
                       std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size), window, near_slots);
     if ((uint64_t)c.tiles * cache->n_heads * 512 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
