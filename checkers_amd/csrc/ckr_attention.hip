@@ -741,8 +741,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     __shared__ __attribute__((aligned(16))) float s_sv[Sh::RING][TK];
     __shared__ uint32_t s_tmp[16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-    // a sequence's later tiles see more keys: they start first
-    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = a.tiles - 1 - blockIdx.x / a.kv_heads, split = blockIdx.y;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
     Tile t;
     if (!find_tile<Sh::BM, 512>(a.b, a.group, tile, s_tmp, t)) return;
     const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + Sh::BM - 1, t.rows - 1) / a.group;
@@ -797,14 +796,27 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     int32_t pg[4] = {-1, -1, -1, -1};  // of the tile that is loaded next (of all of it in pg[0])
     uint64_t valid[4];  // keys of mapped pages: of this tile, and of the next three
     const auto load_pages = [&](int base) {
-        pg[0] = page_id(base);
-        if (!one_page) {
+        if (one_page) {
+            pg[0] = page_id(base);
+            return;
+        }
+        // pages of 16 or 32 slots: the tile starts with one, four columns from it on hold its pages
+        const uint32_t c = c0 + ((uint32_t)base >> a.page_shift);
+        if (base + TK <= end && c + 3 <= last_col) {
+            const int32_t p[4] = {table[c], table[c + 1], table[c + 2], table[c + 3]};
+            const bool small = a.page_shift == 4;
 #pragma unroll
-            for (int g = 1; g < 4; g++) pg[g] = page_id(base + 16 * g);
+            for (int g = 0; g < 4; g++) {
+                const int32_t x = small ? p[g] : p[g / 2];
+                pg[g] = (uint32_t)x < a.n_pages ? x : -1;
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; g++) pg[g] = page_id(base + 16 * g);
         }
     };
     const auto valid_of = [&](int base) {
-        if (one_page && pg[0] >= 0 && base + TK <= end) return ~0ull;
+        if (base + TK <= end && (one_page ? pg[0] : pg[0] | pg[1] | pg[2] | pg[3]) >= 0) return ~0ull;
         uint64_t v = 0;
 #pragma unroll
         for (int g = 0; g < 4; g++) v |= pg[one_page ? 0 : g] >= 0 ? 0xffffull << (16 * g) : 0;
