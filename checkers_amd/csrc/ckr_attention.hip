@@ -38,6 +38,9 @@ struct AttnArg {
     uint32_t flip;  // 0x80008000 when scale is negative: the queries' signs are flipped instead
     KvBatch b;
     uint32_t tiles, splits, split_len;  // row tiles, key ranges of a tile, their length (a multiple of 128)
+    uint32_t* counters;  // few rows: parts of an item that are done, 0 between calls
+    uint32_t items;      // few rows: counters (offsets that ask for more are not a batch)
+    uint32_t min_tiles;  // few rows: tiles of a wave's stretch at least
     float* part_o;  // [tile][kv head][split][rows of a tile][DP], with splits > 1
     float* part_m;  // [tile][kv head][split][rows of a tile][2]: maximum (in powers of two), sum
 };
@@ -104,6 +107,9 @@ template <> struct Prob<ElemF16> { typedef ElemF16 E; static constexpr float up 
 // accumulators are scaled: sums and outputs use the same lagging maximum.
 constexpr float kLag = 8.f;
 
+constexpr uint32_t kFewRows = 16, kManyRows = 128, kWideRows = 256;  // rows of a tile
+constexpr uint32_t kFewWaves = 4;                                    // waves of a block of few rows
+
 // f(0) .. f(N - 1) with constants.
 template <typename F, int... I> __device__ __forceinline__ void unroll_list(F f, std::integer_sequence<int, I...>) {
     (f(std::integral_constant<int, I>{}), ...);
@@ -160,7 +166,7 @@ __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint
 }
 
 // ------------------------------------------------------------ few rows
-// A wave takes tiles of 32 keys against 16 rows (16x16x32 matrix products):
+// A tile of 16 rows against tiles of 32 keys (16x16x32 matrix products), a wave at a time:
 //   S^T = K Q^T: operand A holds a key per lane and row, so a lane reads whole
 //   16-byte pieces of its key's row; the order of the contraction is free, and Q
 //   is laid out to match;
@@ -169,7 +175,16 @@ __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint
 //   exchange between lanes; V's operand holds those keys for one dimension, which
 //   a lane gets by loading NV = DP / 16 dimensions of 8 keys and transposing them in
 //   registers.
-// So nothing goes through LDS but the join of the block's four waves.
+// So no key or value goes through LDS, and two tiles (16 KiB of an 8-bit cache of 128
+// dimensions) are on their way per wave: a tile's registers are loaded again as
+// soon as they have been used.
+//
+// The work of all items (a row tile and a key/value head) is one line of key tiles,
+// of which every block takes an equal stretch, whatever the sequences' lengths; its
+// four waves share each item's tiles and join their sums through LDS.  A stretch
+// that covers an item writes its rows; otherwise the block leaves its part (maximum,
+// sum, weighted values) in the workspace, and the last block of an item's to finish
+// joins the parts, in an order that does not depend on which one that is.
 template <typename C, int DP> struct FewRegs {
     static constexpr int KL = DP * C::bytes / 64;      // 16-byte pieces of a key's row per lane
     static constexpr int VD = DP / 16 * C::bytes / 4;  // dwords of a key's value row per lane
@@ -178,254 +193,471 @@ template <typename C, int DP> struct FewRegs {
     f32x4 sk[2], sv[2];
 };
 
+// Parts of an item go from one CU to another, perhaps on another die: their stores
+// write through and their loads read past the caches (accesses of device scope), so
+// that no cache has to be written back or emptied for them.
+__device__ __forceinline__ void store_far(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), (uint64_t)as_u32(y) << 32 | as_u32(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 load_far(const float* p) {
+    const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return f32x2{as_f32((uint32_t)x), as_f32((uint32_t)(x >> 32))};
+}
+
+// Keys of a row tile: tiles of 32 from `first` on, up to `limit`.
+struct FewSpan { int64_t pos_lo, pos_hi, first, limit; };
+__device__ __forceinline__ FewSpan few_span(const AttnArg& a, int64_t start, uint32_t row0, uint32_t rows) {
+    FewSpan f;
+    f.pos_lo = start + row0 / a.group, f.pos_hi = start + min(row0 + kFewRows - 1, rows - 1) / a.group;
+    f.limit = min(f.pos_hi + 1, (int64_t)a.b.width << a.page_shift);
+    f.first = a.window ? max((int64_t)0, f.pos_lo - (int64_t)a.window + 1) & ~31ll : 0;
+    return f;
+}
+__device__ __forceinline__ uint32_t few_tiles(const FewSpan& f) {  // one at least: a row without keys is written too
+    return f.limit > f.first + 32 ? (uint32_t)((f.limit - f.first + 31) / 32) : 1u;
+}
 template <typename X, typename C, int DP>
-__global__ void __launch_bounds__(256, (DP * C::bytes > 256 ? 1 : 2)) attend_few_kernel(AttnArg a) {
+__global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few_kernel(AttnArg a) {
     typedef typename Prob<C>::E P;
     typedef FewRegs<C, DP> Regs;
     constexpr int KL = Regs::KL, VD = Regs::VD, NV = DP / 16, KS = DP / 32;
-    __shared__ float s_o[4][16][DP + 4];
-    __shared__ float s_m[4][16][2];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
-    Tile t;
-    if (!find_tile<16>(a.b, a.group, tile, reinterpret_cast<uint32_t*>(s_m), t)) return;
-    __syncthreads();
-    // the keys that some row of the tile sees, this split's part of them, this wave's
-    const uint32_t row = t.row0 + col, last_row = min(t.row0 + 15, t.rows - 1);
-    const int64_t pos = t.start + min(row, t.rows - 1) / a.group;
-    const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + last_row / a.group;
-    const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
-    const int64_t first = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) & ~31ll : 0;
-    const int64_t see = a.window ? pos - (int64_t)a.window : -1;  // a row sees keys above this
-    int64_t lo = first + (int64_t)split * a.split_len, hi = split + 1 == a.splits ? limit : min(limit, lo + (int64_t)a.split_len);
-    const int64_t n_tiles = hi > lo ? (hi - lo + 31) / 32 : 0, per = (n_tiles + 3) / 4;
-    const int64_t t0 = lo + 32 * min(n_tiles, per * wave), t1 = lo + 32 * min(n_tiles, per * (wave + 1));
+    constexpr uint32_t THREADS = 64 * kFewWaves, QUADS = DP / 4;  // a row's outputs by fours
+    __shared__ __attribute__((aligned(16))) float s_o[kFewWaves][kFewRows][DP + 4];
+    __shared__ float s_m[kFewWaves][kFewRows][2];
+    __shared__ uint32_t s_sum[kFewWaves][2];
+    __shared__ uint32_t s_at[6];  // the block's first sequence, tiles of it before the block's, its first item; its rows, token, start
+    __shared__ uint32_t s_last;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
 
-    // queries: the elements of each 32-wide step in the order of the keys' pieces
-    u32x4 q[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-        const uint32_t d = C::bytes == 1 ? (ks / 2) * 64 + g * 16 + (ks % 2) * 8 : ks * 32 + g * 8;
-        q[ks] = u32x4{0, 0, 0, 0};
-        if (row < t.rows && d < a.dim) {
-            q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(t.token0 + row / a.group) * a.q_tok +
-                                                          (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
-            q[ks] ^= a.flip;
-        }
-    }
-    const int64_t k_off = (int64_t)col * a.kst[2] + g * 16, v_off = (int64_t)(4 * g) * a.vst[2] + col * (VD * 4);
-    const bool v_in = col * NV < a.dim;
-    const int32_t* table = a.b.table + (int64_t)t.seq * a.b.table_stride;
-    const auto page_lane = [&](int64_t c0) {  // lane i: the page of table column c0 + i
-        const int64_t c = c0 + lane;
-        const int32_t p = c < (int64_t)a.b.width ? table[c] : -1;
-        return (uint32_t)p < a.n_pages ? p : -1;
+    // ---- this block's stretch of the line of key tiles (the launch has seen to it
+    // that the line is shorter than 2^31)
+    struct Seq { uint32_t tiles, items, rows, token0; int32_t start; };
+    const auto count = [&](uint32_t seq) {
+        Seq q = {0, 0, 0, 0, 0};
+        if (seq >= a.b.n_seqs) return q;
+        const int32_t from = a.b.offsets[seq], to = a.b.offsets[seq + 1];
+        q.start = a.b.starts[seq];
+        q.rows = from >= 0 && min(to, (int32_t)a.b.n_tokens) > from ? (uint32_t)(min(to, (int32_t)a.b.n_tokens) - from) * a.group : 0;
+        q.token0 = (uint32_t)from;
+        for (uint32_t r = 0; r < q.rows; r += kFewRows) q.tiles += few_tiles(few_span(a, q.start, r, q.rows)), q.items++;
+        q.tiles *= a.kv_heads, q.items *= a.kv_heads;
+        return q;
     };
-    const auto load = [&](Regs& r, int64_t base, int32_t p0, int32_t p1) {
-        const uint32_t mask = (1u << a.page_shift) - 1;
-        const bool whole = p0 >= 0 && p1 >= 0 && base + 32 <= limit && DP == a.dim;
+    // inclusive sums over the block's threads, and the block's totals
+    const auto scan = [&](uint32_t& tiles, uint32_t& items, uint32_t& all_tiles, uint32_t& all_items) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int32_t page = h ? p1 : p0;
-            const int64_t slot = ((uint32_t)base + 16 * h) & mask;
-            const uint8_t* kp = a.ck + (int64_t)page * a.kst[0] + (int64_t)kvh * a.kst[1] + slot * a.kst[2] + k_off;
-            const uint8_t* vp = a.cv + (int64_t)page * a.vst[0] + (int64_t)kvh * a.vst[1] + slot * a.vst[2] + v_off;
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t x = (uint32_t)__shfl_up((int)tiles, d), y = (uint32_t)__shfl_up((int)items, d);
+            if (lane >= (uint32_t)d) tiles += x, items += y;
+        }
+        __syncthreads();
+        if (lane == 63) s_sum[wave][0] = tiles, s_sum[wave][1] = items;
+        __syncthreads();
+        all_tiles = all_items = 0;
 #pragma unroll
-            for (int j = 0; j < KL; j++) {
-                r.k[h][j] = u32x4{0, 0, 0, 0};
-                if (whole || (page >= 0 && base + 16 * h + col < limit && (j * 64 + g * 16) / C::bytes < a.dim))
-                    r.k[h][j] = *reinterpret_cast<const u32x4*>(kp + j * 64);
+        for (uint32_t w = 0; w < kFewWaves; w++) {
+            if (w == wave) tiles += all_tiles, items += all_items;
+            all_tiles += s_sum[w][0], all_items += s_sum[w][1];
+        }
+    };
+    const Seq q0 = count(threadIdx.x);
+    uint32_t incl = q0.tiles, incl_items = q0.items, total, items;
+    scan(incl, incl_items, total, items);
+    const uint32_t first_total = total, first_items = items;
+    for (uint32_t base = THREADS; base < a.b.n_seqs; base += THREADS) {
+        const Seq x = count(base + threadIdx.x);
+        uint32_t n = x.tiles, it = x.items, more, more_items;
+        scan(n, it, more, more_items);
+        total += more, items += more_items;
+    }
+    if (items > a.items) return;
+    const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, a.min_tiles);
+    if ((uint64_t)blockIdx.x * per >= total) return;
+    const uint32_t p_begin = blockIdx.x * per, p_end = min(p_begin + per, total);
+    {
+        const auto find = [&](uint32_t seq, const Seq& x, uint32_t upto, uint32_t upto_items) {
+            if (p_begin >= upto - x.tiles && p_begin < upto) {
+                s_at[0] = seq, s_at[1] = p_begin - (upto - x.tiles), s_at[2] = upto_items - x.items;
+                s_at[3] = x.rows, s_at[4] = x.token0, s_at[5] = (uint32_t)x.start;
             }
+        };
+        find(threadIdx.x, q0, incl, incl_items);
+        uint32_t before = first_total, before_items = first_items;
+        for (uint32_t base = THREADS; base < a.b.n_seqs; base += THREADS) {
+            const Seq x = count(base + threadIdx.x);
+            uint32_t n = x.tiles, it = x.items, more, more_items;
+            scan(n, it, more, more_items);
+            find(base + threadIdx.x, x, before + n, before_items + it);
+            before += more, before_items += more_items;
+        }
+        __syncthreads();
+    }
+    const auto scalar = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); };
+    uint32_t seq = scalar(s_at[0]), in_seq = scalar(s_at[1]), item0 = scalar(s_at[2]), rows = scalar(s_at[3]), token0 = scalar(s_at[4]), row0 = 0;
+    int32_t start = (int32_t)scalar(s_at[5]);
+    // the item that the stretch begins in
+    FewSpan span = few_span(a, start, 0, rows);
+    uint32_t nt = few_tiles(span);
+    while (in_seq >= nt * a.kv_heads) {
+        in_seq -= nt * a.kv_heads, row0 += kFewRows, item0 += a.kv_heads;
+        span = few_span(a, start, row0, rows), nt = few_tiles(span);
+    }
+    uint32_t kvh = scalar(in_seq / nt), t0 = scalar(in_seq % nt);
+
+    for (uint32_t p = p_begin; p < p_end;) {
+        const uint32_t t1 = scalar(min(nt, t0 + (p_end - p)));
+        // the waves share the item's tiles (or this block's part of them) evenly
+        const uint32_t w0 = (uint32_t)((uint64_t)(t1 - t0) * wave / kFewWaves), w1 = (uint32_t)((uint64_t)(t1 - t0) * (wave + 1) / kFewWaves);
+        const int64_t lo = span.first + 32ll * (t0 + w0);
+        const int n_tiles = w1 - w0;
+        // from here on keys are counted from lo, in 32 bits
+        const auto rel = [&](int64_t x) { return (int)max((int64_t)-0x40000000, min(x - lo, (int64_t)0x7fffffff - 256)); };
+        const uint32_t row = row0 + col;
+        const int64_t my_pos = span.pos_lo - row0 / a.group + min(row, rows - 1) / a.group;
+        const int pos = rel(my_pos), see = a.window ? rel(my_pos - (int64_t)a.window) : -0x40000000;
+        const int end = __builtin_amdgcn_readfirstlane(rel(span.limit));
+        const int full_to = __builtin_amdgcn_readfirstlane(min(rel(span.pos_lo) + 1, end));  // every row sees the keys before this
+        const int full_from = __builtin_amdgcn_readfirstlane(a.window ? rel(span.pos_hi - (int64_t)a.window) + 1 : -0x40000000);  // and from this on
+
+        // queries: the elements of each 32-wide step in the order of the keys' pieces
+        u32x4 q[KS];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t* x = reinterpret_cast<const uint32_t*>(vp + i * a.vst[2]);
-                const bool in = whole || (page >= 0 && base + 16 * h + 4 * g + i < limit && v_in);
+        for (int ks = 0; ks < KS; ks++) {
+            const uint32_t d = C::bytes == 1 ? (ks / 2) * 64 + g * 16 + (ks % 2) * 8 : ks * 32 + g * 8;
+            q[ks] = u32x4{0, 0, 0, 0};
+            if (row < rows && d < a.dim)
+                q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(token0 + row / a.group) * a.q_tok +
+                                                              (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
+        }
+        const uint8_t* const ck = a.ck + (int64_t)kvh * a.kst[1];
+        const uint8_t* const cv = a.cv + (int64_t)kvh * a.vst[1];
+        const float* const skp = a.sk + (int64_t)kvh * a.skst[1];
+        const float* const svp = a.sv + (int64_t)kvh * a.svst[1];
+        const int64_t k_off = (int64_t)col * a.kst[2] + g * 16;
+        int64_t v_off[4];
 #pragma unroll
-                for (int j = 0; j < VD; j++) r.v[4 * h + i][j] = 0;
-                if (in) {
-                    if constexpr (VD == 1) r.v[4 * h + i][0] = *x;
-                    else if constexpr (VD == 2) {
-                        const u32x2 y = *reinterpret_cast<const u32x2*>(x);
-                        r.v[4 * h + i][0] = y[0], r.v[4 * h + i][1] = y[1];
-                    } else {
+        for (int i = 0; i < 4; i++) v_off[i] = (int64_t)(4 * g + i) * a.vst[2] + col * (VD * 4);
+        const bool v_in = col * NV < a.dim;
+        typedef __attribute__((address_space(1))) const int32_t* global_i32;
+        const global_i32 table = (global_i32)(a.b.table + (int64_t)seq * a.b.table_stride);
+        const uint32_t slot_mask = (1u << a.page_shift) - 1, in0 = (uint32_t)lo & slot_mask;
+        // table columns c0 .. c0 + 63 in a register of the wave, the next 64 on their way
+        uint32_t c0 = (uint32_t)(lo >> a.page_shift);
+        const auto page_lane = [&](uint32_t c) {
+            c += lane;
+            const int32_t x = c < a.b.width ? table[c] : -1;
+            return (uint32_t)x < a.n_pages ? x : -1;
+        };
+        int32_t window_now = page_lane(c0), window_next = page_lane(c0 + 64);
+        uint32_t c_now = 0;
+        const auto page_at = [&](int j) {  // of key j; called with j rising by 16
+            const uint32_t c = (in0 + (uint32_t)j) >> a.page_shift;
+            if (c - c_now >= 64) {
+                c_now += 64;
+                window_now = window_next;
+                window_next = page_lane(c0 + c_now + 64);
+            }
+            return (int32_t)__builtin_amdgcn_readlane(window_now, (int)(c - c_now));
+        };
+        const auto load_k = [&](Regs& r, int base, const int32_t* pages) {
+            const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
 #pragma unroll
-                        for (int j = 0; j < VD; j += 4) {
-                            const u32x4 y = *reinterpret_cast<const u32x4*>(x + j);
+            for (int h = 0; h < 2; h++) {
+                const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
+                const uint8_t* at = ck + (int64_t)pages[h] * a.kst[0] + (int64_t)slot * a.kst[2] + k_off;
+                if (whole) {
 #pragma unroll
-                            for (int k = 0; k < 4; k++) r.v[4 * h + i][j + k] = y[k];
-                        }
+                    for (int j = 0; j < KL; j++) r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < KL; j++) {
+                        r.k[h][j] = u32x4{0, 0, 0, 0};
+                        if (pages[h] >= 0 && base + 16 * h + (int)col < end && (j * 64 + g * 16) / C::bytes < a.dim)
+                            r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
+                    }
+                }
+                if constexpr (C::bytes == 1) {
+                    const int64_t x = max(pages[h], 0);
+                    r.sk[h] = *reinterpret_cast<const f32x4*>(skp + x * a.skst[0] + slot + 4 * g);
+                    r.sv[h] = *reinterpret_cast<const f32x4*>(svp + x * a.svst[0] + slot + 4 * g);
+                }
+            }
+        };
+        const auto load_v = [&](Regs& r, int base, const int32_t* pages) {
+            const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
+            const auto get = [&](uint32_t (&v)[VD], const uint8_t* at) {
+                if constexpr (VD == 1) v[0] = *reinterpret_cast<const uint32_t*>(at);
+                else if constexpr (VD == 2) {
+                    const u32x2 y = *reinterpret_cast<const u32x2*>(at);
+                    v[0] = y[0], v[1] = y[1];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VD; j += 4) {
+                        const u32x4 y = *reinterpret_cast<const u32x4*>(at + j * 4);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) v[j + k] = y[k];
+                    }
+                }
+            };
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
+                const uint8_t* at = cv + (int64_t)pages[h] * a.vst[0] + (int64_t)slot * a.vst[2];
+                if (whole) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) get(r.v[4 * h + i], at + v_off[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+#pragma unroll
+                        for (int j = 0; j < VD; j++) r.v[4 * h + i][j] = 0;
+                        if (pages[h] >= 0 && base + 16 * h + 4 * (int)g + i < end && v_in) get(r.v[4 * h + i], at + v_off[i]);
                     }
                 }
             }
-            if constexpr (C::bytes == 1) {
-                r.sk[h] = r.sv[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (page >= 0) {
-                    r.sk[h] = *reinterpret_cast<const f32x4*>(a.sk + (int64_t)page * a.skst[0] + (int64_t)kvh * a.skst[1] + slot + 4 * g);
-                    r.sv[h] = *reinterpret_cast<const f32x4*>(a.sv + (int64_t)page * a.svst[0] + (int64_t)kvh * a.svst[1] + slot + 4 * g);
-                }
-            }
-        }
-    };
+        };
 
-    float m = -INFINITY, l = 0.f;
-    f32x4 o[NV];
+        float m = -INFINITY, l = 0.f;
+        f32x4 o[NV];
 #pragma unroll
-    for (int c = 0; c < NV; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const auto compute = [&](const Regs& r, int64_t base, int32_t p0, int32_t p1) {
-        f32x4 s[2];
+        for (int c = 0; c < NV; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const auto scores = [&](const Regs& r, f32x4 (&s)[2]) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < 2; h++) {
+                s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < KL; j++) {
-                if constexpr (C::bytes == 1) {
-                    const u32x4 x = r.k[h][j];
-                    const u32x2 w0 = widen4<C, X>(x[0]), w1 = widen4<C, X>(x[1]), w2 = widen4<C, X>(x[2]), w3 = widen4<C, X>(x[3]);
-                    s[h] = mfma16<X>(u32x4{w0[0], w0[1], w1[0], w1[1]}, q[2 * j], s[h]);
-                    s[h] = mfma16<X>(u32x4{w2[0], w2[1], w3[0], w3[1]}, q[2 * j + 1], s[h]);
-                } else {
-                    s[h] = mfma16<X>(r.k[h][j], q[j], s[h]);
+                for (int j = 0; j < KL; j++) {
+                    if constexpr (C::bytes == 1) {
+                        const u32x4 x = r.k[h][j];
+                        const u32x2 w0 = widen4<C, X>(x[0]), w1 = widen4<C, X>(x[1]), w2 = widen4<C, X>(x[2]), w3 = widen4<C, X>(x[3]);
+                        s[h] = mfma16<X>(u32x4{w0[0], w0[1], w1[0], w1[1]}, q[2 * j], s[h]);
+                        s[h] = mfma16<X>(u32x4{w2[0], w2[1], w3[0], w3[1]}, q[2 * j + 1], s[h]);
+                    } else {
+                        s[h] = mfma16<X>(r.k[h][j], q[j], s[h]);
+                    }
                 }
             }
-        }
-        // every row sees every key of the tile, or not
-        const bool full = p0 >= 0 && p1 >= 0 && base + 31 <= pos_lo && base + 32 <= limit &&
-                          (!a.window || base > pos_hi - (int64_t)a.window);
-        uint32_t seen = 0xffu;
-        if (!full) {
-            seen = 0;
+        };
+        // the weights of a tile, with the values' scales; what a row does not see weighs 0
+        const auto weights = [&](const Regs& r, const f32x4 (&s)[2], int base, const int32_t* pages) {
+            const bool full = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= full_to && base >= full_from;
+            float x[8], top = -INFINITY;
+            uint32_t seen = 0xffu;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const int64_t j = base + 16 * (i / 4) + 4 * g + i % 4;
-                if ((i < 4 ? p0 : p1) >= 0 && j <= pos && j > see && j < limit) seen |= 1u << i;
+                x[i] = s[i / 4][i % 4] * a.scale2;
+                if constexpr (C::bytes == 1) x[i] *= r.sk[i / 4][i % 4];
             }
-        }
-        float x[8], top = -INFINITY;
+            if (!full) {
+                seen = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[i] = s[i / 4][i % 4] * a.scale2;
-            if constexpr (C::bytes == 1) x[i] *= r.sk[i / 4][i % 4];
-            if (!full) x[i] = seen >> i & 1 ? x[i] : -INFINITY;
-            top = fmaxf(top, x[i]);
-        }
-        top = max_quarters(top);
-        if (__any(top > m + kLag)) {
-            const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
-            m = m2;
-            l *= back;
-#pragma unroll
-            for (int c = 0; c < NV; c++) o[c] *= back;
-        }
-        const float ref = m == -INFINITY ? 0.f : m - Prob<C>::up;
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            p[i] = exp2_fast(x[i] - ref);
-            l += p[i];
-            if constexpr (C::bytes == 1) p[i] *= r.sv[i / 4][i % 4];
-            if (!full) p[i] = seen >> i & 1 ? p[i] : 0.f;
-        }
-        const u32x4 pf = {pack16<P>(p[0], p[1]), pack16<P>(p[2], p[3]), pack16<P>(p[4], p[5]), pack16<P>(p[6], p[7])};
-        if constexpr (C::bytes == 1) {
-#pragma unroll
-            for (int j = 0; j < VD; j++) {  // four dimensions of eight keys
-                uint32_t w[2][4];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t a0 = r.v[4 * h][j], a1 = r.v[4 * h + 1][j], a2 = r.v[4 * h + 2][j], a3 = r.v[4 * h + 3][j];
-                    const uint32_t x0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), x1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
-                    const uint32_t y0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), y1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
-                    w[h][0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u);
-                    w[h][1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
-                    w[h][2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u);
-                    w[h][3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const u32x2 w0 = widen4<C, P>(w[0][k]), w1 = widen4<C, P>(w[1][k]);
-                    o[4 * j + k] = mfma16<P>(u32x4{w0[0], w0[1], w1[0], w1[1]}, pf, o[4 * j + k]);
+                for (int i = 0; i < 8; i++) {
+                    const int j = base + 16 * (i / 4) + 4 * (int)g + i % 4;
+                    if (pages[i / 4] >= 0 && j <= pos && j > see && j < end) seen |= 1u << i;
+                    x[i] = seen >> i & 1 ? x[i] : -INFINITY;
                 }
             }
-        } else {
 #pragma unroll
-            for (int j = 0; j < VD; j++) {  // two dimensions of eight keys
-                u32x4 w0, w1;
+            for (int i = 0; i < 8; i++) top = fmaxf(top, x[i]);
+            if (__any(top > m + kLag)) {
+                top = max_quarters(top);
+                const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
+                m = m2;
+                l *= back;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
-                    w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
-                }
-                o[2 * j] = mfma16<P>(w0, pf, o[2 * j]);
-                o[2 * j + 1] = mfma16<P>(w1, pf, o[2 * j + 1]);
+                for (int c = 0; c < NV; c++) o[c] *= back;
             }
-        }
-    };
-
-    if (t0 < t1) {
-        // table columns c0 .. c0 + 63 in a register of the wave, the next 64 on their way
-        int64_t c0 = t0 >> a.page_shift;
-        int32_t now = page_lane(c0), next = page_lane(c0 + 64);
-        const auto page_at = [&](int64_t base) {
-            int64_t c = base >> a.page_shift;
-            if (c - c0 >= 64) {
-                c0 += 64;
-                now = next;
-                next = page_lane(c0 + 64);
+            const float ref = m == -INFINITY ? 0.f : m - Prob<C>::up;
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w[i] = exp2_fast(x[i] - ref);
+                l += w[i];
+                if constexpr (C::bytes == 1) w[i] *= r.sv[i / 4][i % 4];
             }
-            return (int32_t)__builtin_amdgcn_readlane(now, (int)(c - c0));
+            if (C::bytes == 1 && !full) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i] = seen >> i & 1 ? w[i] : 0.f;  // a scale may be NaN there
+            }
+            return u32x4{pack16<P>(w[0], w[1]), pack16<P>(w[2], w[3]), pack16<P>(w[4], w[5]), pack16<P>(w[6], w[7])};
         };
+        const auto gather = [&](const Regs& r, u32x4 pf) {
+            if constexpr (C::bytes == 1) {
+#pragma unroll
+                for (int j = 0; j < VD; j++) {  // four dimensions of eight keys
+                    uint32_t w[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t a0 = r.v[4 * h][j], a1 = r.v[4 * h + 1][j], a2 = r.v[4 * h + 2][j], a3 = r.v[4 * h + 3][j];
+                        const uint32_t x0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), x1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
+                        const uint32_t y0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), y1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+                        w[h][0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u);
+                        w[h][1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
+                        w[h][2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u);
+                        w[h][3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const u32x2 w0 = widen4<C, P>(w[0][k]), w1 = widen4<C, P>(w[1][k]);
+                        o[4 * j + k] = mfma16<P>(u32x4{w0[0], w0[1], w1[0], w1[1]}, pf, o[4 * j + k]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VD; j++) {  // two dimensions of eight keys
+                    u32x4 w0, w1;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
+                        w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
+                    }
+                    o[2 * j] = mfma16<P>(w0, pf, o[2 * j]);
+                    o[2 * j + 1] = mfma16<P>(w1, pf, o[2 * j + 1]);
+                }
+            }
+        };
+
         Regs r[2];
-        int32_t p[2][2];
-        p[0][0] = page_at(t0), p[0][1] = page_at(t0 + 16);
-        load(r[0], t0, p[0][0], p[0][1]);
-        for (int64_t base = t0; base < t1; base += 64) {
+        int32_t pages[2][2], coming[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (u < n_tiles) {
+                pages[u][0] = page_at(32 * u), pages[u][1] = page_at(32 * u + 16);
+                load_k(r[u], 32 * u, pages[u]);
+                load_v(r[u], 32 * u, pages[u]);
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) q[ks] ^= a.flip;
+        for (int i = 0; i < n_tiles; i += 2) {
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const int64_t at = base + 32 * u;
-                if (at >= t1) break;
-                if (at + 32 < t1) {
-                    p[1 - u][0] = page_at(at + 32), p[1 - u][1] = page_at(at + 48);
-                    load(r[1 - u], at + 32, p[1 - u][0], p[1 - u][1]);
+                if (i + u >= n_tiles) break;
+                const int base = 32 * (i + u);
+                const bool more = i + u + 2 < n_tiles;
+                f32x4 s[2];
+                scores(r[u], s);
+                const u32x4 pf = weights(r[u], s, base, pages[u]);
+                if (more) {  // its keys' registers again, for the tile after the next
+                    coming[0] = page_at(base + 64), coming[1] = page_at(base + 80);
+                    load_k(r[u], base + 64, coming);
                 }
-                compute(r[u], at, p[u][0], p[u][1]);
+                gather(r[u], pf);
+                if (more) {
+                    pages[u][0] = coming[0], pages[u][1] = coming[1];
+                    load_v(r[u], base + 64, pages[u]);
+                }
             }
         }
-    }
-    // join the four waves: lane (col, g) holds dimensions 4 g NV .. 4 (g + 1) NV of row col
-    l = sum_quarters(l);
-    if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+        // ---- join: lane (col, g) holds dimensions 4 g NV .. 4 (g + 1) NV of row col
+        l = sum_quarters(l);
+        if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+        __syncthreads();                        // the last item's sums have been read
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int c = 0; c < NV; c++) s_o[wave][col][(4 * g + i) * NV + c] = o[c][i];
-    if (g == 0) s_m[wave][col][0] = m, s_m[wave][col][1] = l;
-    __syncthreads();
-    const uint64_t part = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * 16;
-    for (uint32_t e = threadIdx.x; e < 16 * (DP / 4); e += 256) {
-        const uint32_t rr = e / (DP / 4), d = e % (DP / 4) * 4, orow = t.row0 + rr;
-        if (orow >= t.rows) continue;
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) top = fmaxf(top, s_m[w][rr][0]);
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float mw = s_m[w][rr][0], f = mw == -INFINITY ? 0.f : exp2_fast(mw - top);
-            sum += s_m[w][rr][1] * f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] += mw == -INFINITY ? 0.f : s_o[w][rr][d + k] * f;
+            for (int c = 0; c < NV; c += 4)
+                *reinterpret_cast<f32x4*>(&s_o[wave][col][(4 * g + i) * NV + c]) = f32x4{o[c][i], o[c + 1][i], o[c + 2][i], o[c + 3][i]};
+        if (g == 0) s_m[wave][col][0] = m, s_m[wave][col][1] = l;
+        __syncthreads();
+        const uint32_t n_rows = min(kFewRows, rows - row0);
+        // the first n sums in LDS of a row's four outputs, joined
+        const auto joined = [&](uint32_t n, uint32_t rr, uint32_t d, float& top, float& sum) {
+            top = -INFINITY, sum = 0.f;
+            for (uint32_t w = 0; w < n; w++) top = fmaxf(top, s_m[w][rr][0]);
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            for (uint32_t w = 0; w < n; w++) {
+                const float mw = s_m[w][rr][0];
+                if (mw == -INFINITY) continue;
+                const float f = exp2_fast(mw - top);
+                sum += s_m[w][rr][1] * f;
+                v += *reinterpret_cast<const f32x4*>(&s_o[w][rr][d]) * f;
+            }
+            return v;
+        };
+        const auto write = [&](uint32_t rr, uint32_t d, f32x4 v, float top, float sum) {
+            const uint32_t orow = row0 + rr, token = token0 + orow / a.group, head = kvh * a.group + orow % a.group;
+            const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+            if (d < a.dim)
+                *reinterpret_cast<u32x2*>(a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head + d) * 2) =
+                    u32x2{pack16<X>(v[0] * inv, v[1] * inv), pack16<X>(v[2] * inv, v[3] * inv)};
+            if (a.lse && d == 0) a.lse[(int64_t)token * a.heads + head] = top == -INFINITY ? -INFINITY : (top - Prob<C>::up + log2f(sum)) * kLn2;
+        };
+        const bool whole = t0 == 0 && t1 == nt;
+        const uint64_t part = ((uint64_t)blockIdx.x * 2 + (t0 == 0)) * kFewRows;
+        for (uint32_t e = threadIdx.x; e < n_rows * QUADS; e += THREADS) {
+            const uint32_t rr = e / QUADS, d = e % QUADS * 4;
+            float top, sum;
+            const f32x4 v = joined(kFewWaves, rr, d, top, sum);
+            if (whole) {
+                write(rr, d, v, top, sum);
+            } else {
+                float* po = a.part_o + (part + rr) * DP + d;
+                store_far(po, v[0], v[1]), store_far(po + 2, v[2], v[3]);
+                if (d == 0) store_far(a.part_m + (part + rr) * 2, top, sum);
+            }
         }
-        if (a.splits > 1) {
-            *reinterpret_cast<f32x4*>(a.part_o + (part + rr) * DP + d) = v;
-            if (d == 0) a.part_m[(part + rr) * 2] = top, a.part_m[(part + rr) * 2 + 1] = sum;
-            continue;
+        if (!whole) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part has arrived
+            __syncthreads();                                  // and the block's
+            const uint32_t begin = p - t0, b_first = begin / per, parts = (begin + nt - 1) / per - b_first + 1;
+            uint32_t* const counter = a.counters + item0 + kvh;
+            if (threadIdx.x == 0) {
+                const uint32_t seen = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                s_last = seen + 1 == parts;
+                if (seen + 1 == parts) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (s_last) {
+                // the last block of the item's to finish joins its parts: groups of threads take
+                // every so many of them each, four at a time (loads without branches, so that
+                // they do not wait for each other), then the groups' sums are joined as the waves' were
+                const uint32_t quads = n_rows * QUADS, groups = min(kFewWaves, max(THREADS / quads, 1u));
+                const auto part_of = [&](uint32_t k) { return (uint64_t)(k == 0 ? b_first * 2 + 1 : (b_first + k) * 2) * kFewRows; };
+                for (uint32_t e = threadIdx.x; e < groups * quads; e += THREADS) {
+                    const uint32_t grp = e / quads, rr = e % quads / QUADS, d = e % QUADS * 4;
+                    float top = -INFINITY, sum = 0.f;
+                    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                    for (uint32_t k = grp; k < parts; k += 4 * groups) {
+                        f32x2 ml[4], x[4], y[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const uint64_t at = part_of(min(k + u * groups, parts - 1)) + rr;
+                            ml[u] = load_far(a.part_m + at * 2);
+                            x[u] = load_far(a.part_o + at * DP + d), y[u] = load_far(a.part_o + at * DP + d + 2);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            if (k + u * groups >= parts || ml[u][0] == -INFINITY) continue;
+                            const float top2 = fmaxf(top, ml[u][0]), f = exp2_fast(top - top2), f2 = exp2_fast(ml[u][0] - top2);
+                            top = top2, sum = sum * f + ml[u][1] * f2;
+                            v = v * f + f32x4{x[u][0], x[u][1], y[u][0], y[u][1]} * f2;
+                        }
+                    }
+                    *reinterpret_cast<f32x4*>(&s_o[grp][rr][d]) = v;
+                    if (d == 0) s_m[grp][rr][0] = top, s_m[grp][rr][1] = sum;
+                }
+                __syncthreads();
+                for (uint32_t e = threadIdx.x; e < quads; e += THREADS) {
+                    const uint32_t rr = e / QUADS, d = e % QUADS * 4;
+                    float top, sum;
+                    const f32x4 v = joined(groups, rr, d, top, sum);
+                    write(rr, d, v, top, sum);
+                }
+            }
         }
-        const uint32_t token = t.token0 + orow / a.group, head = kvh * a.group + orow % a.group;
-        const float inv = top == -INFINITY ? 0.f : 1.f / sum;
-        if (d < a.dim)
-            *reinterpret_cast<u32x2*>(a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head + d) * 2) =
-                u32x2{pack16<X>(v[0] * inv, v[1] * inv), pack16<X>(v[2] * inv, v[3] * inv)};
-        if (a.lse && d == 0) a.lse[(int64_t)token * a.heads + head] = top == -INFINITY ? -INFINITY : (top - Prob<C>::up + log2f(sum)) * kLn2;
+        // ---- on to the next item
+        p += t1 - t0;
+        if (p >= p_end) break;
+        t0 = 0;
+        if (++kvh < a.kv_heads) continue;
+        kvh = 0, row0 += kFewRows, item0 += a.kv_heads;
+        while (row0 >= rows) {  // p < p_end: there is one
+            const int32_t from = a.b.offsets[++seq], to = min(a.b.offsets[seq + 1], (int32_t)a.b.n_tokens);
+            row0 = 0, rows = from >= 0 && to > from ? (uint32_t)(to - from) * a.group : 0;
+            token0 = (uint32_t)from, start = a.b.starts[seq];
+        }
+        span = few_span(a, start, row0, rows), nt = few_tiles(span);
     }
 }
 
@@ -1166,45 +1398,62 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttnArg a, float up) {
 // How a batch is cut: rows of a tile, tiles (an upper bound: each sequence's last
 // tile may be short), key ranges of a tile.
 struct Cut {
-    uint32_t bm, dp, tiles, splits, split_len;
-    uint64_t part_m_bytes, bytes;  // of the workspace: the rows' maxima and sums, then their outputs
+    uint32_t bm, dp, tiles, splits, split_len, blocks, min_tiles;
+    uint64_t counter_bytes, part_m_bytes, bytes;  // of the workspace: counters, the rows' maxima and sums, their outputs
 };
-constexpr uint32_t kFewRows = 16, kManyRows = 128, kWideRows = 256;
-constexpr uint64_t kSplitMin = 128;                   // keys of a split at least
-uint64_t blocks_wanted(uint32_t bm) { return bm == kFewRows ? 2048 : bm == kManyRows ? 512 : 256; }
+constexpr uint64_t kSplitMin = 128;   // keys of a split at least
+constexpr uint32_t kFewBlocks = 512;  // blocks of the few rows' kernel: two a CU
+constexpr uint32_t kFewTiles = 4;     // its tiles of 32 keys a block at least
+uint64_t blocks_wanted(uint32_t bm) { return bm == kManyRows ? 512 : 256; }
 uint32_t padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 uint64_t most_tiles(uint32_t bm, uint64_t group, uint64_t n_seqs, uint64_t n_tokens) {
     return std::min(n_tokens * group / bm + std::min(n_seqs, n_tokens), n_tokens * ((group + bm - 1) / bm));
 }
-uint64_t part_bytes(uint64_t rows, uint32_t dp, uint64_t* m_bytes) {
-    *m_bytes = (rows * 8 + 255) / 256 * 256;
-    return *m_bytes + rows * dp * 4;
+// The workspace of c.counter_bytes counters and `rows` rows of parts.
+void set_bytes(Cut& c, uint64_t counters, uint64_t rows) {
+    c.counter_bytes = (counters * 4 + 255) / 256 * 256, c.part_m_bytes = (rows * 8 + 255) / 256 * 256;
+    c.bytes = c.counter_bytes + c.part_m_bytes + rows * c.dp * 4;
+}
+uint32_t few_blocks(uint64_t items, uint64_t max_context) {
+    return (uint32_t)std::min<uint64_t>(items * ((max_context + 31) / 32) / kFewTiles + 1, kFewBlocks);
 }
 Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t n_tokens, uint32_t max_chunk,
-        uint64_t max_context, uint32_t window, bool near_slots) {
+        uint64_t max_context, uint64_t all_keys, uint32_t window, bool near_slots) {
     Cut c{};
-    const uint64_t group = n_heads / n_kv;
+    const uint64_t group = n_heads / n_kv, rows = (uint64_t)max_chunk * group;
     c.dp = padded_dim(dim);
-    const uint64_t rows = (uint64_t)max_chunk * group;
-    c.bm = rows <= kFewRows ? kFewRows : rows <= kManyRows || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
+    const bool few = rows <= kFewRows && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1) < (1ull << 31);
+    c.bm = few ? kFewRows : rows <= kManyRows || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
     c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
+    c.splits = 1;
     // the keys of a tile: a window's, and as many again as the tile has tokens
     if (window) max_context = std::min<uint64_t>(max_context, (uint64_t)window + c.bm / group + 64);
-    const uint64_t blocks = std::max<uint64_t>((uint64_t)c.tiles * n_kv, 1);
+    const uint64_t items = std::max<uint64_t>((uint64_t)c.tiles * n_kv, 1);
+    if (c.bm == kFewRows) {
+        c.min_tiles = kFewTiles;
+        c.blocks = few_blocks(items, max_context);
+        set_bytes(c, items, (uint64_t)c.blocks * 2 * kFewRows);
+        return c;
+    }
     const uint64_t most = std::max<uint64_t>((max_context + kSplitMin - 1) / kSplitMin, 1);
-    const uint64_t splits = std::min(std::max<uint64_t>(blocks_wanted(c.bm) / blocks, 1), most);
+    const uint64_t splits = std::min(std::max<uint64_t>(blocks_wanted(c.bm) / items, 1), most);
     c.split_len = (uint32_t)std::min<uint64_t>((std::max<uint64_t>(max_context, 1) + splits * kSplitMin - 1) / (splits * kSplitMin) * kSplitMin, 1u << 31);
     c.splits = (uint32_t)std::max<uint64_t>((max_context + c.split_len - 1) / c.split_len, 1);
-    if (c.splits > 1) c.bytes = part_bytes(blocks * c.splits * c.bm, c.dp, &c.part_m_bytes);
+    if (c.splits > 1) set_bytes(c, 0, items * c.splits * c.bm);
     return c;
 }
 // What cut() asks for at most, for any batch up to these sizes.
 uint64_t most_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t n_tokens, uint64_t max_context) {
-    uint64_t most = 0, m;
-    for (const uint32_t bm : {kFewRows, kManyRows, kWideRows}) {
-        const uint64_t blocks = most_tiles(bm, n_heads / n_kv, n_seqs, n_tokens) * n_kv;
-        const uint64_t parts = std::min(blocks_wanted(bm), blocks * ((max_context + kSplitMin - 1) / kSplitMin));
-        if (max_context > kSplitMin) most = std::max(most, part_bytes(parts * bm, padded_dim(dim), &m));
+    const uint64_t group = n_heads / n_kv;
+    Cut c{};
+    c.dp = padded_dim(dim);
+    uint64_t items = std::max<uint64_t>(most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv, 1);
+    set_bytes(c, items, (uint64_t)few_blocks(items, max_context) * 2 * kFewRows);
+    uint64_t most = c.bytes;
+    for (const uint32_t bm : {kManyRows, kWideRows}) {
+        items = most_tiles(bm, group, n_seqs, n_tokens) * n_kv;
+        set_bytes(c, 0, std::min(blocks_wanted(bm), items * ((max_context + kSplitMin - 1) / kSplitMin)) * bm);
+        if (max_context > kSplitMin) most = std::max(most, c.bytes);
     }
     return most;
 }
@@ -1218,8 +1467,7 @@ hipError_t launch_attend(const AttnArg& a, const Cut& c, hipStream_t s) {
         CKR_LAUNCH("kv_attention_join", s, kernel<<<dim3(a.tiles * a.kv_heads, (c.bm + per - 1) / per), 256, 0, s>>>(a, Prob<C>::up));
     };
     if (c.bm == kFewRows) {
-        CKR_LAUNCH("kv_attention_few", s, attend_few_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
-        join(attend_join_kernel<X, DP, kFewRows>);
+        CKR_LAUNCH("kv_attention_few", s, attend_few_kernel<X, C, DP><<<dim3(c.blocks), 64 * kFewWaves, 0, s>>>(a));
     } else if (c.bm == kManyRows) {
         CKR_LAUNCH("kv_attention_many", s, attend_many_kernel<X, C, DP><<<grid, 256, 0, s>>>(a));
         join(attend_join_kernel<X, DP, kManyRows>);
@@ -1291,16 +1539,18 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
     bool near_slots = true;
     for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 26) - 16 && st[0] < (1ll << 36);
     const Cut c = cut(n_heads, cache->n_heads, cache->head_dim, batch->n_seqs, batch->n_tokens, batch->max_chunk,
-                      std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size), window, near_slots);
+                      std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size),
+                      (uint64_t)batch->table_width * cache->page_size, window, near_slots);
     if ((uint64_t)c.tiles * cache->n_heads * 512 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
-    a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len;
+    a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len, a.min_tiles = c.min_tiles, a.items = c.tiles * cache->n_heads;
     if (c.bytes) {
         if (workspace_bytes < c.bytes)
             return err(CKR_E_CAPACITY, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(c.bytes) + " needed");
         if (reinterpret_cast<uintptr_t>(d_workspace) % 256) return err(CKR_E_INVALID, "workspace must be aligned to 256 bytes");
         if ((rc = check_range(d_workspace, c.bytes, "workspace"))) return rc;
-        a.part_m = static_cast<float*>(d_workspace);
-        a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) + c.part_m_bytes);
+        a.counters = static_cast<uint32_t*>(d_workspace);
+        a.part_m = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) + c.counter_bytes);
+        a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) + c.counter_bytes + c.part_m_bytes);
     }
     const hipStream_t s = (hipStream_t)stream;
     hipError_t e;
