@@ -77,6 +77,16 @@ template <typename C, typename E> __device__ __forceinline__ u32x2 widen4(uint32
         return u32x2{pack16<E>(f[0], f[1]), pack16<E>(f[2], f[3])};
     }
 }
+// The same times a power of two, in float16.
+template <typename C> __device__ __forceinline__ u32x2 widen4_by(uint32_t v, float power) {
+    if constexpr (C::tag == CKR_F8)
+        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, power, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, power, true))};
+    else {
+        const f32x4 f = codes4<C>(v) * power;
+        return u32x2{pack16<ElemF16>(f[0], f[1]), pack16<ElemF16>(f[2], f[3])};
+    }
+}
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // Maximum over the lanes l, l ^ 32 (and l ^ 16).
@@ -97,15 +107,67 @@ __device__ __forceinline__ float sum_quarters(float x) {
     return sum_half(as_f32(r[0]) + as_f32(r[1]));
 }
 
-// The probabilities' type: 8-bit values meet bfloat16 weights, which take the
-// value's scale without a range of their own; float16 values meet float16
-// weights, scaled up by 2^7 (their largest is 1, or 2^8 where a running maximum
-// lags, so at most 2^15) so that small ones keep their bits.
-template <typename C> struct Prob { typedef ElemBF16 E; static constexpr float up = 0.f; };
-template <> struct Prob<ElemF16> { typedef ElemF16 E; static constexpr float up = 7.f; };
+// The weights' type is the queries': bfloat16 weights take the value's scale without
+// a range of their own.  float16 weights are scaled up by 2^up so that small ones
+// keep their bits (their largest is 1, or 2^kLag where a running maximum lags, or
+// twice that with a value's scale, so at most 2^15); of an 8-bit value's scale they
+// take the fraction (1 to 2), and the codes its power of two as they are widened,
+// which leaves the values' own range (up to 65504).
+template <typename X, typename C> struct Prob {
+    typedef X E;
+    static constexpr bool split = X::tag == CKR_F16 && C::bytes == 1;
+    static constexpr float up = X::tag == CKR_F16 ? (C::bytes == 1 ? 6.f : 7.f) : 0.f;
+};
+// A scale as a power of two and the rest (zero, subnormal and non-finite scales: 1
+// and themselves; powers that would take the largest code past 65504: the largest
+// that does not).
+struct SplitScale { float power, rest; };
+template <typename C> __device__ __forceinline__ SplitScale split_scale(float s) {
+    const uint32_t top = C::tag == CKR_F8 ? 0x43000000u : 0x44000000u;  // 2^7 x 448, 2^9 x 127
+    const uint32_t e = as_u32(s) & 0x7f800000u, p = min(e, top);
+    const bool normal = e - 0x00800000u < 0x7f000000u;
+    return {normal ? as_f32(p) : 1.f, normal ? as_f32(as_u32(s) - p + 0x3f800000u) : s};
+}
+
 // How far a row's running maximum may lag behind (in powers of two) before the
 // accumulators are scaled: sums and outputs use the same lagging maximum.
 constexpr float kLag = 8.f;
+
+// ---- infinities and NaN in 16-bit values.  A tile of keys that not every row sees
+// meets weights of zero, and zero times an infinity is NaN: there the products
+// take the finite values, and who sees an infinity (or NaN: both) is found by
+// products of ones.
+template <typename E> __device__ __forceinline__ bool any_wild(u32x4 w) {  // E: a 16-bit type
+    constexpr uint32_t one = E::tag == CKR_BF16 ? 0x00800080u : 0x04000400u;  // carries an exponent of ones into the sign's place
+    uint32_t x = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x |= (w[i] & 0x7fff7fffu) + one;
+    return x & 0x80008000u;
+}
+// sign 0: the finite values; 1: ones where +infinity or NaN; -1: ones where -infinity or NaN.
+template <typename E> __device__ __forceinline__ u32x4 wild(u32x4 w, int sign) {
+    constexpr uint32_t inf = E::tag == CKR_BF16 ? 0x7f80u : 0x7c00u, one = E::tag == CKR_BF16 ? 0x3f80u : 0x3c00u;
+    u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t x = w[i / 2] >> (16 * (i % 2)) & 0xffffu;
+        const bool bad = (x & 0x7fffu) >= inf, here = bad && x != (sign > 0 ? inf | 0x8000u : inf);
+        r[i / 2] |= (sign == 0 ? (bad ? 0u : x) : here ? one : 0u) << (16 * (i % 2));
+    }
+    return r;
+}
+// What rows see of wild values, from the two products of ones.
+__device__ __forceinline__ float wild_sum(float plus, float minus) {
+    return (plus > 0.f ? INFINITY : 0.f) + (minus > 0.f ? -INFINITY : 0.f);
+}
+// Ones for the keys a row sees (bits 0 to 7).
+template <typename E> __device__ __forceinline__ u32x4 ones(uint32_t seen) {
+    constexpr uint32_t one = E::tag == CKR_BF16 ? 0x3f80u : 0x3c00u;
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = (seen >> (2 * i) & 1 ? one : 0u) | (seen >> (2 * i + 1) & 1 ? one << 16 : 0u);
+    return r;
+}
 
 constexpr uint32_t kFewRows = 16, kManyRows = 128, kWideRows = 256;  // rows of a tile
 constexpr uint32_t kFewWaves = 4;                                    // waves of a block of few rows
@@ -218,7 +280,7 @@ __device__ __forceinline__ uint32_t few_tiles(const FewSpan& f) {  // one at lea
 }
 template <typename X, typename C, int DP>
 __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few_kernel(AttnArg a) {
-    typedef typename Prob<C>::E P;
+    typedef typename Prob<X, C>::E P;
     typedef FewRegs<C, DP> Regs;
     constexpr int KL = Regs::KL, VD = Regs::VD, NV = DP / 16, KS = DP / 32;
     constexpr uint32_t THREADS = 64 * kFewWaves, QUADS = DP / 4;  // a row's outputs by fours
@@ -376,11 +438,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
                             r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
                     }
                 }
-                if constexpr (C::bytes == 1) {
-                    const int64_t x = max(pages[h], 0);
-                    r.sk[h] = *reinterpret_cast<const f32x4*>(skp + x * a.skst[0] + slot + 4 * g);
-                    r.sv[h] = *reinterpret_cast<const f32x4*>(svp + x * a.svst[0] + slot + 4 * g);
-                }
+                if constexpr (C::bytes == 1) r.sk[h] = *reinterpret_cast<const f32x4*>(skp + (int64_t)max(pages[h], 0) * a.skst[0] + slot + 4 * g);
             }
         };
         const auto load_v = [&](Regs& r, int base, const int32_t* pages) {
@@ -403,6 +461,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
             for (int h = 0; h < 2; h++) {
                 const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
                 const uint8_t* at = cv + (int64_t)pages[h] * a.vst[0] + (int64_t)slot * a.vst[2];
+                if constexpr (C::bytes == 1) r.sv[h] = *reinterpret_cast<const f32x4*>(svp + (int64_t)max(pages[h], 0) * a.svst[0] + slot + 4 * g);
                 if (whole) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) get(r.v[4 * h + i], at + v_off[i]);
@@ -439,10 +498,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
             }
         };
         // the weights of a tile, with the values' scales; what a row does not see weighs 0
-        const auto weights = [&](const Regs& r, const f32x4 (&s)[2], int base, const int32_t* pages) {
+        const auto weights = [&](const Regs& r, const f32x4 (&s)[2], int base, const int32_t* pages, uint32_t& seen) {
             const bool full = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= full_to && base >= full_from;
             float x[8], top = -INFINITY;
-            uint32_t seen = 0xffu;
+            seen = ~0u;  // every row sees every key
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = s[i / 4][i % 4] * a.scale2;
@@ -467,13 +526,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
 #pragma unroll
                 for (int c = 0; c < NV; c++) o[c] *= back;
             }
-            const float ref = m == -INFINITY ? 0.f : m - Prob<C>::up;
+            const float ref = m == -INFINITY ? 0.f : m - Prob<X, C>::up;
             float w[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 w[i] = exp2_fast(x[i] - ref);
                 l += w[i];
-                if constexpr (C::bytes == 1) w[i] *= r.sv[i / 4][i % 4];
+                if constexpr (Prob<X, C>::split) w[i] *= split_scale<C>(r.sv[i / 4][i % 4]).rest;
+                else if constexpr (C::bytes == 1) w[i] *= r.sv[i / 4][i % 4];
             }
             if (C::bytes == 1 && !full) {
 #pragma unroll
@@ -481,8 +541,22 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
             }
             return u32x4{pack16<P>(w[0], w[1]), pack16<P>(w[2], w[3]), pack16<P>(w[4], w[5]), pack16<P>(w[6], w[7])};
         };
-        const auto gather = [&](const Regs& r, u32x4 pf) {
-            if constexpr (C::bytes == 1) {
+        const auto gather = [&](const Regs& r, u32x4 pf, uint32_t seen) {
+            if constexpr (Prob<X, C>::split) {
+#pragma unroll
+                for (int j = 0; j < VD; j++) {  // four dimensions of eight keys, widened first: each key has its power
+                    u32x2 x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x[k] = widen4_by<C>(r.v[k][j], split_scale<C>(r.sv[k / 4][k % 4]).power);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        u32x4 w;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(x[2 * e + 1][k / 2], x[2 * e][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
+                        o[4 * j + k] = mfma16<P>(w, pf, o[4 * j + k]);
+                    }
+                }
+            } else if constexpr (C::bytes == 1) {
 #pragma unroll
                 for (int j = 0; j < VD; j++) {  // four dimensions of eight keys
                     uint32_t w[2][4];
@@ -511,6 +585,15 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
                         w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
                         w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
                     }
+                    if (__any(seen != ~0u && (any_wild<P>(w0) || any_wild<P>(w1)))) {
+                        const u32x4 see = ones<P>(seen);
+                        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+                        const f32x4 p0 = mfma16<P>(wild<P>(w0, 1), see, zero), m0 = mfma16<P>(wild<P>(w0, -1), see, zero);
+                        const f32x4 p1 = mfma16<P>(wild<P>(w1, 1), see, zero), m1 = mfma16<P>(wild<P>(w1, -1), see, zero);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[2 * j][i] += wild_sum(p0[i], m0[i]), o[2 * j + 1][i] += wild_sum(p1[i], m1[i]);
+                        w0 = wild<P>(w0, 0), w1 = wild<P>(w1, 0);
+                    }
                     o[2 * j] = mfma16<P>(w0, pf, o[2 * j]);
                     o[2 * j + 1] = mfma16<P>(w1, pf, o[2 * j + 1]);
                 }
@@ -537,12 +620,13 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
                 const bool more = i + u + 2 < n_tiles;
                 f32x4 s[2];
                 scores(r[u], s);
-                const u32x4 pf = weights(r[u], s, base, pages[u]);
+                uint32_t seen;
+                const u32x4 pf = weights(r[u], s, base, pages[u], seen);
                 if (more) {  // its keys' registers again, for the tile after the next
                     coming[0] = page_at(base + 64), coming[1] = page_at(base + 80);
                     load_k(r[u], base + 64, coming);
                 }
-                gather(r[u], pf);
+                gather(r[u], pf, seen);
                 if (more) {
                     pages[u][0] = coming[0], pages[u][1] = coming[1];
                     load_v(r[u], base + 64, pages[u]);
@@ -581,7 +665,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
             if (d < a.dim)
                 *reinterpret_cast<u32x2*>(a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head + d) * 2) =
                     u32x2{pack16<X>(v[0] * inv, v[1] * inv), pack16<X>(v[2] * inv, v[3] * inv)};
-            if (a.lse && d == 0) a.lse[(int64_t)token * a.heads + head] = top == -INFINITY ? -INFINITY : (top - Prob<C>::up + log2f(sum)) * kLn2;
+            if (a.lse && d == 0) a.lse[(int64_t)token * a.heads + head] = top == -INFINITY ? -INFINITY : (top - Prob<X, C>::up + log2f(sum)) * kLn2;
         };
         const bool whole = t0 == 0 && t1 == nt;
         const uint64_t part = ((uint64_t)blockIdx.x * 2 + (t0 == 0)) * kFewRows;
@@ -682,7 +766,7 @@ template <typename C, int DP> struct ManyShape {
 
 template <typename X, typename C, int DP>
 __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(AttnArg a) {
-    typedef typename Prob<C>::E P;
+    typedef typename Prob<X, C>::E P;
     typedef ManyShape<C, DP> Sh;
     constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, ROWS = Sh::ROWS;
     constexpr int KS = DP / 16, DT = DP / 32, TT = TK / 32;
@@ -744,16 +828,18 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
         if (threadIdx.x < TK) pg_s = page_id(base + (int)threadIdx.x);
     };
     u32x4 kr[LOADS], vr[LOADS];
-    float sk = 0.f, sv = 0.f;
+    float sk = 0.f, sv = 0.f, row_sv[LOADS];
     bool in_s = false;
     const auto load_tile = [&](int base) {
 #pragma unroll
         for (int u = 0; u < LOADS; u++) {
             const int64_t slot = (in0 + (uint32_t)base + r0 + u * ROWS) & slot_mask;
             kr[u] = vr[u] = u32x4{0, 0, 0, 0};
+            row_sv[u] = 0.f;
             if (pg[u] >= 0 && d_in) {
                 kr[u] = *reinterpret_cast<const u32x4*>(a.ck + (int64_t)pg[u] * a.kst[0] + (int64_t)kvh * a.kst[1] + slot * a.kst[2] + piece * 16);
                 vr[u] = *reinterpret_cast<const u32x4*>(a.cv + (int64_t)pg[u] * a.vst[0] + (int64_t)kvh * a.vst[1] + slot * a.vst[2] + piece * 16);
+                if constexpr (Prob<X, C>::split) row_sv[u] = a.sv[(int64_t)pg[u] * a.svst[0] + (int64_t)kvh * a.svst[1] + slot];
             }
         }
         in_s = pg_s >= 0;
@@ -776,7 +862,13 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                 for (int w = 0; w < 2; w++) {
                     const u32x2 x = widen4<C, X>(kr[u][2 * w]), y = widen4<C, X>(kr[u][2 * w + 1]);
                     *reinterpret_cast<u32x4*>(k + piece * 32 + w * 16) = u32x4{x[0], x[1], y[0], y[1]};
-                    const u32x2 z = widen4<C, P>(vr[u][2 * w]), zz = widen4<C, P>(vr[u][2 * w + 1]);
+                    u32x2 z, zz;
+                    if constexpr (Prob<X, C>::split) {
+                        const float power = split_scale<C>(row_sv[u]).power;
+                        z = widen4_by<C>(vr[u][2 * w], power), zz = widen4_by<C>(vr[u][2 * w + 1], power);
+                    } else {
+                        z = widen4<C, P>(vr[u][2 * w]), zz = widen4<C, P>(vr[u][2 * w + 1]);
+                    }
                     *reinterpret_cast<u32x4*>(v + piece * 32 + w * 16) = u32x4{z[0], z[1], zz[0], zz[1]};
                 }
             }
@@ -786,7 +878,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
             // weight of 0 (a key that a row does not see) always gives 0
             const bool fine = abs_bits(sv) < 0x7f800000u;
             s_sk[buf][threadIdx.x] = !in_s ? 0.f : fine ? sk * a.scale2 : as_f32(0x7fc00000u);
-            s_sv[buf][threadIdx.x] = in_s && fine ? sv : 0.f;
+            s_sv[buf][threadIdx.x] = !in_s || !fine ? 0.f : Prob<X, C>::split ? split_scale<C>(sv).rest : sv;
         }
         if (threadIdx.x < 64) {
             const uint64_t ok = __ballot(in_s && lane < TK);
@@ -830,16 +922,30 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                     for (int k = 0; k < 4; k++) s[tt][i + k] *= a.scale2;
                 }
             }
+        uint32_t seen[TT];
+        bool care = false;
         if (!full) {
             valid >>= 4 * half;
             const int k0 = base + 4 * half;
 #pragma unroll
-            for (int tt = 0; tt < TT; tt++)
+            for (int tt = 0; tt < TT; tt++) {
+                seen[tt] = 0;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int key = tt * 32 + 8 * (i / 4) + i % 4;
-                    s[tt][i] = (valid >> key & 1) && k0 + key <= pos && k0 + key > see ? s[tt][i] : -INFINITY;
+                    const bool in = (valid >> key & 1) && k0 + key <= pos && k0 + key > see;
+                    if constexpr (C::bytes == 2) seen[tt] |= in ? 1u << i : 0u;
+                    s[tt][i] = in ? s[tt][i] : -INFINITY;
                 }
+            }
+            if constexpr (C::bytes == 2) {  // is there an infinity or NaN among the values
+#pragma unroll
+                for (int u = 0; u < TK * DP / 8 / 64; u++) {
+                    const uint32_t e = u * 64 + lane;
+                    care |= any_wild<P>(*reinterpret_cast<const u32x4*>(s_v[buf] + e / (DP / 8) * VP + e % (DP / 8) * 16));
+                }
+                care = __any(care);
+            }
         }
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
@@ -855,7 +961,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[dt][i] *= back;
         }
-        const float ref = m == -INFINITY ? 0.f : m - Prob<C>::up;
+        const float ref = m == -INFINITY ? 0.f : m - Prob<X, C>::up;
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
 #pragma unroll
@@ -883,7 +989,18 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at));
                     const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * VP));
                     const u32x2 xa = __builtin_bit_cast(u32x2, x), ya = __builtin_bit_cast(u32x2, y);
-                    o[dt] = mfma32<P>(u32x4{xa[0], xa[1], ya[0], ya[1]}, pf, o[dt]);
+                    u32x4 v = {xa[0], xa[1], ya[0], ya[1]};
+                    if (C::bytes == 2 && care) {
+                        const u32x4 see8 = ones<P>(seen[tt] >> (8 * kb));
+                        f32x16 zero;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) zero[i] = 0.f;
+                        const f32x16 plus = mfma32<P>(wild<P>(v, 1), see8, zero), minus = mfma32<P>(wild<P>(v, -1), see8, zero);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[dt][i] += wild_sum(plus[i], minus[i]);
+                        v = wild<P>(v, 0);
+                    }
+                    o[dt] = mfma32<P>(v, pf, o[dt]);
                 }
             }
     };
@@ -933,7 +1050,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
             if (d < a.dim)
                 *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[dt][i] * inv, o[dt][i + 1] * inv), pack16<X>(o[dt][i + 2] * inv, o[dt][i + 3] * inv)};
         }
-    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<C>::up + log2f(l)) * kLn2;
+    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<X, C>::up + log2f(l)) * kLn2;
 }
 
 // ------------------------------------------------------------ very many rows
@@ -961,12 +1078,12 @@ template <typename C, int DP> struct WideShape {
 
 template <typename X, typename C, int DP>
 __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
-    typedef typename Prob<C>::E P;
+    typedef typename Prob<X, C>::E P;
     typedef WideShape<C, DP> Sh;
     constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, RPW = Sh::RPW, ROWS = Sh::ROWS;
     constexpr int KS = DP / 16, DT = DP / 32, NM = 2 * KS;  // KS products for the scores, as many for the values
     static_assert(KS == 2 * DT && KS % 4 == 0, "pairs of products, operands in rings of four");
-    constexpr float kMost = Prob<C>::up == 0.f ? 256.f : 32768.f;  // 2^(kLag + up)
+    constexpr float kMost = Prob<X, C>::up == 0.f ? 256.f : Prob<X, C>::up == 6.f ? 16384.f : 32768.f;  // 2^(kLag + up)
     __shared__ __attribute__((aligned(16))) uint8_t s_k[Sh::RING * TK * KP];
     __shared__ __attribute__((aligned(16))) uint8_t s_v[Sh::RING * TK * VP];
     __shared__ __attribute__((aligned(16))) float s_sk[Sh::RING + 1][TK];  // the last: ones, for scores that carry their scale
@@ -1055,7 +1172,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         return end - base >= TK ? v : end - base <= 0 ? 0 : v & ((1ull << (end - base)) - 1);
     };
     u32x4 held[LOADS];
-    float sk = 0.f, sv = 0.f;
+    float sk = 0.f, sv = 0.f, row_sv[LOADS];  // row_sv: of the rows held, where values are widened by their scale's power
     uint64_t held_valid = 0;
     const auto load_tile = [&](int base) {
         if (one_page) {
@@ -1063,6 +1180,11 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             const uint8_t* at = from + ((uint64_t)p * st0 + (uint64_t)slot * st2) * 16;
 #pragma unroll
             for (int u = 0; u < LOADS; u++) held[u] = *reinterpret_cast<const u32x4*>(at + (from_lane + (w4_rows + u * ROWS) * st2 * 16));
+            if constexpr (Prob<X, C>::split) {
+                const float* f = scale_v + ((int64_t)p * a.svst[0] + slot) + row_of;
+#pragma unroll
+                for (int u = 0; u < LOADS; u++) row_sv[u] = f[u * ROWS];
+            }
         } else {
 #pragma unroll
             for (int u = 0; u < LOADS; u++) {
@@ -1070,6 +1192,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 const uint32_t p = (uint32_t)max(g == 0 ? pg[0] : g == 1 ? pg[1] : g == 2 ? pg[2] : pg[3], 0);
                 const uint32_t slot = (in0 + (uint32_t)base + 16 * g) & slot_mask;
                 held[u] = *reinterpret_cast<const u32x4*>(from + ((uint64_t)p * st0 + (uint64_t)slot * st2) * 16 + from_lane);
+                if constexpr (Prob<X, C>::split) row_sv[u] = (scale_v + ((int64_t)p * a.svst[0] + slot))[row_of & 15];
             }
         }
         if constexpr (C::bytes == 1) {
@@ -1089,16 +1212,17 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         uint8_t* at = to + slot * to_slot + u * to_rows;
         if constexpr (C::bytes == 2) {
             *reinterpret_cast<u32x4*>(at) = x;
-        } else if (X::tag == P::tag || stage_k) {
+        } else if (!Prob<X, C>::split || stage_k) {
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 const u32x2 y = widen4<C, X>(x[2 * w]), z = widen4<C, X>(x[2 * w + 1]);
                 *reinterpret_cast<u32x4*>(at + w * 16) = u32x4{y[0], y[1], z[0], z[1]};
             }
         } else {
+            const float power = split_scale<C>(row_sv[u]).power;
 #pragma unroll
             for (int w = 0; w < 2; w++) {
-                const u32x2 y = widen4<C, P>(x[2 * w]), z = widen4<C, P>(x[2 * w + 1]);
+                const u32x2 y = widen4_by<C>(x[2 * w], power), z = widen4_by<C>(x[2 * w + 1], power);
                 *reinterpret_cast<u32x4*>(at + w * 16) = u32x4{y[0], y[1], z[0], z[1]};
             }
         }
@@ -1109,7 +1233,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             // weight of 0 (a key that a row does not see) always gives 0
             const bool fine = abs_bits(sv) < 0x7f800000u, in = held_valid >> (16 * w4 + (lane & 15)) & 1;
             if (stage_k) s_sk[slot][16 * w4 + (lane & 15)] = fine ? sk * a.scale2 : as_f32(0x7fc00000u);
-            else s_sv[slot][16 * w4 + (lane & 15)] = in && fine ? sv : 0.f;
+            else s_sv[slot][16 * w4 + (lane & 15)] = !in || !fine ? 0.f : Prob<X, C>::split ? split_scale<C>(sv).rest : sv;
         }
     };
 
@@ -1143,19 +1267,50 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     const auto weight = [&](int k, f32x4 g, float f) {
         return exp2_fast(__builtin_fmaf(s[k], C::bytes == 1 ? g[k % 4] : f, -ref));
     };
-    // scores that some row of the wave must not see: scaled here, -inf where hidden
-    const auto mask = [&](const float* at_fk, int base, uint32_t seen) {
-        seen >>= 4 * half;
+    // scores that some row of the wave must not see: scaled here, -inf where hidden.
+    // 16-bit values: is there an infinity or NaN among them (care), and who sees which
+    // key; those keys' values are then gathered apart, and not by the next turn
+    uint32_t seen = 0;
+    bool care = false;
+    const auto mask = [&](const float* at_fk, const uint8_t* at_v, int base, uint32_t valid) __attribute__((always_inline)) {
+        valid >>= 4 * half;
         const int k0 = base + 4 * half;
+        seen = 0;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int key = 8 * (i / 4) + i % 4;
             const float f = C::bytes == 1 ? at_fk[key + 4 * half] : a.scale2;
-            s[i] = (seen >> key & 1) && k0 + key <= pos && k0 + key > see ? s[i] * f : -INFINITY;
+            const bool in = (valid >> key & 1) && k0 + key <= pos && k0 + key > see;
+            if constexpr (C::bytes == 2) seen |= in ? 1u << i : 0u;
+            s[i] = in ? s[i] * f : -INFINITY;
+        }
+        if constexpr (C::bytes == 2) {
+#pragma unroll
+            for (int u = 0; u < 32 * DP / 8 / 64; u++) {
+                const uint32_t e = u * 64 + lane;
+                care |= any_wild<P>(*reinterpret_cast<const u32x4*>(at_v + e / (DP / 8) * VP + e % (DP / 8) * 16));
+            }
+            care = __any(care);
+        }
+    };
+    const auto gather_with_care = [&](const u32x4 (&w)[2], const uint8_t* at) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < KS; e++) {
+            const uint8_t* row = at + e / DT * 16 * VP + e % DT * 64;
+            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(row)));
+            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(row + 8 * VP)));
+            const u32x4 v = {x[0], x[1], y[0], y[1]}, see8 = ones<P>(seen >> (8 * (e / DT)));
+            f32x16 zero;
+#pragma unroll
+            for (int i = 0; i < 16; i++) zero[i] = 0.f;
+            const f32x16 plus = mfma32<P>(wild<P>(v, 1), see8, zero), minus = mfma32<P>(wild<P>(v, -1), see8, zero);
+            o[e % DT] = mfma32<P>(wild<P>(v, 0), w[e / DT], o[e % DT]);
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[e % DT][i] += wild_sum(plus[i], minus[i]);
         }
     };
     struct Where { const uint8_t *k, *v; const float *fk, *fv; };  // what a turn reads: K(i+1), V(i-1), scales(i)
-    const auto turn = [&](auto sub_tag, float f, const Where& now, const Where& after, auto side) {
+    const auto turn = [&](auto sub_tag, float f, const Where& now, const Where& after, bool gathered, auto side) {
         constexpr int sub = decltype(sub_tag)::value;
         f32x16 z;
 #pragma unroll
@@ -1179,7 +1334,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             if constexpr (S % (16 / NM) == 0) {
                 constexpr int j = S * NM / 16, e = j / 2;
                 if constexpr (j % 2 == 0) {
-                    o[e % DT] = mfma32<P>(vf[e % 4], pf[1 - sub][e / DT], o[e % DT]);
+                    if (C::bytes == 1 || !gathered) o[e % DT] = mfma32<P>(vf[e % 4], pf[1 - sub][e / DT], o[e % DT]);
                     if constexpr (e + 3 < KS) read_v(e + 3, now.v);
                     else read_v(e + 3 - KS, after.v);
                 } else {
@@ -1212,7 +1367,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             most = max_half(most);
             const float m2 = fmaxf(m, most), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
             m = m2;
-            ref = m2 == -INFINITY ? 0.f : m2 - Prob<C>::up;
+            ref = m2 == -INFINITY ? 0.f : m2 - Prob<X, C>::up;
             l *= back;
             sum = 0.f;
 #pragma unroll
@@ -1252,7 +1407,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             for (int g = 0; g < 4; g++) pages[i][g] = pg[g];
         }
         u32x4 rows[3][LOADS];
-        float scales[3][2];
+        float scales[3][2], row_scales[3][LOADS];
 #pragma unroll
         for (int i = 0; i < 3; i++) {
 #pragma unroll
@@ -1260,13 +1415,13 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             load_tile(i * TK);
             valid[i] = held_valid;
 #pragma unroll
-            for (int u = 0; u < LOADS; u++) rows[i][u] = held[u];
+            for (int u = 0; u < LOADS; u++) rows[i][u] = held[u], row_scales[i][u] = row_sv[u];
             scales[i][0] = sk, scales[i][1] = sv;
         }
 #pragma unroll
         for (int i = 0; i < 3; i++) {
 #pragma unroll
-            for (int u = 0; u < LOADS; u++) held[u] = rows[i][u];
+            for (int u = 0; u < LOADS; u++) held[u] = rows[i][u], row_sv[u] = row_scales[i][u];
             sk = scales[i][0], sv = scales[i][1], held_valid = valid[i];
             if (i == 2) break;
 #pragma unroll
@@ -1299,13 +1454,16 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             unroll<2>([&](auto sub_tag) {
                 constexpr int sub = decltype(sub_tag)::value;
                 const int base = i * TK + sub * 32;
-                if (!full) mask(s_sk[cur] + sub * 32, base, (uint32_t)(valid[0] >> (32 * sub)));
+                const bool gathered = care;
+                if (C::bytes == 2 && care) gather_with_care(pf[1 - sub], now.v);
+                care = false;
+                if (!full) mask(s_sk[cur] + sub * 32, s_v + cur * (TK * VP) + sub * 32 * VP, base, (uint32_t)(valid[0] >> (32 * sub)));
                 const float f = full ? a.scale2 : 1.f;
                 const bool full2 = full_at(valid[sub], base + 32);
                 const int slot2 = sub ? next : cur;
                 const Where after = {k_at(next, sub), v_at(cur, sub), s_sk[full2 ? slot2 : Sh::RING] + (1 - sub) * 32,
                                      s_sv[slot2] + (1 - sub) * 32};
-                turn(sub_tag, f, now, after, [&](auto step_tag) {
+                turn(sub_tag, f, now, after, gathered, [&](auto step_tag) {
                     constexpr int S = decltype(step_tag)::value;
                     if constexpr (sub == 0) {  // the next tile but one into LDS
                         if constexpr (S % 2 == 0 && S >= 4 && S / 2 - 2 < LOADS) store_rows(S / 2 - 2, third);
@@ -1331,6 +1489,8 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             __syncthreads();
         }
         // the last turn's values: its first three operands have been read
+        if (C::bytes == 2 && care) gather_with_care(pf[1], now.v);
+        else
 #pragma unroll
         for (int e = 0; e < KS; e++) {
             if (e + 3 < KS) read_v(e + 3, now.v);
@@ -1361,7 +1521,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             if (d < a.dim)
                 *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[dt][i] * inv, o[dt][i + 1] * inv), pack16<X>(o[dt][i + 2] * inv, o[dt][i + 3] * inv)};
         }
-    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<C>::up + log2f(l)) * kLn2;
+    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<X, C>::up + log2f(l)) * kLn2;
 }
 
 // ------------------------------------------------------------ the splits' join
@@ -1464,7 +1624,7 @@ hipError_t launch_attend(const AttnArg& a, const Cut& c, hipStream_t s) {
     const auto join = [&](auto kernel) {
         if (c.splits <= 1) return;
         const uint32_t per = 256 / (DP / 4);
-        CKR_LAUNCH("kv_attention_join", s, kernel<<<dim3(a.tiles * a.kv_heads, (c.bm + per - 1) / per), 256, 0, s>>>(a, Prob<C>::up));
+        CKR_LAUNCH("kv_attention_join", s, kernel<<<dim3(a.tiles * a.kv_heads, (c.bm + per - 1) / per), 256, 0, s>>>(a, Prob<X, C>::up));
     };
     if (c.bm == kFewRows) {
         CKR_LAUNCH("kv_attention_few", s, attend_few_kernel<X, C, DP><<<dim3(c.blocks), 64 * kFewWaves, 0, s>>>(a));

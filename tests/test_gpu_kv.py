@@ -146,7 +146,7 @@ def _check(sq, cache, q, out, lse, fmt, group, window, scale=None):
     D = q.shape[2]
     k, v = (np.nan_to_num(_values(cache, n, fmt), nan=0.0) for n in ("k", "v"))
     ref = ko.attention(sq, k, v, q.cpu().double().numpy(), group, scale or D ** -0.5, window)
-    p_unit = ko.UNIT[torch.float16 if fmt == "f16" else torch.bfloat16]   # weights of 8-bit values are bfloat16
+    p_unit = ko.UNIT[q.dtype]   # weights are rounded to the queries' type
     bound, lbound = ko.attention_bounds(*ref, D, p_unit, q.dtype, np.abs(v).max())
     err = np.abs(out.cpu().double().numpy() - ref[0])
     print(f"  largest error / bound: {(err / bound).max():.3f}", flush=True)
@@ -224,6 +224,38 @@ def test_attention_poisoned_rows_show(gpu, lens):
     cache.v_scale[p, 0, slot] = float("nan")
     assert torch.isnan(plan.run(cache, b, q)).all()
     assert torch.isfinite(plan.run(cache, b, q, window=100)).all()
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,group,lens,window", [(128, 4, [3, 1], 0), (64, 1, [9, 2], 5), (128, 4, [40, 20], 0), (128, 4, [100, 90], 33),
+                                                   (64, 8, [70, 64], 40), (256, 2, [90, 10], 20)])
+def test_infinities_and_nan_in_16_bit_values_reach_who_sees_them_only(gpu, typ, dim, group, lens, window):
+    """Cached values that are infinite or NaN, in the chunk and before it: tokens
+    that see them give what 32-bit sums give (infinities and NaN in those
+    dimensions), tokens that do not (earlier ones, or past their window) the
+    same as with finite values in their place."""
+    print(f"[case] non-finite values {typ} dim={dim} group={group} {lens} window={window}", flush=True)
+    sq, cache, b, q, plan, out, lse = _attend(gpu, typ, typ, 2, group, dim, 16, [50, 0], lens, window)
+    clean = out.clone()
+    at = [(0, 45, 0, 3, float("inf")), (0, 51, 1, dim - 1, float("nan")), (0, 50 + lens[0] // 2, 0, 0, float("-inf")),
+          (0, 50 + lens[0] // 2, 0, 3, float("-inf")), (1, lens[1] - 1, 1, 7, float("inf"))]
+    for s, j, h, d, x in at:
+        p, slot = sq.place(s, j)
+        cache.v[p, h, slot, d] = x
+    got = plan.run(cache, b, q, window=window).float().cpu()
+    want = clean.float().cpu()
+    for s in range(2):
+        for i in range(lens[s]):
+            t, pos = int(sq.offsets[s]) + i, sq.starts[s] + i
+            for s2, j, h, d, x in at:
+                if s2 == s and j <= pos and not (window and j <= pos - window):
+                    want[t, h * group:(h + 1) * group, d] += x
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf])
+    fin = torch.isfinite(want)
+    # where nothing is hidden from anyone the sums are the same; values are never off by more than roundings
+    assert ((got - want)[fin].abs() <= 2 * ko.UNIT[q.dtype] * want[fin].abs() + 1e-2).all()
 
 
 @pytest.mark.parametrize("lens", [[1, 1], [60, 33]])
