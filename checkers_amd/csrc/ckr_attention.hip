@@ -1086,8 +1086,10 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     constexpr float kMost = Prob<X, C>::up == 0.f ? 256.f : Prob<X, C>::up == 6.f ? 16384.f : 32768.f;  // 2^(kLag + up)
     __shared__ __attribute__((aligned(16))) uint8_t s_k[Sh::RING * TK * KP];
     __shared__ __attribute__((aligned(16))) uint8_t s_v[Sh::RING * TK * VP];
-    __shared__ __attribute__((aligned(16))) float s_sk[Sh::RING + 1][TK];  // the last: ones, for scores that carry their scale
-    __shared__ __attribute__((aligned(16))) float s_sv[Sh::RING][TK];
+    constexpr int SCALES = C::bytes == 1 ? TK : 1;
+    __shared__ __attribute__((aligned(16))) float s_sk[Sh::RING + 1][SCALES];  // the last: ones, for scores that carry their scale
+    __shared__ __attribute__((aligned(16))) float s_sv[Sh::RING][SCALES];
+    __shared__ __attribute__((aligned(16))) uint8_t s_zero[C::bytes == 2 ? 32 * VP : 16];  // values of zero
     __shared__ uint32_t s_tmp[16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
@@ -1269,7 +1271,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     };
     // scores that some row of the wave must not see: scaled here, -inf where hidden.
     // 16-bit values: is there an infinity or NaN among them (care), and who sees which
-    // key; those keys' values are then gathered apart, and not by the next turn
+    // key; those keys' values are then gathered apart, and zeros by the next turn
     uint32_t seen = 0;
     bool care = false;
     const auto mask = [&](const float* at_fk, const uint8_t* at_v, int base, uint32_t valid) __attribute__((always_inline)) {
@@ -1310,7 +1312,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         }
     };
     struct Where { const uint8_t *k, *v; const float *fk, *fv; };  // what a turn reads: K(i+1), V(i-1), scales(i)
-    const auto turn = [&](auto sub_tag, float f, const Where& now, const Where& after, bool gathered, auto side) {
+    const auto turn = [&](auto sub_tag, float f, const Where& now, const Where& after, auto side) {
         constexpr int sub = decltype(sub_tag)::value;
         f32x16 z;
 #pragma unroll
@@ -1334,7 +1336,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             if constexpr (S % (16 / NM) == 0) {
                 constexpr int j = S * NM / 16, e = j / 2;
                 if constexpr (j % 2 == 0) {
-                    if (C::bytes == 1 || !gathered) o[e % DT] = mfma32<P>(vf[e % 4], pf[1 - sub][e / DT], o[e % DT]);
+                    o[e % DT] = mfma32<P>(vf[e % 4], pf[1 - sub][e / DT], o[e % DT]);
                     if constexpr (e + 3 < KS) read_v(e + 3, now.v);
                     else read_v(e + 3 - KS, after.v);
                 } else {
@@ -1397,7 +1399,9 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     };
 
     if (n_tiles > 0) {
-        if (wave == 0) s_sk[Sh::RING][lane] = 1.f;
+        if (C::bytes == 1 && wave == 0) s_sk[Sh::RING][lane] = 1.f;
+        if constexpr (C::bytes == 2)
+            for (uint32_t e = threadIdx.x; e < 32 * VP / 16; e += 512) *reinterpret_cast<u32x4*>(s_zero + e * 16) = u32x4{0, 0, 0, 0};
         // the first three tiles: their pages, then their rows, all on their way at once
         int32_t pages[3][4];
 #pragma unroll
@@ -1454,16 +1458,20 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             unroll<2>([&](auto sub_tag) {
                 constexpr int sub = decltype(sub_tag)::value;
                 const int base = i * TK + sub * 32;
-                const bool gathered = care;
-                if (C::bytes == 2 && care) gather_with_care(pf[1 - sub], now.v);
-                care = false;
+                if (C::bytes == 2 && care) {
+                    gather_with_care(pf[1 - sub], now.v);
+                    now.v = s_zero + v_lane;
+#pragma unroll
+                    for (int e = 0; e < 3; e++) vf[e] = u32x4{0, 0, 0, 0};
+                    care = false;
+                }
                 if (!full) mask(s_sk[cur] + sub * 32, s_v + cur * (TK * VP) + sub * 32 * VP, base, (uint32_t)(valid[0] >> (32 * sub)));
                 const float f = full ? a.scale2 : 1.f;
                 const bool full2 = full_at(valid[sub], base + 32);
                 const int slot2 = sub ? next : cur;
                 const Where after = {k_at(next, sub), v_at(cur, sub), s_sk[full2 ? slot2 : Sh::RING] + (1 - sub) * 32,
                                      s_sv[slot2] + (1 - sub) * 32};
-                turn(sub_tag, f, now, after, gathered, [&](auto step_tag) {
+                turn(sub_tag, f, now, after, [&](auto step_tag) {
                     constexpr int S = decltype(step_tag)::value;
                     if constexpr (sub == 0) {  // the next tile but one into LDS
                         if constexpr (S % 2 == 0 && S >= 4 && S / 2 - 2 < LOADS) store_rows(S / 2 - 2, third);
