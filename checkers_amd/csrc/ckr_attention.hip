@@ -38,8 +38,7 @@ struct AttnArg {
     uint32_t flip;  // 0x80008000 when scale is negative: the queries' signs are flipped instead
     KvBatch b;
     uint32_t tiles, splits, split_len;  // row tiles, key ranges of a tile, their length (a multiple of 128)
-    uint32_t* counters;  // few rows: parts of an item that are done, 0 between calls
-    uint32_t items;      // few rows: counters (offsets that ask for more are not a batch)
+    uint32_t* counters;  // few rows: parts done of the item that begins in a block and goes on in the next; 0 between calls
     uint32_t min_tiles;  // few rows: tiles of a wave's stretch at least
     float* part_o;  // [tile][kv head][split][rows of a tile][DP], with splits > 1
     float* part_m;  // [tile][kv head][split][rows of a tile][2]: maximum (in powers of two), sum
@@ -286,82 +285,80 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
     constexpr uint32_t THREADS = 64 * kFewWaves, QUADS = DP / 4;  // a row's outputs by fours
     __shared__ __attribute__((aligned(16))) float s_o[kFewWaves][kFewRows][DP + 4];
     __shared__ float s_m[kFewWaves][kFewRows][2];
-    __shared__ uint32_t s_sum[kFewWaves][2];
-    __shared__ uint32_t s_at[6];  // the block's first sequence, tiles of it before the block's, its first item; its rows, token, start
+    __shared__ uint32_t s_sum[kFewWaves];
+    __shared__ uint32_t s_at[5];  // the block's first sequence, tiles of it before the block's; its rows, token, start
     __shared__ uint32_t s_last;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
 
     // ---- this block's stretch of the line of key tiles (the launch has seen to it
     // that the line is shorter than 2^31)
-    struct Seq { uint32_t tiles, items, rows, token0; int32_t start; };
+    struct Seq { uint32_t tiles, rows, token0; int32_t start; };
     const auto count = [&](uint32_t seq) {
-        Seq q = {0, 0, 0, 0, 0};
+        Seq q = {0, 0, 0, 0};
         if (seq >= a.b.n_seqs) return q;
-        const int32_t from = a.b.offsets[seq], to = a.b.offsets[seq + 1];
+        const int32_t from = a.b.offsets[seq], to = min(a.b.offsets[seq + 1], (int32_t)a.b.n_tokens);
         q.start = a.b.starts[seq];
-        q.rows = from >= 0 && min(to, (int32_t)a.b.n_tokens) > from ? (uint32_t)(min(to, (int32_t)a.b.n_tokens) - from) * a.group : 0;
+        q.rows = from >= 0 && to > from ? (uint32_t)(to - from) * a.group : 0;
         q.token0 = (uint32_t)from;
-        for (uint32_t r = 0; r < q.rows; r += kFewRows) q.tiles += few_tiles(few_span(a, q.start, r, q.rows)), q.items++;
-        q.tiles *= a.kv_heads, q.items *= a.kv_heads;
+        for (uint32_t r = 0; r < q.rows; r += kFewRows) q.tiles += few_tiles(few_span(a, q.start, r, q.rows));
+        q.tiles *= a.kv_heads;
         return q;
     };
-    // inclusive sums over the block's threads, and the block's totals
-    const auto scan = [&](uint32_t& tiles, uint32_t& items, uint32_t& all_tiles, uint32_t& all_items) {
+    // inclusive sum over the block's threads, and the block's total
+    const auto scan = [&](uint32_t tiles, uint32_t& all) {
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-            const uint32_t x = (uint32_t)__shfl_up((int)tiles, d), y = (uint32_t)__shfl_up((int)items, d);
-            if (lane >= (uint32_t)d) tiles += x, items += y;
+            const uint32_t x = (uint32_t)__shfl_up((int)tiles, d);
+            if (lane >= (uint32_t)d) tiles += x;
         }
         __syncthreads();
-        if (lane == 63) s_sum[wave][0] = tiles, s_sum[wave][1] = items;
+        if (lane == 63) s_sum[wave] = tiles;
         __syncthreads();
-        all_tiles = all_items = 0;
+        all = 0;
 #pragma unroll
         for (uint32_t w = 0; w < kFewWaves; w++) {
-            if (w == wave) tiles += all_tiles, items += all_items;
-            all_tiles += s_sum[w][0], all_items += s_sum[w][1];
+            if (w == wave) tiles += all;
+            all += s_sum[w];
         }
+        return tiles;
     };
+    uint32_t total;
     const Seq q0 = count(threadIdx.x);
-    uint32_t incl = q0.tiles, incl_items = q0.items, total, items;
-    scan(incl, incl_items, total, items);
-    const uint32_t first_total = total, first_items = items;
+    const uint32_t upto0 = scan(q0.tiles, total), total0 = total;
     for (uint32_t base = THREADS; base < a.b.n_seqs; base += THREADS) {
-        const Seq x = count(base + threadIdx.x);
-        uint32_t n = x.tiles, it = x.items, more, more_items;
-        scan(n, it, more, more_items);
-        total += more, items += more_items;
+        uint32_t more;
+        scan(count(base + threadIdx.x).tiles, more);
+        total += more;
     }
-    if (items > a.items) return;
     const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, a.min_tiles);
     if ((uint64_t)blockIdx.x * per >= total) return;
     const uint32_t p_begin = blockIdx.x * per, p_end = min(p_begin + per, total);
     {
-        const auto find = [&](uint32_t seq, const Seq& x, uint32_t upto, uint32_t upto_items) {
+        const auto find = [&](uint32_t seq, const Seq& x, uint32_t upto) {
             if (p_begin >= upto - x.tiles && p_begin < upto) {
-                s_at[0] = seq, s_at[1] = p_begin - (upto - x.tiles), s_at[2] = upto_items - x.items;
-                s_at[3] = x.rows, s_at[4] = x.token0, s_at[5] = (uint32_t)x.start;
+                s_at[0] = seq, s_at[1] = p_begin - (upto - x.tiles);
+                s_at[2] = x.rows, s_at[3] = x.token0, s_at[4] = (uint32_t)x.start;
             }
         };
-        find(threadIdx.x, q0, incl, incl_items);
-        uint32_t before = first_total, before_items = first_items;
+        find(threadIdx.x, q0, upto0);
+        uint32_t before = total0;
         for (uint32_t base = THREADS; base < a.b.n_seqs; base += THREADS) {
             const Seq x = count(base + threadIdx.x);
-            uint32_t n = x.tiles, it = x.items, more, more_items;
-            scan(n, it, more, more_items);
-            find(base + threadIdx.x, x, before + n, before_items + it);
-            before += more, before_items += more_items;
+            uint32_t more;
+            const uint32_t upto = scan(x.tiles, more);
+            find(base + threadIdx.x, x, before + upto);
+            before += more;
         }
         __syncthreads();
     }
     const auto scalar = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); };
-    uint32_t seq = scalar(s_at[0]), in_seq = scalar(s_at[1]), item0 = scalar(s_at[2]), rows = scalar(s_at[3]), token0 = scalar(s_at[4]), row0 = 0;
-    int32_t start = (int32_t)scalar(s_at[5]);
+    uint32_t seq = scalar(s_at[0]), in_seq = scalar(s_at[1]), rows = scalar(s_at[2]), token0 = scalar(s_at[3]), row0 = 0;
+    int32_t start = (int32_t)scalar(s_at[4]);
     // the item that the stretch begins in
     FewSpan span = few_span(a, start, 0, rows);
     uint32_t nt = few_tiles(span);
     while (in_seq >= nt * a.kv_heads) {
-        in_seq -= nt * a.kv_heads, row0 += kFewRows, item0 += a.kv_heads;
+        in_seq -= nt * a.kv_heads, row0 += kFewRows;
         span = few_span(a, start, row0, rows), nt = few_tiles(span);
     }
     uint32_t kvh = scalar(in_seq / nt), t0 = scalar(in_seq % nt);
@@ -685,7 +682,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part has arrived
             __syncthreads();                                  // and the block's
             const uint32_t begin = p - t0, b_first = begin / per, parts = (begin + nt - 1) / per - b_first + 1;
-            uint32_t* const counter = a.counters + item0 + kvh;
+            uint32_t* const counter = a.counters + b_first;  // one item at most begins in a block and goes on
             if (threadIdx.x == 0) {
                 const uint32_t seen = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 s_last = seen + 1 == parts;
@@ -735,7 +732,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
         if (p >= p_end) break;
         t0 = 0;
         if (++kvh < a.kv_heads) continue;
-        kvh = 0, row0 += kFewRows, item0 += a.kv_heads;
+        kvh = 0, row0 += kFewRows;
         while (row0 >= rows) {  // p < p_end: there is one
             const int32_t from = a.b.offsets[++seq], to = min(a.b.offsets[seq + 1], (int32_t)a.b.n_tokens);
             row0 = 0, rows = from >= 0 && to > from ? (uint32_t)(to - from) * a.group : 0;
@@ -1567,7 +1564,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttnArg a, float up) {
 // tile may be short), key ranges of a tile.
 struct Cut {
     uint32_t bm, dp, tiles, splits, split_len, blocks, min_tiles;
-    uint64_t counter_bytes, part_m_bytes, bytes;  // of the workspace: counters, the rows' maxima and sums, their outputs
+    uint64_t part_m_bytes, bytes;  // of the workspace: counters, the rows' maxima and sums, their outputs
 };
 constexpr uint64_t kSplitMin = 128;   // keys of a split at least
 constexpr uint32_t kFewBlocks = 512;  // blocks of the few rows' kernel: two a CU
@@ -1577,10 +1574,12 @@ uint32_t padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 2
 uint64_t most_tiles(uint32_t bm, uint64_t group, uint64_t n_seqs, uint64_t n_tokens) {
     return std::min(n_tokens * group / bm + std::min(n_seqs, n_tokens), n_tokens * ((group + bm - 1) / bm));
 }
-// The workspace of c.counter_bytes counters and `rows` rows of parts.
-void set_bytes(Cut& c, uint64_t counters, uint64_t rows) {
-    c.counter_bytes = (counters * 4 + 255) / 256 * 256, c.part_m_bytes = (rows * 8 + 255) / 256 * 256;
-    c.bytes = c.counter_bytes + c.part_m_bytes + rows * c.dp * 4;
+// The workspace begins with the counters, whatever else a call keeps in it: they
+// are 0 between calls, the rest is not.
+constexpr uint64_t kCounterBytes = kFewBlocks * 4;
+void set_bytes(Cut& c, uint64_t rows) {
+    c.part_m_bytes = (rows * 8 + 255) / 256 * 256;
+    c.bytes = kCounterBytes + c.part_m_bytes + rows * c.dp * 4;
 }
 uint32_t few_blocks(uint64_t items, uint64_t max_context) {
     return (uint32_t)std::min<uint64_t>(items * ((max_context + 31) / 32) / kFewTiles + 1, kFewBlocks);
@@ -1600,14 +1599,14 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     if (c.bm == kFewRows) {
         c.min_tiles = kFewTiles;
         c.blocks = few_blocks(items, max_context);
-        set_bytes(c, items, (uint64_t)c.blocks * 2 * kFewRows);
+        set_bytes(c, (uint64_t)c.blocks * 2 * kFewRows);
         return c;
     }
     const uint64_t most = std::max<uint64_t>((max_context + kSplitMin - 1) / kSplitMin, 1);
     const uint64_t splits = std::min(std::max<uint64_t>(blocks_wanted(c.bm) / items, 1), most);
     c.split_len = (uint32_t)std::min<uint64_t>((std::max<uint64_t>(max_context, 1) + splits * kSplitMin - 1) / (splits * kSplitMin) * kSplitMin, 1u << 31);
     c.splits = (uint32_t)std::max<uint64_t>((max_context + c.split_len - 1) / c.split_len, 1);
-    if (c.splits > 1) set_bytes(c, 0, items * c.splits * c.bm);
+    if (c.splits > 1) set_bytes(c, items * c.splits * c.bm);
     return c;
 }
 // What cut() asks for at most, for any batch up to these sizes.
@@ -1616,11 +1615,11 @@ uint64_t most_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_se
     Cut c{};
     c.dp = padded_dim(dim);
     uint64_t items = std::max<uint64_t>(most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv, 1);
-    set_bytes(c, items, (uint64_t)few_blocks(items, max_context) * 2 * kFewRows);
+    set_bytes(c, (uint64_t)few_blocks(items, max_context) * 2 * kFewRows);
     uint64_t most = c.bytes;
     for (const uint32_t bm : {kManyRows, kWideRows}) {
         items = most_tiles(bm, group, n_seqs, n_tokens) * n_kv;
-        set_bytes(c, 0, std::min(blocks_wanted(bm), items * ((max_context + kSplitMin - 1) / kSplitMin)) * bm);
+        set_bytes(c, std::min(blocks_wanted(bm), items * ((max_context + kSplitMin - 1) / kSplitMin)) * bm);
         if (max_context > kSplitMin) most = std::max(most, c.bytes);
     }
     return most;
@@ -1710,15 +1709,15 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
                       std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size),
                       (uint64_t)batch->table_width * cache->page_size, window, near_slots);
     if ((uint64_t)c.tiles * cache->n_heads * 512 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
-    a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len, a.min_tiles = c.min_tiles, a.items = c.tiles * cache->n_heads;
+    a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len, a.min_tiles = c.min_tiles;
     if (c.bytes) {
         if (workspace_bytes < c.bytes)
             return err(CKR_E_CAPACITY, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(c.bytes) + " needed");
         if (reinterpret_cast<uintptr_t>(d_workspace) % 256) return err(CKR_E_INVALID, "workspace must be aligned to 256 bytes");
         if ((rc = check_range(d_workspace, c.bytes, "workspace"))) return rc;
         a.counters = static_cast<uint32_t*>(d_workspace);
-        a.part_m = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) + c.counter_bytes);
-        a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) + c.counter_bytes + c.part_m_bytes);
+        a.part_m = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) + kCounterBytes);
+        a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) + kCounterBytes + c.part_m_bytes);
     }
     const hipStream_t s = (hipStream_t)stream;
     hipError_t e;

@@ -409,3 +409,121 @@ def test_refusals(gpu):
     small._c.d_page_table = 0x1000                     # not device memory
     bad("page table", ck.kv_write, cache, small, kv, kv)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("fmt", ["f8", "f16"])
+def test_many_sequences_and_wrong_hints(gpu, fmt):
+    """More sequences than a block has threads (some empty), one token each and
+    ragged; max_chunk and max_context far from the truth on both sides."""
+    r = np.random.default_rng(3)
+    n = 700
+    for lens in ([1] * n, [int(x) for x in r.integers(0, 4, n)]):
+        starts = [int(x) for x in r.integers(0, 90, n)]
+        sq = ko.Seqs(starts, lens, 16, seed=1)
+        cache = _cache(sq, 1, 64, fmt, gpu)
+        b = _batch(sq, gpu)
+        _fill(sq, cache, b, 1, 64, "f16", gpu, 3)
+        q = torch.randn(sq.tokens, 4, 64, device=gpu).half()
+        plan = ck.KvAttention(4, 1, 64, n, sq.tokens)
+        outs = []
+        for chunk, context in ((max(lens), 100), (1, 1), (1000, 1 << 20), (40, 3)):
+            print(f"[case] many sequences {fmt} hints {chunk} {context}", flush=True)
+            b2 = ck.KvBatch(b.page_table, b.starts, b.offsets, sq.tokens, chunk, context)
+            lse = torch.empty(sq.tokens, 4, device=gpu)
+            outs.append(plan.run(cache, b2, q, lse=lse))
+            torch.cuda.synchronize()
+            if len(outs) in (1, 4):
+                _check(sq, cache, q, outs[-1], lse, fmt, 4, 0)
+            else:
+                assert ((outs[-1].float() - outs[0].float()).abs() < 0.02).all()
+
+
+def test_long_chunks_with_hints_of_one_token(gpu):
+    """The kernel for few rows given long chunks, and the other way round."""
+    sq = ko.Seqs([40, 0, 300], [90, 33, 1], 32, seed=1)
+    for fmt, dim in (("f8", 128), ("bf16", 64), ("i8", 256)):
+        cache = _cache(sq, 2, dim, fmt, gpu)
+        b = _batch(sq, gpu)
+        _fill(sq, cache, b, 2, dim, "bf16", gpu, 3)
+        q = torch.randn(sq.tokens, 10, dim, device=gpu).to(torch.bfloat16)
+        plan = ck.KvAttention(10, 2, dim, 3, sq.tokens)
+        for window in (0, 50):
+            for chunk in (1, 10, 500):
+                print(f"[case] hints {fmt} {dim} window={window} chunk={chunk}", flush=True)
+                lse = torch.empty(sq.tokens, 10, device=gpu)
+                out = plan.run(cache, ck.KvBatch(b.page_table, b.starts, b.offsets, sq.tokens, chunk, 7), q, window=window, lse=lse)
+                torch.cuda.synchronize()
+                _check(sq, cache, q, out, lse, fmt, 5, window)
+
+
+def test_offsets_that_are_no_batch_stay_in_bounds(gpu):
+    """Chunks that overlap, run backwards or past the end: nothing outside the
+    tensors is read or written, and the next call is right."""
+    sq = ko.Seqs([40, 10, 60], [5, 7, 3], 16, seed=1)
+    cache = _cache(sq, 1, 64, "f8", gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 1, 64, "bf16", gpu, 3)
+    q = torch.randn(sq.tokens, 4, 64, device=gpu).to(torch.bfloat16)
+    kv = [torch.randn(sq.tokens, 1, 64, device=gpu).to(torch.bfloat16) for _ in range(2)]
+    plan = ck.KvAttention(4, 1, 64, 3, sq.tokens)
+    for offsets in ([0, 15, 3, 15], [-5, 2, 100, 15], [0, 15, 0, 15], [9, 9, 9, 9]):
+        for chunk in (1, 10, 100):
+            print(f"[case] offsets {offsets} {chunk}", flush=True)
+            bad = ck.KvBatch(b.page_table, b.starts, torch.tensor(offsets, dtype=torch.int32, device=gpu), sq.tokens, chunk, 100)
+            hold = torch.full((sq.tokens + 8, 4, 64), 3.0, device=gpu).to(torch.bfloat16)
+            plan.run(cache, bad, q, out=hold[4:-4])
+            torch.cuda.synchronize()
+            assert (hold[:4] == 3).all() and (hold[-4:] == 3).all()
+            ck.kv_read(cache, bad, ck.BF16, out=(hold[4:-4, :1], hold[4:-4, 1:2]))
+            torch.cuda.synchronize()
+            assert (hold[:4] == 3).all() and (hold[-4:] == 3).all()
+    lse = torch.empty(sq.tokens, 4, device=gpu)
+    _check(sq, cache, q, plan.run(cache, b, q, lse=lse), lse, "f8", 4, 0)
+
+
+def test_slots_far_apart(gpu):
+    """A cache whose slots lie 80 MB from each other (offsets of a page past 32 bits),
+    and one workspace for batches of several sizes."""
+    far = 80 << 20
+    buf = torch.empty(16 * far + (64 << 10), dtype=torch.int8, device=gpu)
+    sq = ko.Seqs([20], [90], 16)
+    k, v = (torch.as_strided(buf, (sq.n_pages, 2, 16, 128), (256, 128, far, 1), 32768 * i) for i in range(2))
+    cache = ck.KvCache(k, v, *(torch.zeros(sq.n_pages, 2, 16, device=gpu) for _ in range(2)))
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 128, "bf16", gpu, 3)
+    q = torch.randn(90, 8, 128, device=gpu).to(torch.bfloat16)
+    plan = ck.KvAttention(8, 2, 128, 1, 90)
+    lse = torch.empty(90, 8, device=gpu)
+    _check(sq, cache, q, plan.run(cache, b, q, lse=lse), lse, "i8", 4, 0)
+    for n in (1, 30, 2):
+        one = ko.Seqs([20], [n], 16)
+        one.table, one.n_pages = sq.table, sq.n_pages
+        lse = torch.empty(n, 8, device=gpu)
+        _check(one, cache, q[:n], plan.run(cache, _batch(one, gpu), q[:n], lse=lse), lse, "i8", 4, 0)
+
+
+def test_one_workspace_for_calls_of_every_kind(gpu):
+    """Calls that split the keys over blocks in the three ways there are, in turn on
+    one workspace: each is right, and repeats bit for bit."""
+    for dim in (64, 128):
+        sq0 = ko.Seqs([0, 0], [700, 900], 16, seed=4)
+        cache = _cache(sq0, 2, dim, "f8", gpu)
+        _fill(sq0, cache, _batch(sq0, gpu), 2, dim, "bf16", gpu, 3)
+        plan = ck.KvAttention(8, 2, dim, 2, 400)
+        first = {}
+        for turn in range(3):
+            for lens in ([1, 1], [150, 90], [1, 2], [20, 30], [4, 4], [1, 1]):
+                print(f"[case] one workspace dim={dim} {lens}", flush=True)
+                sq = ko.Seqs([500, 800], lens, 16)
+                sq.table, sq.n_pages = sq0.table, sq0.n_pages
+                g = torch.Generator(device=gpu).manual_seed(sum(lens))
+                q = torch.randn(sq.tokens, 8, dim, generator=g, device=gpu).to(torch.bfloat16)
+                lse = torch.empty(sq.tokens, 8, device=gpu)
+                out = plan.run(cache, _batch(sq, gpu), q, lse=lse)
+                torch.cuda.synchronize()
+                if turn == 0:
+                    _check(sq, cache, q, out, lse, "f8", 4, 0)
+                key = tuple(lens)
+                if key in first:
+                    assert torch.equal(first[key][0], out) and torch.equal(first[key][1], lse)
+                first.setdefault(key, (out, lse))
