@@ -39,7 +39,7 @@ struct AttnArg {
     KvBatch b;
     uint32_t tiles, splits, split_len;  // row tiles, key ranges of a tile, their length (a multiple of 128)
     uint32_t* counters;  // few rows: parts done of the item that begins in a block and goes on in the next; 0 between calls
-    uint32_t min_tiles;  // few rows: tiles of a wave's stretch at least
+    uint32_t min_tiles;  // few rows: tiles of a block's stretch at least
     float* part_o;  // [tile][kv head][split][rows of a tile][DP], with splits > 1
     float* part_m;  // [tile][kv head][split][rows of a tile][2]: maximum (in powers of two), sum
 };
@@ -179,10 +179,10 @@ template <int N, typename F> __device__ __forceinline__ void unroll(F f) { unrol
 
 // Which sequence and rows a tile of BM rows is: rows of a sequence are its
 // chunk's tokens times the query heads of a key/value head, in that order.
-// Every thread of the block calls it; s_tmp: a word of LDS per wave and two more.
+// Every thread of the block calls it; s_tmp: a word of LDS per wave and five more.
 struct Tile {
     uint32_t seq, row0, rows, token0;  // rows: of the whole sequence; token0: its first packed row
-    int64_t start, end;                // the position of its first token, and after its last
+    int64_t start;                     // the position of its first token
 };
 template <uint32_t BM, uint32_t THREADS = 256>
 __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint32_t tile, uint32_t* s_tmp, Tile& t) {
@@ -192,8 +192,9 @@ __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint
     for (uint32_t base = 0; base < b.n_seqs; base += THREADS) {
         const uint32_t i = base + threadIdx.x;
         uint32_t n = 0;
+        int32_t lo = 0, hi = 0, start = 0;
         if (i < b.n_seqs) {
-            const int32_t lo = b.offsets[i], hi = min(b.offsets[i + 1], (int32_t)b.n_tokens);
+            lo = b.offsets[i], hi = min(b.offsets[i + 1], (int32_t)b.n_tokens), start = b.starts[i];
             n = lo >= 0 && hi > lo ? ((uint32_t)(hi - lo) * group + BM - 1) / BM : 0;
         }
         uint32_t sum = n;
@@ -212,12 +213,14 @@ __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint
         }
         if (tile < done + all) {
             const uint32_t first = before + sum - n;
-            if (tile >= first && tile < first + n) s_tmp[WAVES] = i, s_tmp[WAVES + 1] = tile - first;
+            if (tile >= first && tile < first + n) {
+                s_tmp[WAVES] = i, s_tmp[WAVES + 1] = tile - first;
+                s_tmp[WAVES + 2] = (uint32_t)lo, s_tmp[WAVES + 3] = (uint32_t)hi, s_tmp[WAVES + 4] = (uint32_t)start;
+            }
             __syncthreads();
-            t.seq = s_tmp[WAVES], t.row0 = s_tmp[WAVES + 1] * BM;
-            const int32_t lo = b.offsets[t.seq], hi = min(b.offsets[t.seq + 1], (int32_t)b.n_tokens);
-            t.token0 = (uint32_t)lo, t.rows = (uint32_t)(hi - lo) * group;
-            t.start = b.starts[t.seq], t.end = t.start + (hi - lo);
+            t.seq = s_tmp[WAVES], t.row0 = s_tmp[WAVES + 1] * BM, t.token0 = s_tmp[WAVES + 2];
+            t.rows = (s_tmp[WAVES + 3] - t.token0) * group;
+            t.start = (int32_t)s_tmp[WAVES + 4];
             return true;
         }
         done += all;
@@ -773,7 +776,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     __shared__ __attribute__((aligned(16))) float s_sk[2][TK];
     __shared__ __attribute__((aligned(16))) float s_sv[2][TK];
     __shared__ uint64_t s_valid[2];
-    __shared__ uint32_t s_tmp[8];
+    __shared__ uint32_t s_tmp[16];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
     Tile t;
@@ -1402,11 +1405,13 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         // the first three tiles: their pages, then their rows, all on their way at once
         int32_t pages[3][4];
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-            load_pages(i * TK);
+        for (int i = 0; i < 3; i++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) pages[i][g] = pg[g];
-        }
+            for (int g = 0; g < 4; g++) pages[i][g] = table[min(c0 + ((in0 + (uint32_t)(i * TK + 16 * g)) >> a.page_shift), last_col)];
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) pages[i][g] = ((i * TK + 16 * g < end) & ((uint32_t)pages[i][g] < a.n_pages)) ? pages[i][g] : -1;
         u32x4 rows[3][LOADS];
         float scales[3][2], row_scales[3][LOADS];
 #pragma unroll
@@ -1533,7 +1538,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
 // The splits of a row, in their order: 4 dimensions a thread.
 template <typename X, int DP, uint32_t BM>
 __global__ void __launch_bounds__(256) attend_join_kernel(AttnArg a, float up) {
-    __shared__ uint32_t s_tmp[8];
+    __shared__ uint32_t s_tmp[16];
     const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
     Tile t;
     if (!find_tile<BM>(a.b, a.group, tile, s_tmp, t)) return;
@@ -1568,7 +1573,16 @@ struct Cut {
 };
 constexpr uint64_t kSplitMin = 128;   // keys of a split at least
 constexpr uint32_t kFewBlocks = 512;  // blocks of the few rows' kernel: two a CU
-constexpr uint32_t kFewTiles = 4;     // its tiles of 32 keys a block at least
+// Its tiles of 32 keys a block at least: one a wave (one token over a thousand: 9.5 us;
+// 11.0 with 8, 13.5 with 16).
+constexpr uint32_t kFewTiles = 4;
+// Rows of a chunk up to which it is taken, in tiles of 16 that each read the cache; us,
+// few / many rows, e4m3, 8 heads of 128: 32 rows of 16 sequences over 4096 tokens 55 / 75, of one
+// over 32768 43 / 80, of 64 over 1024 55 / 57; 64 rows of 64 over 1024 100 / 58.
+constexpr uint32_t kFewMost = 32;
+// Rows from which on a tile of 256 pays: 128 rows of 16 sequences over 4096 tokens 108
+// (many) / 131 (very many), 256 rows 150 / 134; 256 of one over 32768 100 / 95.
+constexpr uint32_t kManyMost = 128;
 uint64_t blocks_wanted(uint32_t bm) { return bm == kManyRows ? 512 : 256; }
 uint32_t padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 uint64_t most_tiles(uint32_t bm, uint64_t group, uint64_t n_seqs, uint64_t n_tokens) {
@@ -1589,8 +1603,8 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     Cut c{};
     const uint64_t group = n_heads / n_kv, rows = (uint64_t)max_chunk * group;
     c.dp = padded_dim(dim);
-    const bool few = rows <= kFewRows && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1) < (1ull << 31);
-    c.bm = few ? kFewRows : rows <= kManyRows || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
+    const bool few = rows <= kFewMost && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1) < (1ull << 31);
+    c.bm = few ? kFewRows : rows <= kManyMost || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
     c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
     c.splits = 1;
     // the keys of a tile: a window's, and as many again as the tile has tokens
