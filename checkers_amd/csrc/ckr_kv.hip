@@ -56,7 +56,11 @@ __device__ __forceinline__ uint32_t first_seq(const KvBatch& b, uint32_t token) 
 }
 
 // One kernel for both directions: WRITE quantises packed rows (of X) into the
-// cache's pages (of C), otherwise the cached rows become values of X.
+// cache's pages (of C), otherwise the cached rows become values of X.  Bound by
+// memory, each row read and written once: bfloat16 to e4m3, 21604 tokens of 8 heads of
+// 128, 134 MB written in 29.6 us with the launch (23.2 alone: 5.8 TB/s, part of it out
+// of the last cache); read back, 124592 tokens in 171 us (4.5 TB/s; a copy reaches 4.7
+// to 5.2).  Stores and loads that pass the caches by measured slower in both.
 template <typename X, typename C, int LPR, bool WRITE>
 __global__ void __launch_bounds__(256) kv_rows_kernel(RowsArg a) {
     constexpr uint32_t ROWS = 256 / LPR;
@@ -177,31 +181,40 @@ struct NormArg {
     float* scales;
     uint8_t* total;
     int64_t x_stride, r_stride, out_stride, total_stride;
-    uint64_t row0;
+    uint64_t row0, rows;  // of this launch
     uint32_t n, group;
     float eps;
     int w_f32;
     int wide;  // every row starts on a 16-byte boundary (8-bit output: 8) and n is a multiple of 8
 };
 
-// A row per block.  Thread t holds the 8 values from 8 (t + v THREADS) on, for
-// v < VPT, so a row is read once and stays in registers through both
-// reductions (the sum of squares, then the largest magnitude).
+// THREADS threads a row (a block of at least 256 holds several rows of fewer).
+// Thread t of a row holds the 8 values from 8 (t + v THREADS) on, for v < VPT, so a
+// row is read once and stays in registers through both reductions (the sum of
+// squares, then the largest magnitude).  Bound by memory: rows of 8192 in float16,
+// 16384 of them with residual, total and codes by 128, 943 MB in 181 us (5.2 TB/s, what
+// a copy reaches); 2048 rows of 4096 in 12.3 us; one row 3.5 us, of which the kernel
+// can save nothing (a load, two reductions, a store).
 template <typename E, typename O, int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(NormArg a) {
-    const uint64_t row = a.row0 + blockIdx.x;
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_kernel(NormArg a) {
+    constexpr uint32_t ROWS = THREADS < 256 ? 256 / THREADS : 1;
+    static_assert(THREADS <= 64 || THREADS >= 256, "a row of several waves has its block to itself");
+    const uint32_t tid = threadIdx.x % THREADS;
+    uint64_t row = (uint64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+    if (row >= a.rows) return;
+    row += a.row0;
     const uint8_t* x = a.x + (int64_t)row * a.x_stride * E::bytes;
     const uint8_t* r = a.r ? a.r + (int64_t)row * a.r_stride * E::bytes : nullptr;
     uint8_t* total = a.total ? a.total + (int64_t)row * a.total_stride * E::bytes : nullptr;
     uint8_t* out = a.out + (int64_t)row * a.out_stride * O::bytes;
-    constexpr int WAVES = THREADS / 64;
+    constexpr int WAVES = THREADS < 64 ? 1 : THREADS / 64;
     __shared__ float s_sum[WAVES];
     __shared__ uint32_t s_top[WAVES];
     float h[VPT][8];
     float sum = 0.f;
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
-        const uint32_t col = (v * THREADS + threadIdx.x) * 8;
+        const uint32_t col = (v * THREADS + tid) * 8;
         float q[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) h[v][i] = q[i] = 0.f;
@@ -225,7 +238,7 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(NormArg a) {
         }
     }
 #pragma unroll
-    for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+    for (int d = std::min(THREADS, 64) / 2; d; d /= 2) sum += __shfl_xor(sum, d);
     if constexpr (WAVES > 1) {
         if (threadIdx.x % 64 == 0) s_sum[threadIdx.x / 64] = sum;
         __syncthreads();
@@ -237,7 +250,7 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(NormArg a) {
     uint32_t top = 0;
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
-        const uint32_t col = (v * THREADS + threadIdx.x) * 8;
+        const uint32_t col = (v * THREADS + tid) * 8;
         float w[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) w[i] = 0.f;
@@ -276,7 +289,7 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(NormArg a) {
     if constexpr (O::bytes == 1) {
         if (!a.group) {
 #pragma unroll
-            for (int d = 32; d; d /= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+            for (int d = std::min(THREADS, 64) / 2; d; d /= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
             if constexpr (WAVES > 1) {
                 if (threadIdx.x % 64 == 0) s_top[threadIdx.x / 64] = top;
                 __syncthreads();
@@ -289,12 +302,12 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(NormArg a) {
             for (int v = 0; v < VPT; v++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) h[v][i] = scaled(h[v][i], rs.inv);
-            if (threadIdx.x == 0) a.scales[row] = rs.scale;
+            if (tid == 0) a.scales[row] = rs.scale;
         }
     }
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
-        const uint32_t col = (v * THREADS + threadIdx.x) * 8;
+        const uint32_t col = (v * THREADS + tid) * 8;
         if (a.wide) {
             if (col < a.n) store_vec<O, 8>(out + (int64_t)col * O::bytes, h[v]);
         } else {
@@ -309,15 +322,25 @@ template <typename E, typename O>
 hipError_t launch_norm(const NormArg& a, uint64_t rows, hipStream_t s) {
     const auto go = [&](auto kernel, uint32_t threads) {
         constexpr uint64_t kMost = 1u << 21;  // blocks of a launch: a grid holds fewer than 2^32 threads
-        for (uint64_t r0 = 0; r0 < rows; r0 += kMost) {
+        const uint64_t per = threads < 256 ? 256 / threads : 1;
+        for (uint64_t r0 = 0; r0 < rows; r0 += kMost * per) {
             NormArg b = a;
-            b.row0 = r0;
-            CKR_LAUNCH("add_rms_norm", s, kernel<<<dim3((uint32_t)std::min(rows - r0, kMost)), threads, 0, s>>>(b));
+            b.row0 = r0, b.rows = std::min(rows - r0, kMost * per);
+            CKR_LAUNCH("add_rms_norm", s, kernel<<<dim3((uint32_t)((b.rows + per - 1) / per)), std::max(threads, 256u), 0, s>>>(b));
         }
         return hipGetLastError();
     };
+    // The fewest threads whose registers hold a row in at most four loads of a tensor:
+    // one wave has no barrier, and blocks of four rows keep more loads on their way.
+    // bfloat16 with residual to e4m3, 469 MB in all, us here / otherwise: 256 values 95 /
+    // 154 (a wave a row), 425 (256 threads); 1024: 87 / 140 (256 threads); 2048: 93, and 12 /
+    // 13.5 with 59 MB (256 threads); 4096: 84 / 90 (512 threads); 8192: 92 / 99 (1024
+    // threads); 16384: 88 / 121 (256 threads, eight loads).
+    if (a.n <= 128) return go(add_rms_norm_kernel<E, O, 16, 1>, 16);
+    if (a.n <= 256) return go(add_rms_norm_kernel<E, O, 32, 1>, 32);
     if (a.n <= 512) return go(add_rms_norm_kernel<E, O, 64, 1>, 64);
-    if (a.n <= 2048) return go(add_rms_norm_kernel<E, O, 256, 1>, 256);
+    if (a.n <= 1024) return go(add_rms_norm_kernel<E, O, 64, 2>, 64);
+    if (a.n <= 2048) return go(add_rms_norm_kernel<E, O, 64, 4>, 64);
     if (a.n <= 4096) return go(add_rms_norm_kernel<E, O, 256, 2>, 256);
     if (a.n <= 8192) return go(add_rms_norm_kernel<E, O, 256, 4>, 256);
     if (a.n <= 16384) return go(add_rms_norm_kernel<E, O, 1024, 2>, 1024);

@@ -58,6 +58,22 @@ def test_norm(gpu, typ, rows, n):
                 _check(x, res, wt, 1e-5, out, scales, total, fmt, group)
 
 
+@pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,n", [(33, 8), (17, 100), (16, 128), (15, 129), (9, 256), (7, 257), (6, 768), (5, 1024), (7, 1500)])
+def test_norm_of_short_rows(gpu, typ, rows, n):
+    """Rows that share a block, the last block partly filled."""
+    t = TYPES[typ]
+    x, r = ((torch.randn(rows, n, device=gpu) * s).to(t) for s in (1.0, 3.0))
+    w = torch.randn(n, device=gpu).to(t)
+    for fmt, group in ((typ, 0), ("f8", 0), ("i8", 0), ("f8", 32), ("i8", 64), ("f8", 128), ("i8", 256)):
+        if group and n % group:
+            continue
+        print(f"[case] norm short {typ} {rows}x{n} -> {fmt} group={group}", flush=True)
+        out, scales, total = ck.add_rms_norm(x, r, w, 1e-5, TAGS[fmt], group=group)
+        torch.cuda.synchronize()
+        _check(x, r, w, 1e-5, out, scales, total, fmt, group)
+
+
 @pytest.mark.parametrize("typ", ["bf16", "f32"])
 def test_norm_strides_and_alignment(gpu, typ):
     """Rows inside wider ones, starting at odd elements; outputs likewise."""
