@@ -549,7 +549,8 @@ CKR_API int ckr_make_contiguous(const void* d_src, int ndim, const int64_t* shap
 
 /* A paged cache: keys and values [n_pages][n_heads][page_size][head_dim] in any
  * order of the first three axes (strides in elements, >= 0; the last axis is
- * contiguous).  dtype CKR_F8 or CKR_I8, with a scale per (page, head, slot) whose
+ * contiguous).  A CKR_F8 cache that another program fills holds no NaN codes
+ * (ckr_kv_write stores none).  dtype CKR_F8 or CKR_I8, with a scale per (page, head, slot) whose
  * slots are contiguous, or CKR_BF16 / CKR_F16 without scales.  page_size is a
  * power of two from 16 on, head_dim a multiple of 16 up to 256; every row must
  * start on a 16-byte boundary, every page's scales of a head too. */
@@ -606,7 +607,8 @@ CKR_API int ckr_kv_read(const ckr_kv_cache* cache, const ckr_kv_batch* batch, vo
  * of s with p - window < j <= p (window 0: all j <= p) on mapped pages.  Query
  * head h uses key/value head h / (n_heads / cache->n_heads).  d_q and d_out:
  * [n_tokens][n_heads][head_dim] of dtype (CKR_BF16 or CKR_F16; a 16-bit cache
- * must be of the same type) with token and head strides in elements, rows on
+ * must be of the same type; with CKR_F16 the values of an 8-bit cache reach at
+ * most 65504) with token and head strides in elements, rows on
  * 16-byte boundaries.  d_lse (may be NULL): [n_tokens][n_heads] fp32, the
  * logarithm of the sum of exp(scale * q.k).  A token that attends to nothing
  * gives zeros and -infinity.  The workspace (256-byte aligned) must be all
