@@ -68,19 +68,26 @@ template <> __device__ __forceinline__ uint32_t encode4<ElemI8>(float a, float b
     return x | y << 8 | z << 16 | w << 24;
 }
 
-// N elements (a multiple of 8) at p, aligned for 16-byte loads (8-bit: N bytes).
-template <typename E, int N> __device__ __forceinline__ void load_vec(const void* p, float* x) {
+// The same vectors at any address: global memory takes them whole.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+template <bool ALIGNED> struct Vecs { typedef u32x4 U4; typedef u32x2 U2; typedef f32x4 F4; };
+template <> struct Vecs<false> { typedef u32x4_any U4; typedef u32x2_any U2; typedef f32x4_any F4; };
+
+// N elements (a multiple of 8) at p, ALIGNED: for 16-byte loads (8-bit: N bytes).
+template <typename E, int N, bool ALIGNED = true> __device__ __forceinline__ void load_vec(const void* p, float* x) {
     if constexpr (E::bytes == 4) {
 #pragma unroll
         for (int i = 0; i < N / 4; i++) {
-            const f32x4 v = reinterpret_cast<const f32x4*>(p)[i];
+            const f32x4 v = reinterpret_cast<const typename Vecs<ALIGNED>::F4*>(p)[i];
 #pragma unroll
             for (int j = 0; j < 4; j++) x[4 * i + j] = v[j];
         }
     } else if constexpr (E::bytes == 2) {
 #pragma unroll
         for (int i = 0; i < N / 8; i++) {
-            const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+            const u32x4 v = reinterpret_cast<const typename Vecs<ALIGNED>::U4*>(p)[i];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 x[8 * i + 2 * j] = lo16<E>(v[j]);
@@ -90,7 +97,7 @@ template <typename E, int N> __device__ __forceinline__ void load_vec(const void
     } else {
 #pragma unroll
         for (int i = 0; i < N / 8; i++) {
-            const u32x2 v = reinterpret_cast<const u32x2*>(p)[i];
+            const u32x2 v = reinterpret_cast<const typename Vecs<ALIGNED>::U2*>(p)[i];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const f32x4 c = codes4<E>(v[j]);
@@ -100,18 +107,18 @@ template <typename E, int N> __device__ __forceinline__ void load_vec(const void
         }
     }
 }
-template <typename E, int N> __device__ __forceinline__ void store_vec(void* p, const float* x) {
+template <typename E, int N, bool ALIGNED = true> __device__ __forceinline__ void store_vec(void* p, const float* x) {
     if constexpr (E::bytes == 4) {
 #pragma unroll
         for (int i = 0; i < N / 4; i++)
-            reinterpret_cast<f32x4*>(p)[i] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+            reinterpret_cast<typename Vecs<ALIGNED>::F4*>(p)[i] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
     } else if constexpr (E::bytes == 2) {
 #pragma unroll
         for (int i = 0; i < N / 8; i++) {
             u32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; j++) v[j] = pack16<E>(x[8 * i + 2 * j], x[8 * i + 2 * j + 1]);
-            reinterpret_cast<u32x4*>(p)[i] = v;
+            reinterpret_cast<typename Vecs<ALIGNED>::U4*>(p)[i] = v;
         }
     } else if constexpr (N % 16 == 0) {
 #pragma unroll
@@ -119,17 +126,17 @@ template <typename E, int N> __device__ __forceinline__ void store_vec(void* p, 
             u32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; j++) v[j] = encode4<E>(x[16 * i + 4 * j], x[16 * i + 4 * j + 1], x[16 * i + 4 * j + 2], x[16 * i + 4 * j + 3]);
-            reinterpret_cast<u32x4*>(p)[i] = v;
+            reinterpret_cast<typename Vecs<ALIGNED>::U4*>(p)[i] = v;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < N / 8; i++) {
             const float* y = x + 8 * i;
-            reinterpret_cast<u32x2*>(p)[i] = u32x2{encode4<E>(y[0], y[1], y[2], y[3]), encode4<E>(y[4], y[5], y[6], y[7])};
+            reinterpret_cast<typename Vecs<ALIGNED>::U2*>(p)[i] = u32x2{encode4<E>(y[0], y[1], y[2], y[3]), encode4<E>(y[4], y[5], y[6], y[7])};
         }
     }
 }
-// One element (unaligned or ragged rows).
+// One element (a row's last ones).
 template <typename E> __device__ __forceinline__ float load_one(const void* p, int64_t i) {
     if constexpr (E::bytes == 4) return reinterpret_cast<const float*>(p)[i];
     else return lo16<E>(reinterpret_cast<const uint16_t*>(p)[i]);

@@ -185,9 +185,12 @@ struct NormArg {
     uint32_t n, group;
     float eps;
     int w_f32;
-    int wide;  // every row starts on a 16-byte boundary (8-bit output: 8) and n is a multiple of 8
 };
 
+// RAGGED: n is no multiple of 8, and the last piece of a row goes one element at a
+// time; elsewhere vectors are loaded and stored at any address (rows of 4095 in
+// bfloat16: 130 us, one element at a time 280; a kernel without the last piece saves
+// half its registers: 16384 rows of 8192 in 181 us, 202 with it).
 // THREADS threads a row (a block of at least 256 holds several rows of fewer).
 // Thread t of a row holds the 8 values from 8 (t + v THREADS) on, for v < VPT, so a
 // row is read once and stays in registers through both reductions (the sum of
@@ -195,7 +198,7 @@ struct NormArg {
 // 16384 of them with residual, total and codes by 128, 943 MB in 181 us (5.2 TB/s, what
 // a copy reaches); 2048 rows of 4096 in 12.3 us; one row 3.5 us, of which the kernel
 // can save nothing (a load, two reductions, a store).
-template <typename E, typename O, int THREADS, int VPT>
+template <typename E, typename O, int THREADS, int VPT, bool RAGGED>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_kernel(NormArg a) {
     constexpr uint32_t ROWS = THREADS < 256 ? 256 / THREADS : 1;
     static_assert(THREADS <= 64 || THREADS >= 256, "a row of several waves has its block to itself");
@@ -215,18 +218,17 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_ke
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
         const uint32_t col = (v * THREADS + tid) * 8;
+        const uint32_t left = a.n - min(col, a.n);
         float q[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) h[v][i] = q[i] = 0.f;
-        if (a.wide) {
-            if (col < a.n) {
-                load_vec<E, 8>(x + (int64_t)col * E::bytes, h[v]);
-                if (r) load_vec<E, 8>(r + (int64_t)col * E::bytes, q);
-            }
-        } else {
+        if (left >= 8) {
+            load_vec<E, 8, false>(x + (int64_t)col * E::bytes, h[v]);
+            if (r) load_vec<E, 8, false>(r + (int64_t)col * E::bytes, q);
+        } else if constexpr (RAGGED) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (col + i < a.n) {
+            for (int i = 0; i < 7; i++)
+                if ((uint32_t)i < left) {
                     h[v][i] = load_one<E>(x, col + i);
                     if (r) q[i] = load_one<E>(r, col + i);
                 }
@@ -251,19 +253,18 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_ke
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
         const uint32_t col = (v * THREADS + tid) * 8;
+        const uint32_t left = a.n - min(col, a.n);
         float w[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) w[i] = 0.f;
-        if (a.wide) {
-            if (col < a.n) {
-                if (total) store_vec<E, 8>(total + (int64_t)col * E::bytes, h[v]);
-                if (a.w_f32) load_vec<ElemF32, 8>(a.w + (int64_t)col * 4, w);
-                else load_vec<E, 8>(a.w + (int64_t)col * E::bytes, w);
-            }
-        } else {
+        if (left >= 8) {
+            if (total) store_vec<E, 8, false>(total + (int64_t)col * E::bytes, h[v]);
+            if (a.w_f32) load_vec<ElemF32, 8, false>(a.w + (int64_t)col * 4, w);
+            else load_vec<E, 8, false>(a.w + (int64_t)col * E::bytes, w);
+        } else if constexpr (RAGGED) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (col + i < a.n) {
+            for (int i = 0; i < 7; i++)
+                if ((uint32_t)i < left) {
                     if (total) store_one<E>(total, col + i, h[v][i]);
                     w[i] = a.w_f32 ? load_one<ElemF32>(a.w, col + i) : load_one<E>(a.w, col + i);
                 }
@@ -308,17 +309,18 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_ke
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
         const uint32_t col = (v * THREADS + tid) * 8;
-        if (a.wide) {
-            if (col < a.n) store_vec<O, 8>(out + (int64_t)col * O::bytes, h[v]);
-        } else {
+        const uint32_t left = a.n - min(col, a.n);
+        if (left >= 8) {
+            store_vec<O, 8, false>(out + (int64_t)col * O::bytes, h[v]);
+        } else if constexpr (RAGGED) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (col + i < a.n) store_one<O>(out, col + i, h[v][i]);
+            for (int i = 0; i < 7; i++)
+                if ((uint32_t)i < left) store_one<O>(out, col + i, h[v][i]);
         }
     }
 }
 
-template <typename E, typename O>
+template <typename E, typename O, bool RAGGED>
 hipError_t launch_norm(const NormArg& a, uint64_t rows, hipStream_t s) {
     const auto go = [&](auto kernel, uint32_t threads) {
         constexpr uint64_t kMost = 1u << 21;  // blocks of a launch: a grid holds fewer than 2^32 threads
@@ -336,23 +338,27 @@ hipError_t launch_norm(const NormArg& a, uint64_t rows, hipStream_t s) {
     // 154 (a wave a row), 425 (256 threads); 1024: 87 / 140 (256 threads); 2048: 93, and 12 /
     // 13.5 with 59 MB (256 threads); 4096: 84 / 90 (512 threads); 8192: 92 / 99 (1024
     // threads); 16384: 88 / 121 (256 threads, eight loads).
-    if (a.n <= 128) return go(add_rms_norm_kernel<E, O, 16, 1>, 16);
-    if (a.n <= 256) return go(add_rms_norm_kernel<E, O, 32, 1>, 32);
-    if (a.n <= 512) return go(add_rms_norm_kernel<E, O, 64, 1>, 64);
-    if (a.n <= 1024) return go(add_rms_norm_kernel<E, O, 64, 2>, 64);
-    if (a.n <= 2048) return go(add_rms_norm_kernel<E, O, 64, 4>, 64);
-    if (a.n <= 4096) return go(add_rms_norm_kernel<E, O, 256, 2>, 256);
-    if (a.n <= 8192) return go(add_rms_norm_kernel<E, O, 256, 4>, 256);
-    if (a.n <= 16384) return go(add_rms_norm_kernel<E, O, 1024, 2>, 1024);
-    if (a.n <= 32768) return go(add_rms_norm_kernel<E, O, 1024, 4>, 1024);
-    return go(add_rms_norm_kernel<E, O, 1024, 8>, 1024);
+    if (a.n <= 128) return go(add_rms_norm_kernel<E, O, 16, 1, RAGGED>, 16);
+    if (a.n <= 256) return go(add_rms_norm_kernel<E, O, 32, 1, RAGGED>, 32);
+    if (a.n <= 512) return go(add_rms_norm_kernel<E, O, 64, 1, RAGGED>, 64);
+    if (a.n <= 1024) return go(add_rms_norm_kernel<E, O, 64, 2, RAGGED>, 64);
+    if (a.n <= 2048) return go(add_rms_norm_kernel<E, O, 64, 4, RAGGED>, 64);
+    if (a.n <= 4096) return go(add_rms_norm_kernel<E, O, 256, 2, RAGGED>, 256);
+    if (a.n <= 8192) return go(add_rms_norm_kernel<E, O, 256, 4, RAGGED>, 256);
+    if (a.n <= 16384) return go(add_rms_norm_kernel<E, O, 1024, 2, RAGGED>, 1024);
+    if (a.n <= 32768) return go(add_rms_norm_kernel<E, O, 1024, 4, RAGGED>, 1024);
+    return go(add_rms_norm_kernel<E, O, 1024, 8, RAGGED>, 1024);
 }
 
+template <typename E, typename O>
+hipError_t launch_norm_any(const NormArg& a, uint64_t rows, hipStream_t s) {
+    return a.n % 8 ? launch_norm<E, O, true>(a, rows, s) : launch_norm<E, O, false>(a, rows, s);
+}
 template <typename E>
 hipError_t launch_norm_of(const NormArg& a, int out_dtype, uint64_t rows, hipStream_t s) {
-    if (out_dtype == CKR_F8) return launch_norm<E, ElemF8>(a, rows, s);
-    if (out_dtype == CKR_I8) return launch_norm<E, ElemI8>(a, rows, s);
-    return launch_norm<E, E>(a, rows, s);
+    if (out_dtype == CKR_F8) return launch_norm_any<E, ElemF8>(a, rows, s);
+    if (out_dtype == CKR_I8) return launch_norm_any<E, ElemI8>(a, rows, s);
+    return launch_norm_any<E, E>(a, rows, s);
 }
 
 inline bool multiple(const void* p, uint64_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -479,14 +485,11 @@ int ckr_add_rms_norm(const void* d_x, int64_t x_stride, const void* d_residual, 
     const struct { const void* p; int64_t stride; int es; const char* what; } t[4] = {
         {d_x, x_stride, es, "rows"}, {d_residual, residual_stride, es, "residual"}, {d_total, total_stride, es, "total"},
         {d_out, out_stride, os, "output"}};
-    bool wide = n % 8 == 0 && multiple(d_weight, 16);
     int rc;
     for (const auto& q : t) {
         if (!q.p) continue;
         if (q.stride < 0 || q.stride > (1ll << 40)) return err(CKR_E_INVALID, std::string("stride of the ") + q.what + " out of range");
         if (!multiple(q.p, q.es)) return err(CKR_E_INVALID, std::string(q.what) + " must be aligned to the element size");
-        const uint64_t a = q.es == 1 ? 8 : 16;
-        wide = wide && multiple(q.p, a) && (q.stride * q.es) % a == 0;
         if ((rc = check_range(q.p, ((rows - 1) * (uint64_t)q.stride + n) * q.es, q.what))) return rc;
     }
     if (!multiple(d_weight, ckr_element_size(w_dtype)) || !multiple(d_scales, 4))
@@ -501,7 +504,7 @@ int ckr_add_rms_norm(const void* d_x, int64_t x_stride, const void* d_residual, 
     a.w = static_cast<const uint8_t*>(d_weight), a.out = static_cast<uint8_t*>(d_out), a.scales = d_scales;
     a.total = static_cast<uint8_t*>(d_total);
     a.x_stride = x_stride, a.r_stride = residual_stride, a.out_stride = out_stride, a.total_stride = total_stride;
-    a.n = n, a.group = group, a.eps = eps, a.w_f32 = w_dtype == CKR_F32, a.wide = wide;
+    a.n = n, a.group = group, a.eps = eps, a.w_f32 = w_dtype == CKR_F32;
     const hipStream_t s = (hipStream_t)stream;
     const hipError_t e = dtype == CKR_F32    ? launch_norm_of<ElemF32>(a, out_dtype, rows, s)
                          : dtype == CKR_BF16 ? launch_norm_of<ElemBF16>(a, out_dtype, rows, s)
