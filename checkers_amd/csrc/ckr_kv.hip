@@ -433,8 +433,9 @@ int kv_check_batch(const ckr_kv_cache* c, const ckr_kv_batch* b) {
     if (!b->d_page_table || !b->d_starts || !b->d_offsets) return err(CKR_E_INVALID, "null page table, starts or offsets pointer");
     if (!multiple(b->d_page_table, 4) || !multiple(b->d_starts, 4) || !multiple(b->d_offsets, 4))
         return err(CKR_E_INVALID, "page table, starts and offsets must be aligned to 4 bytes");
-    if (b->table_width == 0 || b->table_stride < b->table_width || b->table_stride > (1ull << 40))
-        return err(CKR_E_INVALID, "the page table's rows must hold table_width entries");
+    // the table is only read, so its rows may overlap
+    if (b->table_width == 0 || b->table_stride > (1ull << 40))
+        return err(CKR_E_INVALID, "the page table's rows must hold table_width entries, their stride at most 2^40");
     int rc;
     const unsigned __int128 entries = (unsigned __int128)(b->n_seqs - 1) * b->table_stride + b->table_width;
     if (entries > (1ull << 46)) return err(CKR_E_INVALID, "the page table is out of range");

@@ -112,7 +112,8 @@ class KvCache:
 class KvBatch:
     """The tokens of a call: sequence s has starts[s] tokens before its chunk,
     rows offsets[s]:offsets[s + 1] of the packed tensors, in the cache pages that
-    page_table[s] lists (negative: unmapped).  All int32 on the GPU; n_tokens is
+    page_table[s] lists (negative: unmapped; a table expanded from one row is read as
+    such).  All int32 on the GPU; n_tokens is
     offsets[-1], max_chunk and max_context (the longest chunk, the largest
     context with its chunk) choose launches and need not be exact."""
 
@@ -129,7 +130,8 @@ class KvBatch:
         self.max_chunk = int(n_tokens if max_chunk is None else max_chunk)
         self.max_context = max_context
         width = page_table.shape[1]
-        self._c = _Batch(page_table.data_ptr(), starts.data_ptr(), offsets.data_ptr(), max(page_table.stride(0), width),
+        stride = page_table.stride(0) if n > 1 else width   # 0, or below the width: rows that share entries
+        self._c = _Batch(page_table.data_ptr(), starts.data_ptr(), offsets.data_ptr(), stride,
                          width, n, self.n_tokens, min(self.max_chunk, 0xffffffff),
                          0xffffffff if max_context is None else min(int(max_context), 0xffffffff), 0)
         self._p = ctypes.byref(self._c)

@@ -572,7 +572,8 @@ typedef struct {
  * tokens before its chunk; its chunk's tokens are rows d_offsets[s] to
  * d_offsets[s + 1] of the packed tensors (d_offsets[0] == 0, d_offsets[n_seqs]
  * == n_tokens), token i at position d_starts[s] + i, which lies in page
- * d_page_table[s * table_stride + position / page_size].  The arrays are on the
+ * d_page_table[s * table_stride + position / page_size] (rows of the table may
+ * overlap, or be one: table_stride 0).  The arrays are on the
  * device and read when the call's kernels run.  A table entry outside
  * [0, n_pages), or a position beyond table_width pages, is an unmapped page:
  * it is not written, reads as zeros and is not attended to.  max_chunk and

@@ -527,3 +527,38 @@ def test_one_workspace_for_calls_of_every_kind(gpu):
                 if key in first:
                     assert torch.equal(first[key][0], out) and torch.equal(first[key][1], lse)
                 first.setdefault(key, (out, lse))
+
+
+def _raw(t):
+    """The bytes of a tensor (NaN equal to itself)."""
+    return t.view(torch.uint8) if t.element_size() == 1 else t.view(torch.int16 if t.element_size() == 2 else torch.int32)
+
+
+@pytest.mark.parametrize("rows", ["one", "shifted"])
+@pytest.mark.parametrize("n", [1, 30])
+def test_page_tables_whose_rows_overlap(gpu, rows, n):
+    """One row of pages for all sequences (stride 0), and rows that start a page
+    further on each (stride 1): as the same rows apart, with page numbers of
+    other sequences right behind the table."""
+    starts, page, S = [0, 40, 90], 16, 3
+    hold = torch.tensor([7, 3, 11, 0, 5, 9, 2, 8, 1, 13, 4, 12] + [6, 10, 14] * 20, dtype=torch.int32, device=gpu)
+    width = 9
+    table = hold[:width].expand(S, width) if rows == "one" else torch.as_strided(hold, (S, width), (1, 1))
+    apart = table.contiguous()
+    assert apart.stride(0) == width and not table.is_contiguous()
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=gpu)  # noqa: E731
+    b, c = (ck.KvBatch(t, i32(starts), i32([n * s for s in range(S + 1)]), S * n, n, 90 + n) for t in (table, apart))
+    g = torch.Generator(device=gpu).manual_seed(n)
+    kv = [torch.randn(S * n, 2, 64, generator=g, device=gpu).to(torch.bfloat16) for _ in range(2)]
+    q = torch.randn(S * n, 8, 64, generator=g, device=gpu).to(torch.bfloat16)
+    plan, got = ck.KvAttention(8, 2, 64, S, S * n, n, 200), []
+    for batch in (b, c):
+        cache = ck.KvCache.empty(15, page, 2, 64, ck.F8, device=gpu)
+        old = [torch.randn(15, 2, page, 64, generator=torch.Generator(device=gpu).manual_seed(s), device=gpu) for s in (5, 6)]
+        every = ck.KvBatch(torch.arange(15, dtype=torch.int32, device=gpu)[None], i32([0]), i32([0, 15 * page]), 15 * page)
+        ck.kv_write(cache, every, *(x.transpose(1, 2).reshape(-1, 2, 64) for x in old))
+        ck.kv_write(cache, batch, *kv)
+        got.append([*(t.clone() for t in cache.tensors()), *ck.kv_read(cache, batch), plan.run(cache, batch, q)])
+    torch.cuda.synchronize()
+    for x, y in zip(*got):
+        assert torch.equal(_raw(x), _raw(y))
