@@ -4,7 +4,7 @@ and add_rms_norm over the C ABI (include/checkers_amd.h).
 A KvCache names the cache's tensors, a KvBatch the tokens a call is about; both
 are descriptors made once and passed to every call (the page table, starts and
 offsets may change in place between calls: the kernels read them on the
-device).  Nothing here copies or synchronises.
+device).  No call here copies or synchronises; only making a KvAttention does.
 """
 import ctypes
 
@@ -204,7 +204,10 @@ def kv_read(cache, batch, dtype=BF16, out=None, stream=None):
 
 class KvAttention:
     """Attention over a paged cache, with the workspace it needs for batches of at
-    most these sizes (n_heads query heads over n_kv_heads; max_context None: any)."""
+    most these sizes (n_heads query heads over n_kv_heads; max_context None: any).
+    Making one waits until the workspace is zero (unless the current stream is
+    being captured), so its first call may be on any stream; its calls must follow
+    each other, in one stream's order or by events."""
 
     def __init__(self, n_heads, n_kv_heads, head_dim, n_seqs, n_tokens, max_chunk=None, max_context=None, device="cuda"):
         torch = _torch()
@@ -214,6 +217,20 @@ class KvAttention:
             n_tokens if max_chunk is None else max_chunk, 0xffffffff if max_context is None else max_context))
         self.ws = torch.zeros(max(self.ws_bytes, 1), dtype=torch.uint8, device=device)
         self._ws_ptr = self.ws.data_ptr()
+        home = torch.cuda.current_stream(self.ws.device)
+        if not torch.cuda.is_current_stream_capturing():
+            home.synchronize()
+        self._streams = {home.cuda_stream}   # whose work the workspace's memory outlives
+
+    def _used_by(self, handle, stream):
+        """A first call on a stream other than the one the workspace was made on."""
+        torch = _torch()
+        if stream is None:
+            if torch.cuda.is_current_stream_capturing():   # whoever keeps the graph keeps the plan
+                return
+            stream = torch.cuda.current_stream(self.ws.device)
+        self.ws.record_stream(stream)
+        self._streams.add(handle)
 
     def run(self, cache, batch, q, scale=None, window=0, out=None, lse=None, stream=None):
         """Attention of the batch's tokens, whose keys and values the cache already
@@ -235,8 +252,11 @@ class KvAttention:
             if lse.shape != q.shape[:2] or lse.dtype != _torch().float32 or not lse.is_contiguous() or not lse.is_cuda:
                 _bad("lse must be a contiguous float32 [tokens, n_heads] on the GPU")
             lse_ptr = lse.data_ptr()
+        handle = _stream_of(stream, q)
+        if handle not in self._streams:
+            self._used_by(handle, stream)
         rc = lib().ckr_kv_attention(cache._p, batch._p, q.data_ptr(), qt, qh, _tag(dtype), h, d ** -0.5 if scale is None else scale,
-                                    window, out.data_ptr(), ot, oh, lse_ptr, self._ws_ptr, self.ws_bytes, _stream_of(stream, q))
+                                    window, out.data_ptr(), ot, oh, lse_ptr, self._ws_ptr, self.ws_bytes, handle)
         if rc:
             _check(rc)
         return out

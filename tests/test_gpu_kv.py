@@ -562,3 +562,68 @@ def test_page_tables_whose_rows_overlap(gpu, rows, n):
     torch.cuda.synchronize()
     for x, y in zip(*got):
         assert torch.equal(_raw(x), _raw(y))
+
+
+def _busy(ms=40):
+    """Work of about so long on the current stream."""
+    torch.cuda._sleep(int(ms * 1.5e6))
+
+
+def _decoding(gpu):
+    """A decoding step whose items are shared by blocks: (cache, batch, q, sizes of
+    its plan, what it gives)."""
+    sq = ko.Seqs([900, 400], [1, 1], 16, seed=5)
+    cache = _cache(sq, 2, 128, "f8", gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 128, "bf16", gpu, 3)
+    q = torch.randn(2, 8, 128, device=gpu).to(torch.bfloat16)
+    sizes = (8, 2, 128, 2, 2, 1, 901)
+    want = ck.KvAttention(*sizes).run(cache, b, q)
+    torch.cuda.synchronize()
+    return cache, b, q, sizes, want
+
+
+@pytest.mark.parametrize("explicit", [True, False])
+def test_plan_made_behind_queued_work_and_run_at_once_on_another_stream(gpu, explicit):
+    """The workspace's memory held other bytes before; the first call, on a stream that
+    waits for nothing, finds zeros."""
+    cache, b, q, sizes, want = _decoding(gpu)
+    side, out = torch.cuda.Stream(), torch.zeros_like(q)
+    n = ck.KvAttention(*sizes).ws.numel()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    dirty = torch.full((n,), 0x5a, dtype=torch.uint8, device=gpu)
+    torch.cuda.synchronize()
+    del dirty
+    _busy()
+    plan = ck.KvAttention(*sizes)
+    if explicit:
+        plan.run(cache, b, q, out=out, stream=side)
+    else:
+        with torch.cuda.stream(side):
+            plan.run(cache, b, q, out=out)
+    side.synchronize()
+    assert torch.equal(out, want)
+    assert (plan.ws[:2048] == 0).all()   # the counters, as the next call needs them
+
+
+@pytest.mark.parametrize("explicit", [True, False])
+def test_plan_dropped_while_another_stream_runs_it(gpu, explicit):
+    """Its workspace is not handed out before that call has ended."""
+    cache, b, q, sizes, want = _decoding(gpu)
+    side, out = torch.cuda.Stream(), torch.zeros_like(q)
+    plan = ck.KvAttention(*sizes)
+    n, at = plan.ws.numel(), plan.ws.data_ptr()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        _busy()
+        if not explicit:
+            plan.run(cache, b, q, out=out)
+    if explicit:
+        plan.run(cache, b, q, out=out, stream=side)
+    del plan
+    other = torch.full((n,), 0x5a, dtype=torch.uint8, device=gpu)
+    assert other.data_ptr() != at
+    side.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and (other == 0x5a).all()
