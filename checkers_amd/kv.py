@@ -5,6 +5,12 @@ A KvCache names the cache's tensors, a KvBatch the tokens a call is about; both
 are descriptors made once and passed to every call (the page table, starts and
 offsets may change in place between calls: the kernels read them on the
 device).  No call here copies or synchronises; only making a KvAttention does.
+
+stream=: the stream a call's work is queued on, None: the current one.  As with
+torch's own operators the caller orders it after the streams that made the
+inputs, and keeps them (or records them on it) until it is done; outputs that
+a call makes belong to that stream and may be used on the current one once that
+waits for it.
 """
 import ctypes
 
@@ -163,12 +169,19 @@ def _rows(t, n_tokens, heads, dim, what):
     return a, b
 
 
-def _used_on(stream, *tensors):
-    """Tensors this module allocated, used on a stream other than the current one."""
-    if stream is not None:
-        for t in tensors:
-            if t is not None:
-                t.record_stream(stream)
+def _new(shape, dtype, device, stream):
+    """An output of a call on `stream` (None: the current one).  Its memory is of that
+    stream's, so whoever had it before has done with it there; the caller may go
+    on with it on the current stream, which therefore delays its next use too."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    here = torch.cuda.current_stream(device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if here.cuda_stream != stream.cuda_stream:
+        t.record_stream(here)
+    return t
 
 
 def kv_write(cache, batch, k, v, stream=None):
@@ -188,9 +201,7 @@ def kv_read(cache, batch, dtype=BF16, out=None, stream=None):
     head_dim] of dtype (a tag), into out (a pair of tensors) when given."""
     n, h, d = batch.n_tokens, cache.n_heads, cache.head_dim
     if out is None:
-        torch = _torch()
-        out = tuple(torch.empty((n, h, d), dtype=_torch_dtype(dtype), device=cache.k.device) for _ in range(2))
-        _used_on(stream, *out)
+        out = tuple(_new((n, h, d), _torch_dtype(dtype), cache.k.device, stream) for _ in range(2))
     k, v = out
     if _tag(k.dtype) != dtype or _tag(v.dtype) != dtype:
         _bad("out must be of the type asked for")
@@ -240,8 +251,7 @@ class KvAttention:
         n, h, d, dtype = batch.n_tokens, self.n_heads, cache.head_dim, q.dtype
         qt, qh = _rows(q, n, h, d, "q")
         if out is None:
-            out = _torch().empty(q.shape, dtype=dtype, device=q.device)
-            _used_on(stream, out)
+            out = _new(q.shape, dtype, q.device, stream)
         if out.dtype != dtype:
             _bad("out must be of q's type")
         ot, oh = _rows(out, n, h, d, "out")
@@ -276,19 +286,16 @@ def add_rms_norm(x, residual, weight, eps=1e-5, dtype=None, group=0, out=None, s
     tag = xt if dtype is None else dtype
     coded = tag == F8 or tag == I8
     if out is None:
-        out = _torch().empty((rows, n), dtype=_torch_dtype(tag), device=x.device)
-        _used_on(stream, out)
+        out = _new(shape, _torch_dtype(tag), x.device, stream)
     if total is None:
-        total = _torch().empty((rows, n), dtype=x_dtype, device=x.device)
-        _used_on(stream, total)
+        total = _new(shape, x_dtype, x.device, stream)
     scales_ptr = None
     if coded:
         if group < 0 or group and n % group:
             _bad("group must divide the row length")
         want = (rows, n // group) if group else (rows,)
         if scales is None:
-            scales = _torch().empty(want, dtype=_torch().float32, device=x.device)
-            _used_on(stream, scales)
+            scales = _new(want, _torch().float32, x.device, stream)
         if scales.shape != want or scales.dtype != _torch().float32 or not scales.is_contiguous() or not scales.is_cuda:
             _bad(f"scales must be contiguous float32 {list(want)} on the GPU")
         scales_ptr = scales.data_ptr()

@@ -627,3 +627,55 @@ def test_plan_dropped_while_another_stream_runs_it(gpu, explicit):
     side.synchronize()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and (other == 0x5a).all()
+
+
+def _calls_that_make_outputs(gpu):
+    """Calls by name, each giving the tensors that it made, on a given stream."""
+    sq = ko.Seqs([90], [1000], 16, seed=5)
+    cache = _cache(sq, 2, 64, "f8", gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 64, "bf16", gpu, 3)
+    q = torch.randn(sq.tokens, 8, 64, device=gpu).to(torch.bfloat16)
+    x, w = torch.randn(1000, 1024, device=gpu).to(torch.bfloat16), torch.ones(1024, device=gpu).to(torch.bfloat16)
+    plan = ck.KvAttention(8, 2, 64, 1, sq.tokens, sq.tokens, 1090)
+    return {"read": lambda s: list(ck.kv_read(cache, b, stream=s)), "attend": lambda s: [plan.run(cache, b, q, stream=s)],
+            "norm": lambda s: list(ck.add_rms_norm(x, None, w, dtype=ck.F8, stream=s))}
+
+
+@pytest.mark.parametrize("name", ["read", "attend", "norm"])
+def test_outputs_made_for_another_stream_are_not_memory_still_read_here(gpu, name):
+    call, side = _calls_that_make_outputs(gpu)[name], torch.cuda.Stream()
+    want = call(None)
+    torch.cuda.synchronize()
+    held = [torch.full((t.numel() * t.element_size(),), 0x5a, dtype=torch.uint8, device=gpu) for t in want]
+    copies = [torch.zeros_like(t) for t in held]
+    at = {t.data_ptr() for t in held}
+    torch.cuda.synchronize()
+    _busy()
+    for t, c in zip(held, copies):
+        c.copy_(t)                     # still to come when the block is given back
+    del held, t
+    got = call(side)
+    assert not at & {t.data_ptr() for t in got}
+    side.synchronize()
+    assert all(torch.equal(_raw(x), _raw(y)) for x, y in zip(got, want))
+    torch.cuda.synchronize()
+    assert all((c == 0x5a).all() for c in copies)
+
+
+@pytest.mark.parametrize("name", ["read", "attend", "norm"])
+def test_outputs_made_for_another_stream_and_dropped_here_are_kept_until_read(gpu, name):
+    call, side = _calls_that_make_outputs(gpu)[name], torch.cuda.Stream()
+    want = call(None)
+    torch.cuda.synchronize()
+    got = call(side)
+    at = {t.data_ptr() for t in got}
+    torch.cuda.current_stream().wait_stream(side)
+    _busy()
+    copies = [_raw(t).clone() for t in got]
+    del got
+    with torch.cuda.stream(side):
+        other = [torch.full_like(_raw(t), 0x5a) for t in want]
+    assert not at & {t.data_ptr() for t in other}
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, _raw(y)) for x, y in zip(copies, want))
