@@ -1616,8 +1616,12 @@ void set_bytes(Cut& c, uint64_t rows) {
 uint32_t few_blocks(uint64_t items, uint64_t max_context) {
     return (uint32_t)std::min<uint64_t>(items * ((max_context + 31) / 32) / kFewTiles + 1, kFewBlocks);
 }
+// Rows of parts that a workspace holds (calls keep multiples of 32, which set_bytes rounds no further).
+uint64_t rows_held(uint64_t bytes, uint32_t dp) { return bytes < kCounterBytes ? 0 : (bytes - kCounterBytes) / (8 + dp * 4); }
+// workspace: its bytes; blocks and splits that it does not hold are left out, down to
+// one block of few rows and no split.
 Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t n_tokens, uint32_t max_chunk,
-        uint64_t max_context, uint64_t all_keys, uint32_t window, bool near_slots) {
+        uint64_t max_context, uint64_t all_keys, uint32_t window, bool near_slots, uint64_t workspace) {
     Cut c{};
     const uint64_t group = n_heads / n_kv, rows = (uint64_t)max_chunk * group;
     c.dp = padded_dim(dim);
@@ -1630,15 +1634,17 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     const uint64_t items = std::max<uint64_t>((uint64_t)c.tiles * n_kv, 1);
     if (c.bm == kFewRows) {
         c.min_tiles = kFewTiles;
-        c.blocks = few_blocks(items, max_context);
+        c.blocks = (uint32_t)std::clamp<uint64_t>(rows_held(workspace, c.dp) / (2 * kFewRows), 1, few_blocks(items, max_context));
         set_bytes(c, (uint64_t)c.blocks * 2 * kFewRows);
         return c;
     }
     const uint64_t most = std::max<uint64_t>((max_context + kSplitMin - 1) / kSplitMin, 1);
-    const uint64_t splits = std::min(std::max<uint64_t>(blocks_wanted(c.bm) / items, 1), most);
-    c.split_len = (uint32_t)std::min<uint64_t>((std::max<uint64_t>(max_context, 1) + splits * kSplitMin - 1) / (splits * kSplitMin) * kSplitMin, 1u << 31);
-    c.splits = (uint32_t)std::max<uint64_t>((max_context + c.split_len - 1) / c.split_len, 1);
-    if (c.splits > 1) set_bytes(c, items * c.splits * c.bm);
+    const uint64_t splits = std::min({blocks_wanted(c.bm) / items, most, rows_held(workspace, c.dp) / (items * c.bm)});
+    if (splits > 1) {
+        c.split_len = (uint32_t)((max_context + splits * kSplitMin - 1) / (splits * kSplitMin) * kSplitMin);  // half of 2^32 at most
+        c.splits = (uint32_t)((max_context + c.split_len - 1) / c.split_len);
+        if (c.splits > 1) set_bytes(c, items * c.splits * c.bm);
+    }
     return c;
 }
 // What cut() asks for at most, for any batch up to these sizes.
@@ -1739,7 +1745,7 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
     for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 26) - 16 && st[0] < (1ll << 36);
     const Cut c = cut(n_heads, cache->n_heads, cache->head_dim, batch->n_seqs, batch->n_tokens, batch->max_chunk,
                       std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size),
-                      (uint64_t)batch->table_width * cache->page_size, window, near_slots);
+                      (uint64_t)batch->table_width * cache->page_size, window, near_slots, workspace_bytes);
     if ((uint64_t)c.tiles * cache->n_heads * 512 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
     a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len, a.min_tiles = c.min_tiles;
     if (c.bytes) {

@@ -214,8 +214,9 @@ def kv_read(cache, batch, dtype=BF16, out=None, stream=None):
 
 
 class KvAttention:
-    """Attention over a paged cache, with the workspace it needs for batches of at
-    most these sizes (n_heads query heads over n_kv_heads; max_context None: any).
+    """Attention over a paged cache, with the workspace for batches of these sizes
+    (n_heads query heads over n_kv_heads; max_context None: any).  Larger batches,
+    or hints above these, are split over fewer blocks, which costs time.
     Making one waits until the workspace is zero (unless the current stream is
     being captured), so its first call may be on any stream; its calls must follow
     each other, in one stream's order or by events."""

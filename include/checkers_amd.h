@@ -615,7 +615,10 @@ CKR_API int ckr_kv_read(const ckr_kv_cache* cache, const ckr_kv_batch* batch, vo
  * gives zeros and -infinity.  The workspace (256-byte aligned) must be all
  * zeros when it is first used and is left fit for the next call; calls that share one
  * must follow each other in stream order.  One sized for the largest n_seqs,
- * n_tokens, max_chunk and max_context serves smaller ones.  Only queues work. */
+ * n_tokens, max_chunk and max_context serves smaller ones; larger ones, and
+ * hints above these, are split over fewer blocks, which costs time (refused,
+ * with CKR_E_CAPACITY, is a workspace too small for one block).  Only queues
+ * work. */
 CKR_API uint64_t ckr_kv_attention_workspace_bytes(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                                                   uint32_t n_seqs, uint32_t n_tokens, uint32_t max_chunk,
                                                   uint32_t max_context);

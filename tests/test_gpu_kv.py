@@ -679,3 +679,30 @@ def test_outputs_made_for_another_stream_and_dropped_here_are_kept_until_read(gp
     assert not at & {t.data_ptr() for t in other}
     torch.cuda.synchronize()
     assert all(torch.equal(x, _raw(y)) for x, y in zip(copies, want))
+
+
+@pytest.mark.parametrize("fmt", ["f8", "f16"])
+@pytest.mark.parametrize("lens", [[1, 1], [3, 8], [9, 20], [70, 90]])
+def test_plans_smaller_than_the_batch_or_its_hints(gpu, fmt, lens):
+    """A plan for short contexts given a wide table and no hints, and one for a single
+    token: less of a split, the same answer."""
+    sq = ko.Seqs([700, 300], lens, 16, seed=4, width=5000)
+    cache = _cache(sq, 2, 128, fmt, gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 128, "f16", gpu, 3)
+    q = torch.randn(sq.tokens, 8, 128, device=gpu).half()
+    chunk = max(lens)
+    for sizes in ((8, 2, 128, 2, sq.tokens, chunk, 100), (8, 2, 128, 1, 1, 1, 1), (8, 2, 128, 2, sq.tokens, chunk, 1000)):
+        plan = ck.KvAttention(*sizes)
+        for context in (None, 1 << 16, 1000):
+            print(f"[case] small plans {fmt} {lens} {sizes[3:]} context={context}", flush=True)
+            lse = torch.empty(sq.tokens, 8, device=gpu)
+            out = plan.run(cache, ck.KvBatch(b.page_table, b.starts, b.offsets, sq.tokens, chunk, context), q, lse=lse)
+            torch.cuda.synchronize()
+            _check(sq, cache, q, out, lse, fmt, 4, 0)
+            assert (plan.ws[:2048] == 0).all()
+    if chunk == 1:
+        plan.ws_bytes = 2048
+        with pytest.raises(ck.CkrError) as e:
+            plan.run(cache, b, q)
+        assert e.value.code == ck.CKR_E_CAPACITY
