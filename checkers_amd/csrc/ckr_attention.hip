@@ -1136,8 +1136,10 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         }
     }
     // staging.  A key of no mapped page is read from page 0 and then cleared (values)
-    // or masked (scores); pieces past the head's size are the last piece again (they
-    // meet queries of zero, and dimensions that are not stored)
+    // or masked (scores); pieces past the head's size are the last piece again: of
+    // values, and of codes, which are finite and meet queries of zero.  A 16-bit key may
+    // hold an infinity, so there the lanes past it store to the 16 bytes between two
+    // rows of LDS, which nobody reads, and the pieces themselves stay zero
     typedef __attribute__((address_space(4))) const int32_t* const_i32;
     const const_i32 table = (const_i32)(a.b.table + (int64_t)__builtin_amdgcn_readfirstlane(t.seq) * a.b.table_stride);
     const bool stage_k = wave < 4;
@@ -1149,7 +1151,8 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     const uint32_t from_lane = ((row_of & 15) * st2 + piece) * 16, w4_rows = w4 * RPW / 16 * 16;
     const float* const scale_k = a.sk + (int64_t)kvh * a.skst[1];
     const float* const scale_v = a.sv + (int64_t)kvh * a.svst[1];
-    uint8_t* const to = (stage_k ? s_k + row_of * KP : s_v + row_of * VP) + place * (C::bytes == 1 ? 32 : 16);
+    const uint32_t to_place = C::bytes == 2 && stage_k && place != piece ? DP * 2 : place * (C::bytes == 1 ? 32 : 16);
+    uint8_t* const to = (stage_k ? s_k + row_of * KP : s_v + row_of * VP) + to_place;
     const uint32_t to_rows = ROWS * (stage_k ? KP : VP), to_slot = TK * (stage_k ? KP : VP);
     const uint32_t c0 = (uint32_t)(lo >> a.page_shift), in0 = (uint32_t)lo & slot_mask, last_col = a.b.width - 1;
     // the page of the 16 keys from j (a multiple of 16) on; -1: none
@@ -1417,6 +1420,9 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         if (C::bytes == 1 && wave == 0) s_sk[Sh::RING][lane] = 1.f;
         if constexpr (C::bytes == 2)
             for (uint32_t e = threadIdx.x; e < 32 * VP / 16; e += 512) *reinterpret_cast<u32x4*>(s_zero + e * 16) = u32x4{0, 0, 0, 0};
+        if (C::bytes == 2 && a.dim < DP)
+            for (uint32_t r = threadIdx.x; r < Sh::RING * TK; r += 512)
+                for (uint32_t d = a.dim; d < DP; d += 8) *reinterpret_cast<u32x4*>(s_k + r * KP + d * 2) = u32x4{0, 0, 0, 0};
         // the first three tiles: their pages, then their rows, all on their way at once
         int32_t pages[3][4];
 #pragma unroll

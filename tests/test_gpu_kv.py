@@ -706,3 +706,37 @@ def test_plans_smaller_than_the_batch_or_its_hints(gpu, fmt, lens):
         with pytest.raises(ck.CkrError) as e:
             plan.run(cache, b, q)
         assert e.value.code == ck.CKR_E_CAPACITY
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [48, 80, 112, 128, 208])
+def test_an_infinite_key_weighs_nothing_where_its_score_is_minus_infinity(gpu, typ, dim):
+    """An infinity in a key's last dimension, seen with a score of -infinity: as if
+    the key were not there, by each of the kernels that hints choose."""
+    sq = ko.Seqs([100], [90], 16, seed=2)
+    cache = _cache(sq, 1, dim, typ, gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 1, dim, typ, gpu, 3)
+    q = torch.randn(90, 8, dim, device=gpu).to(TYPES[typ])
+    q[..., dim - 1] = -q[..., dim - 1].abs() - 0.25
+    p, slot = sq.place(0, 37)
+    for inf in (False, True):
+        cache.k[p, 0, slot, dim - 1] = float("inf") if inf else 0
+        k = _values(cache, "k", typ)
+        if inf:   # a finite stand-in: its weight is 0 in 64 bits too
+            k[p, 0, slot] = 0
+            k[p, 0, slot, dim - 1] = 1e9
+        for chunk in (1, 10, 90):
+            print(f"[case] infinite key {typ} {dim} {inf} chunk={chunk}", flush=True)
+            lse = torch.empty(90, 8, device=gpu)
+            plan = ck.KvAttention(8, 1, dim, 1, 90)
+            out = plan.run(cache, ck.KvBatch(b.page_table, b.starts, b.offsets, 90, chunk, 200), q, lse=lse)
+            torch.cuda.synchronize()
+            v = np.nan_to_num(_values(cache, "v", typ))
+            ref = ko.attention(sq, np.nan_to_num(k), v, q.cpu().double().numpy(), 8, dim ** -0.5, 0)
+            if not inf:
+                slack = ref[3]
+            ref = (*ref[:3], slack, ref[4])   # the stand-in's own products are not what the kernels round
+            bound, lbound = ko.attention_bounds(*ref, dim, ko.UNIT[q.dtype], q.dtype, np.abs(v).max())
+            assert (np.abs(out.cpu().double().numpy() - ref[0]) <= bound).all()
+            assert (np.abs(lse.cpu().double().numpy() - ref[1]) <= lbound).all()
