@@ -180,11 +180,20 @@ template <int N, typename F> __device__ __forceinline__ void unroll(F f) { unrol
 
 // Which sequence and rows a tile of BM rows is: rows of a sequence are its
 // chunk's tokens times the query heads of a key/value head, in that order.
-// Every thread of the block calls it; s_tmp: a word of LDS per wave and five more.
+// Every thread of the block calls it; s_tmp: a word of LDS per wave and five more,
+// which tile_found reads again.
 struct Tile {
     uint32_t seq, row0, rows, token0;  // rows: of the whole sequence; token0: its first packed row
     int64_t start;                     // the position of its first token
 };
+template <uint32_t BM, uint32_t THREADS> __device__ __forceinline__ Tile tile_found(uint32_t group, const uint32_t* s_tmp) {
+    constexpr uint32_t WAVES = THREADS / 64;
+    Tile t;
+    t.seq = s_tmp[WAVES], t.row0 = s_tmp[WAVES + 1] * BM, t.token0 = s_tmp[WAVES + 2];
+    t.rows = (s_tmp[WAVES + 3] - t.token0) * group;
+    t.start = (int32_t)s_tmp[WAVES + 4];
+    return t;
+}
 template <uint32_t BM, uint32_t THREADS = 256>
 __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint32_t tile, uint32_t* s_tmp, Tile& t) {
     constexpr uint32_t WAVES = THREADS / 64;
@@ -219,15 +228,31 @@ __device__ __forceinline__ bool find_tile(const KvBatch& b, uint32_t group, uint
                 s_tmp[WAVES + 2] = (uint32_t)lo, s_tmp[WAVES + 3] = (uint32_t)hi, s_tmp[WAVES + 4] = (uint32_t)start;
             }
             __syncthreads();
-            t.seq = s_tmp[WAVES], t.row0 = s_tmp[WAVES + 1] * BM, t.token0 = s_tmp[WAVES + 2];
-            t.rows = (s_tmp[WAVES + 3] - t.token0) * group;
-            t.start = (int32_t)s_tmp[WAVES + 4];
+            t = tile_found<BM, THREADS>(group, s_tmp);
             return true;
         }
         done += all;
         __syncthreads();
     }
     return false;
+}
+
+// Whether a row of the tile sees a value whose scale is not finite (64 keys a step, the
+// whole wave; for tiles in which there is one).
+template <uint32_t BM>
+__device__ __forceinline__ bool sees_wild_scale(const AttnArg& a, const Tile& t, uint32_t kvh, uint32_t row) {
+    const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + BM - 1, t.rows - 1) / a.group;
+    const int64_t end = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift), pos = t.start + min(row, t.rows - 1) / a.group;
+    const auto below = [](int64_t n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; };
+    bool hit = false;
+    for (int64_t k = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) : 0; k < end; k += 64) {
+        const int64_t key = k + (threadIdx.x & 63);
+        const int32_t page = key < end ? page_of(a.b, t.seq, key, a.page_shift, a.n_pages) : -1;
+        const uint32_t slot = (uint32_t)key & ((1u << a.page_shift) - 1);
+        const bool bad = page >= 0 && abs_bits(a.sv[(int64_t)page * a.svst[0] + (int64_t)kvh * a.svst[1] + slot]) >= 0x7f800000u;
+        hit |= __ballot(bad) & below(pos + 1 - k) & ~(a.window ? below(pos - (int64_t)a.window + 1 - k) : 0);
+    }
+    return hit;
 }
 
 // ------------------------------------------------------------ few rows
@@ -786,10 +811,11 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     __shared__ __attribute__((aligned(16))) float s_sk[2][TK];
     __shared__ __attribute__((aligned(16))) float s_sv[2][TK];
     __shared__ uint64_t s_valid[2];
-    __shared__ uint32_t s_tmp[16];
+    __shared__ uint32_t s_tmp[16], s_wild;  // s_wild: there is a value scale that is not finite
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
     Tile t;
+    if (threadIdx.x == 0) s_wild = 0;
     if (!find_tile<128>(a.b, a.group, tile, s_tmp, t)) return;
     const uint32_t row = t.row0 + wave * 32 + col;
     const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + 127, t.rows - 1) / a.group;
@@ -884,11 +910,12 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
             }
         }
         if (C::bytes == 1 && threadIdx.x < TK) {
-            // a value scale that is not finite shows in the score instead, so that a
-            // weight of 0 (a key that a row does not see) always gives 0
+            // a value scale that is not finite is 0 here, so that a weight of 0 (a key that
+            // a row does not see) always gives 0, and the rows that see it are made NaN at the end
             const bool fine = abs_bits(sv) < 0x7f800000u;
-            s_sk[buf][threadIdx.x] = !in_s ? 0.f : fine ? sk * a.scale2 : as_f32(0x7fc00000u);
+            s_sk[buf][threadIdx.x] = in_s ? sk * a.scale2 : 0.f;
             s_sv[buf][threadIdx.x] = !in_s || !fine ? 0.f : Prob<X, C>::split ? split_scale<C>(sv).rest : sv;
+            if (in_s && !fine) s_wild = 1;
         }
         if (threadIdx.x < 64) {
             const uint64_t ok = __ballot(in_s && lane < TK);
@@ -1038,6 +1065,12 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     }
     l = sum_half(l);
     if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+    if (C::bytes == 1 && s_wild && sees_wild_scale<128>(a, tile_found<128, 256>(a.group, s_tmp), kvh, row)) {
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[dt][i] = as_f32(0x7fc00000u);
+    }
     if (row >= t.rows) return;
     if (a.splits > 1) {
         const uint64_t p = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * 128 + wave * 32 + col;
@@ -1105,10 +1138,11 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     __shared__ __attribute__((aligned(16))) float s_sk[Sh::RING + 1][SCALES];  // the last: ones, for scores that carry their scale
     __shared__ __attribute__((aligned(16))) float s_sv[Sh::RING][SCALES];
     __shared__ __attribute__((aligned(16))) uint8_t s_zero[C::bytes == 2 ? 32 * VP : 16];  // values of zero
-    __shared__ uint32_t s_tmp[16];
+    __shared__ uint32_t s_tmp[16], s_wild;  // s_wild: as in the 128-row kernel
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
     Tile t;
+    if (threadIdx.x == 0) s_wild = 0;
     if (!find_tile<Sh::BM, 512>(a.b, a.group, tile, s_tmp, t)) return;
     const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + Sh::BM - 1, t.rows - 1) / a.group;
     const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
@@ -1249,11 +1283,13 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     };
     const auto store_scales = [&](int slot) {  // four lanes write the same values
         if constexpr (C::bytes == 1) {
-            // a value scale that is not finite shows in the score instead, so that a
-            // weight of 0 (a key that a row does not see) always gives 0
-            const bool fine = abs_bits(sv) < 0x7f800000u, in = held_valid >> (16 * w4 + (lane & 15)) & 1;
-            if (stage_k) s_sk[slot][16 * w4 + (lane & 15)] = fine ? sk * a.scale2 : as_f32(0x7fc00000u);
-            else s_sv[slot][16 * w4 + (lane & 15)] = !in || !fine ? 0.f : Prob<X, C>::split ? split_scale<C>(sv).rest : sv;
+            if (stage_k) {
+                s_sk[slot][16 * w4 + (lane & 15)] = sk * a.scale2;
+            } else {  // as in the 128-row kernel
+                const bool fine = abs_bits(sv) < 0x7f800000u, in = held_valid >> (16 * w4 + (lane & 15)) & 1;
+                s_sv[slot][16 * w4 + (lane & 15)] = !in || !fine ? 0.f : Prob<X, C>::split ? split_scale<C>(sv).rest : sv;
+                if (in && !fine) s_wild = 1;
+            }
         }
     };
 
@@ -1530,6 +1566,12 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     }
     l = sum_half(l);
     if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+    if (C::bytes == 1 && s_wild && sees_wild_scale<Sh::BM>(a, tile_found<Sh::BM, 512>(a.group, s_tmp), kvh, row)) {
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[dt][i] = as_f32(0x7fc00000u);
+    }
     if (row >= t.rows) return;
     if (a.splits > 1) {
         const uint64_t p = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * Sh::BM + wave * 32 + col;

@@ -740,3 +740,39 @@ def test_an_infinite_key_weighs_nothing_where_its_score_is_minus_infinity(gpu, t
             bound, lbound = ko.attention_bounds(*ref, dim, ko.UNIT[q.dtype], q.dtype, np.abs(v).max())
             assert (np.abs(out.cpu().double().numpy() - ref[0]) <= bound).all()
             assert (np.abs(lse.cpu().double().numpy() - ref[1]) <= lbound).all()
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("fmt", ["f8", "i8"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 32)])
+def test_the_log_sum_does_not_depend_on_the_values(gpu, typ, fmt, dim, page):
+    """Value rows of scale NaN: NaN for who sees them, with the log-sum of the scores
+    all the same; for who does not, nothing changes.  By each of the kernels."""
+    sq = ko.Seqs([300, 40], [90, 7], page, seed=2)
+    cache = _cache(sq, 2, dim, fmt, gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, dim, typ, gpu, 3)
+    q = torch.randn(97, 8, dim, device=gpu).to(TYPES[typ])
+    at = ((0, 3, 0), (0, 350, 1), (1, 41, 1))
+    for chunk in (1, 10, 90):
+        b2 = ck.KvBatch(b.page_table, b.starts, b.offsets, 97, chunk, 400)
+        plan = ck.KvAttention(8, 2, dim, 2, 97)
+        for window in (0, 300):
+            print(f"[case] log-sum {typ} {fmt} {dim} {page} chunk={chunk} window={window}", flush=True)
+            lse0, lse = (torch.empty(97, 8, device=gpu) for _ in range(2))
+            clean = plan.run(cache, b2, q, window=window, lse=lse0)
+            held = cache.v_scale.clone()
+            for s, j, h in at:
+                p, slot = sq.place(s, j)
+                cache.v_scale[p, h, slot] = float("nan")
+            got = plan.run(cache, b2, q, window=window, lse=lse)
+            cache.v_scale.copy_(held)
+            sees = torch.zeros(97, 8, dtype=torch.bool, device=gpu)
+            for s, j, h in at:
+                for i in range(sq.lens[s]):
+                    pos = sq.starts[s] + i
+                    if j <= pos and not (window and j <= pos - window):
+                        sees[int(sq.offsets[s]) + i, 4 * h:4 * h + 4] = True
+            assert torch.isnan(got[sees]).all()
+            assert torch.equal(got[~sees], clean[~sees])
+            assert torch.equal(lse, lse0)
