@@ -136,7 +136,8 @@ constexpr float kLag = 8.f;
 // ---- infinities and NaN in 16-bit values.  A tile of keys that not every row sees
 // meets weights of zero, and zero times an infinity is NaN: there the products
 // take the finite values, and who sees an infinity (or NaN: both) is found by
-// products of ones.
+// products of ones.  (Where every row sees the keys, and float16 weights may be zero all
+// the same, the kernels of many rows look at their sums in the end: settle.)
 template <typename E> __device__ __forceinline__ bool any_wild(u32x4 w) {  // E: a 16-bit type
     constexpr uint32_t one = E::tag == CKR_BF16 ? 0x00800080u : 0x04000400u;  // carries an exponent of ones into the sign's place
     uint32_t x = 0;
@@ -253,6 +254,68 @@ __device__ __forceinline__ bool sees_wild_scale(const AttnArg& a, const Tile& t,
         hit |= __ballot(bad) & below(pos + 1 - k) & ~(a.window ? below(pos - (int64_t)a.window + 1 - k) : 0);
     }
     return hit;
+}
+
+// The kernel's arguments once more, for code that hardly ever runs: read where they are
+// used, not kept in (spilled) registers from the kernel's start on.
+__device__ __forceinline__ const AttnArg& args_here() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();  // AttnArg is the kernels' first argument
+    asm volatile("" : "+s"(p));
+    return *(const AttnArg*)p;
+}
+
+// float16 values, a tile whose sums hold NaN: a weight below 2^-31 of the largest is 0 in
+// 16 bits (bfloat16 has the range of 32), and 0 times an infinity is NaN where the
+// sum is infinite.  Such sums begin again at 0, and what the row sees of infinities and
+// NaN is added; others are what they were (an infinity stays one).  The whole wave
+// looks through the tile's keys, 64 pieces of 8 values a load; o as in the kernels of
+// 32x32 products: the lane's dimensions are 32 dt + 8 (i / 4) + 4 (lane / 32) + i % 4.
+template <typename P, int DP, uint32_t BM>
+__device__ __forceinline__ void settle(const Tile& t, uint32_t kvh, uint32_t row, f32x16 (&o)[DP / 32]) {
+    constexpr uint32_t PIECES = DP / 8, KEYS = 64 / PIECES;
+    const AttnArg& a = args_here();
+    uint32_t lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // as args_here: nothing of this is computed before
+    const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + BM - 1, t.rows - 1) / a.group;
+    const int64_t end = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift), pos = t.start + min(row, t.rows - 1) / a.group;
+    const uint32_t piece = lane % PIECES, slot_mask = (1u << a.page_shift) - 1;
+    const uint8_t* const v = a.cv + (int64_t)kvh * a.vst[1];
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; dt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[dt][i] = o[dt][i] == o[dt][i] ? o[dt][i] : 0.f;
+    for (int64_t k = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) : 0; k < end; k += KEYS) {
+        const int64_t mine = k + lane / PIECES;
+        int32_t page = mine < end ? page_of(a.b, t.seq, mine, a.page_shift, a.n_pages) : -1;
+        u32x4 w = {0, 0, 0, 0};
+        if (page >= 0 && piece * 8 < a.dim)
+            w = *reinterpret_cast<const u32x4*>(v + (int64_t)page * a.vst[0] + (int64_t)((uint32_t)mine & slot_mask) * a.vst[2] + piece * 16);
+        if (!__any(any_wild<P>(w))) continue;
+        for (int64_t key = k; key < min(k + KEYS, end); key++) {
+            page = page_of(a.b, t.seq, key, a.page_shift, a.n_pages);
+            if (page < 0 || key > pos || (a.window && key <= pos - (int64_t)a.window)) continue;
+            const uint8_t* const at = v + (int64_t)page * a.vst[0] + (int64_t)((uint32_t)key & slot_mask) * a.vst[2];
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; dt++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const uint32_t d = dt * 32 + 2 * i + 4 * (lane >> 5);
+                    if (d >= a.dim) continue;
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(at + d * 2);
+                    const float y[4] = {lo16<P>(x[0]), hi16<P>(x[0]), lo16<P>(x[1]), hi16<P>(x[1])};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[dt][i + e] += abs_bits(y[e]) >= 0x7f800000u ? y[e] : 0.f;
+                }
+        }
+    }
+}
+template <int N> __device__ __forceinline__ bool any_nan(const f32x16 (&o)[N]) {
+    bool nan = false;
+#pragma unroll
+    for (int dt = 0; dt < N; dt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) nan |= o[dt][i] != o[dt][i];
+    return __any(nan);
 }
 
 // ------------------------------------------------------------ few rows
@@ -617,7 +680,9 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
                         w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
                         w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
                     }
-                    if (__any(seen != ~0u && (any_wild<P>(w0) || any_wild<P>(w1)))) {
+                    // a float16 weight may have become 0 though every row sees the key (see settle; here it
+                    // costs nothing to look: a step of 64 sequences to 16000, 344 us with and without)
+                    if (__any((P::tag == CKR_F16 || seen != ~0u) && (any_wild<P>(w0) || any_wild<P>(w1)))) {
                         const u32x4 see = ones<P>(seen);
                         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
                         const f32x4 p0 = mfma16<P>(wild<P>(w0, 1), see, zero), m0 = mfma16<P>(wild<P>(w0, -1), see, zero);
@@ -1065,6 +1130,8 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     }
     l = sum_half(l);
     if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+    if constexpr (C::tag == CKR_F16)
+        if (any_nan(o)) settle<P, DP, 128>(tile_found<128, 256>(a.group, s_tmp), kvh, row, o);
     if (C::bytes == 1 && s_wild && sees_wild_scale<128>(a, tile_found<128, 256>(a.group, s_tmp), kvh, row)) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
@@ -1566,6 +1633,8 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     }
     l = sum_half(l);
     if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+    if constexpr (C::tag == CKR_F16)
+        if (any_nan(o)) settle<P, DP, Sh::BM>(tile_found<Sh::BM, 512>(a.group, s_tmp), kvh, row, o);
     if (C::bytes == 1 && s_wild && sees_wild_scale<Sh::BM>(a, tile_found<Sh::BM, 512>(a.group, s_tmp), kvh, row)) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)

@@ -776,3 +776,46 @@ def test_the_log_sum_does_not_depend_on_the_values(gpu, typ, fmt, dim, page):
             assert torch.isnan(got[sees]).all()
             assert torch.equal(got[~sees], clean[~sees])
             assert torch.equal(lse, lse0)
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (80, 32), (256, 16)])
+@pytest.mark.parametrize("x", [float("inf"), float("-inf")])
+def test_an_infinity_that_every_row_sees_with_a_small_weight(gpu, dim, page, x):
+    """float16 values: an infinity in a tile that every row sees wholly, whose weight
+    (2^-45 of the largest, 2^-60) is 0 in 16 bits and not in 32: an infinity, by
+    each of the kernels that hints choose; rows that do not see it are as before."""
+    sq = ko.Seqs([300], [90], page, seed=2)
+    cache = _cache(sq, 1, dim, "f16", gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 1, dim, "f16", gpu, 3)
+    cache.k[..., 0] = torch.where(torch.isnan(cache.k[..., 0]), cache.k[..., 0], 2.0)
+    q = torch.zeros(90, 8, dim, dtype=torch.float16, device=gpu)
+    q[..., 0] = 16.0
+    scale = 0.2                            # a key's weight: exp(0.2 * 16 * its first element)
+    for j, first in ((5, -7.75), (131, -11.0)):
+        p, slot = sq.place(0, j)
+        cache.k[p, 0, slot, 0] = first
+    for chunk in (1, 10, 90):
+        b2 = ck.KvBatch(b.page_table, b.starts, b.offsets, 90, chunk, 400)
+        plan = ck.KvAttention(8, 1, dim, 1, 90)
+        for window in (0, 260):
+            print(f"[case] small weight {dim} {page} {x} chunk={chunk} window={window}", flush=True)
+            lse0, lse = (torch.empty(90, 8, device=gpu) for _ in range(2))
+            clean = plan.run(cache, b2, q, scale=scale, window=window, lse=lse0).float().cpu()
+            held = cache.v.clone()
+            for j, d in ((5, 3), (131, dim - 1)):
+                p, slot = sq.place(0, j)
+                cache.v[p, 0, slot, d] = x
+            got = plan.run(cache, b2, q, scale=scale, window=window, lse=lse).float().cpu()
+            cache.v.copy_(held)
+            want = clean.clone()
+            for t in range(90):
+                for j, d in ((5, 3), (131, dim - 1)):
+                    if not window or j > 300 + t - window:
+                        want[t, :, d] = x
+            inf = torch.isinf(want)
+            assert torch.equal(got[inf], want[inf])
+            # the rest: weights in 16 bits of other sums' maxima, roundings only
+            assert ((got - want)[~inf].abs() <= 2 * ko.UNIT[torch.float16] * want[~inf].abs() + 2.0 ** -24).all()
+            # both within their bound of the exact one: scores up to 0.2 * 16 * 11
+            assert ((lse - lse0).abs() <= 2 * ko.U32 * ((dim + 8) * 36 + (400 + 16) + 4 * (1 + lse0.abs()))).all()
