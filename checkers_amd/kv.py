@@ -11,6 +11,9 @@ torch's own operators the caller orders it after the streams that made the
 inputs, and keeps them (or records them on it) until it is done; outputs that
 a call makes belong to that stream and may be used on the current one once that
 waits for it.
+
+None of this has a backward pass: tensors that require gradients are refused
+where gradients are recorded (not under torch.no_grad()).
 """
 import ctypes
 
@@ -156,6 +159,12 @@ def _bad(msg):
     raise CkrError(CKR_E_INVALID, "[ckr] " + msg)
 
 
+def _no_backward():
+    """For inputs that require gradients: refused where one would be lost."""
+    if _torch().is_grad_enabled():
+        _bad("these operators have no backward pass: call them under torch.no_grad(), or on detached tensors")
+
+
 def _rows(t, n_tokens, heads, dim, what):
     """(token stride, head stride) of a [tokens, heads, dim] tensor on a GPU."""
     shape = t.shape
@@ -186,6 +195,8 @@ def _new(shape, dtype, device, stream):
 
 def kv_write(cache, batch, k, v, stream=None):
     """Quantise the batch's keys and values [tokens, heads, head_dim] into the cache."""
+    if k.requires_grad or v.requires_grad:
+        _no_backward()
     dtype, n, h, d = k.dtype, batch.n_tokens, cache.n_heads, cache.head_dim
     if v.dtype != dtype:
         _bad("k and v must be of one type")
@@ -249,6 +260,8 @@ class KvAttention:
         holds: q [tokens, n_heads, head_dim] -> out (of q's type, new when None).
         scale: head_dim ** -0.5 when None.  lse: a contiguous float32 [tokens,
         n_heads] that receives the logarithm of each row's sum of exponentials."""
+        if q.requires_grad:
+            _no_backward()
         n, h, d, dtype = batch.n_tokens, self.n_heads, cache.head_dim, q.dtype
         qt, qh = _rows(q, n, h, d, "q")
         if out is None:
@@ -278,7 +291,10 @@ def add_rms_norm(x, residual, weight, eps=1e-5, dtype=None, group=0, out=None, s
     the last axis of x [rows, n].  Returns (out, scales, h): y of dtype (a tag; x's
     type when None, F8 or I8 with float32 scales per row, or per group of the
     row), scales None for 16 and 32 bits, h rounded to x's type.  out, scales and
-    total (may be x or residual) are written in place when given."""
+    total (may be x or residual) are written in place when given.  There is no
+    backward pass."""
+    if x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad:
+        _no_backward()
     shape, x_dtype = x.shape, x.dtype
     if len(shape) != 2:
         _bad("x must be [rows, n]")

@@ -819,3 +819,21 @@ def test_an_infinity_that_every_row_sees_with_a_small_weight(gpu, dim, page, x):
             assert ((got - want)[~inf].abs() <= 2 * ko.UNIT[torch.float16] * want[~inf].abs() + 2.0 ** -24).all()
             # both within their bound of the exact one: scores up to 0.2 * 16 * 11
             assert ((lse - lse0).abs() <= 2 * ko.U32 * ((dim + 8) * 36 + (400 + 16) + 4 * (1 + lse0.abs()))).all()
+
+
+def test_calls_that_would_lose_a_gradient_are_refused(gpu):
+    sq = ko.Seqs([10], [2], 16)
+    cache = _cache(sq, 2, 64, "f8", gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 64, "bf16", gpu, 3)
+    kv, q = (torch.randn(2, h, 64, device=gpu).to(torch.bfloat16) for h in (2, 4))
+    plan = ck.KvAttention(4, 2, 64, 1, 2)
+    kv2, q2 = (t.clone().requires_grad_() for t in (kv, q))
+    for f, a in ((ck.kv_write, (cache, b, kv2, kv)), (ck.kv_write, (cache, b, kv, kv2)), (plan.run, (cache, b, q2))):
+        with pytest.raises(ck.CkrError) as e:
+            f(*a)
+        assert e.value.code == ck.CKR_E_INVALID and "no backward" in str(e.value)
+    with torch.no_grad():
+        ck.kv_write(cache, b, kv2, kv2)
+        got = plan.run(cache, b, q2)
+    assert torch.equal(got, plan.run(cache, b, q))

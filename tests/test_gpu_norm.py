@@ -170,3 +170,20 @@ def test_norm_refusals(gpu):
     bad("[2, 96]", x.t().contiguous().t(), None, w)
     bad("65536", torch.zeros(1, 65_544, device=gpu), None, torch.zeros(65_544, device=gpu))
     bad("GPU", x.cpu(), None, w)
+
+
+def test_norm_refuses_to_lose_a_gradient(gpu):
+    """Tensors that require gradients: refused where gradients are recorded, taken where not."""
+    x, r = (torch.randn(3, 64, device=gpu) for _ in range(2))
+    w = torch.ones(64, device=gpu)
+    want = ck.add_rms_norm(x, r, w)
+    for i in range(3):
+        t = [x, r, w]
+        t[i] = t[i].clone().requires_grad_()
+        with pytest.raises(ck.CkrError) as e:
+            ck.add_rms_norm(*t)
+        assert e.value.code == ck.CKR_E_INVALID and "no backward" in str(e.value)
+        with torch.no_grad():
+            got = ck.add_rms_norm(*t)
+        again = ck.add_rms_norm(*(y.detach() for y in t))
+        assert torch.equal(got[0], want[0]) and torch.equal(again[2], want[2])
