@@ -1859,7 +1859,7 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
            batch->n_seqs, batch->n_tokens};
     // the slots of a page within 32-bit offsets of each other, pages within 2^36 bytes
     bool near_slots = true;
-    for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 26) - 16 && st[0] < (1ll << 36);
+    for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 26) - 16 && (cache->n_pages == 1 || st[0] < (1ll << 36));
     const Cut c = cut(n_heads, cache->n_heads, cache->head_dim, batch->n_seqs, batch->n_tokens, batch->max_chunk,
                       std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size),
                       (uint64_t)batch->table_width * cache->page_size, window, near_slots, workspace_bytes);

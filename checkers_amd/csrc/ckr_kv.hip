@@ -366,9 +366,12 @@ inline bool multiple(const void* p, uint64_t a) { return reinterpret_cast<uintpt
 }  // namespace
 
 // ---------------------------------------------------------------- argument checks
+// (An axis of one entry may have any stride: it is never taken.)
 int kv_check_rows(const void* p, uint64_t rows, int64_t row_stride, uint64_t heads, int64_t head_stride, uint64_t dim,
                   int es, const char* what) {
     if (!p) return err(CKR_E_INVALID, std::string("null ") + what + " pointer");
+    if (rows == 1) row_stride = 0;
+    if (heads == 1) head_stride = 0;
     if (row_stride < 0 || head_stride < 0) return err(CKR_E_INVALID, std::string("negative stride of the ") + what);
     if (!multiple(p, 16) || (row_stride * es) % 16 || (head_stride * es) % 16)
         return err(CKR_E_INVALID, std::string("rows of the ") + what + " must start on 16-byte boundaries");
@@ -398,6 +401,7 @@ int kv_check_cache(const ckr_kv_cache* c) {
         unsigned __int128 last = c->head_dim;
         const uint64_t shape[3] = {c->n_pages, c->n_heads, c->page_size};
         for (int i = 0; i < 3; i++) {
+            if (shape[i] == 1) continue;
             if (st[i] < 0 || (st[i] * es) % 16)
                 return err(CKR_E_INVALID, std::string("strides of the ") + what + " must be multiples of 16 bytes, not negative");
             last += (unsigned __int128)(shape[i] - 1) * (uint64_t)st[i];
@@ -408,7 +412,8 @@ int kv_check_cache(const ckr_kv_cache* c) {
         if (rc) return rc;
         if (!coded) continue;
         const float* s = which ? c->d_v_scale : c->d_k_scale;
-        const int64_t* ss = which ? c->v_scale_stride : c->k_scale_stride;
+        const int64_t* given = which ? c->v_scale_stride : c->k_scale_stride;
+        const int64_t ss[2] = {c->n_pages == 1 ? 0 : given[0], c->n_heads == 1 ? 0 : given[1]};
         const char* swhat = which ? "value scales" : "key scales";
         if (!s) return err(CKR_E_INVALID, std::string("null ") + swhat + " pointer (an 8-bit cache has scales)");
         if (!multiple(s, 16) || ss[0] < 0 || ss[1] < 0 || ss[0] % 4 || ss[1] % 4)
@@ -489,7 +494,7 @@ int ckr_add_rms_norm(const void* d_x, int64_t x_stride, const void* d_residual, 
     int rc;
     for (const auto& q : t) {
         if (!q.p) continue;
-        if (q.stride < 0 || q.stride > (1ll << 40)) return err(CKR_E_INVALID, std::string("stride of the ") + q.what + " out of range");
+        if (rows > 1 && (q.stride < 0 || q.stride > (1ll << 40))) return err(CKR_E_INVALID, std::string("stride of the ") + q.what + " out of range");
         if (!multiple(q.p, q.es)) return err(CKR_E_INVALID, std::string(q.what) + " must be aligned to the element size");
         if ((rc = check_range(q.p, ((rows - 1) * (uint64_t)q.stride + n) * q.es, q.what))) return rc;
     }

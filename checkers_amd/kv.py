@@ -128,7 +128,7 @@ class KvBatch:
 
     def __init__(self, page_table, starts, offsets, n_tokens, max_chunk=None, max_context=None):
         torch = _torch()
-        _need(page_table.dim() == 2 and page_table.stride(1) == 1, "page_table must be [sequences, pages], its rows contiguous")
+        _need(page_table.dim() == 2 and (page_table.stride(1) == 1 or page_table.shape[1] == 1), "page_table must be [sequences, pages], its rows contiguous")
         n = page_table.shape[0]
         _need(tuple(starts.shape) == (n,) and tuple(offsets.shape) == (n + 1,), "starts and offsets must hold n and n + 1 entries")
         for t, what in ((page_table, "page_table"), (starts, "starts"), (offsets, "offsets")):

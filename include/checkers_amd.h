@@ -553,7 +553,8 @@ CKR_API int ckr_make_contiguous(const void* d_src, int ndim, const int64_t* shap
  * (ckr_kv_write stores none).  dtype CKR_F8 or CKR_I8, with a scale per (page, head, slot) whose
  * slots are contiguous, or CKR_BF16 / CKR_F16 without scales.  page_size is a
  * power of two from 16 on, head_dim a multiple of 16 up to 256; every row must
- * start on a 16-byte boundary, every page's scales of a head too. */
+ * start on a 16-byte boundary, every page's scales of a head too (here and below
+ * the stride of an axis with one entry may be anything). */
 typedef struct {
     void* d_k;
     void* d_v;

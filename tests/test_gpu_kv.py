@@ -837,3 +837,39 @@ def test_calls_that_would_lose_a_gradient_are_refused(gpu):
         ck.kv_write(cache, b, kv2, kv2)
         got = plan.run(cache, b, q2)
     assert torch.equal(got, plan.run(cache, b, q))
+
+
+def test_axes_of_one_entry_may_have_any_stride(gpu):
+    """One token, one head, one page, one sequence, one column of pages: their
+    strides are never taken."""
+    def odd(t, *axes):
+        return torch.as_strided(t, t.shape, [3 if i in axes else s for i, s in enumerate(t.stride())], t.storage_offset())
+
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=gpu)  # noqa: E731
+    kv = [torch.randn(1, 1, 64, device=gpu).half() for _ in range(2)]
+    q = torch.randn(1, 1, 64, device=gpu).half()
+    for fmt in (ck.I8, ck.F16):
+        got = []
+        for strange in (False, True):
+            cache = ck.KvCache.empty(1, 16, 1, 64, fmt, device=gpu)
+            b = ck.KvBatch(i32([[0]]), i32([5]), i32([0, 1]), 1)
+            k, v, x = *kv, q
+            if strange:
+                cache = ck.KvCache(*(odd(t, 0, 1) for t in cache.tensors()))
+                b = ck.KvBatch(odd(i32([[0]]), 0, 1), i32([5]), i32([0, 1]), 1)
+                k, v, x = (odd(t, 0, 1) for t in (k, v, x))
+            ck.kv_write(cache, b, k, v)
+            out = torch.empty(1, 1, 64, device=gpu).half()
+            back = ck.kv_read(cache, b, ck.F16, out=tuple(odd(torch.empty_like(out), 0, 1) if strange else torch.empty_like(out) for _ in range(2)))
+            ck.KvAttention(1, 1, 64, 1, 1).run(cache, b, x, out=odd(out, 0, 1) if strange else out)
+            got.append([t.clone() for t in (*cache.tensors(), *back, out)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(_raw(s.contiguous()), _raw(t.contiguous())) for s, t in zip(*got))
+    table = torch.stack([i32([3, 1, 2]), i32([0, 0, 0])], 1)[:, :1]     # one column, stride 2
+    seqs = ck.KvBatch(table, i32([0, 0, 0]), i32([0, 1, 2, 3]), 3)
+    cache = ck.KvCache.empty(4, 16, 1, 64, ck.F16, device=gpu)
+    x = torch.randn(3, 1, 64, device=gpu).half()
+    ck.kv_write(cache, seqs, x, x)
+    assert torch.equal(cache.k[[3, 1, 2], 0, 0], x[:, 0])
+    turned = ck.KvBatch(torch.stack([i32([3]), i32([0])], 1)[0, :].view(1, 2).t()[:1], i32([0]), i32([0, 1]), 1)
+    assert torch.equal(ck.kv_read(cache, turned, ck.F16)[0], x[:1])
