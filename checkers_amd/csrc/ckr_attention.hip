@@ -14,7 +14,7 @@ namespace ckr {
 int kv_check_cache(const ckr_kv_cache* c);
 int kv_check_batch(const ckr_kv_cache* c, const ckr_kv_batch* b);
 int kv_check_rows(const void* p, uint64_t rows, int64_t row_stride, uint64_t heads, int64_t head_stride, uint64_t dim,
-                  int es, const char* what);
+                  int es, bool written, const char* what);
 
 namespace {
 
@@ -1834,8 +1834,8 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
     if (!std::isfinite(scale)) return err(CKR_E_INVALID, "scale must be finite");
     if ((uint64_t)batch->n_tokens * n_heads > (1ull << 27)) return err(CKR_E_INVALID, "at most 2^27 rows (tokens x query heads)");
     if (batch->n_tokens == 0) return CKR_OK;
-    if ((rc = kv_check_rows(d_q, batch->n_tokens, q_token_stride, n_heads, q_head_stride, cache->head_dim, 2, "queries")) ||
-        (rc = kv_check_rows(d_out, batch->n_tokens, out_token_stride, n_heads, out_head_stride, cache->head_dim, 2, "output")))
+    if ((rc = kv_check_rows(d_q, batch->n_tokens, q_token_stride, n_heads, q_head_stride, cache->head_dim, 2, false, "queries")) ||
+        (rc = kv_check_rows(d_out, batch->n_tokens, out_token_stride, n_heads, out_head_stride, cache->head_dim, 2, true, "output")))
         return rc;
     if (d_lse) {
         if (reinterpret_cast<uintptr_t>(d_lse) % 4) return err(CKR_E_INVALID, "lse must be aligned to 4 bytes");

@@ -3,9 +3,11 @@
 // in 8 bits.  All three are bound by memory: one pass, rows kept in registers
 // between the reduction and the store.
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstring>
 #include <string>
+#include <utility>
 
 #include "ckr_internal.h"
 #include "ckr_kv.h"
@@ -15,13 +17,40 @@ namespace ckr {
 int kv_check_cache(const ckr_kv_cache* c);
 int kv_check_batch(const ckr_kv_cache* c, const ckr_kv_batch* b);
 int kv_check_rows(const void* p, uint64_t rows, int64_t row_stride, uint64_t heads, int64_t head_stride, uint64_t dim,
-                  int es, const char* what);
+                  int es, bool written, const char* what);
 
 namespace {
 
 int err(int code, const std::string& m) { return set_error(code, "[ckr] " + m); }
 int hip_rc(hipError_t e, const char* what) {
     return e == hipSuccess ? CKR_OK : err(CKR_E_HIP, std::string("HIP error in ") + what + ": " + hipGetErrorString(e));
+}
+
+struct Axis { int64_t stride; uint64_t entries; };
+// Whether pieces of `run` elements lie apart when the axes are taken from the
+// nearest entries to the farthest (of tensors whose range has been checked).
+template <size_t N> bool apart(std::array<Axis, N> axes, uint64_t run) {
+    for (size_t i = 1; i < N; i++)
+        for (size_t j = i; j && axes[j].stride < axes[j - 1].stride; j--) std::swap(axes[j], axes[j - 1]);
+    uint64_t extent = run;
+    for (const Axis& x : axes) {
+        if (x.entries <= 1) continue;
+        if ((uint64_t)x.stride < extent) return false;
+        extent += (x.entries - 1) * (uint64_t)x.stride;
+    }
+    return true;
+}
+// A cache that is written: its rows, and its scales.
+int check_rows_apart(const ckr_kv_cache* c) {
+    const uint64_t pages = c->n_pages, heads = c->n_heads, slots = c->page_size;
+    for (int which = 0; which < 2; which++) {
+        const int64_t* st = which ? c->v_stride : c->k_stride;
+        const int64_t* ss = which ? c->v_scale_stride : c->k_scale_stride;
+        if (!apart(std::array<Axis, 3>{{{st[0], pages}, {st[1], heads}, {st[2], slots}}}, c->head_dim) ||
+            (c->d_k_scale && !apart(std::array<Axis, 2>{{{ss[0], pages}, {ss[1], heads}}}, slots)))
+            return err(CKR_E_INVALID, std::string("rows of the cache ") + (which ? "values" : "keys") + " overlap");
+    }
+    return CKR_OK;
 }
 
 // A lane holds 16 values of a (token, head) row: a 16-byte store of codes, and
@@ -153,8 +182,9 @@ int rows_call(const ckr_kv_cache* c, const ckr_kv_batch* b, void* k, int64_t kt,
         return err(CKR_E_INVALID, "keys and values are of float32, bfloat16 or float16, not dtype " + std::to_string(dtype));
     if (b->n_tokens == 0 || b->n_seqs == 0) return CKR_OK;
     const int es = ckr_element_size(dtype);
-    if ((rc = kv_check_rows(k, b->n_tokens, kt, c->n_heads, kh, c->head_dim, es, "keys")) ||
-        (rc = kv_check_rows(v, b->n_tokens, vt, c->n_heads, vh, c->head_dim, es, "values")))
+    if ((rc = kv_check_rows(k, b->n_tokens, kt, c->n_heads, kh, c->head_dim, es, !WRITE, "keys")) ||
+        (rc = kv_check_rows(v, b->n_tokens, vt, c->n_heads, vh, c->head_dim, es, !WRITE, "values")) ||
+        (WRITE && (rc = check_rows_apart(c))))
         return rc;
     RowsArg a{};
     a.k = k, a.v = v, a.k_tok = kt, a.k_head = kh, a.v_tok = vt, a.v_head = vh;
@@ -368,7 +398,7 @@ inline bool multiple(const void* p, uint64_t a) { return reinterpret_cast<uintpt
 // ---------------------------------------------------------------- argument checks
 // (An axis of one entry may have any stride: it is never taken.)
 int kv_check_rows(const void* p, uint64_t rows, int64_t row_stride, uint64_t heads, int64_t head_stride, uint64_t dim,
-                  int es, const char* what) {
+                  int es, bool written, const char* what) {
     if (!p) return err(CKR_E_INVALID, std::string("null ") + what + " pointer");
     if (rows == 1) row_stride = 0;
     if (heads == 1) head_stride = 0;
@@ -378,6 +408,8 @@ int kv_check_rows(const void* p, uint64_t rows, int64_t row_stride, uint64_t hea
     const unsigned __int128 last = (unsigned __int128)(rows - 1) * (uint64_t)row_stride +
                                    (unsigned __int128)(heads - 1) * (uint64_t)head_stride + dim;
     if (last > (1ull << 46)) return err(CKR_E_INVALID, std::string("strides of the ") + what + " are out of range");
+    if (written && !apart(std::array<Axis, 2>{{{row_stride, rows}, {head_stride, heads}}}, dim))
+        return err(CKR_E_INVALID, std::string("rows of the ") + what + " overlap");
     return check_range(p, (uint64_t)last * es, what);
 }
 

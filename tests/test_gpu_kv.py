@@ -873,3 +873,36 @@ def test_axes_of_one_entry_may_have_any_stride(gpu):
     assert torch.equal(cache.k[[3, 1, 2], 0, 0], x[:, 0])
     turned = ck.KvBatch(torch.stack([i32([3]), i32([0])], 1)[0, :].view(1, 2).t()[:1], i32([0]), i32([0, 1]), 1)
     assert torch.equal(ck.kv_read(cache, turned, ck.F16)[0], x[:1])
+
+
+def test_outputs_whose_rows_overlap_are_refused(gpu):
+    """What is written twice would hold either; what is only read may overlap."""
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=gpu)  # noqa: E731
+    b = ck.KvBatch(i32([[1]]), i32([5]), i32([0, 2]), 2)
+    kv, q = torch.randn(2, 2, 64, device=gpu).half(), torch.randn(2, 4, 64, device=gpu).half()
+    cache = ck.KvCache.empty(3, 16, 2, 64, ck.I8, device=gpu)
+    ck.kv_write(cache, b, kv[:, :1].expand(2, 2, 64), kv[:1].expand(2, 2, 64))
+    plan = ck.KvAttention(4, 2, 64, 1, 2)
+
+    def bad(f, *a, **kw):
+        with pytest.raises(ck.CkrError) as e:
+            f(*a, **kw)
+        assert e.value.code == ck.CKR_E_INVALID and "overlap" in str(e.value), str(e.value)
+
+    rows = torch.empty(2, 4, 64, device=gpu).half()
+    for t in (rows[:1].expand(2, 4, 64), rows[:, :1].expand(2, 4, 64), torch.as_strided(rows, (2, 4, 64), (64, 64, 1)),
+              torch.as_strided(rows, (2, 4, 64), (256, 32, 1))):
+        bad(plan.run, cache, b, q, out=t)
+        bad(ck.kv_read, cache, b, ck.F16, out=(t[:, :2], torch.empty_like(kv)))
+        bad(ck.kv_read, cache, b, ck.F16, out=(torch.empty_like(kv), t[:, :2]))
+    plan.run(cache, b, q, out=torch.empty(4, 2, 64, device=gpu).half().transpose(0, 1))
+    # one head's keys and values for all heads: read by the attention, not written
+    k, v, ks, vs = cache.tensors()
+    shared = ck.KvCache(k[:, :1].expand(k.shape), v[:, :1].expand(v.shape), ks[:, :1].expand(ks.shape), vs[:, :1].expand(vs.shape))
+    got = plan.run(shared, b, q)
+    one = ck.KvCache(*(t[:, :1] for t in cache.tensors()))
+    assert torch.equal(got, ck.KvAttention(4, 1, 64, 1, 2).run(one, b, q))
+    bad(ck.kv_write, shared, b, kv, kv)
+    bad(ck.kv_write, ck.KvCache(k, v, ks, vs[:1].expand(vs.shape)), b, kv, kv)
+    bad(ck.kv_write, ck.KvCache(k, v[:1].expand(v.shape), ks, vs), b, kv, kv)
+    torch.cuda.synchronize()
