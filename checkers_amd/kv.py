@@ -280,7 +280,7 @@ class KvAttention:
         if handle not in self._streams:
             self._used_by(handle, stream)
         rc = lib().ckr_kv_attention(cache._p, batch._p, q.data_ptr(), qt, qh, _tag(dtype), h, d ** -0.5 if scale is None else scale,
-                                    window, out.data_ptr(), ot, oh, lse_ptr, self._ws_ptr, self.ws_bytes, handle)
+                                    min(window, 0xffffffff), out.data_ptr(), ot, oh, lse_ptr, self._ws_ptr, self.ws_bytes, handle)
         if rc:
             _check(rc)
         return out

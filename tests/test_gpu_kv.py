@@ -906,3 +906,12 @@ def test_outputs_whose_rows_overlap_are_refused(gpu):
     bad(ck.kv_write, ck.KvCache(k, v, ks, vs[:1].expand(vs.shape)), b, kv, kv)
     bad(ck.kv_write, ck.KvCache(k, v[:1].expand(v.shape), ks, vs), b, kv, kv)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("lens", [[1, 1], [20, 9], [90, 40]])
+def test_windows_longer_than_any_context(gpu, lens):
+    """As no window; 2^32 + 5 is not a window of 5."""
+    sq, cache, b, q, plan, out, lse = _attend(gpu, "bf16", "f8", 2, 4, 64, 16, [100, 30], lens, 0)
+    for window in ((1 << 31) - 1, (1 << 32) - 1, 1 << 32, (1 << 32) + 5, 1 << 40):
+        got = plan.run(cache, b, q, window=window)
+        assert torch.equal(got, out), window
