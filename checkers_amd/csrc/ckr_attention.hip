@@ -388,8 +388,9 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
     __shared__ uint32_t s_last;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
 
-    // ---- this block's stretch of the line of key tiles (the launch has seen to it
-    // that the line is shorter than 2^31)
+    // ---- this block's stretch of the line of key tiles.  The launch has seen to it that
+    // the line of any batch is shorter than 2^31; chunks that overlap, which are no batch,
+    // may add up to more: sums stop at 2^32 - 1, and nothing is done then
     struct Seq { uint32_t tiles, rows, token0; int32_t start; };
     const auto count = [&](uint32_t seq) {
         Seq q = {0, 0, 0, 0};
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const uint32_t x = (uint32_t)__shfl_up((int)tiles, d);
-            if (lane >= (uint32_t)d) tiles += x;
+            if (lane >= (uint32_t)d) tiles = __builtin_elementwise_add_sat(tiles, x);
         }
         __syncthreads();
         if (lane == 63) s_sum[wave] = tiles;
@@ -415,8 +416,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
         all = 0;
 #pragma unroll
         for (uint32_t w = 0; w < kFewWaves; w++) {
-            if (w == wave) tiles += all;
-            all += s_sum[w];
+            if (w == wave) tiles = __builtin_elementwise_add_sat(tiles, all);
+            all = __builtin_elementwise_add_sat(all, s_sum[w]);
         }
         return tiles;
     };
@@ -426,8 +427,9 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
     for (uint32_t base = THREADS; base < a.b.n_seqs; base += THREADS) {
         uint32_t more;
         scan(count(base + threadIdx.x).tiles, more);
-        total += more;
+        total = __builtin_elementwise_add_sat(total, more);
     }
+    if (total >= 1u << 31) return;
     const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, a.min_tiles);
     if ((uint64_t)blockIdx.x * per >= total) return;
     const uint32_t p_begin = blockIdx.x * per, p_end = min(p_begin + per, total);

@@ -915,3 +915,27 @@ def test_windows_longer_than_any_context(gpu, lens):
     for window in ((1 << 31) - 1, (1 << 32) - 1, 1 << 32, (1 << 32) + 5, 1 << 40):
         got = plan.run(cache, b, q, window=window)
         assert torch.equal(got, out), window
+
+
+def test_overlapping_chunks_whose_tiles_exceed_32_bits(gpu):
+    """2500 sequences that each claim the whole of 1000 rows behind a million unmapped
+    keys: 4.9e9 key tiles in all.  Nothing outside the tensors is touched, and the
+    next call is right."""
+    n, tokens, page = 5000, 1000, 256
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=gpu)  # noqa: E731
+    cache = ck.KvCache.empty(2, page, 1, 64, ck.F8, device=gpu)
+    table = torch.full((1, 4096), -1, dtype=torch.int32, device=gpu).expand(n, 4096)
+    ends = [0 if i % 2 == 0 else tokens for i in range(n + 1)]
+    starts = torch.full((n,), 1_000_000, dtype=torch.int32, device=gpu)
+    q = torch.randn(tokens, 1, 64, device=gpu).to(torch.bfloat16)
+    plan = ck.KvAttention(1, 1, 64, n, tokens, 1, 1 << 20)
+    hold = torch.full((tokens + 64, 1, 64), 3.0, device=gpu).to(torch.bfloat16)
+    for offsets in (ends, [0] + [tokens] * n):
+        print("[case] overlapping chunks", offsets[:3], flush=True)
+        plan.run(cache, ck.KvBatch(table, starts, i32(offsets), tokens, 1, 1 << 20), q, out=hold[32:-32])
+        torch.cuda.synchronize()
+        assert (hold[:32] == 3).all() and (hold[-32:] == 3).all()
+        assert (plan.ws[:2048] == 0).all()
+    sq, cache, b, q, _, out, lse = _attend(gpu, "bf16", "f8", 1, 1, 64, 16, [100, 30], [1, 1], 0)
+    assert torch.equal(plan.run(cache, b, q), ck.KvAttention(1, 1, 64, n, tokens, 1, 1 << 20).run(cache, b, q))
+    _check(sq, cache, q, plan.run(cache, b, q, lse=lse), lse, "f8", 1, 0)
