@@ -939,3 +939,48 @@ def test_overlapping_chunks_whose_tiles_exceed_32_bits(gpu):
     sq, cache, b, q, _, out, lse = _attend(gpu, "bf16", "f8", 1, 1, 64, 16, [100, 30], [1, 1], 0)
     assert torch.equal(plan.run(cache, b, q), ck.KvAttention(1, 1, 64, n, tokens, 1, 1 << 20).run(cache, b, q))
     _check(sq, cache, q, plan.run(cache, b, q, lse=lse), lse, "f8", 1, 0)
+
+
+@pytest.mark.parametrize("kernel,starts,lens", [("wide", [1300, 1531], [70, 66]), ("many", [1300, 1531], [20, 9]), ("few", [5300, 4531], [3, 8])])
+@pytest.mark.parametrize("typ,fmt", [("bf16", "f8"), ("bf16", "bf16"), ("f16", "i8"), ("f16", "f8"), ("f16", "f16")])
+@pytest.mark.parametrize("page,dim", [(16, 128), (64, 128), (256, 64), (32, 64), (128, 256)])
+def test_long_contexts_in_one_piece(gpu, kernel, starts, lens, typ, fmt, page, dim):
+    """Twenty key tiles and more in one block (a context hint of 1 splits nothing, and
+    gives few rows two blocks), so that what the kernels load ahead comes round
+    several times: plain, with a window, with a page gone from the middle, and with
+    scores that rise along the context, so that the maximum moves late too."""
+    group = 4
+    sq = ko.Seqs(starts, lens, page, seed=page)
+    cache = _cache(sq, 1, dim, fmt, gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 1, dim, typ, gpu, 3)
+    near = ck.KvBatch(b.page_table, b.starts, b.offsets, sq.tokens, max(lens), 1)
+    g = torch.Generator(device=gpu).manual_seed(4)
+    q = torch.randn(sq.tokens, group, dim, generator=g, device=gpu).to(TYPES[typ])
+    plan = ck.KvAttention(group, 1, dim, 2, sq.tokens, max(lens), 1)
+
+    def check(what, batch, qq, window=0):
+        print(f"[case] one piece {kernel} {typ} {fmt} page={page} {what}", flush=True)
+        lse = torch.empty(sq.tokens, group, device=gpu)
+        out = plan.run(cache, batch, qq, window=window, lse=lse)
+        torch.cuda.synchronize()
+        _check(sq, cache, qq, out, lse, fmt, group, window)
+
+    check("plain", near, q)
+    check("window", near, q, 700)
+    table = sq.table.copy()
+    sq.table[0, 640 // page] = -1
+    sq.table[1, 1100 // page] = sq.n_pages
+    i32 = torch.tensor(sq.table, dtype=torch.int32, device=gpu)
+    check("hole", ck.KvBatch(i32, b.starts, b.offsets, sq.tokens, max(lens), 1), q)
+    sq.table = table
+    # keys whose first element grows by 0.04 a position, queries with 8 there
+    whole = ko.Seqs([0, 0], [o + n for o, n in zip(starts, lens)], page)
+    ramp = torch.cat([torch.arange(n, device=gpu) * 0.04 for n in whole.lens])
+    k, v = (torch.randn(whole.tokens, 1, dim, generator=g, device=gpu) for _ in range(2))
+    k[:, 0, 0] = ramp
+    every = [torch.tensor(x, dtype=torch.int32, device=gpu) for x in (whole.starts, whole.offsets)]
+    ck.kv_write(cache, ck.KvBatch(b.page_table, *every, whole.tokens), k.to(TYPES[typ]), v.to(TYPES[typ]))
+    q = q.clone()
+    q[..., 0] = 8
+    check("rising", near, q)
