@@ -107,8 +107,16 @@ __device__ __forceinline__ float sum_quarters(float x) {
     return sum_half(as_f32(r[0]) + as_f32(r[1]));
 }
 
-// The weights' type is the queries': bfloat16 weights take the value's scale without
-// a range of their own.  float16 weights are scaled up by 2^up so that small ones
+// Weights meet the values in 16 bits, the matrix instructions' operands.  The few rows'
+// kernel gives them two products, of their value rounded and of what that leaves
+// (16 bits in bfloat16, 22 in float16), which memory covers: 175.8 us a step of 64
+// sequences to 16000, 174.3 with one (157 and 152 for heads of 80).  In the others the
+// second product shows in the time (128 rows a head 124 us, 105 with one; a chunk of
+// 2048 behind 30000 1.41 ms and 1.06; prompts in float16 630 us and 505), so there
+// they are rounded once, to 8 or 11 bits: an output's error is 1.3 to 1.4 times that
+// of its own rounding alone.
+// Their type is the queries': bfloat16 weights take the value's scale without a
+// range of their own.  float16 weights are scaled up by 2^up so that small ones
 // keep their bits (their largest is 1, or 2^kLag where a running maximum lags, or
 // twice that with a value's scale, so at most 2^15); of an 8-bit value's scale they
 // take the fraction (1 to 2), and the codes its power of two as they are widened,
@@ -117,6 +125,14 @@ template <typename X, typename C> struct Prob {
     typedef X E;
     static constexpr bool split = X::tag == CKR_F16 && C::bytes == 1;
     static constexpr float up = X::tag == CKR_F16 ? (C::bytes == 1 ? 6.f : 7.f) : 0.f;
+};
+// Eight weights as two 16-bit values each, the second what the first leaves.
+template <typename P> struct Halves {
+    u32x4 hi, lo;
+    __device__ __forceinline__ void add(int i, float x, float y) {
+        const uint32_t h = pack16<P>(x, y);
+        hi[i] = h, lo[i] = pack16<P>(x - lo16<P>(h), y - hi16<P>(h));
+    }
 };
 // A scale as a power of two and the rest (zero, subnormal and non-finite scales: 1
 // and themselves; powers that would take the largest code past 65504: the largest
@@ -340,7 +356,7 @@ template <int N> __device__ __forceinline__ bool any_nan(const f32x16 (&o)[N]) {
 // joins the parts, in an order that does not depend on which one that is.
 //
 // Bound by memory: 64 sequences of 200 to 16000 tokens in e4m3, 8 heads of 128 for 32
-// query heads, 919 MB in 174 us (5.3 TB/s; a kernel that only reads reaches 6.4).  Blocks
+// query heads, 919 MB in 176 us (5.2 TB/s; a kernel that only reads reaches 6.4).  Blocks
 // that each took whole items, longest first, left CUs idle at the end: 234 us.  One
 // sequence of 1000 tokens, 9.5 us: the launch, then a chain of about six dependent
 // reads (chunk, table, rows, counter, parts).
@@ -493,9 +509,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
         const float* const skp = a.sk + (int64_t)kvh * a.skst[1];
         const float* const svp = a.sv + (int64_t)kvh * a.svst[1];
         const int64_t k_off = (int64_t)col * a.kst[2] + g * 16;
-        int64_t v_off[4];
+        // one offset and three sums a load, for 16-bit caches have no registers for four (390 us
+        // a step of 64 sequences to 16000 with them, 342 without; e4m3 177 and 176); four where
+        // values are widened by their scale's power (183 us, 196 with one)
+        constexpr int OFFS = Prob<X, C>::split ? 4 : 1;
+        int64_t v_off[OFFS];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v_off[i] = (int64_t)(4 * g + i) * a.vst[2] + col * (VD * 4);
+        for (int i = 0; i < OFFS; i++) v_off[i] = (int64_t)(4 * g + i) * a.vst[2] + col * (VD * 4);
+        const auto v_row = [&](int i) { return OFFS == 4 ? v_off[i % OFFS] : i * a.vst[2] + v_off[0]; };
         const bool v_in = col * NV < a.dim;
         typedef __attribute__((address_space(1))) const int32_t* global_i32;
         const global_i32 table = (global_i32)(a.b.table + (int64_t)seq * a.b.table_stride);
@@ -561,13 +582,13 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
                 if constexpr (C::bytes == 1) r.sv[h] = *reinterpret_cast<const f32x4*>(svp + (int64_t)max(pages[h], 0) * a.svst[0] + slot + 4 * g);
                 if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) get(r.v[4 * h + i], at + v_off[i]);
+                    for (int i = 0; i < 4; i++) get(r.v[4 * h + i], at + v_row(i));
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
 #pragma unroll
                         for (int j = 0; j < VD; j++) r.v[4 * h + i][j] = 0;
-                        if (pages[h] >= 0 && base + 16 * h + 4 * (int)g + i < end && v_in) get(r.v[4 * h + i], at + v_off[i]);
+                        if (pages[h] >= 0 && base + 16 * h + 4 * (int)g + i < end && v_in) get(r.v[4 * h + i], at + v_row(i));
                     }
                 }
             }
@@ -636,9 +657,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
 #pragma unroll
                 for (int i = 0; i < 8; i++) w[i] = seen >> i & 1 ? w[i] : 0.f;  // a scale may be NaN there
             }
-            return u32x4{pack16<P>(w[0], w[1]), pack16<P>(w[2], w[3]), pack16<P>(w[4], w[5]), pack16<P>(w[6], w[7])};
+            Halves<P> p;
+#pragma unroll
+            for (int i = 0; i < 4; i++) p.add(i, w[2 * i], w[2 * i + 1]);
+            return p;
         };
-        const auto gather = [&](const Regs& r, u32x4 pf, uint32_t seen) {
+        const auto gather = [&](const Regs& r, const Halves<P>& p, uint32_t seen) {
             if constexpr (Prob<X, C>::split) {
 #pragma unroll
                 for (int j = 0; j < VD; j++) {  // four dimensions of eight keys, widened first: each key has its power
@@ -650,7 +674,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
                         u32x4 w;
 #pragma unroll
                         for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(x[2 * e + 1][k / 2], x[2 * e][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
-                        o[4 * j + k] = mfma16<P>(w, pf, o[4 * j + k]);
+                        o[4 * j + k] = mfma16<P>(w, p.lo, mfma16<P>(w, p.hi, o[4 * j + k]));
                     }
                 }
             } else if constexpr (C::bytes == 1) {
@@ -670,7 +694,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const u32x2 w0 = widen4<C, P>(w[0][k]), w1 = widen4<C, P>(w[1][k]);
-                        o[4 * j + k] = mfma16<P>(u32x4{w0[0], w0[1], w1[0], w1[1]}, pf, o[4 * j + k]);
+                        const u32x4 v = {w0[0], w0[1], w1[0], w1[1]};
+                        o[4 * j + k] = mfma16<P>(v, p.lo, mfma16<P>(v, p.hi, o[4 * j + k]));
                     }
                 }
             } else {
@@ -693,8 +718,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
                         for (int i = 0; i < 4; i++) o[2 * j][i] += wild_sum(p0[i], m0[i]), o[2 * j + 1][i] += wild_sum(p1[i], m1[i]);
                         w0 = wild<P>(w0, 0), w1 = wild<P>(w1, 0);
                     }
-                    o[2 * j] = mfma16<P>(w0, pf, o[2 * j]);
-                    o[2 * j + 1] = mfma16<P>(w1, pf, o[2 * j + 1]);
+                    o[2 * j] = mfma16<P>(w0, p.lo, mfma16<P>(w0, p.hi, o[2 * j]));
+                    o[2 * j + 1] = mfma16<P>(w1, p.lo, mfma16<P>(w1, p.hi, o[2 * j + 1]));
                 }
             }
         };
@@ -720,12 +745,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
                 f32x4 s[2];
                 scores(r[u], s);
                 uint32_t seen;
-                const u32x4 pf = weights(r[u], s, base, pages[u], seen);
+                const Halves<P> p = weights(r[u], s, base, pages[u], seen);
                 if (more) {  // its keys' registers again, for the tile after the next
                     coming[0] = page_at(base + 64), coming[1] = page_at(base + 80);
                     load_k(r[u], base + 64, coming);
                 }
-                gather(r[u], pf, seen);
+                gather(r[u], p, seen);
                 if (more) {
                     pages[u][0] = coming[0], pages[u][1] = coming[1];
                     load_v(r[u], base + 64, pages[u]);

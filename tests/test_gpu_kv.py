@@ -984,3 +984,18 @@ def test_long_contexts_in_one_piece(gpu, kernel, starts, lens, typ, fmt, page, d
     q = q.clone()
     q[..., 0] = 8
     check("rising", near, q)
+
+
+@pytest.mark.parametrize("typ,fmt", [("bf16", "f8"), ("bf16", "bf16"), ("bf16", "i8"), ("f16", "i8"), ("f16", "f16")])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (96, 32), (256, 16)])
+def test_weights_of_few_rows_hold_twice_the_bits(gpu, typ, fmt, dim, page):
+    """Two products a value: the sums' error is that of 16 bits (bfloat16) or 22, a small
+    part of what one rounding to 8 or 11 gives where the values cancel."""
+    case = (typ, fmt, 2, 4, dim, page, [1500, 700, 31], [1, 1, 2], 0)
+    sq, cache, b, q, plan, out, lse = _attend(gpu, *case)
+    k, v = (np.nan_to_num(_values(cache, n, fmt), nan=0.0) for n in ("k", "v"))
+    ref = ko.attention(sq, k, v, q.cpu().double().numpy(), 4, dim ** -0.5, 0)
+    bound, _ = ko.attention_bounds(*ref, dim, ko.UNIT[q.dtype] ** 2, q.dtype, np.abs(v).max())
+    err = np.abs(out.cpu().double().numpy() - ref[0])
+    print(f"  largest error / bound: {(err / bound).max():.3f}", flush=True)
+    assert (err <= bound).all()
