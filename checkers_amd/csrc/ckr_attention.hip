@@ -358,8 +358,9 @@ template <int N> __device__ __forceinline__ bool any_nan(const f32x16 (&o)[N]) {
 // Bound by memory: 64 sequences of 200 to 16000 tokens in e4m3, 8 heads of 128 for 32
 // query heads, 919 MB in 176 us (5.2 TB/s; a kernel that only reads reaches 6.4).  Blocks
 // that each took whole items, longest first, left CUs idle at the end: 234 us.  One
-// sequence of 1000 tokens, 9.5 us: the launch, then a chain of about six dependent
-// reads (chunk, table, rows, counter, parts).
+// sequence of 1000 tokens, 9.5 to 10 us: the launch, then a chain of about six dependent
+// reads (chunk, table, rows, counter, parts).  Over 16-bit caches, heads of 128, 15
+// registers spill (1.78 GB in 342 us, 5.2 TB/s all the same).
 template <typename C, int DP> struct FewRegs {
     static constexpr int KL = DP * C::bytes / 64;      // 16-byte pieces of a key's row per lane
     static constexpr int VD = DP / 16 * C::bytes / 4;  // dwords of a key's value row per lane
@@ -880,7 +881,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
 //   V's is read transposed from LDS, four keys of one dimension at a time.
 // Its keys are split over blocks where the tiles do not fill the card.  Bound by the
 // latency of staging and, with few rows, by rows of zeros in the products: 32 tokens
-// of 16 sequences over 4096 (128 rows a head, e4m3) 108 us, 0.32 PFLOP/s.
+// of 16 sequences over 4096 (128 rows a head, e4m3) 105 to 108 us, 0.32 PFLOP/s.  Over
+// 16-bit caches, heads of 128, 5 or 6 registers spill, some of them in its loop (132 us).
 template <typename C, int DP> struct ManyShape {
     static constexpr int TK = DP > 128 ? 32 : 64;
     // bytes of a row in LDS: 16-byte reads of 32 rows run at 206 bytes a cycle with
@@ -1206,11 +1208,12 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 // next but one is stored): waves 0 to 3 stage the keys, 4 to 7 the values.  A wave's
 // rows of a tile lie in one page (16 slots at least), so addresses are the page's,
 // in scalar registers, and an offset that never changes.
-// 2048 tokens behind 30000 in e4m3, 32 query heads: 1.04 ms, 1.0 PFLOP/s (a large
-// library product reaches 1.36); six prompts of 150 to 3000 tokens in float16, 64 query
-// heads: 505 us, 0.68 PFLOP/s: a block is alone on its CU, so of the 50 us that one
-// takes on average the 12 until its first product runs beside nothing.  Over random
-// codes the first takes 1.10 ms, and 1.44 by the 128-row kernel.
+// 2048 tokens behind 30000 in e4m3, 32 query heads: 1.04 to 1.11 ms from card to card,
+// 1.0 PFLOP/s (a large library product reaches 1.36); six prompts of 150 to 3000 tokens
+// in float16, 64 query heads: 505 to 530 us, 0.68 PFLOP/s: a block is alone on its CU
+// and takes one tile of rows, so of the 50 us that one takes on average the 12 until
+// its first product runs beside nothing.  Over random codes the first takes 1.10 ms,
+// and 1.44 by the 128-row kernel.
 template <typename C, int DP> struct WideShape {
     static constexpr int TK = 64, BM = 256, RING = 4;
     static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 64;  // as ManyShape's
@@ -1733,7 +1736,9 @@ struct Cut {
     uint64_t part_m_bytes, bytes;  // of the workspace: counters, the rows' maxima and sums, their outputs
 };
 constexpr uint64_t kSplitMin = 128;   // keys of a split at least
-constexpr uint32_t kFewBlocks = 512;  // blocks of the few rows' kernel: two a CU
+// Blocks of the few rows' kernel: two a CU.  (For heads of 256 its registers leave room
+// for one, so there a full launch runs in two rounds.)
+constexpr uint32_t kFewBlocks = 512;
 // Its tiles of 32 keys a block at least: one a wave (one token over a thousand: 9.5 us;
 // 11.0 with 8, 13.5 with 16).
 constexpr uint32_t kFewTiles = 4;
@@ -1744,7 +1749,7 @@ constexpr uint32_t kFewMost = 32;
 // Rows from which on a tile of 256 pays: 128 rows of 16 sequences over 4096 tokens 108
 // (many) / 131 (very many), 256 rows 150 / 134; 256 of one over 32768 100 / 95.
 constexpr uint32_t kManyMost = 128;
-// Blocks that the card holds at once: two of 128 rows a CU, one of 256.
+// Blocks that the card holds at once: two of 128 rows a CU (of heads of 256 one), one of 256.
 uint64_t blocks_wanted(uint32_t bm) { return bm == kManyRows ? 512 : 256; }
 uint32_t padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 uint64_t most_tiles(uint32_t bm, uint64_t group, uint64_t n_seqs, uint64_t n_tokens) {

@@ -219,14 +219,15 @@ struct NormArg {
 
 // RAGGED: n is no multiple of 8, and the last piece of a row goes one element at a
 // time; elsewhere vectors are loaded and stored at any address (rows of 4095 in
-// bfloat16: 130 us, one element at a time 280; a kernel without the last piece saves
-// half its registers: 16384 rows of 8192 in 181 us, 202 with it).
+// bfloat16: 130 us, one element at a time 280).  A kernel without the last piece takes 91
+// registers instead of 97 for rows of 8192, so five waves a SIMD instead of four: 16384
+// rows in 184 us, 200 with it.
 // THREADS threads a row (a block of at least 256 holds several rows of fewer).
 // Thread t of a row holds the 8 values from 8 (t + v THREADS) on, for v < VPT, so a
 // row is read once and stays in registers through both reductions (the sum of
 // squares, then the largest magnitude).  Bound by memory: rows of 8192 in float16,
-// 16384 of them with residual, total and codes by 128, 943 MB in 181 us (5.2 TB/s, what
-// a copy reaches); 2048 rows of 4096 in 12.3 us; one row 3.5 us, of which the kernel
+// 16384 of them with residual, total and codes by 128, 943 MB in 175 to 185 us from card
+// to card (5.2 TB/s, what a copy reaches); 2048 rows of 4096 in 12.3 us; one row 3.5 us, of which the kernel
 // can save nothing (a load, two reductions, a store).
 template <typename E, typename O, int THREADS, int VPT, bool RAGGED>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_rms_norm_kernel(NormArg a) {
@@ -367,7 +368,9 @@ hipError_t launch_norm(const NormArg& a, uint64_t rows, hipStream_t s) {
     // bfloat16 with residual to e4m3, 469 MB in all, us here / otherwise: 256 values 95 /
     // 154 (a wave a row), 425 (256 threads); 1024: 87 / 140 (256 threads); 2048: 93, and 12 /
     // 13.5 with 59 MB (256 threads); 4096: 84 / 90 (512 threads); 8192: 92 / 99 (1024
-    // threads); 16384: 88 / 121 (256 threads, eight loads).
+    // threads); 16384: 88 / 121 (256 threads, eight loads).  Above 32768 the 64 values of a
+    // thread do not fit the 128 registers that 1024 threads leave it: 22 to 50 spill, in the
+    // ragged kernel 88 to 151 (16-bit rows; 65536: 138 us).
     if (a.n <= 128) return go(add_rms_norm_kernel<E, O, 16, 1, RAGGED>, 16);
     if (a.n <= 256) return go(add_rms_norm_kernel<E, O, 32, 1, RAGGED>, 32);
     if (a.n <= 512) return go(add_rms_norm_kernel<E, O, 64, 1, RAGGED>, 64);

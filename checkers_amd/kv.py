@@ -124,7 +124,9 @@ class KvBatch:
     page_table[s] lists (negative: unmapped; a table expanded from one row is read as
     such).  All int32 on the GPU; n_tokens is
     offsets[-1], max_chunk and max_context (the longest chunk, the largest
-    context with its chunk) choose launches and need not be exact."""
+    context with its chunk) choose launches and need not be exact.  The longest
+    chunk chooses for all sequences, so prompts and sequences that decode are
+    faster in calls of their own."""
 
     def __init__(self, page_table, starts, offsets, n_tokens, max_chunk=None, max_context=None):
         torch = _torch()

@@ -550,7 +550,7 @@ CKR_API int ckr_make_contiguous(const void* d_src, int ndim, const int64_t* shap
 /* A paged cache: keys and values [n_pages][n_heads][page_size][head_dim] in any
  * order of the first three axes (strides in elements, >= 0; the last axis is
  * contiguous).  A CKR_F8 cache that another program fills holds no NaN codes
- * (ckr_kv_write stores none).  dtype CKR_F8 or CKR_I8, with a scale per (page, head, slot) whose
+ * (ckr_kv_write stores none), and a scale is finite or NaN.  dtype CKR_F8 or CKR_I8, with a scale per (page, head, slot) whose
  * slots are contiguous, or CKR_BF16 / CKR_F16 without scales.  page_size is a
  * power of two from 16 on, head_dim a multiple of 16 up to 256; every row must
  * start on a 16-byte boundary, every page's scales of a head too (here and below
