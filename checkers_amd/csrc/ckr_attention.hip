@@ -107,25 +107,60 @@ __device__ __forceinline__ float sum_quarters(float x) {
     return sum_half(as_f32(r[0]) + as_f32(r[1]));
 }
 
-// Weights meet the values in 16 bits, the matrix instructions' operands.  The few rows'
-// kernel gives them two products, of their value rounded and of what that leaves
-// (16 bits in bfloat16, 22 in float16), which memory covers: 175.8 us a step of 64
-// sequences to 16000, 174.3 with one (157 and 152 for heads of 80).  In the others the
-// second product shows in the time (128 rows a head 124 us, 105 with one; a chunk of
-// 2048 behind 30000 1.41 ms and 1.06; prompts in float16 630 us and 505), so there
-// they are rounded once, to 8 or 11 bits: an output's error is 1.3 to 1.4 times that
-// of its own rounding alone.
-// Their type is the queries': bfloat16 weights take the value's scale without a
-// range of their own.  float16 weights are scaled up by 2^up so that small ones
+// Weights meet the values in 16 bits, the matrix instructions' operands.  Rounded
+// once to the queries' type, they make the output's error 1.4 times that of its own
+// rounding over an 8-bit cache (their value's scale is in them; up to 1.75 for short
+// chunks) and 1.1 to 1.4 times over a 16-bit one.  So:
+// - few rows: two products, of the weight rounded and of what that leaves (16 bits in
+//   bfloat16, 22 in float16), which memory covers: a step of 64 sequences to 16000
+//   175.5 us, 174.3 with one (157 and 152 for heads of 80).
+// - many rows, bfloat16 over an 8-bit cache: float16 weights (ProbMany), 11 bits, an
+//   error of 1.01: a chunk of 2048 behind 30000 1.12 ms, 1.06 with bfloat16 ones (the same
+//   instructions otherwise; with two products 1.41); 128 rows a head 109 us and 105.
+// - 128 rows, float16 over an 8-bit cache: two products, 132 us and 109.
+// - many rows else: rounded once.  Two products are 630 us instead of 505 for prompts in
+//   float16, 750 instead of 560 for a chunk over bfloat16.
+// Their type is the queries' but for ProbMany: bfloat16 weights take the value's scale
+// without a range of their own.  float16 weights are scaled up by 2^up so that small ones
 // keep their bits (their largest is 1, or 2^kLag where a running maximum lags, or
 // twice that with a value's scale, so at most 2^15); of an 8-bit value's scale they
 // take the fraction (1 to 2), and the codes its power of two as they are widened,
 // which leaves the values' own range (up to 65504).
 template <typename X, typename C> struct Prob {
     typedef X E;
-    static constexpr bool split = X::tag == CKR_F16 && C::bytes == 1;
+    static constexpr bool split = X::tag == CKR_F16 && C::bytes == 1, scaled = false;
     static constexpr float up = X::tag == CKR_F16 ? (C::bytes == 1 ? 6.f : 7.f) : 0.f;
 };
+// In the kernels of many rows bfloat16 queries have float16 weights too over an 8-bit
+// cache, whose codes are float16 values as well.  There a wave keeps the power of two of
+// the largest value scale so far, e, besides the maximum m of its rows: weights and sums
+// are held against 2^(m + e), so that a weight with its value's whole scale is at most
+// 2^15 whatever the range of the scales, and a small one is off by 2^-31 of the largest
+// value at most.
+template <typename X, typename C> struct ProbMany : Prob<X, C> {};
+struct ProbScaled {
+    typedef ElemF16 E;
+    static constexpr bool split = false, scaled = true;
+    static constexpr float up = 6.f;
+};
+template <> struct ProbMany<ElemBF16, ElemF8> : ProbScaled {};
+template <> struct ProbMany<ElemBF16, ElemI8> : ProbScaled {};
+// e of the largest scale (at least kLeast: sums of weights without values stay in range;
+// above 100, values of 10^32, a sum keeps fewer than 32 octaves below its largest weight).
+constexpr float kLeast = -80.f;
+__device__ __forceinline__ float scale_power(float largest) {
+    return fmaxf((float)(int)(as_u32(largest) >> 23) - 127.f, kLeast);
+}
+// Maximum over each 16 lanes.
+__device__ __forceinline__ float max_row16(float x) {
+    const auto turned = [](float y, auto n) {
+        return as_f32((uint32_t)__builtin_amdgcn_mov_dpp((int)as_u32(y), 0x120 + decltype(n)::value, 0xf, 0xf, true));  // row_ror:n
+    };
+    x = fmaxf(x, turned(x, std::integral_constant<int, 8>{}));
+    x = fmaxf(x, turned(x, std::integral_constant<int, 4>{}));
+    x = fmaxf(x, turned(x, std::integral_constant<int, 2>{}));
+    return fmaxf(x, turned(x, std::integral_constant<int, 1>{}));
+}
 // Eight weights as two 16-bit values each, the second what the first leaves.
 template <typename P> struct Halves {
     u32x4 hi, lo;
@@ -881,8 +916,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
 //   V's is read transposed from LDS, four keys of one dimension at a time.
 // Its keys are split over blocks where the tiles do not fill the card.  Bound by the
 // latency of staging and, with few rows, by rows of zeros in the products: 32 tokens
-// of 16 sequences over 4096 (128 rows a head, e4m3) 105 to 108 us, 0.32 PFLOP/s.  Over
-// 16-bit caches, heads of 128, 5 or 6 registers spill, some of them in its loop (132 us).
+// of 16 sequences over 4096 (128 rows a head, e4m3) 109 us, 0.32 PFLOP/s.  Over 16-bit
+// caches, heads of 128, 5 or 6 registers spill, some of them in its loop (131 us).
 template <typename C, int DP> struct ManyShape {
     static constexpr int TK = DP > 128 ? 32 : 64;
     // bytes of a row in LDS: 16-byte reads of 32 rows run at 206 bytes a cycle with
@@ -895,7 +930,7 @@ template <typename C, int DP> struct ManyShape {
 
 template <typename X, typename C, int DP>
 __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(AttnArg a) {
-    typedef typename Prob<X, C>::E P;
+    typedef typename ProbMany<X, C>::E P;
     typedef ManyShape<C, DP> Sh;
     constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, ROWS = Sh::ROWS;
     constexpr int KS = DP / 16, DT = DP / 32, TT = TK / 32;
@@ -904,6 +939,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     __shared__ __attribute__((aligned(16))) uint8_t s_v[2][TK * VP];
     __shared__ __attribute__((aligned(16))) float s_sk[2][TK];
     __shared__ __attribute__((aligned(16))) float s_sv[2][TK];
+    __shared__ float s_most[2];  // the largest value scale of a tile
     __shared__ uint64_t s_valid[2];
     __shared__ uint32_t s_tmp[16], s_wild;  // s_wild: there is a value scale that is not finite
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
@@ -969,7 +1005,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
             if (pg[u] >= 0 && d_in) {
                 kr[u] = *reinterpret_cast<const u32x4*>(a.ck + (int64_t)pg[u] * a.kst[0] + (int64_t)kvh * a.kst[1] + slot * a.kst[2] + piece * 16);
                 vr[u] = *reinterpret_cast<const u32x4*>(a.cv + (int64_t)pg[u] * a.vst[0] + (int64_t)kvh * a.vst[1] + slot * a.vst[2] + piece * 16);
-                if constexpr (Prob<X, C>::split) row_sv[u] = a.sv[(int64_t)pg[u] * a.svst[0] + (int64_t)kvh * a.svst[1] + slot];
+                if constexpr (ProbMany<X, C>::split) row_sv[u] = a.sv[(int64_t)pg[u] * a.svst[0] + (int64_t)kvh * a.svst[1] + slot];
             }
         }
         in_s = pg_s >= 0;
@@ -993,7 +1029,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                     const u32x2 x = widen4<C, X>(kr[u][2 * w]), y = widen4<C, X>(kr[u][2 * w + 1]);
                     *reinterpret_cast<u32x4*>(k + piece * 32 + w * 16) = u32x4{x[0], x[1], y[0], y[1]};
                     u32x2 z, zz;
-                    if constexpr (Prob<X, C>::split) {
+                    if constexpr (ProbMany<X, C>::split) {
                         const float power = split_scale<C>(row_sv[u]).power;
                         z = widen4_by<C>(vr[u][2 * w], power), zz = widen4_by<C>(vr[u][2 * w + 1], power);
                     } else {
@@ -1008,16 +1044,20 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
             // a row does not see) always gives 0, and the rows that see it are made NaN at the end
             const bool fine = abs_bits(sv) < 0x7f800000u;
             s_sk[buf][threadIdx.x] = in_s ? sk * a.scale2 : 0.f;
-            s_sv[buf][threadIdx.x] = !in_s || !fine ? 0.f : Prob<X, C>::split ? split_scale<C>(sv).rest : sv;
+            s_sv[buf][threadIdx.x] = !in_s || !fine ? 0.f : ProbMany<X, C>::split ? split_scale<C>(sv).rest : sv;
             if (in_s && !fine) s_wild = 1;
         }
         if (threadIdx.x < 64) {
             const uint64_t ok = __ballot(in_s && lane < TK);
             if (lane == 0) s_valid[buf] = ok;
+            if constexpr (ProbMany<X, C>::scaled) {
+                const float most = max_quarters(max_row16(in_s && lane < TK && abs_bits(sv) < 0x7f800000u ? fabsf(sv) : 0.f));
+                if (lane == 0) s_most[buf] = most;
+            }
         }
     };
 
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, e = ProbMany<X, C>::scaled ? kLeast : 0.f;
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
@@ -1083,16 +1123,17 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, s[tt][i]);
         top = max_half(top);
-        if (__any(top > m + kLag)) {
-            const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
-            m = m2;
+        const float e2 = ProbMany<X, C>::scaled ? fmaxf(e, scale_power(s_most[buf])) : 0.f;
+        if (__any(top > m + kLag || e2 > e)) {
+            const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2 + (e - e2));
+            m = m2, e = e2;
             l *= back;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[dt][i] *= back;
         }
-        const float ref = m == -INFINITY ? 0.f : m - Prob<X, C>::up;
+        const float ref = m == -INFINITY ? 0.f : m - ProbMany<X, C>::up + e;
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
 #pragma unroll
@@ -1111,7 +1152,9 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                         for (int k = 0; k < 4; k++) p[i + k] *= f[k];
                     }
                 }
-                const u32x4 pf = {pack16<P>(p[0], p[1]), pack16<P>(p[2], p[3]), pack16<P>(p[4], p[5]), pack16<P>(p[6], p[7])};
+                Halves<P> w;  // the second for float16 queries over 8 bits only
+#pragma unroll
+                for (int i = 0; i < 4; i++) w.add(i, p[2 * i], p[2 * i + 1]);
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
                     typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -1131,7 +1174,8 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                         for (int i = 0; i < 16; i++) o[dt][i] += wild_sum(plus[i], minus[i]);
                         v = wild<P>(v, 0);
                     }
-                    o[dt] = mfma32<P>(v, pf, o[dt]);
+                    o[dt] = mfma32<P>(v, w.hi, o[dt]);
+                    if constexpr (ProbMany<X, C>::split) o[dt] = mfma32<P>(v, w.lo, o[dt]);
                 }
             }
     };
@@ -1158,6 +1202,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
         }
     }
     l = sum_half(l);
+    m += e;  // what sums are held against, from here on
     if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
     if constexpr (C::tag == CKR_F16)
         if (any_nan(o)) settle<P, DP, 128>(tile_found<128, 256>(a.group, s_tmp), kvh, row, o);
@@ -1189,7 +1234,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
             if (d < a.dim)
                 *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[dt][i] * inv, o[dt][i + 1] * inv), pack16<X>(o[dt][i + 2] * inv, o[dt][i + 3] * inv)};
         }
-    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<X, C>::up + log2f(l)) * kLn2;
+    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - ProbMany<X, C>::up + log2f(l)) * kLn2;
 }
 
 // ------------------------------------------------------------ very many rows
@@ -1199,21 +1244,22 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 //   P(i) = exp(S(i) - maximum so far)           on the vector units,
 // three things that do not wait for each other, written as 16 steps of a matrix
 // product, the reads of LDS for the products three steps on, and one score's
-// weight, in that order.  What bounds it is the issue of vector instructions (five
-// and a half per score and lane), so the maximum is not looked for at each turn:
-// weights are taken against the maximum so far, and only where one comes out above
-// 2^kLag, or a row has no maximum yet, is the turn's softmax made again.
+// weight, in that order.  What bounds it is the issue of vector instructions (four
+// and a half per score and lane; and float16 products take 6 to 8 percent longer than
+// bfloat16 ones in otherwise the same code), so the maximum is not looked for at each turn:
+// weights are taken against the maximum so far, and only where the sum of a lane's
+// comes out above 2^kLag, or a row has no maximum yet, is the turn's softmax made
+// again.
 // Tiles of 64 keys go through a ring of four in LDS (the turns of a tile still read
 // the last half of the one before and the first half of the one after, while the
 // next but one is stored): waves 0 to 3 stage the keys, 4 to 7 the values.  A wave's
 // rows of a tile lie in one page (16 slots at least), so addresses are the page's,
 // in scalar registers, and an offset that never changes.
-// 2048 tokens behind 30000 in e4m3, 32 query heads: 1.04 to 1.11 ms from card to card,
-// 1.0 PFLOP/s (a large library product reaches 1.36); six prompts of 150 to 3000 tokens
-// in float16, 64 query heads: 505 to 530 us, 0.68 PFLOP/s: a block is alone on its CU
+// 2048 tokens behind 30000 in e4m3, 32 query heads: 1.10 to 1.13 ms from card to card,
+// 0.94 PFLOP/s (a large library product reaches 1.36); six prompts of 150 to 3000 tokens
+// in float16, 64 query heads: 490 to 505 us, 0.69 PFLOP/s: a block is alone on its CU
 // and takes one tile of rows, so of the 50 us that one takes on average the 12 until
-// its first product runs beside nothing.  Over random codes the first takes 1.10 ms,
-// and 1.44 by the 128-row kernel.
+// its first product runs beside nothing.
 template <typename C, int DP> struct WideShape {
     static constexpr int TK = 64, BM = 256, RING = 4;
     static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 64;  // as ManyShape's
@@ -1223,17 +1269,18 @@ template <typename C, int DP> struct WideShape {
 
 template <typename X, typename C, int DP>
 __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
-    typedef typename Prob<X, C>::E P;
+    typedef typename ProbMany<X, C>::E P;
     typedef WideShape<C, DP> Sh;
     constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, RPW = Sh::RPW, ROWS = Sh::ROWS;
     constexpr int KS = DP / 16, DT = DP / 32, NM = 2 * KS;  // KS products for the scores, as many for the values
     static_assert(KS == 2 * DT && KS % 4 == 0, "pairs of products, operands in rings of four");
-    constexpr float kMost = Prob<X, C>::up == 0.f ? 256.f : Prob<X, C>::up == 6.f ? 16384.f : 32768.f;  // 2^(kLag + up)
+    constexpr bool kScaled = ProbMany<X, C>::scaled;
+    constexpr float kMost = ProbMany<X, C>::up == 0.f ? 256.f : ProbMany<X, C>::up == 6.f ? 16384.f : 32768.f;  // 2^(kLag + up)
     __shared__ __attribute__((aligned(16))) uint8_t s_k[Sh::RING * TK * KP];
     __shared__ __attribute__((aligned(16))) uint8_t s_v[Sh::RING * TK * VP];
     constexpr int SCALES = C::bytes == 1 ? TK : 1;
     __shared__ __attribute__((aligned(16))) float s_sk[Sh::RING + 1][SCALES];  // the last: ones, for scores that carry their scale
-    __shared__ __attribute__((aligned(16))) float s_sv[Sh::RING][SCALES];
+    __shared__ __attribute__((aligned(16))) float s_sv[Sh::RING][SCALES + (kScaled ? 4 : 0)];  // and the largest of each 16
     __shared__ __attribute__((aligned(16))) uint8_t s_zero[C::bytes == 2 ? 32 * VP : 16];  // values of zero
     __shared__ uint32_t s_tmp[16], s_wild;  // s_wild: as in the 128-row kernel
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
@@ -1331,7 +1378,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             const uint8_t* at = from + ((uint64_t)p * st0 + (uint64_t)slot * st2) * 16;
 #pragma unroll
             for (int u = 0; u < LOADS; u++) held[u] = *reinterpret_cast<const u32x4*>(at + (from_lane + (w4_rows + u * ROWS) * st2 * 16));
-            if constexpr (Prob<X, C>::split) {
+            if constexpr (ProbMany<X, C>::split) {
                 const float* f = scale_v + ((int64_t)p * a.svst[0] + slot) + row_of;
 #pragma unroll
                 for (int u = 0; u < LOADS; u++) row_sv[u] = f[u * ROWS];
@@ -1343,7 +1390,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 const uint32_t p = (uint32_t)max(g == 0 ? pg[0] : g == 1 ? pg[1] : g == 2 ? pg[2] : pg[3], 0);
                 const uint32_t slot = (in0 + (uint32_t)base + 16 * g) & slot_mask;
                 held[u] = *reinterpret_cast<const u32x4*>(from + ((uint64_t)p * st0 + (uint64_t)slot * st2) * 16 + from_lane);
-                if constexpr (Prob<X, C>::split) row_sv[u] = (scale_v + ((int64_t)p * a.svst[0] + slot))[row_of & 15];
+                if constexpr (ProbMany<X, C>::split) row_sv[u] = (scale_v + ((int64_t)p * a.svst[0] + slot))[row_of & 15];
             }
         }
         if constexpr (C::bytes == 1) {
@@ -1363,10 +1410,16 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         uint8_t* at = to + slot * to_slot + u * to_rows;
         if constexpr (C::bytes == 2) {
             *reinterpret_cast<u32x4*>(at) = x;
-        } else if (!Prob<X, C>::split || stage_k) {
+        } else if (stage_k || (!ProbMany<X, C>::split && !kScaled)) {
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 const u32x2 y = widen4<C, X>(x[2 * w]), z = widen4<C, X>(x[2 * w + 1]);
+                *reinterpret_cast<u32x4*>(at + w * 16) = u32x4{y[0], y[1], z[0], z[1]};
+            }
+        } else if (kScaled) {
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const u32x2 y = widen4<C, P>(x[2 * w]), z = widen4<C, P>(x[2 * w + 1]);
                 *reinterpret_cast<u32x4*>(at + w * 16) = u32x4{y[0], y[1], z[0], z[1]};
             }
         } else {
@@ -1384,13 +1437,15 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 s_sk[slot][16 * w4 + (lane & 15)] = sk * a.scale2;
             } else {  // as in the 128-row kernel
                 const bool fine = abs_bits(sv) < 0x7f800000u, in = held_valid >> (16 * w4 + (lane & 15)) & 1;
-                s_sv[slot][16 * w4 + (lane & 15)] = !in || !fine ? 0.f : Prob<X, C>::split ? split_scale<C>(sv).rest : sv;
+                const float x = in && fine ? sv : 0.f;
+                s_sv[slot][16 * w4 + (lane & 15)] = ProbMany<X, C>::split && in && fine ? split_scale<C>(sv).rest : x;
+                if constexpr (kScaled) s_sv[slot][TK + w4] = max_row16(fabsf(x));
                 if (in && !fine) s_wild = 1;
             }
         }
     };
 
-    float m = -INFINITY, l = 0.f, ref = 0.f;
+    float m = -INFINITY, l = 0.f, ref = 0.f, e = kScaled ? kLeast : 0.f;
     f32x16 o[DT], s;
     u32x4 pf[2][2], kf[4], vf[4];  // weights of two turns; operands, read three pairs of steps ahead
     f32x4 fk[2], fv[2];            // the keys' scales, of keys 8 j + 4 half on
@@ -1468,15 +1523,15 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         f32x16 z;
 #pragma unroll
         for (int i = 0; i < 16; i++) z[i] = 0.f;
-        float sum = 0.f, top = 0.f, p_even = 0.f, p_last = 0.f;
+        float sum = 0.f, p_even = 0.f, p_last = 0.f;
+        f32x2 scales = {0.f, 0.f};
+        if constexpr (kScaled) scales = *reinterpret_cast<const f32x2*>(now.fv + TK - 30 * sub);  // s_sv's last four from this half's first
         const auto use = [&](auto k_tag) {
             constexpr int k = decltype(k_tag)::value;
             sum += p_last;
             if constexpr (k % 2 == 0) {
                 p_even = C::bytes == 1 ? p_last * fv[k / 4 % 2][k % 4] : p_last;
-                top = fmaxf(top, p_last);
             } else {
-                top = fmaxf(top, p_last);
                 uint32_t w = pack16<P>(p_even, C::bytes == 1 ? p_last * fv[k / 4 % 2][k % 4] : p_last);
                 asm volatile("" : "+v"(w));
                 pf[sub][k / 8][k % 8 / 2] = w;
@@ -1508,8 +1563,10 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             __builtin_amdgcn_sched_barrier(0);
         });
         use(std::integral_constant<int, 15>{});
-        asm volatile("" : "+v"(sum), "+v"(top));
-        if (__any(top > kMost || m == -INFINITY)) {
+        asm volatile("" : "+v"(sum));
+        const float e2 = kScaled ? fmaxf(e, scale_power(fmaxf(scales[0], scales[1]))) : 0.f;
+        const float most_sum = kScaled ? as_f32(as_u32(kMost) - ((uint32_t)(int)e << 23)) : kMost;  // kMost 2^-e
+        if (__any(sum > most_sum || m == -INFINITY || e2 > e)) {
             float most = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 16; k += 4) {
@@ -1518,9 +1575,9 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 for (int i = 0; i < 4; i++) most = fmaxf(most, s[k + i] * g[i]);
             }
             most = max_half(most);
-            const float m2 = fmaxf(m, most), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
-            m = m2;
-            ref = m2 == -INFINITY ? 0.f : m2 - Prob<X, C>::up;
+            const float m2 = fmaxf(m, most), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2 + (e - e2));
+            m = m2, e = e2;
+            ref = m2 == -INFINITY ? 0.f : m2 - ProbMany<X, C>::up + e;
             l *= back;
             sum = 0.f;
 #pragma unroll
@@ -1662,6 +1719,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         }
     }
     l = sum_half(l);
+    m += e;  // what sums are held against, from here on
     if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
     if constexpr (C::tag == CKR_F16)
         if (any_nan(o)) settle<P, DP, Sh::BM>(tile_found<Sh::BM, 512>(a.group, s_tmp), kvh, row, o);
@@ -1693,7 +1751,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
             if (d < a.dim)
                 *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[dt][i] * inv, o[dt][i + 1] * inv), pack16<X>(o[dt][i + 2] * inv, o[dt][i + 3] * inv)};
         }
-    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - Prob<X, C>::up + log2f(l)) * kLn2;
+    if (a.lse && half == 0) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m - ProbMany<X, C>::up + log2f(l)) * kLn2;
 }
 
 // ------------------------------------------------------------ the splits' join
@@ -1743,11 +1801,13 @@ constexpr uint32_t kFewBlocks = 512;
 // 11.0 with 8, 13.5 with 16).
 constexpr uint32_t kFewTiles = 4;
 // Rows of a chunk up to which it is taken, in tiles of 16 that each read the cache; us,
-// few / many rows, e4m3, 8 heads of 128: 32 rows of 16 sequences over 4096 tokens 55 / 75, of one
-// over 32768 43 / 80, of 64 over 1024 55 / 57; 64 rows of 64 over 1024 100 / 58.
+// few / many rows, e4m3, 8 heads of 128: 32 rows of 16 sequences over 4096 tokens 53 / 78, of one
+// over 32768 42 / 79, of 64 over 1024 51 / 58; 64 rows of 64 over 1024 96 / 60, of 16
+// over 4096 66 / 104.
 constexpr uint32_t kFewMost = 32;
-// Rows from which on a tile of 256 pays: 128 rows of 16 sequences over 4096 tokens 108
-// (many) / 131 (very many), 256 rows 150 / 134; 256 of one over 32768 100 / 95.
+// Rows from which on a tile of 256 pays: 128 rows of 16 sequences over 4096 tokens 110
+// (many) / 144 (very many), 256 rows 158 / 148; 256 of one over 32768 102 / 100; float16
+// caches 129 / 111 and 184 / 115.
 constexpr uint32_t kManyMost = 128;
 // Blocks that the card holds at once: two of 128 rows a CU (of heads of 256 one), one of 256.
 uint64_t blocks_wanted(uint32_t bm) { return bm == kManyRows ? 512 : 256; }
@@ -1818,7 +1878,7 @@ hipError_t launch_attend(const AttnArg& a, const Cut& c, hipStream_t s) {
     const auto join = [&](auto kernel) {
         if (c.splits <= 1) return;
         const uint32_t per = 256 / (DP / 4);
-        CKR_LAUNCH("kv_attention_join", s, kernel<<<dim3(a.tiles * a.kv_heads, (c.bm + per - 1) / per), 256, 0, s>>>(a, Prob<X, C>::up));
+        CKR_LAUNCH("kv_attention_join", s, kernel<<<dim3(a.tiles * a.kv_heads, (c.bm + per - 1) / per), 256, 0, s>>>(a, ProbMany<X, C>::up));
     };
     if (c.bm == kFewRows) {
         CKR_LAUNCH("kv_attention_few", s, attend_few_kernel<X, C, DP><<<dim3(c.blocks), 64 * kFewWaves, 0, s>>>(a));

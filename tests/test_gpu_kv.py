@@ -999,3 +999,41 @@ def test_weights_of_few_rows_hold_twice_the_bits(gpu, typ, fmt, dim, page):
     err = np.abs(out.cpu().double().numpy() - ref[0])
     print(f"  largest error / bound: {(err / bound).max():.3f}", flush=True)
     assert (err <= bound).all()
+
+
+@pytest.mark.parametrize("fmt", ["f8", "i8"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("spread", [0, 4, 30])
+def test_bfloat16_queries_over_8_bits_keep_11_bits_of_the_weights(gpu, fmt, dim, page, spread):
+    """Through each kernel, over contexts in one piece and split; with value rows whose
+    magnitudes differ by up to 2^60, some of them zero, growing along one context."""
+    starts, lens, group = [900, 0], [70, 45], 4
+    sq = ko.Seqs(starts, lens, page, seed=page)
+    cache = _cache(sq, 1, dim, fmt, gpu)
+    b = _batch(sq, gpu)
+    whole = ko.Seqs([0, 0], [o + n for o, n in zip(starts, lens)], page)
+    g = torch.Generator(device=gpu).manual_seed(9)
+    k, v = (torch.randn(whole.tokens, 1, dim, generator=g, device=gpu) for _ in range(2))
+    if spread:
+        powers = (torch.rand(whole.tokens, 1, 1, generator=g, device=gpu) * 2 * spread - spread).round()
+        powers[:whole.lens[0]] = powers[:whole.lens[0]].sort(0).values if spread == 4 else powers[:whole.lens[0]]
+        v *= torch.exp2(powers)
+        v[3::17] = 0
+    every = [torch.tensor(x, dtype=torch.int32, device=gpu) for x in (whole.starts, whole.offsets)]
+    ck.kv_write(cache, ck.KvBatch(b.page_table, *every, whole.tokens), k, v)
+    q = (torch.randn(sq.tokens, group, dim, generator=g, device=gpu) * 1.5).to(torch.bfloat16)
+    kd, vd = (np.nan_to_num(_values(cache, n, fmt), nan=0.0) for n in ("k", "v"))
+    ref = ko.attention(sq, kd, vd, q.cpu().double().numpy(), group, dim ** -0.5, 0)
+    # a weight with its value's scale rounds by 2^-25 at least, held against 2^6 of the largest scale: 2^-31 of the largest value
+    bound, lbound = ko.attention_bounds(*ref, dim, ko.UNIT[torch.float16], q.dtype, 2 * np.abs(vd).max())
+    for chunk in (70, 20, 1):
+        for context in (1, 1000):
+            print(f"[case] 11 bits {fmt} {dim} spread={spread} chunk={chunk} context={context}", flush=True)
+            lse = torch.empty(sq.tokens, group, device=gpu)
+            plan = ck.KvAttention(group, 1, dim, 2, sq.tokens, chunk, context)
+            out = plan.run(cache, ck.KvBatch(b.page_table, b.starts, b.offsets, sq.tokens, chunk, context), q, lse=lse)
+            torch.cuda.synchronize()
+            err = np.abs(out.cpu().double().numpy() - ref[0])
+            print(f"  largest error / bound: {(err / bound).max():.3f}", flush=True)
+            assert (err <= bound).all()
+            assert (np.abs(lse.cpu().double().numpy() - ref[1]) <= lbound).all()
