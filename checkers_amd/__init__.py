@@ -42,6 +42,7 @@ EXPORTED = [  # every symbol include/checkers_amd.h declares
     "ckr_stats_slab_bytes", "ckr_carve_stats_slab", "ckr_analyze_device_records",
     "ckr_analyze_device_records_workspace_bytes", "ckr_make_contiguous",
     "ckr_kv_write", "ckr_kv_read", "ckr_kv_attention_workspace_bytes", "ckr_kv_attention", "ckr_add_rms_norm",
+    "ckr_rotary_turns", "ckr_rotate", "ckr_kv_append",
 ]
 
 
@@ -190,6 +191,9 @@ def lib():
         "ckr_make_contiguous": (i32, [vp, i32, vp, vp, i32, vp, vp]),
         "ckr_kv_write": (i32, [vp, vp, vp, i64, i64, vp, i64, i64, i32, vp]),
         "ckr_kv_read": (i32, [vp, vp, vp, i64, i64, vp, i64, i64, i32, vp]),
+        "ckr_rotary_turns": (i32, [vp, u32, vp]),
+        "ckr_rotate": (i32, [vp, vp, vp, vp, u32, u32, u32, u32, i32, i32, vp]),
+        "ckr_kv_append": (i32, [vp, vp, vp, vp, vp, i64, i64, vp, i64, i64, vp, i64, i64, u32, vp, i64, i64, i32, vp]),
         "ckr_kv_attention_workspace_bytes": (u64, [u32] * 7),
         "ckr_kv_attention": (i32, [vp, vp, vp, i64, i64, i32, u32, f32, u32, vp, i64, i64, vp, vp, u64, vp]),
         "ckr_add_rms_norm": (i32, [vp, i64, vp, i64, vp, i32, u64, u32, i32, f32, i32, u32, vp, i64, vp, vp, i64, vp]),
@@ -808,5 +812,5 @@ class Checkpoint:
             pass
 
 
-# ---- operators around an 8-bit key/value cache (checkers_amd/kv.py)
-from .kv import F8, KvAttention, KvBatch, KvCache, add_rms_norm, kv_read, kv_write  # noqa: E402,F401
+# ---- operators around a 4- or 8-bit key/value cache (checkers_amd/kv.py)
+from .kv import F4, F8, KvAttention, KvBatch, KvCache, Rotary, add_rms_norm, kv_append, kv_read, kv_write, rotary  # noqa: E402,F401

@@ -17,7 +17,8 @@ LIB = os.path.join(HERE, "libcheckers_amd.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["ckr_kernels.hip", "ckr_repair.hip", "ckr_api.cpp", "ckr_checkpoint.cpp", "ckr_context.hip",
-           "ckr_container.hip", "ckr_analyzer.hip", "ckr_kv.hip", "ckr_attention.hip"]
+           "ckr_container.hip", "ckr_analyzer.hip", "ckr_kv.hip", "ckr_attention.hip", "ckr_attention4.hip",
+           "ckr_rotary.hip"]
 
 # -packed-fp32-ops: no v_pk_*_f32 generated anywhere (wrong results seen with
 # some of their forms on these machines).
@@ -68,11 +69,11 @@ def _run(cmd, verbose):
         raise subprocess.CalledProcessError(r.returncode, cmd)
 
 
-# ckr_attention.hip: matrix products whose result the vector units read next leave
+# the attention's kernels: matrix products whose result the vector units read next leave
 # it in vector registers (by default a kernel of more than 256 registers keeps all
 # results in accumulation registers and copies them: float16, heads of 256, 16 chunks of
 # 64 tokens over 4096: 456 against 393 us; kernels of fewer registers measure the same)
-SOURCE_FLAGS = {"ckr_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+SOURCE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("ckr_attention.hip", "ckr_attention4.hip")}
 
 
 def _stale(src, obj):
@@ -80,7 +81,7 @@ def _stale(src, obj):
     if not os.path.exists(obj):
         return True
     deps = [src, os.path.join(ROOT, "include", "checkers_amd.h"), os.path.join(CSRC, "ckr_internal.h"),
-            os.path.join(CSRC, "ckr_table.h"), os.path.join(CSRC, "ckr_kv.h"),
+            os.path.join(CSRC, "ckr_table.h"), os.path.join(CSRC, "ckr_kv.h"), os.path.join(CSRC, "ckr_attention.h"),
             os.path.join(CSRC, "ckr_container.h")]
     return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps)
 

@@ -21,6 +21,9 @@ struct ElemBF16 { static constexpr int tag = CKR_BF16, bytes = 2; };
 struct ElemF16 { static constexpr int tag = CKR_F16, bytes = 2; };
 struct ElemI8 { static constexpr int tag = CKR_I8, bytes = 1; };
 struct ElemF8 { static constexpr int tag = CKR_F8, bytes = 1; };
+struct ElemF4 { static constexpr int tag = CKR_F4, bytes = 0; };  // two a byte: none of the sizes that is asked for by `bytes`
+template <typename E> constexpr uint32_t bytes_of(uint32_t n) { return E::tag == CKR_F4 ? n / 2 : n * E::bytes; }
+constexpr uint32_t kGroup = 32;  // values of a CKR_F4 row that share a power of two
 
 __device__ __forceinline__ float as_f32(uint32_t u) { return __builtin_bit_cast(float, u); }
 __device__ __forceinline__ uint32_t as_u32(float f) { return __builtin_bit_cast(uint32_t, f); }
@@ -66,6 +69,57 @@ template <> __device__ __forceinline__ uint32_t encode4<ElemI8>(float a, float b
     const uint32_t x = (uint32_t)(int)__builtin_rintf(a) & 0xffu, y = (uint32_t)(int)__builtin_rintf(b) & 0xffu;
     const uint32_t z = (uint32_t)(int)__builtin_rintf(c) & 0xffu, w = (uint32_t)(int)__builtin_rintf(d);
     return x | y << 8 | z << 16 | w << 24;
+}
+
+// ---- four bits.  The conversions take their power of two from a float's exponent bits,
+// as the scale's byte is (255, NaN, gives NaN), round ties to even and end at 6.
+// Eight codes of a dword, times a scale's power, as four dwords of 16 bits or eight floats (exact
+// within the type's range).
+__device__ __forceinline__ float power_of(uint32_t byte) { return as_f32(byte << 23); }
+template <typename E> __device__ __forceinline__ u32x4 widen8(uint32_t v, float power) {
+    if constexpr (E::tag == CKR_BF16)
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, power, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, power, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, power, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, power, 3))};
+    else
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, power, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, power, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, power, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, power, 3))};
+}
+__device__ __forceinline__ void decode8(uint32_t v, float power, float* x) {
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, power, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, power, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, power, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, power, 3);
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
+}
+__device__ __forceinline__ uint32_t encode8(const float* x, uint32_t byte) {  // zeros where byte is 255 too
+    const float power = power_of(min(byte, 254u));
+    uint32_t v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], power, 0);
+    v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[2], x[3], power, 1);
+    v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[4], x[5], power, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[6], x[7], power, 3);
+}
+// The scale's byte of a group whose largest magnitude has these bits: the least power
+// (2^-100 to 2^125, so that every value is finite) of which it is at most 7 times; 0: a
+// group of zeros, 255: NaN.
+__device__ __forceinline__ uint32_t group_byte(uint32_t top) {
+    if (top >= 0x7f800000u) return 255u;
+    if (as_f32(top) < 0x1p-100f) return 0u;
+    return min(max((top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u), 27u), 252u);
+}
+
+// The same for N values of each of two neighbouring lanes that hold a group; a group that is
+// stored as zeros becomes zeros.
+template <int N> __device__ __forceinline__ uint32_t group_byte_of(float* x) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) top = max(top, as_u32(x[i]) & 0x7fffffffu);
+    const uint32_t byte = group_byte(max(top, (uint32_t)__shfl_xor((int)top, 1)));
+    const bool kept = byte - 1 < 254;
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = kept ? x[i] : 0.f;
+    return byte;
 }
 
 // The same vectors at any address: global memory takes them whole.

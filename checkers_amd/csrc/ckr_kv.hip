@@ -1,5 +1,5 @@
 // checkers_amd/csrc/ckr_kv.hip — writing and reading a paged key/value cache in
-// 8 or 16 bits, and the residual sum and root-mean-square norm with an output
+// 4, 8 or 16 bits, and the residual sum and root-mean-square norm with an output
 // in 8 bits.  All three are bound by memory: one pass, rows kept in registers
 // between the reduction and the store.
 #include <algorithm>
@@ -40,18 +40,25 @@ template <size_t N> bool apart(std::array<Axis, N> axes, uint64_t run) {
     }
     return true;
 }
+// Entries of a row (pairs of codes for CKR_F4) and scales of a page's head that lie side by side.
+uint64_t entries_of_row(const ckr_kv_cache* c) { return c->dtype == CKR_F4 ? c->head_dim / 2 : c->head_dim; }
+uint64_t scales_of_head(const ckr_kv_cache* c) {
+    return (uint64_t)c->page_size * (c->dtype == CKR_F4 ? c->head_dim / kGroup : 1);
+}
+}  // namespace
 // A cache that is written: its rows, and its scales.
-int check_rows_apart(const ckr_kv_cache* c) {
+int kv_check_rows_apart(const ckr_kv_cache* c) {
     const uint64_t pages = c->n_pages, heads = c->n_heads, slots = c->page_size;
     for (int which = 0; which < 2; which++) {
         const int64_t* st = which ? c->v_stride : c->k_stride;
         const int64_t* ss = which ? c->v_scale_stride : c->k_scale_stride;
-        if (!apart(std::array<Axis, 3>{{{st[0], pages}, {st[1], heads}, {st[2], slots}}}, c->head_dim) ||
-            (c->d_k_scale && !apart(std::array<Axis, 2>{{{ss[0], pages}, {ss[1], heads}}}, slots)))
+        if (!apart(std::array<Axis, 3>{{{st[0], pages}, {st[1], heads}, {st[2], slots}}}, entries_of_row(c)) ||
+            (c->d_k_scale && !apart(std::array<Axis, 2>{{{ss[0], pages}, {ss[1], heads}}}, scales_of_head(c))))
             return err(CKR_E_INVALID, std::string("rows of the cache ") + (which ? "values" : "keys") + " overlap");
     }
     return CKR_OK;
 }
+namespace {
 
 // A lane holds 16 values of a (token, head) row: a 16-byte store of codes, and
 // two to four 16-byte loads.  LPR lanes (a power of two) share a row.
@@ -63,8 +70,8 @@ struct RowsArg {
     int64_t k_tok, k_head, v_tok, v_head;
     uint8_t* ck;        // the cache
     uint8_t* cv;
-    float* sk;
-    float* sv;
+    void* sk;
+    void* sv;
     int64_t kst[3], vst[3], skst[2], svst[2];
     uint32_t n_pages, page_shift, heads, dim;
     KvBatch b;
@@ -93,6 +100,7 @@ __device__ __forceinline__ uint32_t first_seq(const KvBatch& b, uint32_t token) 
 template <typename X, typename C, int LPR, bool WRITE>
 __global__ void __launch_bounds__(256) kv_rows_kernel(RowsArg a) {
     constexpr uint32_t ROWS = 256 / LPR;
+    constexpr bool FOUR = C::tag == CKR_F4;
     const uint64_t row0 = (uint64_t)blockIdx.x * ROWS;
     uint32_t seq = first_seq(a.b, (uint32_t)(row0 / a.heads));
     const uint64_t row = row0 + threadIdx.x / LPR;
@@ -116,9 +124,13 @@ __global__ void __launch_bounds__(256) kv_rows_kernel(RowsArg a) {
                       lane * kVals) * X::bytes;
         const int64_t* st = which ? a.vst : a.kst;
         uint8_t* c = (which ? a.cv : a.ck) +
-                     ((int64_t)page * st[0] + (int64_t)head * st[1] + (int64_t)slot * st[2] + lane * kVals) * C::bytes;
+                     ((int64_t)page * st[0] + (int64_t)head * st[1] + (int64_t)slot * st[2]) * (FOUR ? 1 : C::bytes) +
+                     lane * bytes_of<C>(kVals);
         const int64_t* sst = which ? a.svst : a.skst;
-        float* s = (which ? a.sv : a.sk) + ((int64_t)page * sst[0] + (int64_t)head * sst[1] + slot);
+        const int64_t s_at = (int64_t)page * sst[0] + (int64_t)head * sst[1] + slot;
+        float* s = static_cast<float*>(which ? a.sv : a.sk) + s_at;
+        // four bits: the pair of lanes that hold a group share its byte
+        uint8_t* s4 = static_cast<uint8_t*>(which ? a.sv : a.sk) + s_at + ((int64_t)(lane * kVals / kGroup) << a.page_shift);
         float f[kVals];
 #pragma unroll
         for (int i = 0; i < kVals; i++) f[i] = 0.f;
@@ -135,10 +147,24 @@ __global__ void __launch_bounds__(256) kv_rows_kernel(RowsArg a) {
                 for (int i = 0; i < kVals; i++) f[i] = scaled(f[i], rs.inv);
                 if (mine && page >= 0 && lane == 0) *s = rs.scale;
             }
-            if (mine && page >= 0) store_vec<C, kVals>(c, f);
+            if constexpr (FOUR) {
+                const uint32_t byte = group_byte_of<kVals>(f);
+                if (mine && page >= 0) {
+                    *reinterpret_cast<u32x2*>(c) = u32x2{encode8(f, byte), encode8(f + 8, byte)};
+                    if (lane % 2 == 0) *s4 = (uint8_t)byte;
+                }
+            } else if (mine && page >= 0) {
+                store_vec<C, kVals>(c, f);
+            }
         } else {
             if (mine && page >= 0) {
-                load_vec<C, kVals>(c, f);
+                if constexpr (FOUR) {
+                    const u32x2 codes = *reinterpret_cast<const u32x2*>(c);
+                    const float power = power_of(*s4);
+                    decode8(codes[0], power, f), decode8(codes[1], power, f + 8);
+                } else {
+                    load_vec<C, kVals>(c, f);
+                }
                 if constexpr (C::bytes == 1) {
                     const float scale = *s;
 #pragma unroll
@@ -168,6 +194,7 @@ hipError_t launch_rows_of(const RowsArg& a, int cache_dtype, hipStream_t s) {
     switch (cache_dtype) {
         case CKR_F8: return launch_rows<X, ElemF8, WRITE>(a, s);
         case CKR_I8: return launch_rows<X, ElemI8, WRITE>(a, s);
+        case CKR_F4: return launch_rows<X, ElemF4, WRITE>(a, s);
         case CKR_BF16: return launch_rows<X, ElemBF16, WRITE>(a, s);
         default: return launch_rows<X, ElemF16, WRITE>(a, s);
     }
@@ -184,7 +211,7 @@ int rows_call(const ckr_kv_cache* c, const ckr_kv_batch* b, void* k, int64_t kt,
     const int es = ckr_element_size(dtype);
     if ((rc = kv_check_rows(k, b->n_tokens, kt, c->n_heads, kh, c->head_dim, es, !WRITE, "keys")) ||
         (rc = kv_check_rows(v, b->n_tokens, vt, c->n_heads, vh, c->head_dim, es, !WRITE, "values")) ||
-        (WRITE && (rc = check_rows_apart(c))))
+        (WRITE && (rc = kv_check_rows_apart(c))))
         return rc;
     RowsArg a{};
     a.k = k, a.v = v, a.k_tok = kt, a.k_head = kh, a.v_tok = vt, a.v_head = vh;
@@ -418,13 +445,15 @@ int kv_check_rows(const void* p, uint64_t rows, int64_t row_stride, uint64_t hea
 
 int kv_check_cache(const ckr_kv_cache* c) {
     if (!c) return err(CKR_E_INVALID, "null cache");
-    const bool coded = c->dtype == CKR_F8 || c->dtype == CKR_I8;
+    const bool four = c->dtype == CKR_F4, coded = four || c->dtype == CKR_F8 || c->dtype == CKR_I8;
     if (!coded && c->dtype != CKR_BF16 && c->dtype != CKR_F16)
-        return err(CKR_E_INVALID, "a cache holds 8-bit floats, int8, bfloat16 or float16, not dtype " + std::to_string(c->dtype));
+        return err(CKR_E_INVALID, "a cache holds 4- or 8-bit floats, int8, bfloat16 or float16, not dtype " + std::to_string(c->dtype));
     if (c->page_size < 16 || (c->page_size & (c->page_size - 1)))
         return err(CKR_E_INVALID, "page size " + std::to_string(c->page_size) + ": a power of two from 16 on");
     if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16)
         return err(CKR_E_INVALID, "head size " + std::to_string(c->head_dim) + ": a multiple of 16 up to 256");
+    if (four && c->head_dim % kGroup)
+        return err(CKR_E_INVALID, "head size " + std::to_string(c->head_dim) + ": a multiple of 32 in 4 bits");
     if (c->n_heads == 0 || c->n_heads > 65535) return err(CKR_E_INVALID, "a cache has 1 to 65535 heads");
     if (c->n_pages == 0 || c->n_pages > 0x7fffffffu) return err(CKR_E_INVALID, "a cache has 1 to 2^31 - 1 pages");
     const int es = coded ? 1 : 2;
@@ -433,7 +462,7 @@ int kv_check_cache(const ckr_kv_cache* c) {
         const int64_t* st = which ? c->v_stride : c->k_stride;
         const char* what = which ? "cache values" : "cache keys";
         if (!p) return err(CKR_E_INVALID, std::string("null ") + what + " pointer");
-        unsigned __int128 last = c->head_dim;
+        unsigned __int128 last = entries_of_row(c);
         const uint64_t shape[3] = {c->n_pages, c->n_heads, c->page_size};
         for (int i = 0; i < 3; i++) {
             if (shape[i] == 1) continue;
@@ -446,17 +475,18 @@ int kv_check_cache(const ckr_kv_cache* c) {
         int rc = check_range(p, (uint64_t)last * es, what);
         if (rc) return rc;
         if (!coded) continue;
-        const float* s = which ? c->d_v_scale : c->d_k_scale;
+        const void* s = which ? c->d_v_scale : c->d_k_scale;
         const int64_t* given = which ? c->v_scale_stride : c->k_scale_stride;
         const int64_t ss[2] = {c->n_pages == 1 ? 0 : given[0], c->n_heads == 1 ? 0 : given[1]};
         const char* swhat = which ? "value scales" : "key scales";
-        if (!s) return err(CKR_E_INVALID, std::string("null ") + swhat + " pointer (an 8-bit cache has scales)");
-        if (!multiple(s, 16) || ss[0] < 0 || ss[1] < 0 || ss[0] % 4 || ss[1] % 4)
+        if (!s) return err(CKR_E_INVALID, std::string("null ") + swhat + " pointer (" + (four ? "a 4" : "an 8") + "-bit cache has scales)");
+        const int64_t unit = four ? 16 : 4;  // scales in 16 bytes
+        if (!multiple(s, 16) || ss[0] < 0 || ss[1] < 0 || ss[0] % unit || ss[1] % unit)
             return err(CKR_E_INVALID, std::string(swhat) + " must start on 16-byte boundaries for every page and head");
         const unsigned __int128 slast = (unsigned __int128)(c->n_pages - 1) * (uint64_t)ss[0] +
-                                        (unsigned __int128)(c->n_heads - 1) * (uint64_t)ss[1] + c->page_size;
+                                        (unsigned __int128)(c->n_heads - 1) * (uint64_t)ss[1] + scales_of_head(c);
         if (slast > (1ull << 46)) return err(CKR_E_INVALID, std::string("strides of the ") + swhat + " are out of range");
-        if ((rc = check_range(s, (uint64_t)slast * 4, swhat))) return rc;
+        if ((rc = check_range(s, (uint64_t)slast * (four ? 1 : 4), swhat))) return rc;
     }
     return CKR_OK;
 }

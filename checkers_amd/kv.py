@@ -1,10 +1,11 @@
-"""The operators around an 8-bit key/value cache: kv_write, kv_read, KvAttention
-and add_rms_norm over the C ABI (include/checkers_amd.h).
+"""The operators around a 4- or 8-bit key/value cache: kv_write, kv_append, kv_read,
+KvAttention, add_rms_norm and rotary over the C ABI (include/checkers_amd.h).
 
 A KvCache names the cache's tensors, a KvBatch the tokens a call is about; both
 are descriptors made once and passed to every call (the page table, starts and
 offsets may change in place between calls: the kernels read them on the
-device).  No call here copies or synchronises; only making a KvAttention does.
+device).  No call here copies or synchronises; only making a KvAttention or a
+Rotary does.
 
 stream=: the stream a call's work is queued on, None: the current one.  As with
 torch's own operators the caller orders it after the streams that made the
@@ -12,14 +13,16 @@ inputs, and keeps them (or records them on it) until it is done; outputs that
 a call makes belong to that stream and may be used on the current one once that
 waits for it.
 
-None of this has a backward pass: tensors that require gradients are refused
-where gradients are recorded (not under torch.no_grad()).
+Only rotary has a backward pass: elsewhere tensors that require gradients are
+refused where gradients are recorded (not under torch.no_grad()).
 """
 import ctypes
+import math
 
 from . import CKR_E_INVALID, BF16, F16, F32, I8, CkrError, _check, _torch, lib
 
 F8 = 16  # 8-bit floating point (e4m3, largest value 448), a type of these operators only
+F4 = 17  # 4-bit floating point (e2m1, two a byte) with a power of two for each 32 values, a type of caches only
 
 _i64x3, _i64x2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
 
@@ -47,7 +50,7 @@ def _tag(dtype):
     if not _TAGS:
         torch = _torch()
         _TAGS.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int8: I8,
-                      torch.float8_e4m3fn: F8})
+                      torch.float8_e4m3fn: F8, torch.float4_e2m1fn_x2: F4})
     tag = _TAGS.get(dtype)
     if tag is None:
         raise CkrError(CKR_E_INVALID, f"[ckr] {dtype} is not a type of the cache and norm operators")
@@ -74,27 +77,39 @@ def _on_gpu(t, what):
 class KvCache:
     """A paged cache over the caller's tensors: k and v [pages, heads, page_size,
     head_dim] with any strides of the first three axes, for 8-bit types k_scale
-    and v_scale [pages, heads, page_size] in float32 (slots contiguous)."""
+    and v_scale [pages, heads, page_size] in float32 (slots contiguous).  In 4 bits
+    k and v are float4_e2m1fn_x2 [pages, heads, page_size, head_dim / 2] (two values an
+    entry, the first in its low half), their scales float8_e8m0fnu [pages, heads,
+    head_dim / 32, page_size], the last two axes contiguous."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype, "k and v must be alike, [pages, heads, page_size, head_dim]")
         _need(k.stride(3) == 1 and v.stride(3) == 1, "the last axis of k and v must be contiguous")
         self.dtype = _tag(k.dtype)
-        coded = self.dtype in (F8, I8)
-        _need(coded == (k_scale is not None) == (v_scale is not None), "scales belong to 8-bit caches, and to both k and v")
+        coded = self.dtype in (F4, F8, I8)
+        _need(coded == (k_scale is not None) == (v_scale is not None), "scales belong to 4- and 8-bit caches, and to both k and v")
         for t, what in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
             if t is not None:
                 _on_gpu(t, what)
                 _need(t.device == k.device, "the cache's tensors must be on one GPU")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_pages, self.n_heads, self.page_size, self.head_dim = k.shape
+        self.n_pages, self.n_heads, self.page_size, row = k.shape
+        self.head_dim = row * 2 if self.dtype == F4 else row
         c = _Cache(k.data_ptr(), v.data_ptr(), None, None, _i64x3(*k.stride()[:3]), _i64x3(*v.stride()[:3]),
-                   _i64x2(0, 0), _i64x2(0, 0), *(int(n) for n in (k.shape[0], k.shape[2], k.shape[1], k.shape[3])),
+                   _i64x2(0, 0), _i64x2(0, 0), *(int(n) for n in (k.shape[0], k.shape[2], k.shape[1], self.head_dim)),
                    self.dtype, 0)
-        if coded:
+        if self.dtype == F4:
+            groups = self.head_dim // 32
+            _need(groups * 32 == self.head_dim, f"head size {self.head_dim}: a multiple of 32 in 4 bits")
+            for t in (k_scale, v_scale):
+                _need(t.shape == (*k.shape[:2], groups, self.page_size) and t.dtype == _torch().float8_e8m0fnu and t.stride(3) == 1
+                      and (groups == 1 or t.stride(2) == self.page_size),
+                      "scales must be float8_e8m0fnu [pages, heads, head_dim / 32, page_size], the last two axes contiguous")
+        elif coded:
             for t in (k_scale, v_scale):
                 _need(t.shape == k.shape[:3] and t.dtype == _torch().float32 and t.stride(2) == 1,
                       "scales must be float32 [pages, heads, page_size], slots contiguous")
+        if coded:
             c.d_k_scale, c.d_v_scale = k_scale.data_ptr(), v_scale.data_ptr()
             c.k_scale_stride, c.v_scale_stride = _i64x2(*k_scale.stride()[:2]), _i64x2(*v_scale.stride()[:2])
         self._c = c
@@ -102,19 +117,25 @@ class KvCache:
 
     @classmethod
     def empty(cls, n_pages, page_size, n_heads, head_dim, dtype, device="cuda"):
-        """A cache of new tensors (dtype: F8, I8, BF16 or F16), zeroed."""
+        """A cache of new tensors (dtype: F4, F8, I8, BF16 or F16), zeroed."""
         torch = _torch()
         t = _torch_dtype(dtype)
-        kv = [torch.zeros((n_pages, n_heads, page_size, head_dim), dtype=torch.uint8 if dtype == F8 else t, device=device)
-              for _ in range(2)]
-        if dtype == F8:
+        if dtype == F4:
+            _need(head_dim % 32 == 0, f"head size {head_dim}: a multiple of 32 in 4 bits")
+        kv = [torch.zeros((n_pages, n_heads, page_size, head_dim // 2 if dtype == F4 else head_dim),
+                          dtype=torch.uint8 if dtype in (F4, F8) else t, device=device) for _ in range(2)]
+        if dtype in (F4, F8):
             kv = [x.view(t) for x in kv]
-        sc = [torch.zeros((n_pages, n_heads, page_size), dtype=torch.float32, device=device) if dtype in (F8, I8) else None
-              for _ in range(2)]
+        if dtype == F4:
+            sc = [torch.zeros((n_pages, n_heads, head_dim // 32, page_size), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+                  for _ in range(2)]
+        else:
+            sc = [torch.zeros((n_pages, n_heads, page_size), dtype=torch.float32, device=device) if dtype in (F8, I8) else None
+                  for _ in range(2)]
         return cls(kv[0], kv[1], sc[0], sc[1])
 
     def tensors(self):
-        """The cache's tensors (k, v and, in 8 bits, their scales)."""
+        """The cache's tensors (k, v and, in 4 and 8 bits, their scales)."""
         return [t for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None]
 
 
@@ -195,6 +216,17 @@ def _new(shape, dtype, device, stream):
     return t
 
 
+def _used_by(owner, tensor, handle, stream):
+    """A first call on a stream other than the one an owner's tensor was made on."""
+    torch = _torch()
+    if stream is None:
+        if torch.cuda.is_current_stream_capturing():   # whoever keeps the graph keeps its owner
+            return
+        stream = torch.cuda.current_stream(tensor.device)
+    tensor.record_stream(stream)
+    owner._streams.add(handle)
+
+
 def kv_write(cache, batch, k, v, stream=None):
     """Quantise the batch's keys and values [tokens, heads, head_dim] into the cache."""
     if k.requires_grad or v.requires_grad:
@@ -207,6 +239,45 @@ def kv_write(cache, batch, k, v, stream=None):
     rc = lib().ckr_kv_write(cache._p, batch._p, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _tag(dtype), _stream_of(stream, k))
     if rc:
         _check(rc)
+
+
+def kv_append(cache, batch, rotary, k, v, q=None, out=None, positions=None, stream=None):
+    """kv_write of keys that are turned by their positions on the way (rotary: a Rotary,
+    None: not turned).  q [tokens, heads, head_dim], of the keys' type: the chunk's queries,
+    turned as well, into out (may be q; new when None), which is returned (None without q).
+    positions: a contiguous int32 [tokens] where they are not those in the cache."""
+    if k.requires_grad or v.requires_grad or q is not None and q.requires_grad:
+        _no_backward()
+    dtype, n, h, d = k.dtype, batch.n_tokens, cache.n_heads, cache.head_dim
+    if v.dtype != dtype:
+        _bad("k and v must be of one type")
+    kt, kh = _rows(k, n, h, d, "k")
+    vt, vh = _rows(v, n, h, d, "v")
+    heads, q_ptr, out_ptr, qt, qh, ot, oh = 0, None, None, 0, 0, 0, 0
+    if q is not None:
+        if q.dtype != dtype:
+            _bad("q must be of k's type")
+        heads = q.shape[1] if q.dim() == 3 else 0
+        qt, qh = _rows(q, n, heads, d, "q")
+        if out is None:
+            out = _new(q.shape, dtype, q.device, stream)
+        if out.dtype != dtype:
+            _bad("out must be of q's type")
+        ot, oh = _rows(out, n, heads, d, "out")
+        q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    elif out is not None:
+        _bad("out belongs to q")
+    if positions is not None and (positions.dtype != _torch().int32 or positions.shape != (n,) or not positions.is_contiguous() or not positions.is_cuda):
+        _bad(f"positions must be a contiguous int32 [{n}] on the GPU")
+    handle = _stream_of(stream, k)
+    if rotary is not None and handle not in rotary._streams:
+        _used_by(rotary, rotary.turns, handle, stream)
+    rc = lib().ckr_kv_append(cache._p, batch._p, None if rotary is None else rotary._p, None if positions is None else positions.data_ptr(),
+                             k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, q_ptr, qt, qh, heads, out_ptr, ot, oh, _tag(dtype),
+                             handle)
+    if rc:
+        _check(rc)
+    return out
 
 
 def kv_read(cache, batch, dtype=BF16, out=None, stream=None):
@@ -247,16 +318,6 @@ class KvAttention:
             home.synchronize()
         self._streams = {home.cuda_stream}   # whose work the workspace's memory outlives
 
-    def _used_by(self, handle, stream):
-        """A first call on a stream other than the one the workspace was made on."""
-        torch = _torch()
-        if stream is None:
-            if torch.cuda.is_current_stream_capturing():   # whoever keeps the graph keeps the plan
-                return
-            stream = torch.cuda.current_stream(self.ws.device)
-        self.ws.record_stream(stream)
-        self._streams.add(handle)
-
     def run(self, cache, batch, q, scale=None, window=0, out=None, lse=None, stream=None):
         """Attention of the batch's tokens, whose keys and values the cache already
         holds: q [tokens, n_heads, head_dim] -> out (of q's type, new when None).
@@ -280,7 +341,7 @@ class KvAttention:
             lse_ptr = lse.data_ptr()
         handle = _stream_of(stream, q)
         if handle not in self._streams:
-            self._used_by(handle, stream)
+            _used_by(self, self.ws, handle, stream)
         rc = lib().ckr_kv_attention(cache._p, batch._p, q.data_ptr(), qt, qh, _tag(dtype), h, d ** -0.5 if scale is None else scale,
                                     min(window, 0xffffffff), out.data_ptr(), ot, oh, lse_ptr, self._ws_ptr, self.ws_bytes, handle)
         if rc:
@@ -345,3 +406,181 @@ def _row_stride(t, shape, what):
     if b != 1 and shape[1] > 1:
         _bad(f"the last axis of {what} must be contiguous, {what} {list(shape)}")
     return a
+
+
+# ---- rotary positions
+class _Rot(ctypes.Structure):
+    _fields_ = [("d_turns", ctypes.c_void_p), ("magnitude", ctypes.c_double), ("n_pairs", ctypes.c_uint32),
+                ("interleaved", ctypes.c_uint32)]
+
+
+def _frequencies(rotary_dim, base, scaling):
+    """(radians a position of each pair, the factor on both of its values)."""
+    f = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    if scaling is None:
+        return f, 1.0
+    s = dict(scaling)
+    kind, factor = s.pop("kind", None), float(s.pop("factor", 0.0))
+    known = {"linear": (), "base": (), "bands": ("length", "low", "high"), "yarn": ("length", "fast", "slow", "magnitude")}
+    _need(kind in known, f"scaling kind {kind!r}: one of {', '.join(known)}")
+    _need(factor > 0 and math.isfinite(factor), f"scaling factor {factor}: above 0")
+    _need(set(s) <= set(known[kind]), f"scaling {kind!r} takes {', '.join(('factor',) + known[kind])}, not {', '.join(map(str, s))}")
+    if kind == "linear":
+        return [x / factor for x in f], 1.0
+    if kind == "base":
+        _need(rotary_dim > 2, "scaling 'base' needs two pairs at least")
+        return [(base * factor ** (rotary_dim / (rotary_dim - 2))) ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)], 1.0
+    length = float(s.get("length", 0.0))
+    _need(length > 0, f"scaling {kind!r} needs the original length")
+    if kind == "bands":
+        low, high = float(s.get("low", 1.0)), float(s.get("high", 4.0))
+        _need(high > low, f"scaling 'bands': high {high} must be above low {low}")
+        keep = [min(max((length * x / (2 * math.pi) - low) / (high - low), 0.0), 1.0) for x in f]
+        return [x * (w + (1 - w) / factor) for x, w in zip(f, keep)], 1.0
+    fast, slow = float(s.get("fast", 32.0)), float(s.get("slow", 1.0))
+    _need(fast > slow > 0 and base > 1, "scaling 'yarn': fast above slow above 0, base above 1")
+    at = [rotary_dim * math.log(length / (t * 2 * math.pi)) / (2 * math.log(base)) for t in (fast, slow)]
+    lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary_dim - 1)
+    ramp = [min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0) for i in range(len(f))]
+    magnitude = s.get("magnitude")
+    if magnitude is None:
+        magnitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    return [x * (1 - w) + x / factor * w for x, w in zip(f, ramp)], float(magnitude)
+
+
+class Rotary:
+    """How heads are turned by their positions: the pairs of a head's first rotary_dim
+    values, i and i + rotary_dim / 2 (interleaved: 2 i and 2 i + 1), by position *
+    frequency, that of pair i being base ** (-2 i / rotary_dim).  scaling, for contexts
+    longer than a model was trained on, a dict with a "kind" and a "factor":
+      linear  all frequencies / factor
+      base    base * factor ** (rotary_dim / (rotary_dim - 2))
+      bands   frequencies of fewer than `low` (1) turns within `length`, the original context,
+              / factor, of more than `high` (4) kept, in between interpolated by their turns
+      yarn    / factor and kept likewise, by a ramp over the pairs from the one of `fast` (32) turns
+              within `length` to that of `slow` (1); values times `magnitude` (0.1 ln factor + 1)
+    Making one copies its table to the GPU and waits for that."""
+
+    def __init__(self, rotary_dim, base=10000.0, interleaved=False, scaling=None, device="cuda"):
+        _need(rotary_dim > 0 and rotary_dim % 2 == 0, f"rotary_dim {rotary_dim}: even, from 2 on")
+        _need(base > 0 and math.isfinite(base), f"base {base}: above 0")
+        self._make(*_frequencies(int(rotary_dim), float(base), scaling), interleaved, device)
+
+    @classmethod
+    def of(cls, frequencies, interleaved=False, magnitude=1.0, device="cuda"):
+        """One of given frequencies (radians a position, one of each pair)."""
+        self = cls.__new__(cls)
+        self._make([float(x) for x in frequencies], float(magnitude), interleaved, device)
+        return self
+
+    def _make(self, frequencies, magnitude, interleaved, device):
+        torch = _torch()
+        n = len(frequencies)
+        _need(n > 0, "a rotary has one pair at least")
+        _need(math.isfinite(magnitude), "the rotary's magnitude must be finite")
+        self.frequencies, self.magnitude, self.interleaved, self.rotary_dim = frequencies, magnitude, bool(interleaved), 2 * n
+        host = torch.empty(n, dtype=torch.int64)
+        _check(lib().ckr_rotary_turns((ctypes.c_double * n)(*frequencies), n, host.data_ptr()))
+        self.turns = host.to(device)   # complete when this returns
+        _on_gpu(self.turns, "a rotary")
+        self._streams = {torch.cuda.current_stream(self.turns.device).cuda_stream}   # whose work the table outlives
+        self._c = _Rot(self.turns.data_ptr(), magnitude, n, self.interleaved)
+        self._p = ctypes.byref(self._c)
+
+
+_i64x18, _i64x2v = ctypes.c_int64 * 18, ctypes.c_int64 * 2
+
+
+def _heads_of(x, lead, dim, dtype, what):
+    """(batch, token and head stride, heads) of a [batch, tokens, heads, dim] tensor, or of one without batch."""
+    shape = x.shape
+    if shape[:-2] != lead or shape[-1] != dim or x.dtype != dtype or not x.is_cuda:
+        _bad(f"{what} must be {[*lead, 'heads', dim]} of {dtype} on the GPU")
+    st = x.stride()
+    if st[-1] != 1 and x.numel():
+        _bad(f"the last axis of {what} must be contiguous")
+    return (st[0], st[1], st[2], shape[2]) if len(shape) == 4 else (0, st[0], st[1], shape[1])
+
+
+def _rotate(rotary, positions, xs, outs, inverse, stream):
+    """xs (one or two tensors) turned into outs."""
+    q = xs[0]
+    lead, dim, dtype = q.shape[:-2], q.shape[-1], q.dtype
+    if positions.dtype != _torch().int32 or not positions.is_cuda or positions.shape != lead and positions.shape != lead[-1:]:
+        _bad(f"positions must be int32 {list(lead)} or {list(lead[-1:])} on the GPU")
+    ps = positions.stride()
+    handle = _stream_of(stream, q)
+    if handle not in rotary._streams:
+        _used_by(rotary, rotary.turns, handle, stream)
+    flat = []
+    for i, (x, y) in enumerate(zip(xs, outs)):
+        b, t, h, n = _heads_of(x, lead, dim, dtype, "qk"[i])
+        ob, ot, oh, on = _heads_of(y, lead, dim, dtype, f"out of {'qk'[i]}")
+        if on != n:
+            _bad(f"out of {'qk'[i]} must have its heads")
+        if x.data_ptr() == y.data_ptr() and x.stride() != y.stride():
+            _bad(f"{'qk'[i]} turned in place must have its own strides")
+        flat += (x.data_ptr(), y.data_ptr(), b, t, h, ob, ot, oh, n)
+    rc = lib().ckr_rotate(rotary._p, positions.data_ptr(), _i64x2v(*(ps if len(ps) == 2 else (0, ps[0]))), _i64x18(*flat), len(xs),
+                          lead[0] if len(lead) == 2 else 1, lead[-1], dim, _tag(dtype), inverse, handle)
+    if rc:
+        _check(rc)
+
+
+_Turn = None
+
+
+def _turn():
+    """The operator with its backward pass, made when it is first needed."""
+    global _Turn
+    if _Turn is None:
+        torch = _torch()
+
+        class Turn(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, rotary, positions, inverse, *xs):
+                ctx.rotary, ctx.inverse = rotary, inverse
+                ctx.save_for_backward(positions)
+                ctx.set_materialize_grads(False)
+                outs = tuple(torch.empty_like(x) for x in xs)
+                _rotate(rotary, positions, xs, outs, inverse, None)
+                return outs
+
+            @staticmethod
+            def backward(ctx, *grads):
+                positions, = ctx.saved_tensors
+                here = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[3 + i]]
+                out = [None] * len(grads)
+                if here:
+                    got = Turn.apply(ctx.rotary, positions, not ctx.inverse,
+                                     *(grads[i] if grads[i].stride(-1) == 1 else grads[i].contiguous() for i in here))
+                    for i, g in zip(here, got):
+                        out[i] = g
+                return (None, None, None, *out)
+
+        _Turn = Turn
+    return _Turn
+
+
+def rotary(rotary, positions, q, k=None, out=None, inverse=False, stream=None):
+    """Heads turned by their tokens' positions (a Rotary): q, and k with it, [tokens, heads, dim] or
+    [batch, tokens, heads, dim] with any strides but the last axis'; positions int32 [tokens] or
+    [batch, tokens].  Returns the turned q, with k a pair; into out (a tensor, with k a pair; may
+    be q and k themselves) when given.  inverse turns back, but for the magnitude: it is the transposed
+    matrix.  Gradients are recorded where q or k requires them (then without out and stream)."""
+    xs = (q,) if k is None else (q, k)
+    if not 3 <= q.dim() <= 4 or any(x.dim() != q.dim() for x in xs):
+        _bad("q and k must be [tokens, heads, dim] or [batch, tokens, heads, dim]")
+    if _torch().is_grad_enabled() and any(x.requires_grad for x in xs):
+        if out is not None or stream is not None:
+            _bad("where gradients are recorded rotary takes neither out nor stream")
+        outs = _turn().apply(rotary, positions, bool(inverse), *xs)
+    else:
+        if out is None:
+            outs = tuple(_new(x.shape, x.dtype, x.device, stream) for x in xs)
+        else:
+            outs = (out,) if k is None else tuple(out)
+            if len(outs) != len(xs) or any(y.requires_grad for y in outs) and _torch().is_grad_enabled():
+                _bad("out must be as many tensors as are turned, and require no gradients")
+        _rotate(rotary, positions, xs, outs, bool(inverse), stream)
+    return outs[0] if k is None else outs

@@ -60,6 +60,9 @@ extern "C" {
  * value 448): a type of the cache and norm operators only, not of tensors (the
  * codec takes such bytes as CKR_I8). */
 #define CKR_F8       16
+/* 4-bit floating point (OCP e2m1: 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives),
+ * two a byte, the first in the low half: a type of caches only. */
+#define CKR_F4       17
 
 /* rANS constants: include/checkers/ANSCompressor.hpp:51-55 */
 #define CKR_SCALE_BITS 12u
@@ -545,21 +548,30 @@ CKR_API int ckr_make_contiguous(const void* d_src, int ndim, const int64_t* shap
  * type's largest value (CKR_F8 448, CKR_I8 127):
  *   scale = a / T,  code = round(x * (T / a)) (ties to even),  value = code * scale
  * in fp32; a < 2^-100 gives scale 0 and codes 0, and a row that holds an
- * infinity or NaN gives scale NaN and codes 0, so that it reads back as NaN. ---- */
+ * infinity or NaN gives scale NaN and codes 0, so that it reads back as NaN.
+ *
+ * CKR_F4: each 32 values of a row share a power of two 2^e, kept as the byte e + 127
+ * (OCP e8m0).  With a = max |x| of the 32, e is the least from -100 to 125 with
+ * a <= 7 * 2^e (125 where none is), code = round(x / 2^e) (ties to even; above 6: 6, which is at most
+ * half a step off), value = code * 2^e exactly; a < 2^-100 gives byte 0 and
+ * codes 0, and 32 values that hold an infinity or NaN give byte 255 (NaN) and codes 0. ---- */
 
 /* A paged cache: keys and values [n_pages][n_heads][page_size][head_dim] in any
- * order of the first three axes (strides in elements, >= 0; the last axis is
- * contiguous).  A CKR_F8 cache that another program fills holds no NaN codes
- * (ckr_kv_write stores none), and a scale is finite or NaN.  dtype CKR_F8 or CKR_I8, with a scale per (page, head, slot) whose
- * slots are contiguous, or CKR_BF16 / CKR_F16 without scales.  page_size is a
- * power of two from 16 on, head_dim a multiple of 16 up to 256; every row must
+ * order of the first three axes (strides in elements, of CKR_F4 in bytes, >= 0; the
+ * last axis is contiguous).  A CKR_F8 cache that another program fills holds no NaN codes
+ * (ckr_kv_write stores none), and a scale is finite or NaN (CKR_F4: a byte up to 252,
+ * or 255).  dtype CKR_F8 or CKR_I8, with an
+ * fp32 scale per (page, head, slot) whose slots are contiguous; CKR_F4, with a byte per
+ * (page, head, 32 dimensions, slot), [head_dim / 32][page_size] contiguous in each
+ * page and head; or CKR_BF16 / CKR_F16 without scales.  page_size is a
+ * power of two from 16 on, head_dim a multiple of 16 (CKR_F4: 32) up to 256; every row must
  * start on a 16-byte boundary, every page's scales of a head too (here and below
  * the stride of an axis with one entry may be anything). */
 typedef struct {
     void* d_k;
     void* d_v;
-    float* d_k_scale;           /* NULL without scales                          */
-    float* d_v_scale;
+    void* d_k_scale;            /* fp32, of CKR_F4 bytes; NULL without scales   */
+    void* d_v_scale;
     int64_t k_stride[3];        /* page, head, slot                             */
     int64_t v_stride[3];
     int64_t k_scale_stride[2];  /* page, head                                   */
@@ -603,6 +615,55 @@ CKR_API int ckr_kv_write(const ckr_kv_cache* cache, const ckr_kv_batch* batch, c
 CKR_API int ckr_kv_read(const ckr_kv_cache* cache, const ckr_kv_batch* batch, void* d_k, int64_t k_token_stride,
                         int64_t k_head_stride, void* d_v, int64_t v_token_stride, int64_t v_head_stride, int dtype,
                         void* stream);
+
+/* Rotary positions: the pairs (x, y) of a head's first 2 * n_pairs values are
+ * turned by the angle position * frequency of their pair,
+ *   (x, y) -> magnitude * (x cos - y sin, y cos + x sin),
+ * values behind them stay.  Pair i is the values i and i + n_pairs, or with
+ * interleaved 2 i and 2 i + 1.  d_turns [n_pairs] on the device: each pair's turns a
+ * position (its frequency / 2 pi, whole turns left out) times 2^64, as
+ * ckr_rotary_turns makes them on the host of frequencies in radians: angles are
+ * products of 64-bit integers, so far positions are as exact as near ones.
+ * Cosine and sine are rounded once to fp32; each product and sum of the formula is one
+ * fp32 operation. */
+typedef struct {
+    const uint64_t* d_turns;
+    double magnitude;
+    uint32_t n_pairs;
+    uint32_t interleaved;       /* 0 or 1                                       */
+} ckr_rotary;
+CKR_API int ckr_rotary_turns(const double* h_frequencies, uint32_t n, uint64_t* h_turns);
+
+/* Heads [batch][tokens][n_heads][head_dim] (strides in elements, >= 0, the last axis
+ * contiguous); d_out is d_in itself with the same strides, or overlaps nothing. */
+typedef struct {
+    const void* d_in;
+    void* d_out;
+    int64_t in_stride[3];       /* batch, token, head                           */
+    int64_t out_stride[3];
+    uint32_t n_heads;
+    uint32_t pad;
+} ckr_rotary_heads;
+/* One or two tensors of heads (queries and keys) turned by d_positions
+ * [batch][tokens] (int32, any value, with its two strides; 0: shared), the other way
+ * round with inverse, which is the transposed matrix: of gradients of the turned
+ * heads it makes those of the heads.  dtype CKR_F32, BF16 or F16, head_dim 2 to 1024.
+ * Only queues work. */
+CKR_API int ckr_rotate(const ckr_rotary* rotary, const int32_t* d_positions, const int64_t* position_stride,
+                       const ckr_rotary_heads* heads, uint32_t n, uint32_t batch, uint32_t tokens, uint32_t head_dim,
+                       int dtype, int inverse, void* stream);
+
+/* ckr_kv_write of keys that are turned on the way, and the batch's queries turned with
+ * them (n_heads 0: none): d_q and d_out [n_tokens][n_heads][head_dim] of the keys'
+ * dtype, laid out as they are; d_out may be d_q, and overlaps nothing else.
+ * Positions are the cache's, or d_positions [n_tokens] (int32) where given; rotary
+ * NULL turns nothing (queries are copied).  Keys are quantised from fp32, without a
+ * rounding to dtype between.  Rows of tokens that no sequence has are left alone.  Only queues work. */
+CKR_API int ckr_kv_append(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const ckr_rotary* rotary,
+                          const int32_t* d_positions, const void* d_k, int64_t k_token_stride, int64_t k_head_stride,
+                          const void* d_v, int64_t v_token_stride, int64_t v_head_stride, const void* d_q,
+                          int64_t q_token_stride, int64_t q_head_stride, uint32_t n_heads, void* d_out,
+                          int64_t out_token_stride, int64_t out_head_stride, int dtype, void* stream);
 
 /* Attention of the batch's tokens over the cache, which already holds them
  * (ckr_kv_write): token at position p of sequence s attends to the positions j
