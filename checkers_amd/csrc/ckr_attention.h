@@ -229,6 +229,7 @@ template <typename E> __device__ __forceinline__ u32x4 ones(uint32_t seen) {
 
 constexpr uint32_t kFewRows = 16, kManyRows = 128, kWideRows = 256;  // rows of a tile
 constexpr uint32_t kFewWaves = 4;                                    // waves of a block of few rows
+constexpr int kFourTiles = 2, kFourWaves = 2;                         // four bits: tiles on their way a wave, waves a SIMD
 
 // f(0) .. f(N - 1) with constants.
 template <typename F, int... I> __device__ __forceinline__ void unroll_list(F f, std::integer_sequence<int, I...>) {
@@ -444,12 +445,273 @@ __device__ __forceinline__ FewSpan few_span(const AttnArg& a, int64_t start, uin
 __device__ __forceinline__ uint32_t few_tiles(const FewSpan& f) {  // one at least: a row without keys is written too
     return f.limit > f.first + 32 ? (uint32_t)((f.limit - f.first + 31) / 32) : 1u;
 }
+// Four bits: a wave's share of an item, n_tiles tiles of 32 keys from lo on.  The same products as
+// below, with K's operand made of the 16 bytes (32 dimensions, one group) that a lane holds of a key,
+// V's of the 4 (8 dimensions) that it holds of each of 8 keys: widened by their groups' powers,
+// which the conversions take as they come.  Strides are in 16 bytes and fit 32 bits (the launch
+// has seen to it), so what a tile's page adds to an address is made in scalar registers.
+template <typename X, int DP>
+__device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, uint32_t kvh, uint32_t token0, uint32_t row0, uint32_t rows,
+                                              const FewSpan& span, int64_t lo, int n_tiles, float& m, float& l, f32x4 (&o)[DP / 16]) {
+    typedef ElemBF16 P;
+    typedef FewRegs<ElemF4, DP> Regs;
+    constexpr int KL = Regs::KL, KW = Regs::KW, VD = Regs::VD, NV = DP / 16, KS = DP / 32, NB = DP > 128 ? 2 : kFourTiles;
+    constexpr bool TWICE = X::tag == CKR_F16;  // queries in two halves
+    const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    // keys are counted from lo, in 32 bits
+    const auto rel = [&](int64_t x) { return (int)max((int64_t)-0x40000000, min(x - lo, (int64_t)0x7fffffff - 256)); };
+    const uint32_t row = row0 + col;
+    const int64_t my_pos = span.pos_lo - row0 / a.group + min(row, rows - 1) / a.group;
+    const int pos = rel(my_pos), see = a.window ? rel(my_pos - (int64_t)a.window) : -0x40000000;
+    const int end = __builtin_amdgcn_readfirstlane(rel(span.limit));
+    const int full_to = __builtin_amdgcn_readfirstlane(min(rel(span.pos_lo) + 1, end));  // every row sees the keys before this
+    const int full_from = __builtin_amdgcn_readfirstlane(a.window ? rel(span.pos_hi - (int64_t)a.window) + 1 : -0x40000000);  // and from this on
+
+    // queries: the elements of each 32-wide step in the order of the keys' pieces
+    u32x4 q[KS], q_lo[TWICE ? KS : 1];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        const uint32_t d = DP > 64 ? (ks / 4) * 128 + g * 32 + (ks % 4) * 8 : g * 16 + ks * 8;
+        q[ks] = u32x4{0, 0, 0, 0};
+        if (row < rows && d < a.dim)
+            q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(token0 + row / a.group) * a.q_tok +
+                                                          (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
+    }
+    const uint8_t* const ck = a.ck + (int64_t)kvh * a.kst[1];
+    const uint8_t* const cv = a.cv + (int64_t)kvh * a.vst[1];
+    const uint8_t* const ckp = reinterpret_cast<const uint8_t*>(a.sk) + (int64_t)kvh * a.skst[1];
+    const uint8_t* const cvp = reinterpret_cast<const uint8_t*>(a.sv) + (int64_t)kvh * a.svst[1];
+    const uint32_t kst0 = (uint32_t)(a.kst[0] >> 4), kst2 = (uint32_t)(a.kst[2] >> 4), vst0 = (uint32_t)(a.vst[0] >> 4), vst2 = (uint32_t)(a.vst[2] >> 4);
+    const uint32_t skst0 = (uint32_t)(a.skst[0] >> 4), svst0 = (uint32_t)(a.svst[0] >> 4);
+    // the lane's places in the 16 keys that a page holds at least; past the head's size (where
+    // queries are zero and outputs go nowhere) its last ones again
+    const uint32_t k_piece = DP == 64 ? min(g, a.dim / 16 - 1) : min(g, a.dim / 32 - 1);
+    const uint32_t k_off = col * kst2 * 16 + k_piece * (DP == 64 ? 8 : 16), kp_off = ((DP == 64 ? k_piece / 2 : k_piece) << a.page_shift) + col;
+    const uint32_t k_next = DP > 128 ? (min(4 + g, a.dim / 32 - 1) - k_piece) * 16 : 0;  // from a key's first piece to its second
+    const uint32_t v_col = min(col, a.dim / NV - 1);
+    const uint32_t vp_off = (v_col * NV / kGroup << a.page_shift) + 4 * g;
+    uint32_t v_off[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v_off[i] = (4 * g + i) * vst2 * 16 + v_col * (NV / 2);
+    typedef __attribute__((address_space(1))) const int32_t* global_i32;
+    const global_i32 table = (global_i32)(a.b.table + (int64_t)seq * a.b.table_stride);
+    const uint32_t slot_mask = (1u << a.page_shift) - 1, in0 = (uint32_t)lo & slot_mask, last_col = a.b.width - 1;
+    // table columns c0 + c_now .. + 63 in a register of the wave
+    const uint32_t c0 = (uint32_t)(lo >> a.page_shift);
+    const auto page_lane = [&](uint32_t c) {
+        c += lane;
+        const int32_t x = table[min(c, last_col)];
+        return c <= last_col && (uint32_t)x < a.n_pages ? x : -1;
+    };
+    uint32_t c_now = 0;
+    int32_t window = page_lane(c0);
+    const auto page_at = [&](int j) {  // of key j; called with j rising by 16
+        const uint32_t c = (in0 + (uint32_t)j) >> a.page_shift;
+        if (c - c_now >= 64) {
+            c_now = c;
+            window = page_lane(c0 + c_now);
+        }
+        return (int32_t)__builtin_amdgcn_readlane(window, (int)(c - c_now));
+    };
+    struct Pages { int32_t p[2]; };
+    const auto pages_at = [&](int base) {
+        Pages x;
+        x.p[0] = page_at(base);
+        x.p[1] = a.page_shift > 4 ? x.p[0] : page_at(base + 16);
+        return x;
+    };
+    // Every load is made for every tile, a few tiles behind the last too, so that the waits between
+    // can count: what is not mapped is read from page 0, and what no row sees is masked.
+    const auto load_k = [&](Regs& r, int base, const Pages& pages) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask, p = (uint32_t)max(pages.p[h], 0);
+            const uint8_t* const k = ck + ((uint64_t)p * kst0 + slot * kst2) * 16;
+            const uint8_t* const kp = ckp + ((uint64_t)p * skst0 * 16 + slot);
+#pragma unroll
+            for (int j = 0; j < KL; j++) {
+                if constexpr (DP == 64) {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(k + k_off);
+                    r.k[h][j][0] = x[0], r.k[h][j][1] = x[1];
+                } else {
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(k + (k_off + j * k_next));
+#pragma unroll
+                    for (int w = 0; w < 4; w++) r.k[h][j][w] = x[w];
+                }
+                r.kp[h][j] = kp[kp_off + (j * (k_next / 16) << a.page_shift)];
+            }
+        }
+    };
+    const auto load_v = [&](Regs& r, int base, const Pages& pages) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask, p = (uint32_t)max(pages.p[h], 0);
+            const uint8_t* const v = cv + ((uint64_t)p * vst0 + slot * vst2) * 16;
+            const uint8_t* const vp = cvp + ((uint64_t)p * svst0 * 16 + slot);
+            r.vp[h] = *reinterpret_cast<const uint32_t*>(vp + vp_off);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (DP == 64) {
+                    r.v[4 * h + i][0] = *reinterpret_cast<const uint16_t*>(v + v_off[i]);
+                } else if constexpr (VD == 1) {
+                    r.v[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(v + v_off[i]);
+                } else {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(v + v_off[i]);
+                    r.v[4 * h + i][0] = x[0], r.v[4 * h + i][VD - 1] = x[1];
+                }
+            }
+        }
+    };
+    const auto scores = [&](const Regs& r, f32x4 (&s)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KL; j++)
+#pragma unroll
+                for (int w = 0; w < KW; w++) {
+                    const u32x4 x = widen8<ElemBF16>(r.k[h][j][w], power_of(r.kp[h][j]));
+                    s[h] = mfma16<ElemBF16>(x, q[j * KW + w], s[h]);
+                    if constexpr (TWICE) s[h] = mfma16<ElemBF16>(x, q_lo[j * KW + w], s[h]);
+                }
+        }
+    };
+    // the weights of a tile; seen: the keys that the lane's row sees, kept: those that are keys at all
+    const auto weights = [&](f32x4 (&s)[2], int base, const Pages& pages, uint32_t& seen, uint32_t& kept) {
+        const bool full = (pages.p[0] | pages.p[1]) >= 0 && base + 32 <= full_to && base >= full_from;
+        seen = kept = 255u;
+        if (!full) {
+            seen = kept = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int j = base + 16 * (i / 4) + 4 * (int)g + i % 4;
+                const bool key = pages.p[i / 4] >= 0 && j < end, in = key && j <= pos && j > see;
+                kept |= key ? 1u << i : 0u, seen |= in ? 1u << i : 0u;
+                s[i / 4][i % 4] = in ? s[i / 4][i % 4] : -INFINITY;
+            }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) top = fmaxf(top, s[i / 4][i % 4]);
+        top *= a.scale2;
+        if (__any(top > m + kLag)) {
+            top = max_quarters(top);
+            const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
+            m = m2;
+            l *= back;
+#pragma unroll
+            for (int c = 0; c < NV; c++) o[c] *= back;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        Halves<P> p;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const float x = exp2_fast(__builtin_fmaf(s[i / 4][i % 4], a.scale2, -ref)), y = exp2_fast(__builtin_fmaf(s[i / 4][i % 4 + 1], a.scale2, -ref));
+            l += x, l += y;
+            p.add(i / 2, x, y);
+        }
+        return p;
+    };
+    // values of NaN are looked for where a sum came out as NaN, in a second go
+    bool careful = false;
+    const auto gather = [&](const Regs& r, const Halves<P>& p, uint32_t seen, uint32_t kept) {
+        uint32_t vp[2] = {r.vp[0], r.vp[1]};
+        if (careful || kept != 255u) {
+            // what is no key may hold a power of NaN; one of a key makes the rows that see it NaN, and is 0 here
+            uint32_t nan = 0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const bool bad = (vp[k / 4] >> (8 * (k % 4)) & 255u) == 255u;
+                nan |= careful && bad ? 1u << k : 0u;
+                if (!(kept >> k & 1) || (careful && bad)) vp[k / 4] &= ~(255u << (8 * (k % 4)));
+            }
+            if (careful) {
+                const f32x4 hit = mfma16<P>(ones<P>(nan & kept), ones<P>(seen), f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int c = 0; c < NV; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[c][i] += hit[i] > 0.f ? as_f32(0x7fc00000u) : 0.f;
+            }
+        }
+        float power[8];  // the conversions look at a float's exponent only
+#pragma unroll
+        for (int k = 0; k < 8; k++) power[k] = as_f32(k % 4 == 3 ? vp[k / 4] >> 1 : vp[k / 4] << (23 - 8 * (k % 4)));
+        unroll<VD>([&](auto j_tag) {
+            unroll<std::min(NV / 2, 4)>([&](auto b_tag) {  // two dimensions of eight keys
+                constexpr int j = decltype(j_tag)::value, b = decltype(b_tag)::value;
+                uint32_t x[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    x[k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(r.v[k][j], power[k], b));
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    u32x4 w;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], c ? 0x07060302u : 0x05040100u);
+                    f32x4& to = o[8 * j + 2 * b + c];
+                    to = mfma16<P>(w, p.lo, mfma16<P>(w, p.hi, to));
+                }
+            });
+        });
+    };
+
+    if (n_tiles <= 0) return;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        q[ks] ^= a.flip;
+        if constexpr (TWICE) {
+            Halves<ElemBF16> x;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x.add(i, lo16<X>(q[ks][i]), hi16<X>(q[ks][i]));
+            q[ks] = x.hi, q_lo[ks] = x.lo;
+        }
+    }
+    for (;;) {
+        Regs r[NB];
+        Pages pages[NB];
+#pragma unroll
+        for (int u = 0; u < NB; u++) {
+            pages[u] = pages_at(32 * u);
+            load_k(r[u], 32 * u, pages[u]);
+            load_v(r[u], 32 * u, pages[u]);
+        }
+        for (int i = 0; i < n_tiles; i += NB) {
+#pragma unroll
+            for (int u = 0; u < NB; u++) {
+                if (i + u >= n_tiles) break;
+                const int base = 32 * (i + u);
+                f32x4 s[2];
+                scores(r[u], s);
+                const Pages coming = pages_at(base + 32 * NB);
+                load_k(r[u], base + 32 * NB, coming);
+                uint32_t seen, kept;
+                const Halves<P> p = weights(s, base, pages[u], seen, kept);
+                gather(r[u], p, seen, kept);
+                load_v(r[u], base + 32 * NB, coming);
+                pages[u] = coming;
+            }
+        }
+        bool nan = false;
+#pragma unroll
+        for (int c = 0; c < NV; c++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) nan |= o[c][k] != o[c][k];
+        if (careful || !__any(nan)) break;
+        careful = true, m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int c = 0; c < NV; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        window = page_lane(c0), c_now = 0;
+    }
+}
+// Waves of a SIMD that a block's registers leave room for.
+template <typename C> constexpr int few_waves(int dp) { return dp > 128 ? 1 : C::tag == CKR_F4 ? kFourWaves : 2; }
+
 template <typename X, typename C, int DP>
-__global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few_kernel(AttnArg a) {
+__global__ void __launch_bounds__(64 * kFewWaves, few_waves<C>(DP)) attend_few_kernel(AttnArg arg) {
+    const AttnArg& a = arg;
     typedef typename Prob<X, C>::E P;
-    typedef FewRegs<C, DP> Regs;
+    typedef std::conditional_t<C::tag == CKR_F4, FewRegs<ElemF8, DP>, FewRegs<C, DP>> Regs;
     constexpr int KL = Regs::KL, VD = Regs::VD, NV = DP / 16, KS = DP / 32;
-    constexpr bool FOUR = C::tag == CKR_F4, TWICE = FOUR && X::tag == CKR_F16;  // TWICE: queries in two halves
     constexpr uint32_t THREADS = 64 * kFewWaves, QUADS = DP / 4;  // a row's outputs by fours
     __shared__ __attribute__((aligned(16))) float s_o[kFewWaves][kFewRows][DP + 4];
     __shared__ float s_m[kFewWaves][kFewRows][2];
@@ -534,354 +796,285 @@ __global__ void __launch_bounds__(64 * kFewWaves, (DP > 128 ? 1 : 2)) attend_few
     uint32_t kvh = scalar(in_seq / nt), t0 = scalar(in_seq % nt);
 
     for (uint32_t p = p_begin; p < p_end;) {
+        const AttnArg& a = C::tag == CKR_F4 ? args_here() : arg;
         const uint32_t t1 = scalar(min(nt, t0 + (p_end - p)));
         // the waves share the item's tiles (or this block's part of them) evenly
         const uint32_t w0 = (uint32_t)((uint64_t)(t1 - t0) * wave / kFewWaves), w1 = (uint32_t)((uint64_t)(t1 - t0) * (wave + 1) / kFewWaves);
         const int64_t lo = span.first + 32ll * (t0 + w0);
         const int n_tiles = w1 - w0;
-        // from here on keys are counted from lo, in 32 bits
-        const auto rel = [&](int64_t x) { return (int)max((int64_t)-0x40000000, min(x - lo, (int64_t)0x7fffffff - 256)); };
-        const uint32_t row = row0 + col;
-        const int64_t my_pos = span.pos_lo - row0 / a.group + min(row, rows - 1) / a.group;
-        const int pos = rel(my_pos), see = a.window ? rel(my_pos - (int64_t)a.window) : -0x40000000;
-        const int end = __builtin_amdgcn_readfirstlane(rel(span.limit));
-        const int full_to = __builtin_amdgcn_readfirstlane(min(rel(span.pos_lo) + 1, end));  // every row sees the keys before this
-        const int full_from = __builtin_amdgcn_readfirstlane(a.window ? rel(span.pos_hi - (int64_t)a.window) + 1 : -0x40000000);  // and from this on
-
-        // queries: the elements of each 32-wide step in the order of the keys' pieces
-        u32x4 q[KS], q_lo[TWICE ? KS : 1];
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const uint32_t d = FOUR && DP > 64      ? (ks / 4) * 128 + g * 32 + (ks % 4) * 8
-                               : FOUR || C::bytes == 1 ? (ks / 2) * 64 + g * 16 + (ks % 2) * 8
-                                                       : ks * 32 + g * 8;
-            q[ks] = u32x4{0, 0, 0, 0};
-            if (row < rows && d < a.dim)
-                q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(token0 + row / a.group) * a.q_tok +
-                                                              (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
-        }
-        const uint8_t* const ck = a.ck + (int64_t)kvh * a.kst[1];
-        const uint8_t* const cv = a.cv + (int64_t)kvh * a.vst[1];
-        const float* const skp = a.sk + (int64_t)kvh * a.skst[1];
-        const float* const svp = a.sv + (int64_t)kvh * a.svst[1];
-        const int64_t k_off = (int64_t)col * a.kst[2] + g * (FOUR && DP == 64 ? 8 : 16);
-        // four bits: the bytes of this lane's groups
-        const uint8_t* const kp4 = reinterpret_cast<const uint8_t*>(a.sk) + (int64_t)kvh * a.skst[1] + ((DP == 64 ? g / 2 : g) << a.page_shift) + col;
-        const uint8_t* const vp4 = reinterpret_cast<const uint8_t*>(a.sv) + (int64_t)kvh * a.svst[1] + (min(col * NV, a.dim - 1) / kGroup << a.page_shift) + 4 * g;
-        // one offset and three sums a load, for 16-bit caches have no registers for four (390 us
-        // a step of 64 sequences to 16000 with them, 342 without; e4m3 177 and 176); four where
-        // values are widened by their scale's power (183 us, 196 with one)
-        constexpr int OFFS = Prob<X, C>::split ? 4 : 1;
-        int64_t v_off[OFFS];
-#pragma unroll
-        for (int i = 0; i < OFFS; i++) v_off[i] = (int64_t)(4 * g + i) * a.vst[2] + col * bytes_of<C>(NV);
-        const auto v_row = [&](int i) { return OFFS == 4 ? v_off[i % OFFS] : i * a.vst[2] + v_off[0]; };
-        const bool v_in = col * NV < a.dim;
-        typedef __attribute__((address_space(1))) const int32_t* global_i32;
-        const global_i32 table = (global_i32)(a.b.table + (int64_t)seq * a.b.table_stride);
-        const uint32_t slot_mask = (1u << a.page_shift) - 1, in0 = (uint32_t)lo & slot_mask;
-        // table columns c0 .. c0 + 63 in a register of the wave, the next 64 on their way
-        uint32_t c0 = (uint32_t)(lo >> a.page_shift);
-        const auto page_lane = [&](uint32_t c) {
-            c += lane;
-            const int32_t x = c < a.b.width ? table[c] : -1;
-            return (uint32_t)x < a.n_pages ? x : -1;
-        };
-        int32_t window_now = page_lane(c0), window_next = page_lane(c0 + 64);
-        uint32_t c_now = 0;
-        const auto page_at = [&](int j) {  // of key j; called with j rising by 16
-            const uint32_t c = (in0 + (uint32_t)j) >> a.page_shift;
-            if (c - c_now >= 64) {
-                c_now += 64;
-                window_now = window_next;
-                window_next = page_lane(c0 + c_now + 64);
-            }
-            return (int32_t)__builtin_amdgcn_readlane(window_now, (int)(c - c_now));
-        };
-        const auto load_k = [&](Regs& r, int base, const int32_t* pages) {
-            const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
-                const uint8_t* at = ck + (int64_t)pages[h] * a.kst[0] + (int64_t)slot * a.kst[2] + k_off;
-                if constexpr (FOUR) {
-                    const uint8_t* from = kp4 + (int64_t)pages[h] * a.skst[0] + slot;
-#pragma unroll
-                    for (int j = 0; j < KL; j++) {
-                        const bool in = whole || (pages[h] >= 0 && base + 16 * h + (int)col < end && (DP == 64 ? g * 16 : j * 128 + g * 32) < a.dim);
-#pragma unroll
-                        for (int w = 0; w < Regs::KW; w++) r.k[h][j][w] = 0;
-                        r.kp[h][j] = 0;
-                        if (in) {
-                            if constexpr (DP == 64) {
-                                const u32x2 x = *reinterpret_cast<const u32x2*>(at);
-                                r.k[h][j][0] = x[0], r.k[h][j][1] = x[1];
-                            } else {
-                                const u32x4 x = *reinterpret_cast<const u32x4*>(at + j * 64);
-#pragma unroll
-                                for (int w = 0; w < 4; w++) r.k[h][j][w] = x[w];
-                            }
-                            r.kp[h][j] = from[(int64_t)(4 * j) << a.page_shift];
-                        }
-                    }
-                } else if (whole) {
-#pragma unroll
-                    for (int j = 0; j < KL; j++) r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < KL; j++) {
-                        r.k[h][j] = u32x4{0, 0, 0, 0};
-                        if (pages[h] >= 0 && base + 16 * h + (int)col < end && (j * 64 + g * 16) / std::max(C::bytes, 1) < a.dim)
-                            r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
-                    }
-                }
-                if constexpr (C::bytes == 1) r.sk[h] = *reinterpret_cast<const f32x4*>(skp + (int64_t)max(pages[h], 0) * a.skst[0] + slot + 4 * g);
-            }
-        };
-        const auto load_v = [&](Regs& r, int base, const int32_t* pages) {
-            const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
-            const auto get = [&](uint32_t (&v)[VD], const uint8_t* at) {
-                if constexpr (FOUR && DP == 64) v[0] = *reinterpret_cast<const uint16_t*>(at);
-                else if constexpr (VD == 1) v[0] = *reinterpret_cast<const uint32_t*>(at);
-                else if constexpr (VD == 2) {
-                    const u32x2 y = *reinterpret_cast<const u32x2*>(at);
-                    v[0] = y[0], v[1] = y[1];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VD; j += 4) {
-                        const u32x4 y = *reinterpret_cast<const u32x4*>(at + j * 4);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) v[j + k] = y[k];
-                    }
-                }
-            };
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
-                const uint8_t* at = cv + (int64_t)pages[h] * a.vst[0] + (int64_t)slot * a.vst[2];
-                if constexpr (FOUR) {
-                    r.vp[h] = 0;
-                    if (pages[h] >= 0) r.vp[h] = *reinterpret_cast<const uint32_t*>(vp4 + (int64_t)pages[h] * a.svst[0] + slot);
-                }
-                if constexpr (C::bytes == 1) r.sv[h] = *reinterpret_cast<const f32x4*>(svp + (int64_t)max(pages[h], 0) * a.svst[0] + slot + 4 * g);
-                if (whole) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) get(r.v[4 * h + i], at + v_row(i));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-#pragma unroll
-                        for (int j = 0; j < VD; j++) r.v[4 * h + i][j] = 0;
-                        if (pages[h] >= 0 && base + 16 * h + 4 * (int)g + i < end && v_in) get(r.v[4 * h + i], at + v_row(i));
-                    }
-                }
-            }
-        };
-
         float m = -INFINITY, l = 0.f;
         f32x4 o[NV];
 #pragma unroll
         for (int c = 0; c < NV; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const auto scores = [&](const Regs& r, f32x4 (&s)[2]) {
+        if constexpr (C::tag == CKR_F4) {
+            few_item_four<X, DP>(a, seq, kvh, token0, row0, rows, span, lo, n_tiles, m, l, o);
+        } else {
+            // from here on keys are counted from lo, in 32 bits
+            const auto rel = [&](int64_t x) { return (int)max((int64_t)-0x40000000, min(x - lo, (int64_t)0x7fffffff - 256)); };
+            const uint32_t row = row0 + col;
+            const int64_t my_pos = span.pos_lo - row0 / a.group + min(row, rows - 1) / a.group;
+            const int pos = rel(my_pos), see = a.window ? rel(my_pos - (int64_t)a.window) : -0x40000000;
+            const int end = __builtin_amdgcn_readfirstlane(rel(span.limit));
+            const int full_to = __builtin_amdgcn_readfirstlane(min(rel(span.pos_lo) + 1, end));  // every row sees the keys before this
+            const int full_from = __builtin_amdgcn_readfirstlane(a.window ? rel(span.pos_hi - (int64_t)a.window) + 1 : -0x40000000);  // and from this on
+
+            // queries: the elements of each 32-wide step in the order of the keys' pieces
+            u32x4 q[KS];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int ks = 0; ks < KS; ks++) {
+                const uint32_t d = C::bytes == 1 ? (ks / 2) * 64 + g * 16 + (ks % 2) * 8 : ks * 32 + g * 8;
+                q[ks] = u32x4{0, 0, 0, 0};
+                if (row < rows && d < a.dim)
+                    q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(token0 + row / a.group) * a.q_tok +
+                                                                  (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
+            }
+            const uint8_t* const ck = a.ck + (int64_t)kvh * a.kst[1];
+            const uint8_t* const cv = a.cv + (int64_t)kvh * a.vst[1];
+            const float* const skp = a.sk + (int64_t)kvh * a.skst[1];
+            const float* const svp = a.sv + (int64_t)kvh * a.svst[1];
+            const int64_t k_off = (int64_t)col * a.kst[2] + g * 16;
+            // one offset and three sums a load, for 16-bit caches have no registers for four (390 us
+            // a step of 64 sequences to 16000 with them, 342 without; e4m3 177 and 176); four where
+            // values are widened by their scale's power (183 us, 196 with one)
+            constexpr int OFFS = Prob<X, C>::split ? 4 : 1;
+            int64_t v_off[OFFS];
 #pragma unroll
-                for (int j = 0; j < KL; j++) {
-                    if constexpr (FOUR) {
-                        const float power = power_of(r.kp[h][j]);
+            for (int i = 0; i < OFFS; i++) v_off[i] = (int64_t)(4 * g + i) * a.vst[2] + col * (VD * 4);
+            const auto v_row = [&](int i) { return OFFS == 4 ? v_off[i % OFFS] : i * a.vst[2] + v_off[0]; };
+            const bool v_in = col * NV < a.dim;
+            typedef __attribute__((address_space(1))) const int32_t* global_i32;
+            const global_i32 table = (global_i32)(a.b.table + (int64_t)seq * a.b.table_stride);
+            const uint32_t slot_mask = (1u << a.page_shift) - 1, in0 = (uint32_t)lo & slot_mask;
+            // table columns c0 .. c0 + 63 in a register of the wave, the next 64 on their way
+            uint32_t c0 = (uint32_t)(lo >> a.page_shift);
+            const auto page_lane = [&](uint32_t c) {
+                c += lane;
+                const int32_t x = c < a.b.width ? table[c] : -1;
+                return (uint32_t)x < a.n_pages ? x : -1;
+            };
+            int32_t window_now = page_lane(c0), window_next = page_lane(c0 + 64);
+            uint32_t c_now = 0;
+            const auto page_at = [&](int j) {  // of key j; called with j rising by 16
+                const uint32_t c = (in0 + (uint32_t)j) >> a.page_shift;
+                if (c - c_now >= 64) {
+                    c_now += 64;
+                    window_now = window_next;
+                    window_next = page_lane(c0 + c_now + 64);
+                }
+                return (int32_t)__builtin_amdgcn_readlane(window_now, (int)(c - c_now));
+            };
+            const auto load_k = [&](Regs& r, int base, const int32_t* pages) {
+                const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
 #pragma unroll
-                        for (int w = 0; w < Regs::KW; w++) {
-                            const u32x4 x = widen8<ElemBF16>(r.k[h][j][w], power);
-                            s[h] = mfma16<ElemBF16>(x, q[j * Regs::KW + w], s[h]);
-                            if constexpr (TWICE) s[h] = mfma16<ElemBF16>(x, q_lo[j * Regs::KW + w], s[h]);
-                        }
-                    } else if constexpr (C::bytes == 1) {
-                        const u32x4 x = r.k[h][j];
-                        const u32x2 w0 = widen4<C, X>(x[0]), w1 = widen4<C, X>(x[1]), w2 = widen4<C, X>(x[2]), w3 = widen4<C, X>(x[3]);
-                        s[h] = mfma16<X>(u32x4{w0[0], w0[1], w1[0], w1[1]}, q[2 * j], s[h]);
-                        s[h] = mfma16<X>(u32x4{w2[0], w2[1], w3[0], w3[1]}, q[2 * j + 1], s[h]);
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
+                    const uint8_t* at = ck + (int64_t)pages[h] * a.kst[0] + (int64_t)slot * a.kst[2] + k_off;
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < KL; j++) r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
                     } else {
-                        s[h] = mfma16<X>(r.k[h][j], q[j], s[h]);
+#pragma unroll
+                        for (int j = 0; j < KL; j++) {
+                            r.k[h][j] = u32x4{0, 0, 0, 0};
+                            if (pages[h] >= 0 && base + 16 * h + (int)col < end && (j * 64 + g * 16) / C::bytes < a.dim)
+                                r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
+                        }
+                    }
+                    if constexpr (C::bytes == 1) r.sk[h] = *reinterpret_cast<const f32x4*>(skp + (int64_t)max(pages[h], 0) * a.skst[0] + slot + 4 * g);
+                }
+            };
+            const auto load_v = [&](Regs& r, int base, const int32_t* pages) {
+                const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
+                const auto get = [&](uint32_t (&v)[VD], const uint8_t* at) {
+                    if constexpr (VD == 1) v[0] = *reinterpret_cast<const uint32_t*>(at);
+                    else if constexpr (VD == 2) {
+                        const u32x2 y = *reinterpret_cast<const u32x2*>(at);
+                        v[0] = y[0], v[1] = y[1];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < VD; j += 4) {
+                            const u32x4 y = *reinterpret_cast<const u32x4*>(at + j * 4);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) v[j + k] = y[k];
+                        }
+                    }
+                };
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
+                    const uint8_t* at = cv + (int64_t)pages[h] * a.vst[0] + (int64_t)slot * a.vst[2];
+                    if constexpr (C::bytes == 1) r.sv[h] = *reinterpret_cast<const f32x4*>(svp + (int64_t)max(pages[h], 0) * a.svst[0] + slot + 4 * g);
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) get(r.v[4 * h + i], at + v_row(i));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+#pragma unroll
+                            for (int j = 0; j < VD; j++) r.v[4 * h + i][j] = 0;
+                            if (pages[h] >= 0 && base + 16 * h + 4 * (int)g + i < end && v_in) get(r.v[4 * h + i], at + v_row(i));
+                        }
                     }
                 }
-            }
-        };
-        // the weights of a tile, with the values' scales; what a row does not see weighs 0
-        const auto weights = [&](const Regs& r, const f32x4 (&s)[2], int base, const int32_t* pages, uint32_t& seen) {
-            const bool full = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= full_to && base >= full_from;
-            float x[8], top = -INFINITY;
-            seen = ~0u;  // every row sees every key
+            };
+
+            const auto scores = [&](const Regs& r, f32x4 (&s)[2]) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                x[i] = s[i / 4][i % 4] * a.scale2;
-                if constexpr (C::bytes == 1) x[i] *= r.sk[i / 4][i % 4];
-            }
-            if (!full) {
-                seen = 0;
+                for (int h = 0; h < 2; h++) {
+                    s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < KL; j++) {
+                        if constexpr (C::bytes == 1) {
+                            const u32x4 x = r.k[h][j];
+                            const u32x2 w0 = widen4<C, X>(x[0]), w1 = widen4<C, X>(x[1]), w2 = widen4<C, X>(x[2]), w3 = widen4<C, X>(x[3]);
+                            s[h] = mfma16<X>(u32x4{w0[0], w0[1], w1[0], w1[1]}, q[2 * j], s[h]);
+                            s[h] = mfma16<X>(u32x4{w2[0], w2[1], w3[0], w3[1]}, q[2 * j + 1], s[h]);
+                        } else {
+                            s[h] = mfma16<X>(r.k[h][j], q[j], s[h]);
+                        }
+                    }
+                }
+            };
+            // the weights of a tile, with the values' scales; what a row does not see weighs 0
+            const auto weights = [&](const Regs& r, const f32x4 (&s)[2], int base, const int32_t* pages, uint32_t& seen) {
+                const bool full = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= full_to && base >= full_from;
+                float x[8], top = -INFINITY;
+                seen = ~0u;  // every row sees every key
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const int j = base + 16 * (i / 4) + 4 * (int)g + i % 4;
-                    if (pages[i / 4] >= 0 && j <= pos && j > see && j < end) seen |= 1u << i;
-                    x[i] = seen >> i & 1 ? x[i] : -INFINITY;
+                    x[i] = s[i / 4][i % 4] * a.scale2;
+                    if constexpr (C::bytes == 1) x[i] *= r.sk[i / 4][i % 4];
                 }
-            }
+                if (!full) {
+                    seen = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, x[i]);
-            if (__any(top > m + kLag)) {
-                top = max_quarters(top);
-                const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
-                m = m2;
-                l *= back;
-#pragma unroll
-                for (int c = 0; c < NV; c++) o[c] *= back;
-            }
-            const float ref = m == -INFINITY ? 0.f : m - Prob<X, C>::up;
-            float w[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                w[i] = exp2_fast(x[i] - ref);
-                l += w[i];
-                if constexpr (Prob<X, C>::split) w[i] *= split_scale<C>(r.sv[i / 4][i % 4]).rest;
-                else if constexpr (C::bytes == 1) w[i] *= r.sv[i / 4][i % 4];
-            }
-            if (C::bytes == 1 && !full) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = seen >> i & 1 ? w[i] : 0.f;  // a scale may be NaN there
-            }
-            Halves<P> p;
-#pragma unroll
-            for (int i = 0; i < 4; i++) p.add(i, w[2 * i], w[2 * i + 1]);
-            return p;
-        };
-        const auto gather = [&](const Regs& r, const Halves<P>& p, uint32_t seen) {
-            if constexpr (FOUR) {
-                uint32_t vp[2] = {r.vp[0], r.vp[1]};
-                // a group of NaN: values of zero here, and NaN for the rows that see one
-                const auto nan_byte = [](uint32_t x) { return x & ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
-                if (__any(nan_byte(vp[0]) | nan_byte(vp[1]))) {
-                    uint32_t nan = 0;
-#pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        if ((vp[k / 4] >> (8 * (k % 4)) & 255u) == 255u) nan |= 1u << k, vp[k / 4] &= ~(255u << (8 * (k % 4)));
-                    const f32x4 hit = mfma16<P>(ones<P>(nan), ones<P>(seen), f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                    for (int c = 0; c < NV; c++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) o[c][i] += hit[i] > 0.f ? as_f32(0x7fc00000u) : 0.f;
-                }
-#pragma unroll
-                for (int j = 0; j < VD; j++) {  // eight dimensions of eight keys (of 64 in all: four)
-                    u32x4 x[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] = widen8<P>(r.v[k][j], power_of(vp[k / 4] >> (8 * (k % 4)) & 255u));
-#pragma unroll
-                    for (int k = 0; k < std::min(NV, 8); k++) {
-                        u32x4 w;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(x[2 * e + 1][k / 2], x[2 * e][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
-                        o[8 * j + k] = mfma16<P>(w, p.lo, mfma16<P>(w, p.hi, o[8 * j + k]));
+                    for (int i = 0; i < 8; i++) {
+                        const int j = base + 16 * (i / 4) + 4 * (int)g + i % 4;
+                        if (pages[i / 4] >= 0 && j <= pos && j > see && j < end) seen |= 1u << i;
+                        x[i] = seen >> i & 1 ? x[i] : -INFINITY;
                     }
                 }
-            } else if constexpr (Prob<X, C>::split) {
 #pragma unroll
-                for (int j = 0; j < VD; j++) {  // four dimensions of eight keys, widened first: each key has its power
-                    u32x2 x[8];
+                for (int i = 0; i < 8; i++) top = fmaxf(top, x[i]);
+                if (__any(top > m + kLag)) {
+                    top = max_quarters(top);
+                    const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
+                    m = m2;
+                    l *= back;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] = widen4_by<C>(r.v[k][j], split_scale<C>(r.sv[k / 4][k % 4]).power);
+                    for (int c = 0; c < NV; c++) o[c] *= back;
+                }
+                const float ref = m == -INFINITY ? 0.f : m - Prob<X, C>::up;
+                float w[8];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        u32x4 w;
+                for (int i = 0; i < 8; i++) {
+                    w[i] = exp2_fast(x[i] - ref);
+                    l += w[i];
+                    if constexpr (Prob<X, C>::split) w[i] *= split_scale<C>(r.sv[i / 4][i % 4]).rest;
+                    else if constexpr (C::bytes == 1) w[i] *= r.sv[i / 4][i % 4];
+                }
+                if (C::bytes == 1 && !full) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(x[2 * e + 1][k / 2], x[2 * e][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
-                        o[4 * j + k] = mfma16<P>(w, p.lo, mfma16<P>(w, p.hi, o[4 * j + k]));
+                    for (int i = 0; i < 8; i++) w[i] = seen >> i & 1 ? w[i] : 0.f;  // a scale may be NaN there
+                }
+                Halves<P> p;
+#pragma unroll
+                for (int i = 0; i < 4; i++) p.add(i, w[2 * i], w[2 * i + 1]);
+                return p;
+            };
+            const auto gather = [&](const Regs& r, const Halves<P>& p, uint32_t seen) {
+                if constexpr (Prob<X, C>::split) {
+#pragma unroll
+                    for (int j = 0; j < VD; j++) {  // four dimensions of eight keys, widened first: each key has its power
+                        u32x2 x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) x[k] = widen4_by<C>(r.v[k][j], split_scale<C>(r.sv[k / 4][k % 4]).power);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            u32x4 w;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(x[2 * e + 1][k / 2], x[2 * e][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
+                            o[4 * j + k] = mfma16<P>(w, p.lo, mfma16<P>(w, p.hi, o[4 * j + k]));
+                        }
+                    }
+                } else if constexpr (C::bytes == 1) {
+#pragma unroll
+                    for (int j = 0; j < VD; j++) {  // four dimensions of eight keys
+                        uint32_t w[2][4];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t a0 = r.v[4 * h][j], a1 = r.v[4 * h + 1][j], a2 = r.v[4 * h + 2][j], a3 = r.v[4 * h + 3][j];
+                            const uint32_t x0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), x1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
+                            const uint32_t y0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), y1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+                            w[h][0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u);
+                            w[h][1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
+                            w[h][2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u);
+                            w[h][3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const u32x2 w0 = widen4<C, P>(w[0][k]), w1 = widen4<C, P>(w[1][k]);
+                            const u32x4 v = {w0[0], w0[1], w1[0], w1[1]};
+                            o[4 * j + k] = mfma16<P>(v, p.lo, mfma16<P>(v, p.hi, o[4 * j + k]));
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VD; j++) {  // two dimensions of eight keys
+                        u32x4 w0, w1;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
+                            w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
+                        }
+                        // a float16 weight may have become 0 though every row sees the key (see settle; here it
+                        // costs nothing to look: a step of 64 sequences to 16000, 344 us with and without)
+                        if (__any((P::tag == CKR_F16 || seen != ~0u) && (any_wild<P>(w0) || any_wild<P>(w1)))) {
+                            const u32x4 see = ones<P>(seen);
+                            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+                            const f32x4 p0 = mfma16<P>(wild<P>(w0, 1), see, zero), m0 = mfma16<P>(wild<P>(w0, -1), see, zero);
+                            const f32x4 p1 = mfma16<P>(wild<P>(w1, 1), see, zero), m1 = mfma16<P>(wild<P>(w1, -1), see, zero);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[2 * j][i] += wild_sum(p0[i], m0[i]), o[2 * j + 1][i] += wild_sum(p1[i], m1[i]);
+                            w0 = wild<P>(w0, 0), w1 = wild<P>(w1, 0);
+                        }
+                        o[2 * j] = mfma16<P>(w0, p.lo, mfma16<P>(w0, p.hi, o[2 * j]));
+                        o[2 * j + 1] = mfma16<P>(w1, p.lo, mfma16<P>(w1, p.hi, o[2 * j + 1]));
                     }
                 }
-            } else if constexpr (C::bytes == 1) {
-#pragma unroll
-                for (int j = 0; j < VD; j++) {  // four dimensions of eight keys
-                    uint32_t w[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t a0 = r.v[4 * h][j], a1 = r.v[4 * h + 1][j], a2 = r.v[4 * h + 2][j], a3 = r.v[4 * h + 3][j];
-                        const uint32_t x0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), x1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
-                        const uint32_t y0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), y1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
-                        w[h][0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u);
-                        w[h][1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
-                        w[h][2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u);
-                        w[h][3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const u32x2 w0 = widen4<C, P>(w[0][k]), w1 = widen4<C, P>(w[1][k]);
-                        const u32x4 v = {w0[0], w0[1], w1[0], w1[1]};
-                        o[4 * j + k] = mfma16<P>(v, p.lo, mfma16<P>(v, p.hi, o[4 * j + k]));
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < VD; j++) {  // two dimensions of eight keys
-                    u32x4 w0, w1;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
-                        w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
-                    }
-                    // a float16 weight may have become 0 though every row sees the key (see settle; here it
-                    // costs nothing to look: a step of 64 sequences to 16000, 344 us with and without)
-                    if (__any((P::tag == CKR_F16 || seen != ~0u) && (any_wild<P>(w0) || any_wild<P>(w1)))) {
-                        const u32x4 see = ones<P>(seen);
-                        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                        const f32x4 p0 = mfma16<P>(wild<P>(w0, 1), see, zero), m0 = mfma16<P>(wild<P>(w0, -1), see, zero);
-                        const f32x4 p1 = mfma16<P>(wild<P>(w1, 1), see, zero), m1 = mfma16<P>(wild<P>(w1, -1), see, zero);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) o[2 * j][i] += wild_sum(p0[i], m0[i]), o[2 * j + 1][i] += wild_sum(p1[i], m1[i]);
-                        w0 = wild<P>(w0, 0), w1 = wild<P>(w1, 0);
-                    }
-                    o[2 * j] = mfma16<P>(w0, p.lo, mfma16<P>(w0, p.hi, o[2 * j]));
-                    o[2 * j + 1] = mfma16<P>(w1, p.lo, mfma16<P>(w1, p.hi, o[2 * j + 1]));
-                }
-            }
-        };
+            };
 
-        Regs r[2];
-        int32_t pages[2][2], coming[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (u < n_tiles) {
-                pages[u][0] = page_at(32 * u), pages[u][1] = page_at(32 * u + 16);
-                load_k(r[u], 32 * u, pages[u]);
-                load_v(r[u], 32 * u, pages[u]);
-            }
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            q[ks] ^= a.flip;
-            if constexpr (TWICE) {
-                Halves<ElemBF16> x;
-#pragma unroll
-                for (int i = 0; i < 4; i++) x.add(i, lo16<X>(q[ks][i]), hi16<X>(q[ks][i]));
-                q[ks] = x.hi, q_lo[ks] = x.lo;
-            }
-        }
-        for (int i = 0; i < n_tiles; i += 2) {
+            Regs r[2];
+            int32_t pages[2][2], coming[2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                if (i + u >= n_tiles) break;
-                const int base = 32 * (i + u);
-                const bool more = i + u + 2 < n_tiles;
-                f32x4 s[2];
-                scores(r[u], s);
-                uint32_t seen;
-                const Halves<P> p = weights(r[u], s, base, pages[u], seen);
-                if (more) {  // its keys' registers again, for the tile after the next
-                    coming[0] = page_at(base + 64), coming[1] = page_at(base + 80);
-                    load_k(r[u], base + 64, coming);
+                if (u < n_tiles) {
+                    pages[u][0] = page_at(32 * u), pages[u][1] = page_at(32 * u + 16);
+                    load_k(r[u], 32 * u, pages[u]);
+                    load_v(r[u], 32 * u, pages[u]);
                 }
-                gather(r[u], p, seen);
-                if (more) {
-                    pages[u][0] = coming[0], pages[u][1] = coming[1];
-                    load_v(r[u], base + 64, pages[u]);
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) q[ks] ^= a.flip;
+            for (int i = 0; i < n_tiles; i += 2) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    if (i + u >= n_tiles) break;
+                    const int base = 32 * (i + u);
+                    const bool more = i + u + 2 < n_tiles;
+                    f32x4 s[2];
+                    scores(r[u], s);
+                    uint32_t seen;
+                    const Halves<P> p = weights(r[u], s, base, pages[u], seen);
+                    if (more) {  // its keys' registers again, for the tile after the next
+                        coming[0] = page_at(base + 64), coming[1] = page_at(base + 80);
+                        load_k(r[u], base + 64, coming);
+                    }
+                    gather(r[u], p, seen);
+                    if (more) {
+                        pages[u][0] = coming[0], pages[u][1] = coming[1];
+                        load_v(r[u], base + 64, pages[u]);
+                    }
                 }
             }
         }

@@ -22,6 +22,8 @@ constexpr uint64_t kSplitMin = 128;   // keys of a split at least
 // Blocks of the few rows' kernel: two a CU.  (For heads of 256 its registers leave room
 // for one, so there a full launch runs in two rounds.)
 constexpr uint32_t kFewBlocks = 512;
+constexpr uint32_t kFourBlocks = 512;  // over a cache of 4 bits
+uint32_t most_blocks(bool four) { return four ? kFourBlocks : kFewBlocks; }
 // Its tiles of 32 keys a block at least: one a wave (one token over a thousand: 9.5 us;
 // 11.0 with 8, 13.5 with 16).
 constexpr uint32_t kFewTiles = 4;
@@ -42,24 +44,24 @@ uint64_t most_tiles(uint32_t bm, uint64_t group, uint64_t n_seqs, uint64_t n_tok
 }
 // The workspace begins with the counters, whatever else a call keeps in it: they
 // are 0 between calls, the rest is not.
-constexpr uint64_t kCounterBytes = kFewBlocks * 4;
+constexpr uint64_t kCounterBytes = kFourBlocks * 4;
 void set_bytes(Cut& c, uint64_t rows) {
     c.part_m_bytes = (rows * 8 + 255) / 256 * 256;
     c.bytes = kCounterBytes + c.part_m_bytes + rows * c.dp * 4;
 }
-uint32_t few_blocks(uint64_t items, uint64_t max_context) {
-    return (uint32_t)std::min<uint64_t>(items * ((max_context + 31) / 32) / kFewTiles + 1, kFewBlocks);
+uint32_t few_blocks(uint64_t items, uint64_t max_context, bool four) {
+    return (uint32_t)std::min<uint64_t>(items * ((max_context + 31) / 32) / kFewTiles + 1, most_blocks(four));
 }
 // Rows of parts that a workspace holds (calls keep multiples of 32, which set_bytes rounds no further).
 uint64_t rows_held(uint64_t bytes, uint32_t dp) { return bytes < kCounterBytes ? 0 : (bytes - kCounterBytes) / (8 + dp * 4); }
 // workspace: its bytes; blocks and splits that it does not hold are left out, down to
 // one block of few rows and no split.
 Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t n_tokens, uint32_t max_chunk,
-        uint64_t max_context, uint64_t all_keys, uint32_t window, bool near_slots, uint64_t workspace) {
+        uint64_t max_context, uint64_t all_keys, uint32_t window, bool near_slots, bool four, uint64_t workspace) {
     Cut c{};
     const uint64_t group = n_heads / n_kv, rows = (uint64_t)max_chunk * group;
     c.dp = padded_dim(dim);
-    const bool few = rows <= kFewMost && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1) < (1ull << 31);
+    const bool few = rows <= kFewMost && (near_slots || !four) && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1) < (1ull << 31);
     c.bm = few ? kFewRows : rows <= kManyMost || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
     c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
     c.splits = 1;
@@ -68,7 +70,7 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     const uint64_t items = std::max<uint64_t>((uint64_t)c.tiles * n_kv, 1);
     if (c.bm == kFewRows) {
         c.min_tiles = kFewTiles;
-        c.blocks = (uint32_t)std::clamp<uint64_t>(rows_held(workspace, c.dp) / (2 * kFewRows), 1, few_blocks(items, max_context));
+        c.blocks = (uint32_t)std::clamp<uint64_t>(rows_held(workspace, c.dp) / (2 * kFewRows), 1, few_blocks(items, max_context, four));
         set_bytes(c, (uint64_t)c.blocks * 2 * kFewRows);
         return c;
     }
@@ -87,7 +89,7 @@ uint64_t most_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_se
     Cut c{};
     c.dp = padded_dim(dim);
     uint64_t items = std::max<uint64_t>(most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv, 1);
-    set_bytes(c, (uint64_t)few_blocks(items, max_context) * 2 * kFewRows);
+    set_bytes(c, (uint64_t)few_blocks(items, max_context, true) * 2 * kFewRows);
     uint64_t most = c.bytes;
     for (const uint32_t bm : {kManyRows, kWideRows}) {
         items = most_tiles(bm, group, n_seqs, n_tokens) * n_kv;
@@ -150,10 +152,12 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
            batch->n_seqs, batch->n_tokens};
     // the slots of a page within 32-bit offsets of each other, pages within 2^36 bytes
     bool near_slots = true;
+    const bool four = cache->dtype == CKR_F4;
     for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 26) - 16 && (cache->n_pages == 1 || st[0] < (1ll << 36));
+    for (const int64_t* st : {a.skst, a.svst}) near_slots = near_slots && (!four || cache->n_pages == 1 || st[0] < (1ll << 36));
     const Cut c = cut(n_heads, cache->n_heads, cache->head_dim, batch->n_seqs, batch->n_tokens, batch->max_chunk,
                       std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size),
-                      (uint64_t)batch->table_width * cache->page_size, window, near_slots, workspace_bytes);
+                      (uint64_t)batch->table_width * cache->page_size, window, near_slots, four, workspace_bytes);
     if ((uint64_t)c.tiles * cache->n_heads * 512 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
     a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len, a.min_tiles = c.min_tiles;
     if (c.bytes) {
@@ -167,7 +171,7 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
     }
     const hipStream_t s = (hipStream_t)stream;
     hipError_t e;
-    if (cache->dtype == CKR_F4)
+    if (four)
         e = attend_four(a, c, dtype, s);
     else if (dtype == CKR_BF16)
         e = cache->dtype == CKR_F8   ? launch_attend_dim<ElemBF16, ElemF8>(a, c, s)
