@@ -31,6 +31,7 @@ struct AttnArg {
     uint32_t tiles, splits, split_len;  // row tiles, key ranges of a tile, their length (a multiple of 128)
     uint32_t* counters;  // few rows: parts done of the item that begins in a block and goes on in the next; 0 between calls
     uint32_t min_tiles;  // few rows: tiles of a block's stretch at least
+    uint32_t item_pad;   // few rows, 4 bits: tiles that an item counts for besides its own
     // with splits > 1; few rows: [block][its first item's part, its last one's][row]
     float* part_o;  // [tile][kv head][split][rows of a tile][DP]
     float* part_m;  // [tile][kv head][split][rows of a tile][2]: maximum (in powers of two), sum
@@ -229,7 +230,7 @@ template <typename E> __device__ __forceinline__ u32x4 ones(uint32_t seen) {
 
 constexpr uint32_t kFewRows = 16, kManyRows = 128, kWideRows = 256;  // rows of a tile
 constexpr uint32_t kFewWaves = 4;                                    // waves of a block of few rows
-constexpr int kFourTiles = 2, kFourWaves = 2;                         // four bits: tiles on their way a wave, waves a SIMD
+constexpr int kFourTiles = 1, kFourWaves = 3;                         // four bits: tiles on their way a wave, waves a SIMD
 
 // f(0) .. f(N - 1) with constants.
 template <typename F, int... I> __device__ __forceinline__ void unroll_list(F f, std::integer_sequence<int, I...>) {
@@ -455,7 +456,7 @@ __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, ui
                                               const FewSpan& span, int64_t lo, int n_tiles, float& m, float& l, f32x4 (&o)[DP / 16]) {
     typedef ElemBF16 P;
     typedef FewRegs<ElemF4, DP> Regs;
-    constexpr int KL = Regs::KL, KW = Regs::KW, VD = Regs::VD, NV = DP / 16, KS = DP / 32, NB = DP > 128 ? 2 : kFourTiles;
+    constexpr int KL = Regs::KL, KW = Regs::KW, VD = Regs::VD, NV = DP / 16, KS = DP / 32, NB = kFourTiles;
     constexpr bool TWICE = X::tag == CKR_F16;  // queries in two halves
     const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     // keys are counted from lo, in 32 bits
@@ -704,11 +705,12 @@ __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, ui
     }
 }
 // Waves of a SIMD that a block's registers leave room for.
-template <typename C> constexpr int few_waves(int dp) { return dp > 128 ? 1 : C::tag == CKR_F4 ? kFourWaves : 2; }
+template <typename C> constexpr int few_waves(int dp) { return C::tag == CKR_F4 ? (dp > 128 ? 2 : kFourWaves) : dp > 128 ? 1 : 2; }
 
 template <typename X, typename C, int DP>
 __global__ void __launch_bounds__(64 * kFewWaves, few_waves<C>(DP)) attend_few_kernel(AttnArg arg) {
     const AttnArg& a = arg;
+    const uint32_t pad = C::tag == CKR_F4 ? arg.item_pad : 0;
     typedef typename Prob<X, C>::E P;
     typedef std::conditional_t<C::tag == CKR_F4, FewRegs<ElemF8, DP>, FewRegs<C, DP>> Regs;
     constexpr int KL = Regs::KL, VD = Regs::VD, NV = DP / 16, KS = DP / 32;
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, few_waves<C>(DP)) attend_few_k
         q.start = a.b.starts[seq];
         q.rows = from >= 0 && to > from ? (uint32_t)(to - from) * a.group : 0;
         q.token0 = (uint32_t)from;
-        for (uint32_t r = 0; r < q.rows; r += kFewRows) q.tiles += few_tiles(few_span(a, q.start, r, q.rows));
+        for (uint32_t r = 0; r < q.rows; r += kFewRows) q.tiles += few_tiles(few_span(a, q.start, r, q.rows)) + pad;
         q.tiles *= a.kv_heads;
         return q;
     };
@@ -789,394 +791,396 @@ __global__ void __launch_bounds__(64 * kFewWaves, few_waves<C>(DP)) attend_few_k
     // the item that the stretch begins in
     FewSpan span = few_span(a, start, 0, rows);
     uint32_t nt = few_tiles(span);
-    while (in_seq >= nt * a.kv_heads) {
-        in_seq -= nt * a.kv_heads, row0 += kFewRows;
+    while (in_seq >= (nt + pad) * a.kv_heads) {
+        in_seq -= (nt + pad) * a.kv_heads, row0 += kFewRows;
         span = few_span(a, start, row0, rows), nt = few_tiles(span);
     }
-    uint32_t kvh = scalar(in_seq / nt), t0 = scalar(in_seq % nt);
+    uint32_t kvh = scalar(in_seq / (nt + pad)), t0 = scalar(in_seq % (nt + pad));
 
     for (uint32_t p = p_begin; p < p_end;) {
         const AttnArg& a = C::tag == CKR_F4 ? args_here() : arg;
-        const uint32_t t1 = scalar(min(nt, t0 + (p_end - p)));
-        // the waves share the item's tiles (or this block's part of them) evenly
-        const uint32_t w0 = (uint32_t)((uint64_t)(t1 - t0) * wave / kFewWaves), w1 = (uint32_t)((uint64_t)(t1 - t0) * (wave + 1) / kFewWaves);
-        const int64_t lo = span.first + 32ll * (t0 + w0);
-        const int n_tiles = w1 - w0;
-        float m = -INFINITY, l = 0.f;
-        f32x4 o[NV];
+        const uint32_t t2 = scalar(min(nt + pad, t0 + (p_end - p))), t1 = min(nt, t2);
+        if (pad == 0 || t0 < nt) {
+            // the waves share the item's tiles (or this block's part of them) evenly
+            const uint32_t w0 = (uint32_t)((uint64_t)(t1 - t0) * wave / kFewWaves), w1 = (uint32_t)((uint64_t)(t1 - t0) * (wave + 1) / kFewWaves);
+            const int64_t lo = span.first + 32ll * (t0 + w0);
+            const int n_tiles = w1 - w0;
+            float m = -INFINITY, l = 0.f;
+            f32x4 o[NV];
 #pragma unroll
-        for (int c = 0; c < NV; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (C::tag == CKR_F4) {
-            few_item_four<X, DP>(a, seq, kvh, token0, row0, rows, span, lo, n_tiles, m, l, o);
-        } else {
-            // from here on keys are counted from lo, in 32 bits
-            const auto rel = [&](int64_t x) { return (int)max((int64_t)-0x40000000, min(x - lo, (int64_t)0x7fffffff - 256)); };
-            const uint32_t row = row0 + col;
-            const int64_t my_pos = span.pos_lo - row0 / a.group + min(row, rows - 1) / a.group;
-            const int pos = rel(my_pos), see = a.window ? rel(my_pos - (int64_t)a.window) : -0x40000000;
-            const int end = __builtin_amdgcn_readfirstlane(rel(span.limit));
-            const int full_to = __builtin_amdgcn_readfirstlane(min(rel(span.pos_lo) + 1, end));  // every row sees the keys before this
-            const int full_from = __builtin_amdgcn_readfirstlane(a.window ? rel(span.pos_hi - (int64_t)a.window) + 1 : -0x40000000);  // and from this on
+            for (int c = 0; c < NV; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (C::tag == CKR_F4) {
+                few_item_four<X, DP>(a, seq, kvh, token0, row0, rows, span, lo, n_tiles, m, l, o);
+            } else {
+                // from here on keys are counted from lo, in 32 bits
+                const auto rel = [&](int64_t x) { return (int)max((int64_t)-0x40000000, min(x - lo, (int64_t)0x7fffffff - 256)); };
+                const uint32_t row = row0 + col;
+                const int64_t my_pos = span.pos_lo - row0 / a.group + min(row, rows - 1) / a.group;
+                const int pos = rel(my_pos), see = a.window ? rel(my_pos - (int64_t)a.window) : -0x40000000;
+                const int end = __builtin_amdgcn_readfirstlane(rel(span.limit));
+                const int full_to = __builtin_amdgcn_readfirstlane(min(rel(span.pos_lo) + 1, end));  // every row sees the keys before this
+                const int full_from = __builtin_amdgcn_readfirstlane(a.window ? rel(span.pos_hi - (int64_t)a.window) + 1 : -0x40000000);  // and from this on
 
-            // queries: the elements of each 32-wide step in the order of the keys' pieces
-            u32x4 q[KS];
+                // queries: the elements of each 32-wide step in the order of the keys' pieces
+                u32x4 q[KS];
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const uint32_t d = C::bytes == 1 ? (ks / 2) * 64 + g * 16 + (ks % 2) * 8 : ks * 32 + g * 8;
-                q[ks] = u32x4{0, 0, 0, 0};
-                if (row < rows && d < a.dim)
-                    q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(token0 + row / a.group) * a.q_tok +
-                                                                  (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
-            }
-            const uint8_t* const ck = a.ck + (int64_t)kvh * a.kst[1];
-            const uint8_t* const cv = a.cv + (int64_t)kvh * a.vst[1];
-            const float* const skp = a.sk + (int64_t)kvh * a.skst[1];
-            const float* const svp = a.sv + (int64_t)kvh * a.svst[1];
-            const int64_t k_off = (int64_t)col * a.kst[2] + g * 16;
-            // one offset and three sums a load, for 16-bit caches have no registers for four (390 us
-            // a step of 64 sequences to 16000 with them, 342 without; e4m3 177 and 176); four where
-            // values are widened by their scale's power (183 us, 196 with one)
-            constexpr int OFFS = Prob<X, C>::split ? 4 : 1;
-            int64_t v_off[OFFS];
-#pragma unroll
-            for (int i = 0; i < OFFS; i++) v_off[i] = (int64_t)(4 * g + i) * a.vst[2] + col * (VD * 4);
-            const auto v_row = [&](int i) { return OFFS == 4 ? v_off[i % OFFS] : i * a.vst[2] + v_off[0]; };
-            const bool v_in = col * NV < a.dim;
-            typedef __attribute__((address_space(1))) const int32_t* global_i32;
-            const global_i32 table = (global_i32)(a.b.table + (int64_t)seq * a.b.table_stride);
-            const uint32_t slot_mask = (1u << a.page_shift) - 1, in0 = (uint32_t)lo & slot_mask;
-            // table columns c0 .. c0 + 63 in a register of the wave, the next 64 on their way
-            uint32_t c0 = (uint32_t)(lo >> a.page_shift);
-            const auto page_lane = [&](uint32_t c) {
-                c += lane;
-                const int32_t x = c < a.b.width ? table[c] : -1;
-                return (uint32_t)x < a.n_pages ? x : -1;
-            };
-            int32_t window_now = page_lane(c0), window_next = page_lane(c0 + 64);
-            uint32_t c_now = 0;
-            const auto page_at = [&](int j) {  // of key j; called with j rising by 16
-                const uint32_t c = (in0 + (uint32_t)j) >> a.page_shift;
-                if (c - c_now >= 64) {
-                    c_now += 64;
-                    window_now = window_next;
-                    window_next = page_lane(c0 + c_now + 64);
+                for (int ks = 0; ks < KS; ks++) {
+                    const uint32_t d = C::bytes == 1 ? (ks / 2) * 64 + g * 16 + (ks % 2) * 8 : ks * 32 + g * 8;
+                    q[ks] = u32x4{0, 0, 0, 0};
+                    if (row < rows && d < a.dim)
+                        q[ks] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(token0 + row / a.group) * a.q_tok +
+                                                                      (int64_t)(kvh * a.group + row % a.group) * a.q_head + d) * 2);
                 }
-                return (int32_t)__builtin_amdgcn_readlane(window_now, (int)(c - c_now));
-            };
-            const auto load_k = [&](Regs& r, int base, const int32_t* pages) {
-                const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
+                const uint8_t* const ck = a.ck + (int64_t)kvh * a.kst[1];
+                const uint8_t* const cv = a.cv + (int64_t)kvh * a.vst[1];
+                const float* const skp = a.sk + (int64_t)kvh * a.skst[1];
+                const float* const svp = a.sv + (int64_t)kvh * a.svst[1];
+                const int64_t k_off = (int64_t)col * a.kst[2] + g * 16;
+                // one offset and three sums a load, for 16-bit caches have no registers for four (390 us
+                // a step of 64 sequences to 16000 with them, 342 without; e4m3 177 and 176); four where
+                // values are widened by their scale's power (183 us, 196 with one)
+                constexpr int OFFS = Prob<X, C>::split ? 4 : 1;
+                int64_t v_off[OFFS];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
-                    const uint8_t* at = ck + (int64_t)pages[h] * a.kst[0] + (int64_t)slot * a.kst[2] + k_off;
-                    if (whole) {
-#pragma unroll
-                        for (int j = 0; j < KL; j++) r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < KL; j++) {
-                            r.k[h][j] = u32x4{0, 0, 0, 0};
-                            if (pages[h] >= 0 && base + 16 * h + (int)col < end && (j * 64 + g * 16) / C::bytes < a.dim)
-                                r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
-                        }
+                for (int i = 0; i < OFFS; i++) v_off[i] = (int64_t)(4 * g + i) * a.vst[2] + col * (VD * 4);
+                const auto v_row = [&](int i) { return OFFS == 4 ? v_off[i % OFFS] : i * a.vst[2] + v_off[0]; };
+                const bool v_in = col * NV < a.dim;
+                typedef __attribute__((address_space(1))) const int32_t* global_i32;
+                const global_i32 table = (global_i32)(a.b.table + (int64_t)seq * a.b.table_stride);
+                const uint32_t slot_mask = (1u << a.page_shift) - 1, in0 = (uint32_t)lo & slot_mask;
+                // table columns c0 .. c0 + 63 in a register of the wave, the next 64 on their way
+                uint32_t c0 = (uint32_t)(lo >> a.page_shift);
+                const auto page_lane = [&](uint32_t c) {
+                    c += lane;
+                    const int32_t x = c < a.b.width ? table[c] : -1;
+                    return (uint32_t)x < a.n_pages ? x : -1;
+                };
+                int32_t window_now = page_lane(c0), window_next = page_lane(c0 + 64);
+                uint32_t c_now = 0;
+                const auto page_at = [&](int j) {  // of key j; called with j rising by 16
+                    const uint32_t c = (in0 + (uint32_t)j) >> a.page_shift;
+                    if (c - c_now >= 64) {
+                        c_now += 64;
+                        window_now = window_next;
+                        window_next = page_lane(c0 + c_now + 64);
                     }
-                    if constexpr (C::bytes == 1) r.sk[h] = *reinterpret_cast<const f32x4*>(skp + (int64_t)max(pages[h], 0) * a.skst[0] + slot + 4 * g);
-                }
-            };
-            const auto load_v = [&](Regs& r, int base, const int32_t* pages) {
-                const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
-                const auto get = [&](uint32_t (&v)[VD], const uint8_t* at) {
-                    if constexpr (VD == 1) v[0] = *reinterpret_cast<const uint32_t*>(at);
-                    else if constexpr (VD == 2) {
-                        const u32x2 y = *reinterpret_cast<const u32x2*>(at);
-                        v[0] = y[0], v[1] = y[1];
-                    } else {
+                    return (int32_t)__builtin_amdgcn_readlane(window_now, (int)(c - c_now));
+                };
+                const auto load_k = [&](Regs& r, int base, const int32_t* pages) {
+                    const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
 #pragma unroll
-                        for (int j = 0; j < VD; j += 4) {
-                            const u32x4 y = *reinterpret_cast<const u32x4*>(at + j * 4);
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
+                        const uint8_t* at = ck + (int64_t)pages[h] * a.kst[0] + (int64_t)slot * a.kst[2] + k_off;
+                        if (whole) {
 #pragma unroll
-                            for (int k = 0; k < 4; k++) v[j + k] = y[k];
+                            for (int j = 0; j < KL; j++) r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < KL; j++) {
+                                r.k[h][j] = u32x4{0, 0, 0, 0};
+                                if (pages[h] >= 0 && base + 16 * h + (int)col < end && (j * 64 + g * 16) / C::bytes < a.dim)
+                                    r.k[h][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
+                            }
+                        }
+                        if constexpr (C::bytes == 1) r.sk[h] = *reinterpret_cast<const f32x4*>(skp + (int64_t)max(pages[h], 0) * a.skst[0] + slot + 4 * g);
+                    }
+                };
+                const auto load_v = [&](Regs& r, int base, const int32_t* pages) {
+                    const bool whole = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= end && DP == a.dim;
+                    const auto get = [&](uint32_t (&v)[VD], const uint8_t* at) {
+                        if constexpr (VD == 1) v[0] = *reinterpret_cast<const uint32_t*>(at);
+                        else if constexpr (VD == 2) {
+                            const u32x2 y = *reinterpret_cast<const u32x2*>(at);
+                            v[0] = y[0], v[1] = y[1];
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < VD; j += 4) {
+                                const u32x4 y = *reinterpret_cast<const u32x4*>(at + j * 4);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) v[j + k] = y[k];
+                            }
+                        }
+                    };
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
+                        const uint8_t* at = cv + (int64_t)pages[h] * a.vst[0] + (int64_t)slot * a.vst[2];
+                        if constexpr (C::bytes == 1) r.sv[h] = *reinterpret_cast<const f32x4*>(svp + (int64_t)max(pages[h], 0) * a.svst[0] + slot + 4 * g);
+                        if (whole) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) get(r.v[4 * h + i], at + v_row(i));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                                for (int j = 0; j < VD; j++) r.v[4 * h + i][j] = 0;
+                                if (pages[h] >= 0 && base + 16 * h + 4 * (int)g + i < end && v_in) get(r.v[4 * h + i], at + v_row(i));
+                            }
                         }
                     }
                 };
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask;
-                    const uint8_t* at = cv + (int64_t)pages[h] * a.vst[0] + (int64_t)slot * a.vst[2];
-                    if constexpr (C::bytes == 1) r.sv[h] = *reinterpret_cast<const f32x4*>(svp + (int64_t)max(pages[h], 0) * a.svst[0] + slot + 4 * g);
-                    if (whole) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) get(r.v[4 * h + i], at + v_row(i));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-#pragma unroll
-                            for (int j = 0; j < VD; j++) r.v[4 * h + i][j] = 0;
-                            if (pages[h] >= 0 && base + 16 * h + 4 * (int)g + i < end && v_in) get(r.v[4 * h + i], at + v_row(i));
-                        }
-                    }
-                }
-            };
 
-            const auto scores = [&](const Regs& r, f32x4 (&s)[2]) {
+                const auto scores = [&](const Regs& r, f32x4 (&s)[2]) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int h = 0; h < 2; h++) {
+                        s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < KL; j++) {
-                        if constexpr (C::bytes == 1) {
-                            const u32x4 x = r.k[h][j];
-                            const u32x2 w0 = widen4<C, X>(x[0]), w1 = widen4<C, X>(x[1]), w2 = widen4<C, X>(x[2]), w3 = widen4<C, X>(x[3]);
-                            s[h] = mfma16<X>(u32x4{w0[0], w0[1], w1[0], w1[1]}, q[2 * j], s[h]);
-                            s[h] = mfma16<X>(u32x4{w2[0], w2[1], w3[0], w3[1]}, q[2 * j + 1], s[h]);
-                        } else {
-                            s[h] = mfma16<X>(r.k[h][j], q[j], s[h]);
+                        for (int j = 0; j < KL; j++) {
+                            if constexpr (C::bytes == 1) {
+                                const u32x4 x = r.k[h][j];
+                                const u32x2 w0 = widen4<C, X>(x[0]), w1 = widen4<C, X>(x[1]), w2 = widen4<C, X>(x[2]), w3 = widen4<C, X>(x[3]);
+                                s[h] = mfma16<X>(u32x4{w0[0], w0[1], w1[0], w1[1]}, q[2 * j], s[h]);
+                                s[h] = mfma16<X>(u32x4{w2[0], w2[1], w3[0], w3[1]}, q[2 * j + 1], s[h]);
+                            } else {
+                                s[h] = mfma16<X>(r.k[h][j], q[j], s[h]);
+                            }
                         }
                     }
-                }
-            };
-            // the weights of a tile, with the values' scales; what a row does not see weighs 0
-            const auto weights = [&](const Regs& r, const f32x4 (&s)[2], int base, const int32_t* pages, uint32_t& seen) {
-                const bool full = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= full_to && base >= full_from;
-                float x[8], top = -INFINITY;
-                seen = ~0u;  // every row sees every key
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    x[i] = s[i / 4][i % 4] * a.scale2;
-                    if constexpr (C::bytes == 1) x[i] *= r.sk[i / 4][i % 4];
-                }
-                if (!full) {
-                    seen = 0;
+                };
+                // the weights of a tile, with the values' scales; what a row does not see weighs 0
+                const auto weights = [&](const Regs& r, const f32x4 (&s)[2], int base, const int32_t* pages, uint32_t& seen) {
+                    const bool full = pages[0] >= 0 && pages[1] >= 0 && base + 32 <= full_to && base >= full_from;
+                    float x[8], top = -INFINITY;
+                    seen = ~0u;  // every row sees every key
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int j = base + 16 * (i / 4) + 4 * (int)g + i % 4;
-                        if (pages[i / 4] >= 0 && j <= pos && j > see && j < end) seen |= 1u << i;
-                        x[i] = seen >> i & 1 ? x[i] : -INFINITY;
+                        x[i] = s[i / 4][i % 4] * a.scale2;
+                        if constexpr (C::bytes == 1) x[i] *= r.sk[i / 4][i % 4];
                     }
-                }
+                    if (!full) {
+                        seen = 0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, x[i]);
-                if (__any(top > m + kLag)) {
-                    top = max_quarters(top);
-                    const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
-                    m = m2;
-                    l *= back;
-#pragma unroll
-                    for (int c = 0; c < NV; c++) o[c] *= back;
-                }
-                const float ref = m == -INFINITY ? 0.f : m - Prob<X, C>::up;
-                float w[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    w[i] = exp2_fast(x[i] - ref);
-                    l += w[i];
-                    if constexpr (Prob<X, C>::split) w[i] *= split_scale<C>(r.sv[i / 4][i % 4]).rest;
-                    else if constexpr (C::bytes == 1) w[i] *= r.sv[i / 4][i % 4];
-                }
-                if (C::bytes == 1 && !full) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) w[i] = seen >> i & 1 ? w[i] : 0.f;  // a scale may be NaN there
-                }
-                Halves<P> p;
-#pragma unroll
-                for (int i = 0; i < 4; i++) p.add(i, w[2 * i], w[2 * i + 1]);
-                return p;
-            };
-            const auto gather = [&](const Regs& r, const Halves<P>& p, uint32_t seen) {
-                if constexpr (Prob<X, C>::split) {
-#pragma unroll
-                    for (int j = 0; j < VD; j++) {  // four dimensions of eight keys, widened first: each key has its power
-                        u32x2 x[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) x[k] = widen4_by<C>(r.v[k][j], split_scale<C>(r.sv[k / 4][k % 4]).power);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            u32x4 w;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(x[2 * e + 1][k / 2], x[2 * e][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
-                            o[4 * j + k] = mfma16<P>(w, p.lo, mfma16<P>(w, p.hi, o[4 * j + k]));
+                        for (int i = 0; i < 8; i++) {
+                            const int j = base + 16 * (i / 4) + 4 * (int)g + i % 4;
+                            if (pages[i / 4] >= 0 && j <= pos && j > see && j < end) seen |= 1u << i;
+                            x[i] = seen >> i & 1 ? x[i] : -INFINITY;
                         }
                     }
-                } else if constexpr (C::bytes == 1) {
 #pragma unroll
-                    for (int j = 0; j < VD; j++) {  // four dimensions of eight keys
-                        uint32_t w[2][4];
+                    for (int i = 0; i < 8; i++) top = fmaxf(top, x[i]);
+                    if (__any(top > m + kLag)) {
+                        top = max_quarters(top);
+                        const float m2 = fmaxf(m, top), back = m2 == -INFINITY ? 1.f : exp2_fast(m - m2);
+                        m = m2;
+                        l *= back;
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint32_t a0 = r.v[4 * h][j], a1 = r.v[4 * h + 1][j], a2 = r.v[4 * h + 2][j], a3 = r.v[4 * h + 3][j];
-                            const uint32_t x0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), x1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
-                            const uint32_t y0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), y1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
-                            w[h][0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u);
-                            w[h][1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
-                            w[h][2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u);
-                            w[h][3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
+                        for (int c = 0; c < NV; c++) o[c] *= back;
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m - Prob<X, C>::up;
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        w[i] = exp2_fast(x[i] - ref);
+                        l += w[i];
+                        if constexpr (Prob<X, C>::split) w[i] *= split_scale<C>(r.sv[i / 4][i % 4]).rest;
+                        else if constexpr (C::bytes == 1) w[i] *= r.sv[i / 4][i % 4];
+                    }
+                    if (C::bytes == 1 && !full) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) w[i] = seen >> i & 1 ? w[i] : 0.f;  // a scale may be NaN there
+                    }
+                    Halves<P> p;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p.add(i, w[2 * i], w[2 * i + 1]);
+                    return p;
+                };
+                const auto gather = [&](const Regs& r, const Halves<P>& p, uint32_t seen) {
+                    if constexpr (Prob<X, C>::split) {
+#pragma unroll
+                        for (int j = 0; j < VD; j++) {  // four dimensions of eight keys, widened first: each key has its power
+                            u32x2 x[8];
+#pragma unroll
+                            for (int k = 0; k < 8; k++) x[k] = widen4_by<C>(r.v[k][j], split_scale<C>(r.sv[k / 4][k % 4]).power);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                u32x4 w;
+#pragma unroll
+                                for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(x[2 * e + 1][k / 2], x[2 * e][k / 2], k % 2 ? 0x07060302u : 0x05040100u);
+                                o[4 * j + k] = mfma16<P>(w, p.lo, mfma16<P>(w, p.hi, o[4 * j + k]));
+                            }
                         }
+                    } else if constexpr (C::bytes == 1) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const u32x2 w0 = widen4<C, P>(w[0][k]), w1 = widen4<C, P>(w[1][k]);
-                            const u32x4 v = {w0[0], w0[1], w1[0], w1[1]};
-                            o[4 * j + k] = mfma16<P>(v, p.lo, mfma16<P>(v, p.hi, o[4 * j + k]));
+                        for (int j = 0; j < VD; j++) {  // four dimensions of eight keys
+                            uint32_t w[2][4];
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const uint32_t a0 = r.v[4 * h][j], a1 = r.v[4 * h + 1][j], a2 = r.v[4 * h + 2][j], a3 = r.v[4 * h + 3][j];
+                                const uint32_t x0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), x1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
+                                const uint32_t y0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), y1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+                                w[h][0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u);
+                                w[h][1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
+                                w[h][2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u);
+                                w[h][3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const u32x2 w0 = widen4<C, P>(w[0][k]), w1 = widen4<C, P>(w[1][k]);
+                                const u32x4 v = {w0[0], w0[1], w1[0], w1[1]};
+                                o[4 * j + k] = mfma16<P>(v, p.lo, mfma16<P>(v, p.hi, o[4 * j + k]));
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < VD; j++) {  // two dimensions of eight keys
+                            u32x4 w0, w1;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
+                                w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
+                            }
+                            // a float16 weight may have become 0 though every row sees the key (see settle; here it
+                            // costs nothing to look: a step of 64 sequences to 16000, 344 us with and without)
+                            if (__any((P::tag == CKR_F16 || seen != ~0u) && (any_wild<P>(w0) || any_wild<P>(w1)))) {
+                                const u32x4 see = ones<P>(seen);
+                                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+                                const f32x4 p0 = mfma16<P>(wild<P>(w0, 1), see, zero), m0 = mfma16<P>(wild<P>(w0, -1), see, zero);
+                                const f32x4 p1 = mfma16<P>(wild<P>(w1, 1), see, zero), m1 = mfma16<P>(wild<P>(w1, -1), see, zero);
+#pragma unroll
+                                for (int i = 0; i < 4; i++) o[2 * j][i] += wild_sum(p0[i], m0[i]), o[2 * j + 1][i] += wild_sum(p1[i], m1[i]);
+                                w0 = wild<P>(w0, 0), w1 = wild<P>(w1, 0);
+                            }
+                            o[2 * j] = mfma16<P>(w0, p.lo, mfma16<P>(w0, p.hi, o[2 * j]));
+                            o[2 * j + 1] = mfma16<P>(w1, p.lo, mfma16<P>(w1, p.hi, o[2 * j + 1]));
                         }
                     }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VD; j++) {  // two dimensions of eight keys
-                        u32x4 w0, w1;
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            w0[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x05040100u);
-                            w1[k] = __builtin_amdgcn_perm(r.v[2 * k + 1][j], r.v[2 * k][j], 0x07060302u);
-                        }
-                        // a float16 weight may have become 0 though every row sees the key (see settle; here it
-                        // costs nothing to look: a step of 64 sequences to 16000, 344 us with and without)
-                        if (__any((P::tag == CKR_F16 || seen != ~0u) && (any_wild<P>(w0) || any_wild<P>(w1)))) {
-                            const u32x4 see = ones<P>(seen);
-                            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                            const f32x4 p0 = mfma16<P>(wild<P>(w0, 1), see, zero), m0 = mfma16<P>(wild<P>(w0, -1), see, zero);
-                            const f32x4 p1 = mfma16<P>(wild<P>(w1, 1), see, zero), m1 = mfma16<P>(wild<P>(w1, -1), see, zero);
-#pragma unroll
-                            for (int i = 0; i < 4; i++) o[2 * j][i] += wild_sum(p0[i], m0[i]), o[2 * j + 1][i] += wild_sum(p1[i], m1[i]);
-                            w0 = wild<P>(w0, 0), w1 = wild<P>(w1, 0);
-                        }
-                        o[2 * j] = mfma16<P>(w0, p.lo, mfma16<P>(w0, p.hi, o[2 * j]));
-                        o[2 * j + 1] = mfma16<P>(w1, p.lo, mfma16<P>(w1, p.hi, o[2 * j + 1]));
-                    }
-                }
-            };
+                };
 
-            Regs r[2];
-            int32_t pages[2][2], coming[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                if (u < n_tiles) {
-                    pages[u][0] = page_at(32 * u), pages[u][1] = page_at(32 * u + 16);
-                    load_k(r[u], 32 * u, pages[u]);
-                    load_v(r[u], 32 * u, pages[u]);
-                }
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) q[ks] ^= a.flip;
-            for (int i = 0; i < n_tiles; i += 2) {
+                Regs r[2];
+                int32_t pages[2][2], coming[2];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    if (i + u >= n_tiles) break;
-                    const int base = 32 * (i + u);
-                    const bool more = i + u + 2 < n_tiles;
-                    f32x4 s[2];
-                    scores(r[u], s);
-                    uint32_t seen;
-                    const Halves<P> p = weights(r[u], s, base, pages[u], seen);
-                    if (more) {  // its keys' registers again, for the tile after the next
-                        coming[0] = page_at(base + 64), coming[1] = page_at(base + 80);
-                        load_k(r[u], base + 64, coming);
+                    if (u < n_tiles) {
+                        pages[u][0] = page_at(32 * u), pages[u][1] = page_at(32 * u + 16);
+                        load_k(r[u], 32 * u, pages[u]);
+                        load_v(r[u], 32 * u, pages[u]);
                     }
-                    gather(r[u], p, seen);
-                    if (more) {
-                        pages[u][0] = coming[0], pages[u][1] = coming[1];
-                        load_v(r[u], base + 64, pages[u]);
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) q[ks] ^= a.flip;
+                for (int i = 0; i < n_tiles; i += 2) {
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        if (i + u >= n_tiles) break;
+                        const int base = 32 * (i + u);
+                        const bool more = i + u + 2 < n_tiles;
+                        f32x4 s[2];
+                        scores(r[u], s);
+                        uint32_t seen;
+                        const Halves<P> p = weights(r[u], s, base, pages[u], seen);
+                        if (more) {  // its keys' registers again, for the tile after the next
+                            coming[0] = page_at(base + 64), coming[1] = page_at(base + 80);
+                            load_k(r[u], base + 64, coming);
+                        }
+                        gather(r[u], p, seen);
+                        if (more) {
+                            pages[u][0] = coming[0], pages[u][1] = coming[1];
+                            load_v(r[u], base + 64, pages[u]);
+                        }
                     }
                 }
             }
-        }
-        // ---- join: lane (col, g) holds dimensions 4 g NV .. 4 (g + 1) NV of row col
-        l = sum_quarters(l);
-        if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
-        __syncthreads();                        // the last item's sums have been read
+            // ---- join: lane (col, g) holds dimensions 4 g NV .. 4 (g + 1) NV of row col
+            l = sum_quarters(l);
+            if (l != l && m == -INFINITY) m = 0.f;  // only NaN scores so far: not a row without keys
+            __syncthreads();                        // the last item's sums have been read
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int c = 0; c < NV; c += 4)
-                *reinterpret_cast<f32x4*>(&s_o[wave][col][(4 * g + i) * NV + c]) = f32x4{o[c][i], o[c + 1][i], o[c + 2][i], o[c + 3][i]};
-        if (g == 0) s_m[wave][col][0] = m, s_m[wave][col][1] = l;
-        __syncthreads();
-        const uint32_t n_rows = min(kFewRows, rows - row0);
-        // the first n sums in LDS of a row's four outputs, joined
-        const auto joined = [&](uint32_t n, uint32_t rr, uint32_t d, float& top, float& sum) {
-            top = -INFINITY, sum = 0.f;
-            for (uint32_t w = 0; w < n; w++) top = fmaxf(top, s_m[w][rr][0]);
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            for (uint32_t w = 0; w < n; w++) {
-                const float mw = s_m[w][rr][0];
-                if (mw == -INFINITY) continue;
-                const float f = exp2_fast(mw - top);
-                sum += s_m[w][rr][1] * f;
-                v += *reinterpret_cast<const f32x4*>(&s_o[w][rr][d]) * f;
-            }
-            return v;
-        };
-        const auto write = [&](uint32_t rr, uint32_t d, f32x4 v, float top, float sum) {
-            const uint32_t orow = row0 + rr, token = token0 + orow / a.group, head = kvh * a.group + orow % a.group;
-            const float inv = top == -INFINITY ? 0.f : 1.f / sum;
-            if (d < a.dim)
-                *reinterpret_cast<u32x2*>(a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head + d) * 2) =
-                    u32x2{pack16<X>(v[0] * inv, v[1] * inv), pack16<X>(v[2] * inv, v[3] * inv)};
-            if (a.lse && d == 0) a.lse[(int64_t)token * a.heads + head] = top == -INFINITY ? -INFINITY : (top - Prob<X, C>::up + log2f(sum)) * kLn2;
-        };
-        const bool whole = t0 == 0 && t1 == nt;
-        const uint64_t part = ((uint64_t)blockIdx.x * 2 + (t0 == 0)) * kFewRows;
-        for (uint32_t e = threadIdx.x; e < n_rows * QUADS; e += THREADS) {
-            const uint32_t rr = e / QUADS, d = e % QUADS * 4;
-            float top, sum;
-            const f32x4 v = joined(kFewWaves, rr, d, top, sum);
-            if (whole) {
-                write(rr, d, v, top, sum);
-            } else {
-                float* po = a.part_o + (part + rr) * DP + d;
-                store_far(po, v[0], v[1]), store_far(po + 2, v[2], v[3]);
-                if (d == 0) store_far(a.part_m + (part + rr) * 2, top, sum);
-            }
-        }
-        if (!whole) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part has arrived
-            __syncthreads();                                  // and the block's
-            const uint32_t begin = p - t0, b_first = begin / per, parts = (begin + nt - 1) / per - b_first + 1;
-            uint32_t* const counter = a.counters + b_first;  // one item at most begins in a block and goes on
-            if (threadIdx.x == 0) {
-                const uint32_t seen = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                s_last = seen + 1 == parts;
-                if (seen + 1 == parts) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+                for (int c = 0; c < NV; c += 4)
+                    *reinterpret_cast<f32x4*>(&s_o[wave][col][(4 * g + i) * NV + c]) = f32x4{o[c][i], o[c + 1][i], o[c + 2][i], o[c + 3][i]};
+            if (g == 0) s_m[wave][col][0] = m, s_m[wave][col][1] = l;
             __syncthreads();
-            if (s_last) {
-                // the last block of the item's to finish joins its parts: groups of threads take
-                // every so many of them each, four at a time (loads without branches, so that
-                // they do not wait for each other), then the groups' sums are joined as the waves' were
-                const uint32_t quads = n_rows * QUADS, groups = min(kFewWaves, max(THREADS / quads, 1u));
-                const auto part_of = [&](uint32_t k) { return (uint64_t)(k == 0 ? b_first * 2 + 1 : (b_first + k) * 2) * kFewRows; };
-                for (uint32_t e = threadIdx.x; e < groups * quads; e += THREADS) {
-                    const uint32_t grp = e / quads, rr = e % quads / QUADS, d = e % QUADS * 4;
-                    float top = -INFINITY, sum = 0.f;
-                    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                    for (uint32_t k = grp; k < parts; k += 4 * groups) {
-                        f32x2 ml[4], x[4], y[4];
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            const uint64_t at = part_of(min(k + u * groups, parts - 1)) + rr;
-                            ml[u] = load_far(a.part_m + at * 2);
-                            x[u] = load_far(a.part_o + at * DP + d), y[u] = load_far(a.part_o + at * DP + d + 2);
-                        }
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            if (k + u * groups >= parts || ml[u][0] == -INFINITY) continue;
-                            const float top2 = fmaxf(top, ml[u][0]), f = exp2_fast(top - top2), f2 = exp2_fast(ml[u][0] - top2);
-                            top = top2, sum = sum * f + ml[u][1] * f2;
-                            v = v * f + f32x4{x[u][0], x[u][1], y[u][0], y[u][1]} * f2;
-                        }
-                    }
-                    *reinterpret_cast<f32x4*>(&s_o[grp][rr][d]) = v;
-                    if (d == 0) s_m[grp][rr][0] = top, s_m[grp][rr][1] = sum;
+            const uint32_t n_rows = min(kFewRows, rows - row0);
+            // the first n sums in LDS of a row's four outputs, joined
+            const auto joined = [&](uint32_t n, uint32_t rr, uint32_t d, float& top, float& sum) {
+                top = -INFINITY, sum = 0.f;
+                for (uint32_t w = 0; w < n; w++) top = fmaxf(top, s_m[w][rr][0]);
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                for (uint32_t w = 0; w < n; w++) {
+                    const float mw = s_m[w][rr][0];
+                    if (mw == -INFINITY) continue;
+                    const float f = exp2_fast(mw - top);
+                    sum += s_m[w][rr][1] * f;
+                    v += *reinterpret_cast<const f32x4*>(&s_o[w][rr][d]) * f;
+                }
+                return v;
+            };
+            const auto write = [&](uint32_t rr, uint32_t d, f32x4 v, float top, float sum) {
+                const uint32_t orow = row0 + rr, token = token0 + orow / a.group, head = kvh * a.group + orow % a.group;
+                const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+                if (d < a.dim)
+                    *reinterpret_cast<u32x2*>(a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head + d) * 2) =
+                        u32x2{pack16<X>(v[0] * inv, v[1] * inv), pack16<X>(v[2] * inv, v[3] * inv)};
+                if (a.lse && d == 0) a.lse[(int64_t)token * a.heads + head] = top == -INFINITY ? -INFINITY : (top - Prob<X, C>::up + log2f(sum)) * kLn2;
+            };
+            const bool whole = t0 == 0 && t1 == nt;
+            const uint64_t part = ((uint64_t)blockIdx.x * 2 + (t0 == 0)) * kFewRows;
+            for (uint32_t e = threadIdx.x; e < n_rows * QUADS; e += THREADS) {
+                const uint32_t rr = e / QUADS, d = e % QUADS * 4;
+                float top, sum;
+                const f32x4 v = joined(kFewWaves, rr, d, top, sum);
+                if (whole) {
+                    write(rr, d, v, top, sum);
+                } else {
+                    float* po = a.part_o + (part + rr) * DP + d;
+                    store_far(po, v[0], v[1]), store_far(po + 2, v[2], v[3]);
+                    if (d == 0) store_far(a.part_m + (part + rr) * 2, top, sum);
+                }
+            }
+            if (!whole) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part has arrived
+                __syncthreads();                                  // and the block's
+                const uint32_t begin = p - t0, b_first = begin / per, parts = (begin + nt - 1) / per - b_first + 1;
+                uint32_t* const counter = a.counters + b_first;  // one item at most begins in a block and goes on
+                if (threadIdx.x == 0) {
+                    const uint32_t seen = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    s_last = seen + 1 == parts;
+                    if (seen + 1 == parts) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
                 __syncthreads();
-                for (uint32_t e = threadIdx.x; e < quads; e += THREADS) {
-                    const uint32_t rr = e / QUADS, d = e % QUADS * 4;
-                    float top, sum;
-                    const f32x4 v = joined(groups, rr, d, top, sum);
-                    write(rr, d, v, top, sum);
+                if (s_last) {
+                    // the last block of the item's to finish joins its parts: groups of threads take
+                    // every so many of them each, four at a time (loads without branches, so that
+                    // they do not wait for each other), then the groups' sums are joined as the waves' were
+                    const uint32_t quads = n_rows * QUADS, groups = min(kFewWaves, max(THREADS / quads, 1u));
+                    const auto part_of = [&](uint32_t k) { return (uint64_t)(k == 0 ? b_first * 2 + 1 : (b_first + k) * 2) * kFewRows; };
+                    for (uint32_t e = threadIdx.x; e < groups * quads; e += THREADS) {
+                        const uint32_t grp = e / quads, rr = e % quads / QUADS, d = e % QUADS * 4;
+                        float top = -INFINITY, sum = 0.f;
+                        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                        for (uint32_t k = grp; k < parts; k += 4 * groups) {
+                            f32x2 ml[4], x[4], y[4];
+#pragma unroll
+                            for (int u = 0; u < 4; u++) {
+                                const uint64_t at = part_of(min(k + u * groups, parts - 1)) + rr;
+                                ml[u] = load_far(a.part_m + at * 2);
+                                x[u] = load_far(a.part_o + at * DP + d), y[u] = load_far(a.part_o + at * DP + d + 2);
+                            }
+#pragma unroll
+                            for (int u = 0; u < 4; u++) {
+                                if (k + u * groups >= parts || ml[u][0] == -INFINITY) continue;
+                                const float top2 = fmaxf(top, ml[u][0]), f = exp2_fast(top - top2), f2 = exp2_fast(ml[u][0] - top2);
+                                top = top2, sum = sum * f + ml[u][1] * f2;
+                                v = v * f + f32x4{x[u][0], x[u][1], y[u][0], y[u][1]} * f2;
+                            }
+                        }
+                        *reinterpret_cast<f32x4*>(&s_o[grp][rr][d]) = v;
+                        if (d == 0) s_m[grp][rr][0] = top, s_m[grp][rr][1] = sum;
+                    }
+                    __syncthreads();
+                    for (uint32_t e = threadIdx.x; e < quads; e += THREADS) {
+                        const uint32_t rr = e / QUADS, d = e % QUADS * 4;
+                        float top, sum;
+                        const f32x4 v = joined(groups, rr, d, top, sum);
+                        write(rr, d, v, top, sum);
+                    }
                 }
             }
         }
         // ---- on to the next item
-        p += t1 - t0;
+        p += t2 - t0;
         if (p >= p_end) break;
         t0 = 0;
         if (++kvh < a.kv_heads) continue;
@@ -2279,7 +2283,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttnArg a, float up) {
 // How a batch is cut: rows of a tile, tiles (an upper bound: each sequence's last
 // tile may be short), key ranges of a tile.
 struct Cut {
-    uint32_t bm, dp, tiles, splits, split_len, blocks, min_tiles;
+    uint32_t bm, dp, tiles, splits, split_len, blocks, min_tiles, item_pad;
     uint64_t part_m_bytes, bytes;  // of the workspace: counters, the rows' maxima and sums, their outputs
 };
 template <typename X, typename C, int DP>

@@ -22,8 +22,11 @@ constexpr uint64_t kSplitMin = 128;   // keys of a split at least
 // Blocks of the few rows' kernel: two a CU.  (For heads of 256 its registers leave room
 // for one, so there a full launch runs in two rounds.)
 constexpr uint32_t kFewBlocks = 512;
-constexpr uint32_t kFourBlocks = 512;  // over a cache of 4 bits
-uint32_t most_blocks(bool four) { return four ? kFourBlocks : kFewBlocks; }
+constexpr uint32_t kFourBlocks = 768;  // over a cache of 4 bits: three a CU (of heads of 256 two)
+// There an item (its queries, the first tiles' way, the join) costs a block as much as so many tiles, so
+// that stretches with many short items are given fewer tiles; in stretches from kPadFrom tiles on.
+constexpr uint32_t kItemPad = 16, kPadFrom = 32;
+uint32_t most_blocks(bool four, uint32_t dp) { return four && dp <= 128 ? kFourBlocks : kFewBlocks; }
 // Its tiles of 32 keys a block at least: one a wave (one token over a thousand: 9.5 us;
 // 11.0 with 8, 13.5 with 16).
 constexpr uint32_t kFewTiles = 4;
@@ -49,8 +52,8 @@ void set_bytes(Cut& c, uint64_t rows) {
     c.part_m_bytes = (rows * 8 + 255) / 256 * 256;
     c.bytes = kCounterBytes + c.part_m_bytes + rows * c.dp * 4;
 }
-uint32_t few_blocks(uint64_t items, uint64_t max_context, bool four) {
-    return (uint32_t)std::min<uint64_t>(items * ((max_context + 31) / 32) / kFewTiles + 1, most_blocks(four));
+uint32_t few_blocks(uint64_t items, uint64_t max_context, bool four, uint32_t dp) {
+    return (uint32_t)std::min<uint64_t>(items * ((max_context + 31) / 32) / kFewTiles + 1, most_blocks(four, dp));
 }
 // Rows of parts that a workspace holds (calls keep multiples of 32, which set_bytes rounds no further).
 uint64_t rows_held(uint64_t bytes, uint32_t dp) { return bytes < kCounterBytes ? 0 : (bytes - kCounterBytes) / (8 + dp * 4); }
@@ -61,7 +64,7 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     Cut c{};
     const uint64_t group = n_heads / n_kv, rows = (uint64_t)max_chunk * group;
     c.dp = padded_dim(dim);
-    const bool few = rows <= kFewMost && (near_slots || !four) && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1) < (1ull << 31);
+    const bool few = rows <= kFewMost && (near_slots || !four) && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1 + (four ? kItemPad : 0)) < (1ull << 31);
     c.bm = few ? kFewRows : rows <= kManyMost || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
     c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
     c.splits = 1;
@@ -70,7 +73,8 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     const uint64_t items = std::max<uint64_t>((uint64_t)c.tiles * n_kv, 1);
     if (c.bm == kFewRows) {
         c.min_tiles = kFewTiles;
-        c.blocks = (uint32_t)std::clamp<uint64_t>(rows_held(workspace, c.dp) / (2 * kFewRows), 1, few_blocks(items, max_context, four));
+        c.blocks = (uint32_t)std::clamp<uint64_t>(rows_held(workspace, c.dp) / (2 * kFewRows), 1, few_blocks(items, max_context, four, c.dp));
+        c.item_pad = four && items * ((max_context + 31) / 32) >= (uint64_t)c.blocks * kPadFrom ? kItemPad : 0;
         set_bytes(c, (uint64_t)c.blocks * 2 * kFewRows);
         return c;
     }
@@ -89,7 +93,7 @@ uint64_t most_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_se
     Cut c{};
     c.dp = padded_dim(dim);
     uint64_t items = std::max<uint64_t>(most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv, 1);
-    set_bytes(c, (uint64_t)few_blocks(items, max_context, true) * 2 * kFewRows);
+    set_bytes(c, (uint64_t)few_blocks(items, max_context, true, c.dp) * 2 * kFewRows);
     uint64_t most = c.bytes;
     for (const uint32_t bm : {kManyRows, kWideRows}) {
         items = most_tiles(bm, group, n_seqs, n_tokens) * n_kv;
@@ -159,7 +163,7 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
                       std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size),
                       (uint64_t)batch->table_width * cache->page_size, window, near_slots, four, workspace_bytes);
     if ((uint64_t)c.tiles * cache->n_heads * 512 > 0xffffffffull) return err(CKR_E_INVALID, "the batch is too large for one launch");
-    a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len, a.min_tiles = c.min_tiles;
+    a.tiles = c.tiles, a.splits = c.splits, a.split_len = c.split_len, a.min_tiles = c.min_tiles, a.item_pad = c.item_pad;
     if (c.bytes) {
         if (workspace_bytes < c.bytes)
             return err(CKR_E_CAPACITY, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(c.bytes) + " needed");

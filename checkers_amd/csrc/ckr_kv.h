@@ -5,6 +5,7 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "checkers_amd.h"
 
@@ -109,16 +110,21 @@ __device__ __forceinline__ uint32_t group_byte(uint32_t top) {
     return min(max((top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u), 27u), 252u);
 }
 
-// The same for N values of each of two neighbouring lanes that hold a group; a group that is
+// The same for 8 values of each of four neighbouring lanes that hold a group; a group that is
 // stored as zeros becomes zeros.
-template <int N> __device__ __forceinline__ uint32_t group_byte_of(float* x) {
+__device__ __forceinline__ uint32_t group_byte_of(float* x) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < N; i++) top = max(top, as_u32(x[i]) & 0x7fffffffu);
-    const uint32_t byte = group_byte(max(top, (uint32_t)__shfl_xor((int)top, 1)));
+    for (int i = 0; i < 8; i++) top = max(top, as_u32(x[i]) & 0x7fffffffu);
+    const auto other = [](uint32_t v, auto n) {
+        return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(n)::value, 0xf, 0xf, true);
+    };
+    top = max(top, other(top, std::integral_constant<int, 0xb1>{}));  // quad_perm 1 0 3 2
+    top = max(top, other(top, std::integral_constant<int, 0x4e>{}));  // quad_perm 2 3 0 1
+    const uint32_t byte = group_byte(top);
     const bool kept = byte - 1 < 254;
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] = kept ? x[i] : 0.f;
+    for (int i = 0; i < 8; i++) x[i] = kept ? x[i] : 0.f;
     return byte;
 }
 

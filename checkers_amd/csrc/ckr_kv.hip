@@ -1,5 +1,5 @@
 // checkers_amd/csrc/ckr_kv.hip — writing and reading a paged key/value cache in
-// 4, 8 or 16 bits, and the residual sum and root-mean-square norm with an output
+// 8 or 16 bits (4 bits: ckr_rotary.hip), and the residual sum and root-mean-square norm with an output
 // in 8 bits.  All three are bound by memory: one pass, rows kept in registers
 // between the reduction and the store.
 #include <algorithm>
@@ -18,6 +18,8 @@ int kv_check_cache(const ckr_kv_cache* c);
 int kv_check_batch(const ckr_kv_cache* c, const ckr_kv_batch* b);
 int kv_check_rows(const void* p, uint64_t rows, int64_t row_stride, uint64_t heads, int64_t head_stride, uint64_t dim,
                   int es, bool written, const char* what);
+int kv_read_four(const ckr_kv_cache* c, const ckr_kv_batch* b, void* k, int64_t kt, int64_t kh, void* v, int64_t vt, int64_t vh,
+                 int dtype, void* stream);
 
 namespace {
 
@@ -70,8 +72,8 @@ struct RowsArg {
     int64_t k_tok, k_head, v_tok, v_head;
     uint8_t* ck;        // the cache
     uint8_t* cv;
-    void* sk;
-    void* sv;
+    float* sk;
+    float* sv;
     int64_t kst[3], vst[3], skst[2], svst[2];
     uint32_t n_pages, page_shift, heads, dim;
     KvBatch b;
@@ -100,7 +102,6 @@ __device__ __forceinline__ uint32_t first_seq(const KvBatch& b, uint32_t token) 
 template <typename X, typename C, int LPR, bool WRITE>
 __global__ void __launch_bounds__(256) kv_rows_kernel(RowsArg a) {
     constexpr uint32_t ROWS = 256 / LPR;
-    constexpr bool FOUR = C::tag == CKR_F4;
     const uint64_t row0 = (uint64_t)blockIdx.x * ROWS;
     uint32_t seq = first_seq(a.b, (uint32_t)(row0 / a.heads));
     const uint64_t row = row0 + threadIdx.x / LPR;
@@ -124,13 +125,9 @@ __global__ void __launch_bounds__(256) kv_rows_kernel(RowsArg a) {
                       lane * kVals) * X::bytes;
         const int64_t* st = which ? a.vst : a.kst;
         uint8_t* c = (which ? a.cv : a.ck) +
-                     ((int64_t)page * st[0] + (int64_t)head * st[1] + (int64_t)slot * st[2]) * (FOUR ? 1 : C::bytes) +
-                     lane * bytes_of<C>(kVals);
+                     ((int64_t)page * st[0] + (int64_t)head * st[1] + (int64_t)slot * st[2] + lane * kVals) * C::bytes;
         const int64_t* sst = which ? a.svst : a.skst;
-        const int64_t s_at = (int64_t)page * sst[0] + (int64_t)head * sst[1] + slot;
-        float* s = static_cast<float*>(which ? a.sv : a.sk) + s_at;
-        // four bits: the pair of lanes that hold a group share its byte
-        uint8_t* s4 = static_cast<uint8_t*>(which ? a.sv : a.sk) + s_at + ((int64_t)(lane * kVals / kGroup) << a.page_shift);
+        float* s = (which ? a.sv : a.sk) + ((int64_t)page * sst[0] + (int64_t)head * sst[1] + slot);
         float f[kVals];
 #pragma unroll
         for (int i = 0; i < kVals; i++) f[i] = 0.f;
@@ -147,24 +144,10 @@ __global__ void __launch_bounds__(256) kv_rows_kernel(RowsArg a) {
                 for (int i = 0; i < kVals; i++) f[i] = scaled(f[i], rs.inv);
                 if (mine && page >= 0 && lane == 0) *s = rs.scale;
             }
-            if constexpr (FOUR) {
-                const uint32_t byte = group_byte_of<kVals>(f);
-                if (mine && page >= 0) {
-                    *reinterpret_cast<u32x2*>(c) = u32x2{encode8(f, byte), encode8(f + 8, byte)};
-                    if (lane % 2 == 0) *s4 = (uint8_t)byte;
-                }
-            } else if (mine && page >= 0) {
-                store_vec<C, kVals>(c, f);
-            }
+            if (mine && page >= 0) store_vec<C, kVals>(c, f);
         } else {
             if (mine && page >= 0) {
-                if constexpr (FOUR) {
-                    const u32x2 codes = *reinterpret_cast<const u32x2*>(c);
-                    const float power = power_of(*s4);
-                    decode8(codes[0], power, f), decode8(codes[1], power, f + 8);
-                } else {
-                    load_vec<C, kVals>(c, f);
-                }
+                load_vec<C, kVals>(c, f);
                 if constexpr (C::bytes == 1) {
                     const float scale = *s;
 #pragma unroll
@@ -194,7 +177,6 @@ hipError_t launch_rows_of(const RowsArg& a, int cache_dtype, hipStream_t s) {
     switch (cache_dtype) {
         case CKR_F8: return launch_rows<X, ElemF8, WRITE>(a, s);
         case CKR_I8: return launch_rows<X, ElemI8, WRITE>(a, s);
-        case CKR_F4: return launch_rows<X, ElemF4, WRITE>(a, s);
         case CKR_BF16: return launch_rows<X, ElemBF16, WRITE>(a, s);
         default: return launch_rows<X, ElemF16, WRITE>(a, s);
     }
@@ -213,9 +195,12 @@ int rows_call(const ckr_kv_cache* c, const ckr_kv_batch* b, void* k, int64_t kt,
         (rc = kv_check_rows(v, b->n_tokens, vt, c->n_heads, vh, c->head_dim, es, !WRITE, "values")) ||
         (WRITE && (rc = kv_check_rows_apart(c))))
         return rc;
+    if (c->dtype == CKR_F4)
+        return WRITE ? ckr_kv_append(c, b, nullptr, nullptr, k, kt, kh, v, vt, vh, nullptr, 0, 0, 0, nullptr, 0, 0, dtype, stream)
+                     : kv_read_four(c, b, k, kt, kh, v, vt, vh, dtype, stream);
     RowsArg a{};
     a.k = k, a.v = v, a.k_tok = kt, a.k_head = kh, a.v_tok = vt, a.v_head = vh;
-    a.ck = static_cast<uint8_t*>(c->d_k), a.cv = static_cast<uint8_t*>(c->d_v), a.sk = c->d_k_scale, a.sv = c->d_v_scale;
+    a.ck = static_cast<uint8_t*>(c->d_k), a.cv = static_cast<uint8_t*>(c->d_v), a.sk = static_cast<float*>(c->d_k_scale), a.sv = static_cast<float*>(c->d_v_scale);
     std::copy(c->k_stride, c->k_stride + 3, a.kst);
     std::copy(c->v_stride, c->v_stride + 3, a.vst);
     std::copy(c->k_scale_stride, c->k_scale_stride + 2, a.skst);

@@ -1,6 +1,6 @@
 // checkers_amd/csrc/ckr_rotary.hip — rotary positions: heads turned by their tokens'
-// positions (ckr_rotate, forward and backward), and a chunk's keys turned on their way
-// into a paged cache (ckr_kv_append).
+// positions (ckr_rotate, forward and backward), a chunk's keys turned on their way into a
+// paged cache (ckr_kv_append), and the rows of a cache of 4 bits read back.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -61,39 +61,51 @@ __device__ __forceinline__ float turned_second(float x, float y, float c, float 
     return y * c + x * s;
 }
 
-// Cosines and sines of a block's tokens in LDS, `padded` pairs a token (a multiple of 8).
-constexpr uint32_t kMostTokens = 8;               // of a block
-constexpr uint64_t kMostBlocks = (1u << 24) - 1;  // a grid holds fewer than 2^32 threads
-
-// How rows are cut into blocks: `tokens` tokens a block with `slab` of their rows (one
-// token where it has more rows than a block), 256 / lanes of them at a time.
+// ---- how tokens' rows are cut into blocks.  A thread keeps its row (a head) and its place in it
+// for all of its block's tokens, so that the products of strides are made once a thread or
+// once a token (whose share lies in LDS), not for each row: with all of them made for each,
+// what bound these kernels was integer multiplication (22448 tokens of 48 heads of 128 appended in 145 us,
+// now XXX).
+constexpr uint32_t kThreads = 512;                // of a block at most
+constexpr uint32_t kMostTokens = 64;              // of a block
+constexpr uint32_t kMostAngles = 32768;           // bytes of LDS for them
+constexpr uint64_t kMostBlocks = (1u << 23) - 1;  // a grid holds fewer than 2^32 threads
 struct RowCut {
-    uint32_t tokens, slab, slabs;  // slabs: blocks of a token
-    uint32_t shift;                // log2 of the lanes of a row
-    uint32_t magic;                // ceil(2^32 / slab)
+    uint32_t shift;        // log2 of the lanes of a row
+    uint32_t slab, slabs;  // rows of a token that a block takes, blocks of a token
+    uint32_t sub, passes;  // tokens side by side, and one after another
+    uint32_t threads;
     uint64_t blocks;
 };
-// Blocks take one pass over their threads when there are few, up to four (a block's
-// angles and, in the cache, its look-ups are then shared by more rows).
-RowCut row_cut(uint64_t tokens, uint64_t rows, uint32_t lanes) {
+RowCut row_cut(uint64_t tokens, uint64_t rows, uint32_t lanes, uint32_t pairs) {
     RowCut c{};
     while ((1u << c.shift) < lanes) c.shift++;
-    const uint64_t pass = 256u >> c.shift, passes = std::clamp<uint64_t>(tokens * rows / pass / 2048, 1, 4);
-    const uint64_t per = pass * passes;
-    if (rows >= per) {
-        c.slabs = (uint32_t)((rows + per - 1) / per);
-        c.slab = (uint32_t)((rows + c.slabs - 1) / c.slabs);
-        c.tokens = 1;
-    } else {
-        c.slabs = 1, c.slab = (uint32_t)rows;
-        c.tokens = (uint32_t)std::min<uint64_t>({per / rows, kMostTokens, std::max<uint64_t>(tokens, 1)});
-    }
-    c.magic = c.slab == 1 ? 0xffffffffu : (uint32_t)(((1ull << 32) + c.slab - 1) / c.slab);
-    c.blocks = (tokens + c.tokens - 1) / c.tokens * c.slabs;
+    c.slabs = (uint32_t)(((rows << c.shift) + kThreads - 1) / kThreads);
+    c.slab = (uint32_t)((rows + c.slabs - 1) / c.slabs);
+    const uint32_t most = std::min(kMostTokens, kMostAngles / std::max((pairs + 7) / 8 * 64, 1u));
+    c.sub = std::clamp(256u / (c.slab << c.shift), 1u, most);
+    c.threads = ((c.sub * c.slab << c.shift) + 63) / 64 * 64;
+    // one after another where there are blocks enough all the same: they share the look-ups and angles
+    c.passes = (uint32_t)std::clamp<uint64_t>(tokens * c.slabs / c.sub / 2048, 1, std::min(8u, most / c.sub));
+    c.blocks = (tokens + c.sub * c.passes - 1) / (c.sub * c.passes) * c.slabs;
     return c;
 }
-// i / slab for i < 2^16 (slab <= 2^16).
-__device__ __forceinline__ uint32_t by_slab(uint32_t i, const RowCut& c) { return c.slab == 1 ? i : __umulhi(i, c.magic); }
+struct Mine { uint32_t sub, row, lane; bool in; };
+__device__ __forceinline__ Mine my_row(const RowCut& c) {
+    const uint32_t item = threadIdx.x >> c.shift, sub = item / c.slab;
+    return {sub, blockIdx.x % c.slabs * c.slab + (item - sub * c.slab), threadIdx.x & ((1u << c.shift) - 1), sub < c.sub};
+}
+// Cosines and sines of n tokens in LDS, `padded` pairs a token (a multiple of 8); position(t): of token t.
+template <typename F> __device__ __forceinline__ void make_angles(f32x2* to, const Rot& rot, uint32_t n, F position, bool inverse) {
+    const uint32_t padded = (rot.pairs + 7) & ~7u;
+    for (uint32_t i = threadIdx.x; i < n * padded; i += blockDim.x) {
+        const uint32_t t = i / padded, pair = i - t * padded;
+        f32x2 cs = {1.f, 0.f};
+        if (pair < rot.pairs) cs = cos_sin((uint64_t)(int64_t)position(t) * rot.turns[pair], rot.magnitude);
+        if (inverse) cs.y = -cs.y;
+        to[i] = cs;
+    }
+}
 
 // ------------------------------------------------------------ rotate
 struct Heads {
@@ -107,7 +119,7 @@ struct RotateArg {
     const int32_t* positions;
     int64_t pos_st[2];
     Heads x[2];
-    uint64_t n_tokens;  // batch x tokens
+    uint32_t n_tokens;  // batch x tokens
     uint32_t tokens, dim, chunks, inverse;
     RowCut cut;
 };
@@ -130,73 +142,69 @@ template <typename E, int N> __device__ __forceinline__ void store_some(uint8_t*
     }
 }
 
-template <typename E> __global__ void __launch_bounds__(256) rotate_kernel(RotateArg a) {
+template <typename E> __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArg a) {
     extern __shared__ __attribute__((aligned(16))) f32x2 s_cs[];
+    __shared__ int64_t s_at[kMostTokens][4];  // a token's place in the inputs and outputs
     const RowCut& c = a.cut;
+    const uint32_t per = c.sub * c.passes, token0 = blockIdx.x / c.slabs * per, n = min(per, a.n_tokens - token0);
     const uint32_t padded = (a.rot.pairs + 7) & ~7u;
-    const uint64_t token0 = (uint64_t)(blockIdx.x / c.slabs) * c.tokens;
-    const uint32_t row0 = blockIdx.x % c.slabs * c.slab, n = (uint32_t)min((uint64_t)c.tokens, a.n_tokens - token0);
-    for (uint32_t i = threadIdx.x; i < n * padded; i += 256) {
-        const uint32_t t = i / padded, pair = i % padded;
-        const uint64_t token = token0 + t, b = token / a.tokens;
-        f32x2 cs = {1.f, 0.f};
-        if (pair < a.rot.pairs) {
-            const int64_t p = a.positions[(int64_t)b * a.pos_st[0] + (int64_t)(token - b * a.tokens) * a.pos_st[1]];
-            cs = cos_sin((uint64_t)p * a.rot.turns[pair], a.rot.magnitude);
-            if (a.inverse) cs.y = -cs.y;
+    if (threadIdx.x < n) {
+        const uint32_t token = token0 + threadIdx.x, b = token / a.tokens, t = token - b * a.tokens;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            s_at[threadIdx.x][2 * x] = ((int64_t)b * a.x[x].in_st[0] + (int64_t)t * a.x[x].in_st[1]) * E::bytes;
+            s_at[threadIdx.x][2 * x + 1] = ((int64_t)b * a.x[x].out_st[0] + (int64_t)t * a.x[x].out_st[1]) * E::bytes;
         }
-        s_cs[i] = cs;
     }
+    make_angles(s_cs, a.rot, n, [&](uint32_t i) {
+        const uint32_t token = token0 + i, b = token / a.tokens;
+        return a.positions[(int64_t)b * a.pos_st[0] + (int64_t)(token - b * a.tokens) * a.pos_st[1]];
+    }, a.inverse);
     __syncthreads();
-    const uint32_t chunk = threadIdx.x & ((1u << c.shift) - 1), turned = (a.rot.pairs + 7) / 8;
-    const uint32_t all = a.x[0].heads + a.x[1].heads;
-    if (chunk >= a.chunks) return;
-    for (uint32_t i = threadIdx.x >> c.shift; i < n * c.slab; i += 256 >> c.shift) {
-        const uint32_t t = by_slab(i, c), r = row0 + (i - t * c.slab);
-        if (r >= all) continue;
-        const bool second = r >= a.x[0].heads;
-        const Heads& x = a.x[second];
-        const uint64_t token = token0 + t, b = token / a.tokens;
-        const int64_t at_b = (int64_t)b, at_t = (int64_t)(token - b * a.tokens), at_h = r - (second ? a.x[0].heads : 0);
-        const uint8_t* in = x.in + (at_b * x.in_st[0] + at_t * x.in_st[1] + at_h * x.in_st[2]) * E::bytes;
-        uint8_t* out = x.out + (at_b * x.out_st[0] + at_t * x.out_st[1] + at_h * x.out_st[2]) * E::bytes;
-        float f[16];
-        if (chunk >= turned) {  // values behind the pairs
-            const uint32_t d = 2 * a.rot.pairs + (chunk - turned) * 16;
-            if (!x.copy) continue;
-            load_some<E, 16>(in + (int64_t)d * E::bytes, a.dim - d, f);
-            store_some<E, 16>(out + (int64_t)d * E::bytes, a.dim - d, f);
+    const Mine me = my_row(c);
+    const uint32_t turned = (a.rot.pairs + 7) / 8, w = me.row >= a.x[0].heads, head = me.row - (w ? a.x[0].heads : 0);
+    if (!me.in || me.lane >= a.chunks || me.row >= a.x[0].heads + a.x[1].heads) return;
+    const bool rest = me.lane >= turned;  // values behind the pairs
+    if (rest && !(w ? a.x[1].copy : a.x[0].copy)) return;
+    const uint32_t pair = me.lane * 8, left = a.rot.pairs - pair, half = a.rot.half;
+    const uint32_t d = rest ? 2 * a.rot.pairs + (me.lane - turned) * 16 : half ? pair : 2 * pair;
+    const uint8_t* const in0 = (w ? a.x[1].in : a.x[0].in) + ((int64_t)head * (w ? a.x[1].in_st[2] : a.x[0].in_st[2]) + d) * E::bytes;
+    uint8_t* const out0 = (w ? a.x[1].out : a.x[0].out) + ((int64_t)head * (w ? a.x[1].out_st[2] : a.x[0].out_st[2]) + d) * E::bytes;
+    for (uint32_t t = me.sub; t < n; t += c.sub) {
+        const uint8_t* const in = in0 + s_at[t][2 * w];
+        uint8_t* const out = out0 + s_at[t][2 * w + 1];
+        float f[16], y[16];
+        if (rest) {
+            load_some<E, 16>(in, a.dim - d, f);
+            store_some<E, 16>(out, a.dim - d, f);
             continue;
         }
-        const uint32_t pair = chunk * 8, left = a.rot.pairs - pair;
-        float y[16];
         const f32x2* cs = s_cs + t * padded + pair;
-        if (a.rot.half) {
-            const int64_t d0 = (int64_t)pair * E::bytes, d1 = (int64_t)(pair + a.rot.half) * E::bytes;
-            load_some<E, 8>(in + d0, left, f), load_some<E, 8>(in + d1, left, f + 8);
+        if (half) {
+            load_some<E, 8>(in, left, f), load_some<E, 8>(in + half * E::bytes, left, f + 8);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 y[k] = turned_first(f[k], f[8 + k], cs[k].x, cs[k].y);
                 y[8 + k] = turned_second(f[k], f[8 + k], cs[k].x, cs[k].y);
             }
-            store_some<E, 8>(out + d0, left, y), store_some<E, 8>(out + d1, left, y + 8);
+            store_some<E, 8>(out, left, y), store_some<E, 8>(out + half * E::bytes, left, y + 8);
         } else {
-            load_some<E, 16>(in + (int64_t)pair * 2 * E::bytes, 2 * left, f);
+            load_some<E, 16>(in, 2 * left, f);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 y[2 * k] = turned_first(f[2 * k], f[2 * k + 1], cs[k].x, cs[k].y);
                 y[2 * k + 1] = turned_second(f[2 * k], f[2 * k + 1], cs[k].x, cs[k].y);
             }
-            store_some<E, 16>(out + (int64_t)pair * 2 * E::bytes, 2 * left, y);
+            store_some<E, 16>(out, 2 * left, y);
         }
     }
 }
 
-// ------------------------------------------------------------ append
+// ------------------------------------------------------------ rows of a cache
 struct AppendArg {
     Rot rot;                   // pairs 0: nothing is turned
     const int32_t* positions;  // of the angles, NULL: the cache's
-    const uint8_t* in[3];      // queries, keys, values
+    uint8_t* x[3];             // queries, keys, values
     uint8_t* q_out;
     int64_t tok[3], head[3], o_tok, o_head;
     uint8_t* cache[2];
@@ -210,133 +218,202 @@ struct AppendArg {
 // The count of chunks that end at or before a token, by all threads at once.
 __device__ __forceinline__ uint32_t seq_of(const KvBatch& b, uint32_t token) {
     uint32_t s = 0;
-    for (uint32_t base = 0; base < b.n_seqs; base += 256) {
+    for (uint32_t base = 0; base < b.n_seqs; base += blockDim.x) {
         const uint32_t i = base + threadIdx.x;
         const int n = __syncthreads_count(i < b.n_seqs && b.offsets[i + 1] <= (int32_t)token);
         s += n;
-        if (n < 256) break;
+        if ((uint32_t)n < blockDim.x) break;
     }
     return s;
 }
-
-// A token's rows are its query heads, its keys' and its values'.  A lane holds 16 values of a
-// row; those of a turned row also load the 16 that they are paired with, which the row's
-// other lanes bring in anyway.
-template <typename X, typename C> __global__ void __launch_bounds__(256) kv_append_kernel(AppendArg a) {
-    extern __shared__ __attribute__((aligned(16))) f32x2 s_cs[];
-    __shared__ int32_t s_page[kMostTokens], s_known[kMostTokens];
-    __shared__ int64_t s_pos[kMostTokens];
-    constexpr bool FOUR = C::tag == CKR_F4;
-    const RowCut& c = a.cut;
-    const uint32_t pairs = a.rot.pairs, half = a.rot.half, padded = (pairs + 7) & ~7u, rot = 2 * pairs;
-    const uint32_t token0 = blockIdx.x / c.slabs * c.tokens, row0 = blockIdx.x % c.slabs * c.slab;
-    const uint32_t n = min(c.tokens, a.b.n_tokens - token0);
-    const uint32_t first = seq_of(a.b, token0);
-    if (threadIdx.x < n) {
-        const uint32_t token = token0 + threadIdx.x;
-        uint32_t seq = first;
-        while (seq < a.b.n_seqs && a.b.offsets[seq + 1] <= (int32_t)token) seq++;
-        int64_t pos = 0;
-        int32_t page = -1;
-        if (seq < a.b.n_seqs) {
-            pos = (int64_t)a.b.starts[seq] + (int64_t)token - a.b.offsets[seq];
-            page = page_of(a.b, seq, pos, a.page_shift, a.n_pages);
-        }
-        s_page[threadIdx.x] = page, s_pos[threadIdx.x] = pos, s_known[threadIdx.x] = seq < a.b.n_seqs;
+// Where a block's tokens lie in the cache.
+struct Places {
+    int64_t row[kMostTokens][2], scale[kMostTokens][2];  // of keys and values: bytes, elements
+    int64_t pos[kMostTokens];
+    int32_t state[kMostTokens];                          // 0: of no sequence, 1: of no page, 2: held
+};
+__device__ __forceinline__ void find_places(const AppendArg& a, uint32_t token0, uint32_t n, Places& p) {
+    uint32_t seq = seq_of(a.b, token0);
+    const uint32_t i = threadIdx.x, token = token0 + i;
+    if (i >= n) return;
+    while (seq < a.b.n_seqs && a.b.offsets[seq + 1] <= (int32_t)token) seq++;
+    int64_t pos = 0;
+    int32_t page = -1;
+    if (seq < a.b.n_seqs) {
+        pos = (int64_t)a.b.starts[seq] + (int64_t)token - a.b.offsets[seq];
+        page = page_of(a.b, seq, pos, a.page_shift, a.n_pages);
     }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n * padded; i += 256) {
-        const uint32_t t = i / padded, pair = i % padded;
-        const int64_t p = a.positions ? a.positions[token0 + t] : s_pos[t];
-        s_cs[i] = pair < pairs ? cos_sin((uint64_t)p * a.rot.turns[pair], a.rot.magnitude) : f32x2{1.f, 0.f};
-    }
-    __syncthreads();
-    const uint32_t lanes = 1u << c.shift, lane = threadIdx.x & (lanes - 1), d = lane * 16, all = a.q_heads + 2 * a.heads;
-    for (uint32_t i0 = 0; i0 < n * c.slab; i0 += 256 >> c.shift) {  // every lane, for the rows' maxima
-        const uint32_t i = i0 + (threadIdx.x >> c.shift), t = by_slab(i, c), r = row0 + (i - t * c.slab);
-        const bool in = i < n * c.slab && r < all && d < a.dim;
-        const uint32_t kind = r < a.q_heads ? 0 : r < a.q_heads + a.heads ? 1 : 2;
-        const uint32_t h = r - (kind == 0 ? 0 : kind == 1 ? a.q_heads : a.q_heads + a.heads), tt = in ? t : 0;
-        const bool mine = in && s_known[tt];
-        float f[16];
+    const int64_t slot = (uint32_t)pos & ((1u << a.page_shift) - 1);
 #pragma unroll
-        for (int k = 0; k < 16; k++) f[k] = 0.f;
-        if (mine) {
-            const uint8_t* row = (kind == 0 ? a.in[0] : kind == 1 ? a.in[1] : a.in[2]) +
-                                 ((int64_t)(token0 + t) * (kind == 0 ? a.tok[0] : kind == 1 ? a.tok[1] : a.tok[2]) +
-                                  (int64_t)h * (kind == 0 ? a.head[0] : kind == 1 ? a.head[1] : a.head[2])) * X::bytes;
-            load_vec<X, 16>(row + d * X::bytes, f);
-            if (kind < 2 && d < rot) {
-                const f32x2* cs = s_cs + t * padded;
+    for (int v = 0; v < 2; v++) {
+        p.row[i][v] = (int64_t)page * a.st[v][0] + slot * a.st[v][2];
+        p.scale[i][v] = (int64_t)page * a.sst[v][0] + slot;
+    }
+    p.pos[i] = pos, p.state[i] = seq >= a.b.n_seqs ? 0 : page < 0 ? 1 : 2;
+}
+
+// A token's rows are its query heads, its keys' and its values'.  A lane holds 8 values of a
+// row and 8 that lie 8 times the row's lanes behind them, so that loads and stores are whole lines, and for
+// heads of 64, 128 and 256 dimensions that are turned as a whole, halves apart, both of its pairs; else those
+// of a turned row also load the values that they are paired with, which the row's other lanes bring
+// in anyway.  A row's lanes are of one wave, whose loads of a row come before its stores, so that queries
+// may be turned in place.
+template <typename X, typename C> __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendArg a) {
+    extern __shared__ __attribute__((aligned(16))) f32x2 s_cs[];
+    __shared__ Places s_p;
+    const RowCut& c = a.cut;
+    const uint32_t per = c.sub * c.passes, token0 = blockIdx.x / c.slabs * per, n = min(per, a.b.n_tokens - token0);
+    const uint32_t pairs = a.rot.pairs, half = a.rot.half, padded = (pairs + 7) & ~7u, rot = 2 * pairs;
+    find_places(a, token0, n, s_p);
+    __syncthreads();
+    if (pairs) {
+        make_angles(s_cs, a.rot, n, [&](uint32_t t) { return a.positions ? a.positions[token0 + t] : s_p.pos[t]; }, false);
+        __syncthreads();
+    }
+    const Mine me = my_row(c);
+    const uint32_t lanes = 1u << c.shift, kind = me.row < a.q_heads ? 0 : me.row < a.q_heads + a.heads ? 1 : 2, v = kind == 2;
+    const uint32_t h = me.row - (kind == 0 ? 0 : kind == 1 ? a.q_heads : a.q_heads + a.heads);
+    if (!me.in || me.row >= a.q_heads + 2 * a.heads) return;  // whole rows of lanes
+    const auto of = [&](const auto* x) { return kind == 0 ? x[0] : kind == 1 ? x[1] : x[2]; };
+    const uint32_t d0 = me.lane * 8, dist = lanes * 8;
+    const bool in0 = d0 < a.dim, in1 = d0 + dist < a.dim, paired = half == dist && rot == a.dim && kind < 2, apart = half && half % 8 == 0;
+    const int64_t tok = of(a.tok) * X::bytes;
+    const uint8_t* row = of(a.x) + (int64_t)(token0 + me.sub) * tok + (int64_t)h * of(a.head) * X::bytes;
+    uint8_t* q_out = a.q_out + ((int64_t)(token0 + me.sub) * a.o_tok + (int64_t)h * a.o_head + d0) * X::bytes;
+    const int64_t step = tok * c.sub, q_step = a.o_tok * c.sub * X::bytes;
+    uint8_t* const cache = (v ? a.cache[1] : a.cache[0]) + (int64_t)h * (v ? a.st[1][1] : a.st[0][1]) + bytes_of<C>(d0);
+    const int64_t s_head = (int64_t)h * (v ? a.sst[1][1] : a.sst[0][1]);
+    for (uint32_t t = me.sub; t < n; t += c.sub, row += step, q_out += q_step) {
+        const int32_t state = s_p.state[t];
+        float f[2][8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) f[0][k] = f[1][k] = 0.f;
+        if (state && in0) load_vec<X, 8>(row + d0 * X::bytes, f[0]);
+        if (state && in1) load_vec<X, 8>(row + (d0 + dist) * X::bytes, f[1]);
+        const f32x2* const cs = s_cs + t * padded;
+        if (paired) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const f32x2 w = cs[d0 + k];
+                const float x = f[0][k], y = f[1][k];
+                f[0][k] = turned_first(x, y, w.x, w.y), f[1][k] = turned_second(x, y, w.x, w.y);
+            }
+        } else if (kind < 2 && state) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const uint32_t d = d0 + u * dist;
+                if (d >= rot) continue;
                 if (!half) {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
+                    for (int k = 0; k < 4; k++) {
                         if (d / 2 + k < pairs) {
                             const f32x2 w = cs[d / 2 + k];
-                            const float x = f[2 * k], y = f[2 * k + 1];
-                            f[2 * k] = turned_first(x, y, w.x, w.y), f[2 * k + 1] = turned_second(x, y, w.x, w.y);
+                            const float x = f[u][2 * k], y = f[u][2 * k + 1];
+                            f[u][2 * k] = turned_first(x, y, w.x, w.y), f[u][2 * k + 1] = turned_second(x, y, w.x, w.y);
                         }
                     }
-                } else if (half % 8 == 0) {  // 8 values lie on one side of the pairs
+                } else if (apart) {  // 8 values lie on one side of the pairs
+                    const bool low = d < half;
+                    float p[8];
+                    load_vec<X, 8, false>(row + (low ? d + half : d - half) * X::bytes, p);
 #pragma unroll
-                    for (int u = 0; u < 16; u += 8) {
-                        const uint32_t e = d + u;
-                        if (e >= rot) continue;
-                        const bool low = e < half;
-                        const uint32_t pair = low ? e : e - half;
-                        float p[8];
-                        load_vec<X, 8, false>(row + (low ? e + half : e - half) * X::bytes, p);
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const f32x2 w = cs[pair + k];
-                            f[u + k] = low ? turned_first(f[u + k], p[k], w.x, w.y) : turned_second(p[k], f[u + k], w.x, w.y);
-                        }
+                    for (int k = 0; k < 8; k++) {
+                        const f32x2 w = cs[(low ? d : d - half) + k];
+                        f[u][k] = low ? turned_first(f[u][k], p[k], w.x, w.y) : turned_second(p[k], f[u][k], w.x, w.y);
                     }
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 16; k++) {
+                    for (int k = 0; k < 8; k++) {
                         const uint32_t e = d + k;
                         if (e >= rot) continue;
-                        const bool low = e < half;
-                        const float p = load_one<X>(row, low ? e + half : e - half);
-                        const f32x2 w = cs[low ? e : e - half];
-                        f[k] = low ? turned_first(f[k], p, w.x, w.y) : turned_second(p, f[k], w.x, w.y);
+                        const float p = load_one<X>(row, e < half ? e + half : e - half);
+                        const f32x2 w = cs[e < half ? e : e - half];
+                        f[u][k] = e < half ? turned_first(f[u][k], p, w.x, w.y) : turned_second(p, f[u][k], w.x, w.y);
                     }
                 }
             }
         }
-        // ---- a query's row goes out as it is, others into the cache
-        const int32_t page = s_page[tt];
-        const uint32_t slot = (uint32_t)s_pos[tt] & ((1u << a.page_shift) - 1), v = kind == 2;
-        const bool held = mine && kind > 0 && page >= 0;
-        uint8_t* to = a.cache[v] + (int64_t)page * a.st[v][0] + (int64_t)h * a.st[v][1] + (int64_t)slot * a.st[v][2] + bytes_of<C>(d);
-        const int64_t s_at = (int64_t)page * a.sst[v][0] + (int64_t)h * a.sst[v][1] + slot;
-        if (mine && kind == 0) store_vec<X, 16>(a.q_out + ((int64_t)(token0 + t) * a.o_tok + (int64_t)h * a.o_head + d) * X::bytes, f);
-        if constexpr (FOUR) {
-            const uint32_t byte = group_byte_of<16>(f);
-            if (held) {
-                *reinterpret_cast<u32x2*>(to) = u32x2{encode8(f, byte), encode8(f + 8, byte)};
-                if (lane % 2 == 0) static_cast<uint8_t*>(a.scales[v])[s_at + ((int64_t)(d / kGroup) << a.page_shift)] = (uint8_t)byte;
+        // a query's row goes out as it is, others into the cache
+        if (kind == 0) {
+            if (state && in0) store_vec<X, 8>(q_out, f[0]);
+            if (state && in1) store_vec<X, 8>(q_out + dist * X::bytes, f[1]);
+            continue;
+        }
+        const bool held = state == 2;
+        uint8_t* const to = cache + s_p.row[t][v];
+        const int64_t s_at = s_head + s_p.scale[t][v];
+        if constexpr (C::tag == CKR_F4) {
+            uint8_t* const bytes = static_cast<uint8_t*>(v ? a.scales[1] : a.scales[0]) + s_at;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const uint32_t d = d0 + u * dist, byte = group_byte_of(f[u]);
+                if (held && (u ? in1 : in0)) {
+                    *reinterpret_cast<uint32_t*>(to + u * dist / 2) = encode8(f[u], byte);
+                    if (me.lane % 4 == 0) bytes[(int64_t)(d / kGroup) << a.page_shift] = (uint8_t)byte;
+                }
             }
         } else {
             if constexpr (C::bytes == 1) {
                 uint32_t top = 0;
 #pragma unroll
-                for (int k = 0; k < 16; k++) top = max(top, abs_bits(f[k]));
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) top = max(top, abs_bits(f[u][k]));
                 for (uint32_t e = 1; e < lanes; e *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, (int)e));
                 const RowScale rs = row_scale<C>(top);
 #pragma unroll
-                for (int k = 0; k < 16; k++) f[k] = scaled(f[k], rs.inv);
-                if (held && lane == 0) static_cast<float*>(a.scales[v])[s_at] = rs.scale;
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) f[u][k] = scaled(f[u][k], rs.inv);
+                if (held && me.lane == 0) static_cast<float*>(v ? a.scales[1] : a.scales[0])[s_at] = rs.scale;
             }
-            if (held) store_vec<C, 16>(to, f);
+            if (held && in0) store_vec<C, 8>(to, f[0]);
+            if (held && in1) store_vec<C, 8>(to + dist * C::bytes, f[1]);
+        }
+    }
+}
+
+// A cache of 4 bits read back: the same rows (no queries), the other way round.
+template <typename X> __global__ void __launch_bounds__(kThreads) kv_read_four_kernel(AppendArg a) {
+    __shared__ Places s_p;
+    const RowCut& c = a.cut;
+    const uint32_t per = c.sub * c.passes, token0 = blockIdx.x / c.slabs * per, n = min(per, a.b.n_tokens - token0);
+    find_places(a, token0, n, s_p);
+    __syncthreads();
+    const Mine me = my_row(c);
+    const uint32_t v = me.row >= a.heads, h = me.row - (v ? a.heads : 0), d0 = me.lane * 8, dist = 8u << c.shift;
+    if (!me.in || me.row >= 2 * a.heads || d0 >= a.dim) return;
+    const bool in1 = d0 + dist < a.dim;
+    const int64_t tok = (v ? a.tok[2] : a.tok[1]) * X::bytes, step = tok * c.sub;
+    uint8_t* out = (v ? a.x[2] : a.x[1]) + (int64_t)(token0 + me.sub) * tok + ((int64_t)h * (v ? a.head[2] : a.head[1]) + d0) * X::bytes;
+    const uint8_t* const codes = (v ? a.cache[1] : a.cache[0]) + (int64_t)h * (v ? a.st[1][1] : a.st[0][1]) + d0 / 2;
+    const uint8_t* const bytes = static_cast<const uint8_t*>(v ? a.scales[1] : a.scales[0]) + (int64_t)h * (v ? a.sst[1][1] : a.sst[0][1]) +
+                                 ((int64_t)(d0 / kGroup) << a.page_shift);
+    for (uint32_t t = me.sub; t < n; t += c.sub, out += step) {
+        uint32_t x[2] = {0, 0}, b[2] = {0, 0};
+        if (s_p.state[t] == 2) {
+            const uint8_t* at = codes + s_p.row[t][v];
+            const uint8_t* bt = bytes + s_p.scale[t][v];
+            x[0] = *reinterpret_cast<const uint32_t*>(at), b[0] = *bt;
+            if (in1) x[1] = *reinterpret_cast<const uint32_t*>(at + dist / 2), b[1] = bt[(int64_t)(dist / kGroup) << a.page_shift];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (u && !in1) break;
+            if constexpr (X::bytes == 2) {
+                *reinterpret_cast<u32x4*>(out + u * dist * X::bytes) = widen8<X>(x[u], power_of(b[u]));
+            } else {
+                float f[8];
+                decode8(x[u], power_of(b[u]), f);
+                store_vec<X, 8>(out + u * dist * X::bytes, f);
+            }
         }
     }
 }
 
 template <typename X> hipError_t launch_append(const AppendArg& a, int cache_dtype, uint32_t lds, hipStream_t s) {
     const auto go = [&](auto kernel) {
-        CKR_LAUNCH("kv_append", s, kernel<<<dim3((uint32_t)a.cut.blocks), 256, lds, s>>>(a));
+        CKR_LAUNCH("kv_append", s, kernel<<<dim3((uint32_t)a.cut.blocks), a.cut.threads, lds, s>>>(a));
         return hipGetLastError();
     };
     switch (cache_dtype) {
@@ -346,6 +423,20 @@ template <typename X> hipError_t launch_append(const AppendArg& a, int cache_dty
         case CKR_BF16: return go(kv_append_kernel<X, ElemBF16>);
         default: return go(kv_append_kernel<X, ElemF16>);
     }
+}
+
+// The cache's and the batch's part, and the cut (after the rows').
+void set_cache(AppendArg& a, const ckr_kv_cache* cache, const ckr_kv_batch* batch) {
+    a.cache[0] = static_cast<uint8_t*>(cache->d_k), a.cache[1] = static_cast<uint8_t*>(cache->d_v);
+    a.scales[0] = cache->d_k_scale, a.scales[1] = cache->d_v_scale;
+    const int ces = cache->dtype == CKR_BF16 || cache->dtype == CKR_F16 ? 2 : 1;  // of a stride's unit
+    for (int i = 0; i < 3; i++) a.st[0][i] = cache->k_stride[i] * ces, a.st[1][i] = cache->v_stride[i] * ces;
+    for (int i = 0; i < 2; i++) a.sst[0][i] = cache->k_scale_stride[i], a.sst[1][i] = cache->v_scale_stride[i];
+    a.n_pages = cache->n_pages, a.page_shift = (uint32_t)__builtin_ctz(cache->page_size);
+    a.heads = cache->n_heads, a.dim = cache->head_dim;
+    a.b = {batch->d_page_table, batch->d_starts, batch->d_offsets, (int64_t)batch->table_stride, batch->table_width,
+           batch->n_seqs, batch->n_tokens};
+    a.cut = row_cut(batch->n_tokens, a.q_heads + 2ull * a.heads, std::max((a.dim / 8 + 1) / 2, 4u), a.rot.pairs);
 }
 
 inline bool multiple(const void* p, uint64_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -362,6 +453,23 @@ int check_rotary(const ckr_rotary* r, uint32_t dim, Rot& rot) {
 }
 
 }  // namespace
+
+// ckr_kv_read of a cache of 4 bits, whose arguments have been checked.
+int kv_read_four(const ckr_kv_cache* c, const ckr_kv_batch* b, void* k, int64_t kt, int64_t kh, void* v, int64_t vt, int64_t vh,
+                 int dtype, void* stream) {
+    AppendArg a{};
+    a.x[1] = static_cast<uint8_t*>(k), a.x[2] = static_cast<uint8_t*>(v);
+    a.tok[1] = kt, a.tok[2] = vt, a.head[1] = kh, a.head[2] = vh;
+    set_cache(a, c, b);
+    if (a.cut.blocks > kMostBlocks) return err(CKR_E_INVALID, "the batch is too large for one launch");
+    const hipStream_t s = (hipStream_t)stream;
+    const auto go = [&](auto kernel) { CKR_LAUNCH("kv_read", s, kernel<<<dim3((uint32_t)a.cut.blocks), a.cut.threads, 0, s>>>(a)); };
+    if (dtype == CKR_F32) go(kv_read_four_kernel<ElemF32>);
+    else if (dtype == CKR_BF16) go(kv_read_four_kernel<ElemBF16>);
+    else go(kv_read_four_kernel<ElemF16>);
+    return hip_rc(hipGetLastError(), "kv_read");
+}
+
 }  // namespace ckr
 
 using namespace ckr;
@@ -391,14 +499,14 @@ int ckr_rotate(const ckr_rotary* rotary, const int32_t* d_positions, const int64
     RotateArg a{};
     int rc;
     if ((rc = check_rotary(rotary, head_dim, a.rot))) return rc;
-    a.n_tokens = (uint64_t)batch * tokens;
+    const uint64_t n_tokens = (uint64_t)batch * tokens;
     uint64_t rows = 0;
     for (uint32_t i = 0; i < n; i++) {
         if (heads[i].n_heads > 65535) return err(CKR_E_INVALID, "at most 65535 heads");
         rows += heads[i].n_heads;
     }
-    if (a.n_tokens * rows > 0x7fffffffull) return err(CKR_E_INVALID, "at most 2^31 - 1 rows (tokens x heads)");
-    if (a.n_tokens == 0 || rows == 0) return CKR_OK;
+    if (n_tokens > 0x7fffffffull || n_tokens * rows > 0x7fffffffull) return err(CKR_E_INVALID, "at most 2^31 - 1 rows (tokens x heads)");
+    if (n_tokens == 0 || rows == 0) return CKR_OK;
     if (!d_positions) return err(CKR_E_INVALID, "null positions pointer");
     if (!multiple(d_positions, 4)) return err(CKR_E_INVALID, "positions must be aligned to 4 bytes");
     const int es = ckr_element_size(dtype);
@@ -449,13 +557,13 @@ int ckr_rotate(const ckr_rotary* rotary, const int32_t* d_positions, const int64
         y.copy = x.d_in != x.d_out && 2 * a.rot.pairs < head_dim;
         copy = copy || y.copy;
     }
-    a.tokens = tokens, a.dim = head_dim, a.inverse = inverse != 0;
+    a.n_tokens = (uint32_t)n_tokens, a.tokens = tokens, a.dim = head_dim, a.inverse = inverse != 0;
     a.chunks = (a.rot.pairs + 7) / 8 + (copy ? (head_dim - 2 * a.rot.pairs + 15) / 16 : 0);
-    a.cut = row_cut(a.n_tokens, rows, a.chunks);
+    a.cut = row_cut(n_tokens, rows, a.chunks, a.rot.pairs);
     if (a.cut.blocks > kMostBlocks) return err(CKR_E_INVALID, "the heads are too many for one launch");
-    const uint32_t lds = a.cut.tokens * ((a.rot.pairs + 7) / 8 * 8) * 8;
+    const uint32_t lds = a.cut.sub * a.cut.passes * ((a.rot.pairs + 7) / 8 * 8) * 8;
     const hipStream_t s = (hipStream_t)stream;
-    const auto go = [&](auto kernel) { CKR_LAUNCH("rotate", s, kernel<<<dim3((uint32_t)a.cut.blocks), 256, lds, s>>>(a)); };
+    const auto go = [&](auto kernel) { CKR_LAUNCH("rotate", s, kernel<<<dim3((uint32_t)a.cut.blocks), a.cut.threads, lds, s>>>(a)); };
     if (dtype == CKR_F32) go(rotate_kernel<ElemF32>);
     else if (dtype == CKR_BF16) go(rotate_kernel<ElemBF16>);
     else go(rotate_kernel<ElemF16>);
@@ -492,23 +600,14 @@ int ckr_kv_append(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const ck
         if ((rc = check_range(d_positions, (uint64_t)T * 4, "positions"))) return rc;
     }
     a.positions = d_positions;
-    a.in[0] = static_cast<const uint8_t*>(d_q), a.in[1] = static_cast<const uint8_t*>(d_k), a.in[2] = static_cast<const uint8_t*>(d_v);
+    a.x[0] = static_cast<uint8_t*>(const_cast<void*>(d_q)), a.x[1] = static_cast<uint8_t*>(const_cast<void*>(d_k)), a.x[2] = static_cast<uint8_t*>(const_cast<void*>(d_v));
     a.q_out = static_cast<uint8_t*>(d_out);
     a.tok[0] = q_token_stride, a.tok[1] = k_token_stride, a.tok[2] = v_token_stride;
     a.head[0] = q_head_stride, a.head[1] = k_head_stride, a.head[2] = v_head_stride;
-    a.o_tok = out_token_stride, a.o_head = out_head_stride;
-    a.cache[0] = static_cast<uint8_t*>(cache->d_k), a.cache[1] = static_cast<uint8_t*>(cache->d_v);
-    a.scales[0] = cache->d_k_scale, a.scales[1] = cache->d_v_scale;
-    const int ces = cache->dtype == CKR_BF16 || cache->dtype == CKR_F16 ? 2 : 1;  // of a stride's unit
-    for (int i = 0; i < 3; i++) a.st[0][i] = cache->k_stride[i] * ces, a.st[1][i] = cache->v_stride[i] * ces;
-    for (int i = 0; i < 2; i++) a.sst[0][i] = cache->k_scale_stride[i], a.sst[1][i] = cache->v_scale_stride[i];
-    a.n_pages = cache->n_pages, a.page_shift = (uint32_t)__builtin_ctz(cache->page_size);
-    a.q_heads = n_heads, a.heads = cache->n_heads, a.dim = D;
-    a.b = {batch->d_page_table, batch->d_starts, batch->d_offsets, (int64_t)batch->table_stride, batch->table_width,
-           batch->n_seqs, batch->n_tokens};
-    a.cut = row_cut(T, n_heads + 2ull * cache->n_heads, D / 16);
+    a.o_tok = out_token_stride, a.o_head = out_head_stride, a.q_heads = n_heads;
+    set_cache(a, cache, batch);
     if (a.cut.blocks > kMostBlocks) return err(CKR_E_INVALID, "the batch is too large for one launch");
-    const uint32_t lds = a.cut.tokens * ((a.rot.pairs + 7) / 8 * 8) * 8;
+    const uint32_t lds = a.cut.sub * a.cut.passes * ((a.rot.pairs + 7) / 8 * 8) * 8;
     const hipStream_t s = (hipStream_t)stream;
     const hipError_t e = dtype == CKR_F32    ? launch_append<ElemF32>(a, cache->dtype, lds, s)
                          : dtype == CKR_BF16 ? launch_append<ElemBF16>(a, cache->dtype, lds, s)
