@@ -77,7 +77,7 @@ struct RowCut {
     uint32_t threads;
     uint64_t blocks;
 };
-RowCut row_cut(uint64_t tokens, uint64_t rows, uint32_t lanes, uint32_t pairs) {
+RowCut row_cut(uint64_t tokens, uint64_t rows, uint32_t lanes, uint32_t pairs, uint32_t passes) {
     RowCut c{};
     while ((1u << c.shift) < lanes) c.shift++;
     c.slabs = (uint32_t)(((rows << c.shift) + kThreads - 1) / kThreads);
@@ -85,8 +85,9 @@ RowCut row_cut(uint64_t tokens, uint64_t rows, uint32_t lanes, uint32_t pairs) {
     const uint32_t most = std::min(kMostTokens, kMostAngles / std::max((pairs + 7) / 8 * 64, 1u));
     c.sub = std::clamp(256u / (c.slab << c.shift), 1u, most);
     c.threads = ((c.sub * c.slab << c.shift) + 63) / 64 * 64;
-    // one after another where there are blocks enough all the same: they share the look-ups and angles
-    c.passes = (uint32_t)std::clamp<uint64_t>(tokens * c.slabs / c.sub / 2048, 1, std::min(8u, most / c.sub));
+    // one after another where there are blocks enough all the same: they share the look-ups and angles, and
+    // the lines that neighbouring tokens' scales lie in
+    c.passes = (uint32_t)std::clamp<uint64_t>(tokens * c.slabs / c.sub / 2048, 1, std::min(passes, most / c.sub));
     c.blocks = (tokens + c.sub * c.passes - 1) / (c.sub * c.passes) * c.slabs;
     return c;
 }
@@ -123,6 +124,18 @@ struct RotateArg {
     uint32_t tokens, dim, chunks, inverse;
     RowCut cut;
 };
+
+// Eight values as they lie in memory (at any address), and unpacked: rows of several tokens are
+// loaded before the first of them is used.
+template <typename E> struct Raw {
+    typename Vecs<false>::U4 v[E::bytes / 2];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+#pragma unroll
+        for (int i = 0; i < E::bytes / 2; i++) v[i] = reinterpret_cast<const typename Vecs<false>::U4*>(p)[i];
+    }
+    __device__ __forceinline__ void get(float* x) const { load_vec<E, 8, false>(&v, x); }
+};
+template <typename E> constexpr int kAhead = E::bytes == 2 ? 4 : 2;  // tokens whose rows are loaded at once
 
 template <typename E, int N> __device__ __forceinline__ void load_some(const uint8_t* p, uint32_t n, float* x) {
     if (n >= N) {
@@ -166,22 +179,20 @@ template <typename E> __global__ void __launch_bounds__(kThreads) rotate_kernel(
     if (!me.in || me.lane >= a.chunks || me.row >= a.x[0].heads + a.x[1].heads) return;
     const bool rest = me.lane >= turned;  // values behind the pairs
     if (rest && !(w ? a.x[1].copy : a.x[0].copy)) return;
-    const uint32_t pair = me.lane * 8, left = a.rot.pairs - pair, half = a.rot.half;
-    const uint32_t d = rest ? 2 * a.rot.pairs + (me.lane - turned) * 16 : half ? pair : 2 * pair;
+    // 8 pairs, or 16 values behind them: the last ones end with the row (some are then done twice, alike,
+    // by lanes of one wave, whose loads come before their stores), `left` of them where a row has fewer
+    const uint32_t half = a.rot.half, behind = a.dim - 2 * a.rot.pairs, at = (me.lane - (rest ? turned : 0)) * (rest ? 16 : 8);
+    const uint32_t all = rest ? behind : a.rot.pairs, size = rest ? 16 : 8;
+    const bool back = all >= size && c.shift <= 6;
+    const uint32_t pair = back ? min(at, all - size) : at, left = all - pair;
+    const uint32_t d = rest ? 2 * a.rot.pairs + pair : half ? pair : 2 * pair;
     const uint8_t* const in0 = (w ? a.x[1].in : a.x[0].in) + ((int64_t)head * (w ? a.x[1].in_st[2] : a.x[0].in_st[2]) + d) * E::bytes;
     uint8_t* const out0 = (w ? a.x[1].out : a.x[0].out) + ((int64_t)head * (w ? a.x[1].out_st[2] : a.x[0].out_st[2]) + d) * E::bytes;
-    for (uint32_t t = me.sub; t < n; t += c.sub) {
-        const uint8_t* const in = in0 + s_at[t][2 * w];
-        uint8_t* const out = out0 + s_at[t][2 * w + 1];
-        float f[16], y[16];
-        if (rest) {
-            load_some<E, 16>(in, a.dim - d, f);
-            store_some<E, 16>(out, a.dim - d, f);
-            continue;
-        }
+    const auto put = [&](uint32_t t, const float* f) {
+        float y[16];
         const f32x2* cs = s_cs + t * padded + pair;
+        uint8_t* const out = out0 + s_at[t][2 * w + 1];
         if (half) {
-            load_some<E, 8>(in, left, f), load_some<E, 8>(in + half * E::bytes, left, f + 8);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 y[k] = turned_first(f[k], f[8 + k], cs[k].x, cs[k].y);
@@ -189,13 +200,44 @@ template <typename E> __global__ void __launch_bounds__(kThreads) rotate_kernel(
             }
             store_some<E, 8>(out, left, y), store_some<E, 8>(out + half * E::bytes, left, y + 8);
         } else {
-            load_some<E, 16>(in, 2 * left, f);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 y[2 * k] = turned_first(f[2 * k], f[2 * k + 1], cs[k].x, cs[k].y);
                 y[2 * k + 1] = turned_second(f[2 * k], f[2 * k + 1], cs[k].x, cs[k].y);
             }
             store_some<E, 16>(out, 2 * left, y);
+        }
+    };
+    if (left < size) {
+        for (uint32_t t = me.sub; t < n; t += c.sub) {
+            const uint8_t* const in = in0 + s_at[t][2 * w];
+            float f[16];
+            if (rest) {
+                load_some<E, 16>(in, left, f);
+                store_some<E, 16>(out0 + s_at[t][2 * w + 1], left, f);
+            } else {
+                if (half) load_some<E, 8>(in, left, f), load_some<E, 8>(in + half * E::bytes, left, f + 8);
+                else load_some<E, 16>(in, 2 * left, f);
+                put(t, f);
+            }
+        }
+        return;
+    }
+    const uint32_t second = (half && !rest ? half : 8) * E::bytes;
+    for (uint32_t t = me.sub; t < n; t += kAhead<E> * c.sub) {
+        Raw<E> x[kAhead<E>][2];
+#pragma unroll
+        for (int u = 0; u < kAhead<E>; u++) {  // behind the last token it once more
+            const uint8_t* const in = in0 + s_at[min(t + u * c.sub, n - 1)][2 * w];
+            x[u][0].load(in), x[u][1].load(in + second);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead<E>; u++) {
+            if (t + u * c.sub >= n) break;
+            float f[16];
+            x[u][0].get(f), x[u][1].get(f + 8);
+            if (rest) store_vec<E, 16, false>(out0 + s_at[t + u * c.sub][2 * w + 1], f);
+            else put(t + u * c.sub, f);
         }
     }
 }
@@ -246,8 +288,8 @@ __device__ __forceinline__ void find_places(const AppendArg& a, uint32_t token0,
     const int64_t slot = (uint32_t)pos & ((1u << a.page_shift) - 1);
 #pragma unroll
     for (int v = 0; v < 2; v++) {
-        p.row[i][v] = (int64_t)page * a.st[v][0] + slot * a.st[v][2];
-        p.scale[i][v] = (int64_t)page * a.sst[v][0] + slot;
+        p.row[i][v] = (int64_t)max(page, 0) * a.st[v][0] + slot * a.st[v][2];
+        p.scale[i][v] = (int64_t)max(page, 0) * a.sst[v][0] + slot;
     }
     p.pos[i] = pos, p.state[i] = seq >= a.b.n_seqs ? 0 : page < 0 ? 1 : 2;
 }
@@ -278,18 +320,30 @@ template <typename X, typename C> __global__ void __launch_bounds__(kThreads) kv
     const uint32_t d0 = me.lane * 8, dist = lanes * 8;
     const bool in0 = d0 < a.dim, in1 = d0 + dist < a.dim, paired = half == dist && rot == a.dim && kind < 2, apart = half && half % 8 == 0;
     const int64_t tok = of(a.tok) * X::bytes;
-    const uint8_t* row = of(a.x) + (int64_t)(token0 + me.sub) * tok + (int64_t)h * of(a.head) * X::bytes;
-    uint8_t* q_out = a.q_out + ((int64_t)(token0 + me.sub) * a.o_tok + (int64_t)h * a.o_head + d0) * X::bytes;
-    const int64_t step = tok * c.sub, q_step = a.o_tok * c.sub * X::bytes;
+    const uint8_t* const row0 = of(a.x) + (int64_t)token0 * tok + (int64_t)h * of(a.head) * X::bytes;
+    uint8_t* const q_out0 = a.q_out + ((int64_t)token0 * a.o_tok + (int64_t)h * a.o_head + d0) * X::bytes;
+    const int64_t q_tok = a.o_tok * X::bytes;
+    const uint32_t l0 = in0 ? d0 : 0, l1 = in1 ? d0 + dist : l0;
     uint8_t* const cache = (v ? a.cache[1] : a.cache[0]) + (int64_t)h * (v ? a.st[1][1] : a.st[0][1]) + bytes_of<C>(d0);
     const int64_t s_head = (int64_t)h * (v ? a.sst[1][1] : a.sst[0][1]);
-    for (uint32_t t = me.sub; t < n; t += c.sub, row += step, q_out += q_step) {
+    for (uint32_t tt = me.sub; tt < n; tt += kAhead<X> * c.sub) {
+    Raw<X> raw[kAhead<X>][2];
+#pragma unroll
+    for (int u = 0; u < kAhead<X>; u++) {  // behind the last token it once more
+        const uint8_t* const row = row0 + (int64_t)min(tt + u * c.sub, n - 1) * tok;
+        raw[u][0].load(row + l0 * X::bytes), raw[u][1].load(row + l1 * X::bytes);
+    }
+#pragma unroll
+    for (int ahead = 0; ahead < kAhead<X>; ahead++) {
+        const uint32_t t = tt + ahead * c.sub;
+        if (t >= n) break;
+        const uint8_t* const row = row0 + (int64_t)t * tok;
+        uint8_t* const q_out = q_out0 + (int64_t)t * q_tok;
         const int32_t state = s_p.state[t];
         float f[2][8];
+        raw[ahead][0].get(f[0]), raw[ahead][1].get(f[1]);
 #pragma unroll
-        for (int k = 0; k < 8; k++) f[0][k] = f[1][k] = 0.f;
-        if (state && in0) load_vec<X, 8>(row + d0 * X::bytes, f[0]);
-        if (state && in1) load_vec<X, 8>(row + (d0 + dist) * X::bytes, f[1]);
+        for (int k = 0; k < 8; k++) f[0][k] = in0 ? f[0][k] : 0.f, f[1][k] = in1 ? f[1][k] : 0.f;
         const f32x2* const cs = s_cs + t * padded;
         if (paired) {
 #pragma unroll
@@ -371,6 +425,7 @@ template <typename X, typename C> __global__ void __launch_bounds__(kThreads) kv
             if (held && in1) store_vec<C, 8>(to + dist * C::bytes, f[1]);
         }
     }
+    }
 }
 
 // A cache of 4 bits read back: the same rows (no queries), the other way round.
@@ -384,28 +439,40 @@ template <typename X> __global__ void __launch_bounds__(kThreads) kv_read_four_k
     const uint32_t v = me.row >= a.heads, h = me.row - (v ? a.heads : 0), d0 = me.lane * 8, dist = 8u << c.shift;
     if (!me.in || me.row >= 2 * a.heads || d0 >= a.dim) return;
     const bool in1 = d0 + dist < a.dim;
-    const int64_t tok = (v ? a.tok[2] : a.tok[1]) * X::bytes, step = tok * c.sub;
-    uint8_t* out = (v ? a.x[2] : a.x[1]) + (int64_t)(token0 + me.sub) * tok + ((int64_t)h * (v ? a.head[2] : a.head[1]) + d0) * X::bytes;
+    const int64_t tok = (v ? a.tok[2] : a.tok[1]) * X::bytes;
+    uint8_t* const out0 = (v ? a.x[2] : a.x[1]) + (int64_t)token0 * tok + ((int64_t)h * (v ? a.head[2] : a.head[1]) + d0) * X::bytes;
     const uint8_t* const codes = (v ? a.cache[1] : a.cache[0]) + (int64_t)h * (v ? a.st[1][1] : a.st[0][1]) + d0 / 2;
     const uint8_t* const bytes = static_cast<const uint8_t*>(v ? a.scales[1] : a.scales[0]) + (int64_t)h * (v ? a.sst[1][1] : a.sst[0][1]) +
                                  ((int64_t)(d0 / kGroup) << a.page_shift);
-    for (uint32_t t = me.sub; t < n; t += c.sub, out += step) {
-        uint32_t x[2] = {0, 0}, b[2] = {0, 0};
-        if (s_p.state[t] == 2) {
+    const uint32_t next = in1 ? dist / 2 : 0, next_b = in1 ? dist / kGroup << a.page_shift : 0;
+    constexpr int AHEAD = 4;
+    for (uint32_t tt = me.sub; tt < n; tt += AHEAD * c.sub) {
+        uint32_t x[AHEAD][2], b[AHEAD][2];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {  // behind the last token it once more
+            const uint32_t t = min(tt + u * c.sub, n - 1);
             const uint8_t* at = codes + s_p.row[t][v];
             const uint8_t* bt = bytes + s_p.scale[t][v];
-            x[0] = *reinterpret_cast<const uint32_t*>(at), b[0] = *bt;
-            if (in1) x[1] = *reinterpret_cast<const uint32_t*>(at + dist / 2), b[1] = bt[(int64_t)(dist / kGroup) << a.page_shift];
+            x[u][0] = *reinterpret_cast<const uint32_t*>(at), x[u][1] = *reinterpret_cast<const uint32_t*>(at + next);
+            b[u][0] = bt[0], b[u][1] = bt[next_b];
         }
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (u && !in1) break;
-            if constexpr (X::bytes == 2) {
-                *reinterpret_cast<u32x4*>(out + u * dist * X::bytes) = widen8<X>(x[u], power_of(b[u]));
-            } else {
-                float f[8];
-                decode8(x[u], power_of(b[u]), f);
-                store_vec<X, 8>(out + u * dist * X::bytes, f);
+        for (int u = 0; u < AHEAD; u++) {
+            const uint32_t t = tt + u * c.sub;
+            if (t >= n) break;
+            const bool held = s_p.state[t] == 2;
+            uint8_t* const out = out0 + (int64_t)t * tok;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                if (w && !in1) break;
+                const uint32_t code = held ? x[u][w] : 0, byte = held ? b[u][w] : 0;
+                if constexpr (X::bytes == 2) {
+                    *reinterpret_cast<u32x4*>(out + w * dist * X::bytes) = widen8<X>(code, power_of(byte));
+                } else {
+                    float f[8];
+                    decode8(code, power_of(byte), f);
+                    store_vec<X, 8>(out + w * dist * X::bytes, f);
+                }
             }
         }
     }
@@ -426,7 +493,7 @@ template <typename X> hipError_t launch_append(const AppendArg& a, int cache_dty
 }
 
 // The cache's and the batch's part, and the cut (after the rows').
-void set_cache(AppendArg& a, const ckr_kv_cache* cache, const ckr_kv_batch* batch) {
+void set_cache(AppendArg& a, const ckr_kv_cache* cache, const ckr_kv_batch* batch, uint32_t passes) {
     a.cache[0] = static_cast<uint8_t*>(cache->d_k), a.cache[1] = static_cast<uint8_t*>(cache->d_v);
     a.scales[0] = cache->d_k_scale, a.scales[1] = cache->d_v_scale;
     const int ces = cache->dtype == CKR_BF16 || cache->dtype == CKR_F16 ? 2 : 1;  // of a stride's unit
@@ -436,7 +503,7 @@ void set_cache(AppendArg& a, const ckr_kv_cache* cache, const ckr_kv_batch* batc
     a.heads = cache->n_heads, a.dim = cache->head_dim;
     a.b = {batch->d_page_table, batch->d_starts, batch->d_offsets, (int64_t)batch->table_stride, batch->table_width,
            batch->n_seqs, batch->n_tokens};
-    a.cut = row_cut(batch->n_tokens, a.q_heads + 2ull * a.heads, std::max((a.dim / 8 + 1) / 2, 4u), a.rot.pairs);
+    a.cut = row_cut(batch->n_tokens, a.q_heads + 2ull * a.heads, std::max((a.dim / 8 + 1) / 2, 4u), a.rot.pairs, passes);
 }
 
 inline bool multiple(const void* p, uint64_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -460,7 +527,7 @@ int kv_read_four(const ckr_kv_cache* c, const ckr_kv_batch* b, void* k, int64_t 
     AppendArg a{};
     a.x[1] = static_cast<uint8_t*>(k), a.x[2] = static_cast<uint8_t*>(v);
     a.tok[1] = kt, a.tok[2] = vt, a.head[1] = kh, a.head[2] = vh;
-    set_cache(a, c, b);
+    set_cache(a, c, b, 4);
     if (a.cut.blocks > kMostBlocks) return err(CKR_E_INVALID, "the batch is too large for one launch");
     const hipStream_t s = (hipStream_t)stream;
     const auto go = [&](auto kernel) { CKR_LAUNCH("kv_read", s, kernel<<<dim3((uint32_t)a.cut.blocks), a.cut.threads, 0, s>>>(a)); };
@@ -559,7 +626,7 @@ int ckr_rotate(const ckr_rotary* rotary, const int32_t* d_positions, const int64
     }
     a.n_tokens = (uint32_t)n_tokens, a.tokens = tokens, a.dim = head_dim, a.inverse = inverse != 0;
     a.chunks = (a.rot.pairs + 7) / 8 + (copy ? (head_dim - 2 * a.rot.pairs + 15) / 16 : 0);
-    a.cut = row_cut(n_tokens, rows, a.chunks, a.rot.pairs);
+    a.cut = row_cut(n_tokens, rows, a.chunks, a.rot.pairs, 4);
     if (a.cut.blocks > kMostBlocks) return err(CKR_E_INVALID, "the heads are too many for one launch");
     const uint32_t lds = a.cut.sub * a.cut.passes * ((a.rot.pairs + 7) / 8 * 8) * 8;
     const hipStream_t s = (hipStream_t)stream;
@@ -605,7 +672,7 @@ int ckr_kv_append(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const ck
     a.tok[0] = q_token_stride, a.tok[1] = k_token_stride, a.tok[2] = v_token_stride;
     a.head[0] = q_head_stride, a.head[1] = k_head_stride, a.head[2] = v_head_stride;
     a.o_tok = out_token_stride, a.o_head = out_head_stride, a.q_heads = n_heads;
-    set_cache(a, cache, batch);
+    set_cache(a, cache, batch, 8);
     if (a.cut.blocks > kMostBlocks) return err(CKR_E_INVALID, "the batch is too large for one launch");
     const uint32_t lds = a.cut.sub * a.cut.passes * ((a.rot.pairs + 7) / 8 * 8) * 8;
     const hipStream_t s = (hipStream_t)stream;
