@@ -491,38 +491,43 @@ class Rotary:
 _i64x18, _i64x2v = ctypes.c_int64 * 18, ctypes.c_int64 * 2
 
 
-def _heads_of(x, lead, dim, dtype, what):
-    """(batch, token and head stride, heads) of a [batch, tokens, heads, dim] tensor, or of one without batch."""
-    shape = x.shape
-    if shape[:-2] != lead or shape[-1] != dim or x.dtype != dtype or not x.is_cuda:
-        _bad(f"{what} must be {[*lead, 'heads', dim]} of {dtype} on the GPU")
-    st = x.stride()
-    if st[-1] != 1 and x.numel():
-        _bad(f"the last axis of {what} must be contiguous")
-    return (st[0], st[1], st[2], shape[2]) if len(shape) == 4 else (0, st[0], st[1], shape[1])
-
-
 def _rotate(rotary, positions, xs, outs, inverse, stream):
     """xs (one or two tensors) turned into outs."""
     q = xs[0]
-    lead, dim, dtype = q.shape[:-2], q.shape[-1], q.dtype
-    if positions.dtype != _torch().int32 or not positions.is_cuda or positions.shape != lead and positions.shape != lead[-1:]:
-        _bad(f"positions must be int32 {list(lead)} or {list(lead[-1:])} on the GPU")
-    ps = positions.stride()
+    shape, dtype = q.shape, q.dtype
+    four, dim = len(shape) == 4, shape[-1]
+    batch, tokens = (shape[0], shape[1]) if four else (1, shape[0])
+    at = positions.shape
+    if len(at) == 1 and at[0] == tokens:
+        ps = (0, positions.stride(0))
+    elif four and len(at) == 2 and at[0] == batch and at[1] == tokens:
+        ps = positions.stride()
+    else:
+        ps = None
+    if ps is None or positions.dtype is not _torch().int32 or not positions.is_cuda:
+        _bad(f"positions must be int32 {list(shape[:-2])} or {[tokens]} on the GPU")
     handle = _stream_of(stream, q)
     if handle not in rotary._streams:
         _used_by(rotary, rotary.turns, handle, stream)
     flat = []
-    for i, (x, y) in enumerate(zip(xs, outs)):
-        b, t, h, n = _heads_of(x, lead, dim, dtype, "qk"[i])
-        ob, ot, oh, on = _heads_of(y, lead, dim, dtype, f"out of {'qk'[i]}")
-        if on != n:
+    for i, x in enumerate(xs):
+        y = outs[i]
+        places = []
+        for t, what in ((x, "qk"[i]), (y, "out of " + "qk"[i])):
+            n = t.shape
+            if len(n) != len(shape) or n[0] != shape[0] or n[-1] != dim or t.dtype is not dtype or four and n[1] != tokens or not t.is_cuda:
+                _bad(f"{what} must be {[*shape[:-2], 'heads', dim]} of {dtype} on the GPU")
+            st = t.stride()
+            if st[-1] != 1 and t.numel():
+                _bad(f"the last axis of {what} must be contiguous")
+            places.append(st[:3] if four else (0, st[0], st[1]))
+        if y.shape[-2] != x.shape[-2]:
             _bad(f"out of {'qk'[i]} must have its heads")
-        if x.data_ptr() == y.data_ptr() and x.stride() != y.stride():
+        x_ptr, y_ptr = x.data_ptr(), y.data_ptr()
+        if x_ptr == y_ptr and places[0] != places[1]:
             _bad(f"{'qk'[i]} turned in place must have its own strides")
-        flat += (x.data_ptr(), y.data_ptr(), b, t, h, ob, ot, oh, n)
-    rc = lib().ckr_rotate(rotary._p, positions.data_ptr(), _i64x2v(*(ps if len(ps) == 2 else (0, ps[0]))), _i64x18(*flat), len(xs),
-                          lead[0] if len(lead) == 2 else 1, lead[-1], dim, _tag(dtype), inverse, handle)
+        flat += (x_ptr, y_ptr, *places[0], *places[1], x.shape[-2])
+    rc = lib().ckr_rotate(rotary._p, positions.data_ptr(), _i64x2v(*ps), _i64x18(*flat), len(xs), batch, tokens, dim, _tag(dtype), inverse, handle)
     if rc:
         _check(rc)
 
@@ -552,8 +557,12 @@ def _turn():
                 here = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[3 + i]]
                 out = [None] * len(grads)
                 if here:
-                    got = Turn.apply(ctx.rotary, positions, not ctx.inverse,
-                                     *(grads[i] if grads[i].stride(-1) == 1 else grads[i].contiguous() for i in here))
+                    gs = [grads[i] if grads[i].stride(-1) == 1 else grads[i].contiguous() for i in here]
+                    if torch.is_grad_enabled():
+                        got = Turn.apply(ctx.rotary, positions, not ctx.inverse, *gs)
+                    else:
+                        got = [torch.empty_like(g) for g in gs]
+                        _rotate(ctx.rotary, positions, gs, got, not ctx.inverse, None)
                     for i, g in zip(here, got):
                         out[i] = g
                 return (None, None, None, *out)
