@@ -450,7 +450,7 @@ __device__ __forceinline__ uint32_t few_tiles(const FewSpan& f) {  // one at lea
 // below, with K's operand made of the 16 bytes (32 dimensions, one group) that a lane holds of a key,
 // V's of the 4 (8 dimensions) that it holds of each of 8 keys: widened by their groups' powers,
 // which the conversions take as they come.  Strides are in 16 bytes and fit 32 bits (the launch
-// has seen to it), so what a tile's page adds to an address is made in scalar registers.
+// has seen to it, and to the bytes of a page's head), so what a tile's page adds to an address is made in scalar registers.
 template <typename X, int DP>
 __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, uint32_t kvh, uint32_t token0, uint32_t row0, uint32_t rows,
                                               const FewSpan& span, int64_t lo, int n_tiles, float& m, float& l, f32x4 (&o)[DP / 16]) {
@@ -527,7 +527,7 @@ __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, ui
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask, p = (uint32_t)max(pages.p[h], 0);
-            const uint8_t* const k = ck + ((uint64_t)p * kst0 + slot * kst2) * 16;
+            const uint8_t* const k = ck + ((uint64_t)p * kst0 + (uint64_t)slot * kst2) * 16;
             const uint8_t* const kp = ckp + ((uint64_t)p * skst0 * 16 + slot);
 #pragma unroll
             for (int j = 0; j < KL; j++) {
@@ -547,7 +547,7 @@ __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, ui
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint32_t slot = (in0 + (uint32_t)base + 16 * h) & slot_mask, p = (uint32_t)max(pages.p[h], 0);
-            const uint8_t* const v = cv + ((uint64_t)p * vst0 + slot * vst2) * 16;
+            const uint8_t* const v = cv + ((uint64_t)p * vst0 + (uint64_t)slot * vst2) * 16;
             const uint8_t* const vp = cvp + ((uint64_t)p * svst0 * 16 + slot);
             r.vp[h] = *reinterpret_cast<const uint32_t*>(vp + vp_off);
 #pragma unroll
@@ -1225,11 +1225,17 @@ __device__ __forceinline__ uint32_t sees_wild_groups(const AttnArg& a, const Til
         const uint32_t slot = (uint32_t)key & ((1u << a.page_shift) - 1);
         const uint64_t seen = below(pos + 1 - k) & ~(a.window ? below(pos - (int64_t)a.window + 1 - k) : 0);
         for (uint32_t g = 0; g < a.dim / kGroup; g++) {
-            const bool bad = page >= 0 && bytes[(int64_t)page * a.svst[0] + (int64_t)(g << a.page_shift) + slot] == 255;
+            const bool bad = page >= 0 && bytes[(int64_t)page * a.svst[0] + ((int64_t)g << a.page_shift) + slot] == 255;
             if (__ballot(bad) & seen) hit |= 1u << g;
         }
     }
     return hit;
+}
+
+// Which tile the n-th block takes.  Four bits: from the last one on, whose rows see the most keys, so that
+// short ones fill up the end (six prompts of 150 to 3000 tokens 648 us, 670 from the first on).
+template <typename C> __device__ __forceinline__ uint32_t nth_tile(const AttnArg& a, uint32_t n) {
+    return C::tag == CKR_F4 ? a.tiles - 1 - n : n;
 }
 
 // ------------------------------------------------------------ many rows
@@ -1274,7 +1280,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     __shared__ uint32_t s_tmp[16], s_wild;  // s_wild: there is a value scale that is not finite
     __shared__ FourShift s_shift;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = nth_tile<C>(a, blockIdx.x / a.kv_heads), split = blockIdx.y;
     Tile t;
     if (threadIdx.x == 0) s_wild = 0;
     if (FOUR && threadIdx.x < 9) s_shift.top[threadIdx.x] = 0;
@@ -1312,8 +1318,8 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     const uint32_t r0 = threadIdx.x / LPR, piece = threadIdx.x % LPR;
     const bool d_in = piece * PIECE < bytes_of<C>(a.dim);
     const uint32_t my_group = FOUR ? piece * PIECE * 2 / kGroup : 0;  // that this thread's pieces lie in
-    const uint8_t* const kp4 = reinterpret_cast<const uint8_t*>(a.sk) + (int64_t)kvh * a.skst[1] + (my_group << a.page_shift);
-    const uint8_t* const vp4 = reinterpret_cast<const uint8_t*>(a.sv) + (int64_t)kvh * a.svst[1] + (my_group << a.page_shift);
+    const uint8_t* const kp4 = reinterpret_cast<const uint8_t*>(a.sk) + (int64_t)kvh * a.skst[1] + ((int64_t)my_group << a.page_shift);
+    const uint8_t* const vp4 = reinterpret_cast<const uint8_t*>(a.sv) + (int64_t)kvh * a.svst[1] + ((int64_t)my_group << a.page_shift);
     uint32_t k_used = 127, v_used = 127, k_most = 0, v_most = 0;  // bytes: of the shifts, the largest so far
     const uint32_t slot_mask = (1u << a.page_shift) - 1;
     const int64_t c0 = lo >> a.page_shift;               // table column of lo, and lo's place in its page
@@ -1694,7 +1700,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     __shared__ uint32_t s_tmp[16], s_wild;  // s_wild: as in the 128-row kernel
     __shared__ FourShift s_shift;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, split = blockIdx.y;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = nth_tile<C>(a, blockIdx.x / a.kv_heads), split = blockIdx.y;
     Tile t;
     if (threadIdx.x == 0) s_wild = 0;
     if (FOUR && threadIdx.x < 9) s_shift.top[threadIdx.x] = 0;
@@ -1745,7 +1751,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     const uint32_t my_group = FOUR ? piece * PIECE * 2 / kGroup : 0;
     const int64_t st_b = stage_k ? a.skst[0] : a.svst[0];
     const uint8_t* const bytes4 = reinterpret_cast<const uint8_t*>(stage_k ? a.sk : a.sv) +
-                                  (int64_t)kvh * (stage_k ? a.skst[1] : a.svst[1]) + (my_group << a.page_shift) + (row_of & 15);
+                                  (int64_t)kvh * (stage_k ? a.skst[1] : a.svst[1]) + ((int64_t)my_group << a.page_shift) + (row_of & 15);
     uint32_t used = 127, most = 0;
     float scale2 = a.scale2;
     uint8_t* const to = (stage_k ? s_k + row_of * KP : s_v + row_of * VP) + to_place;

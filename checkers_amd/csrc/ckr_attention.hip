@@ -35,6 +35,11 @@ constexpr uint32_t kFewTiles = 4;
 // over 32768 42 / 79, of 64 over 1024 51 / 58; 64 rows of 64 over 1024 96 / 60, of 16
 // over 4096 66 / 104.
 constexpr uint32_t kFewMost = 32;
+// Over 4 bits, whose tiles cost few rows half as much (e4m3's figures above; here 48 rows of 16 sequences over
+// 4096 tokens 48 / 101, of one over 32768 42 / 79, of 64 over 1024 47 / 59; 64 rows 60 / 100, 45 / 80 and 73 /
+// 59; 96 rows 70 / 102, 53 / 82 and 90 / 62; 128 rows 106 / 106, 60 / 86 and 127 / 64): more rows, and
+// more again over long contexts.
+constexpr uint32_t kFourMost = 48, kFourMostLong = 96, kFourLong = 2048;
 // Rows from which on a tile of 256 pays: 128 rows of 16 sequences over 4096 tokens 110
 // (many) / 144 (very many), 256 rows 158 / 148; 256 of one over 32768 102 / 100; float16
 // caches 129 / 111 and 184 / 115.
@@ -64,7 +69,7 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     Cut c{};
     const uint64_t group = n_heads / n_kv, rows = (uint64_t)max_chunk * group;
     c.dp = padded_dim(dim);
-    const bool few = rows <= kFewMost && (near_slots || !four) && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1 + (four ? kItemPad : 0)) < (1ull << 31);
+    const bool few = rows <= (!four ? kFewMost : max_context < kFourLong ? kFourMost : kFourMostLong) && (near_slots || !four) && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1 + (four ? kItemPad : 0)) < (1ull << 31);
     c.bm = few ? kFewRows : rows <= kManyMost || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
     c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
     c.splits = 1;
@@ -158,7 +163,7 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
     bool near_slots = true;
     const bool four = cache->dtype == CKR_F4;
     for (const int64_t* st : {a.kst, a.vst}) near_slots = near_slots && st[2] < (1ll << 26) - 16 && (cache->n_pages == 1 || st[0] < (1ll << 36));
-    for (const int64_t* st : {a.skst, a.svst}) near_slots = near_slots && (!four || cache->n_pages == 1 || st[0] < (1ll << 36));
+    for (const int64_t* st : {a.skst, a.svst}) near_slots = near_slots && (!four || (a.page_shift < 29 && (cache->n_pages == 1 || st[0] < (1ll << 36))));
     const Cut c = cut(n_heads, cache->n_heads, cache->head_dim, batch->n_seqs, batch->n_tokens, batch->max_chunk,
                       std::min<uint64_t>(batch->max_context, (uint64_t)batch->table_width * cache->page_size),
                       (uint64_t)batch->table_width * cache->page_size, window, near_slots, four, workspace_bytes);

@@ -64,8 +64,7 @@ __device__ __forceinline__ float turned_second(float x, float y, float c, float 
 // ---- how tokens' rows are cut into blocks.  A thread keeps its row (a head) and its place in it
 // for all of its block's tokens, so that the products of strides are made once a thread or
 // once a token (whose share lies in LDS), not for each row: with all of them made for each,
-// what bound these kernels was integer multiplication (22448 tokens of 48 heads of 128 appended in 145 us,
-// now XXX).
+// integer multiplication took a third of their time.
 constexpr uint32_t kThreads = 512;                // of a block at most
 constexpr uint32_t kMostTokens = 64;              // of a block
 constexpr uint32_t kMostAngles = 32768;           // bytes of LDS for them
@@ -444,7 +443,8 @@ template <typename X> __global__ void __launch_bounds__(kThreads) kv_read_four_k
     const uint8_t* const codes = (v ? a.cache[1] : a.cache[0]) + (int64_t)h * (v ? a.st[1][1] : a.st[0][1]) + d0 / 2;
     const uint8_t* const bytes = static_cast<const uint8_t*>(v ? a.scales[1] : a.scales[0]) + (int64_t)h * (v ? a.sst[1][1] : a.sst[0][1]) +
                                  ((int64_t)(d0 / kGroup) << a.page_shift);
-    const uint32_t next = in1 ? dist / 2 : 0, next_b = in1 ? dist / kGroup << a.page_shift : 0;
+    const uint32_t next = in1 ? dist / 2 : 0;
+    const uint64_t next_b = in1 ? (uint64_t)(dist / kGroup) << a.page_shift : 0;
     constexpr int AHEAD = 4;
     for (uint32_t tt = me.sub; tt < n; tt += AHEAD * c.sub) {
         uint32_t x[AHEAD][2], b[AHEAD][2];
@@ -620,6 +620,8 @@ int ckr_rotate(const ckr_rotary* rotary, const int32_t* d_positions, const int64
             }
             for (int k = 0; k < 3; k++) (w ? y.out_st : y.in_st)[k] = size[k] > 1 ? st[k] : 0;
         }
+        for (int k = 0; k < 3; k++)
+            if (x.d_in == x.d_out && y.in_st[k] != y.out_st[k]) return err(CKR_E_INVALID, "heads turned in place have the output's strides");
         y.in = static_cast<const uint8_t*>(x.d_in), y.out = static_cast<uint8_t*>(x.d_out);
         y.copy = x.d_in != x.d_out && 2 * a.rot.pairs < head_dim;
         copy = copy || y.copy;

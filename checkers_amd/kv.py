@@ -93,6 +93,7 @@ class KvCache:
                 _on_gpu(t, what)
                 _need(t.device == k.device, "the cache's tensors must be on one GPU")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._device = k.get_device()
         self.n_pages, self.n_heads, self.page_size, row = k.shape
         self.head_dim = row * 2 if self.dtype == F4 else row
         c = _Cache(k.data_ptr(), v.data_ptr(), None, None, _i64x3(*k.stride()[:3]), _i64x3(*v.stride()[:3]),
@@ -242,8 +243,8 @@ def kv_write(cache, batch, k, v, stream=None):
 
 
 def kv_append(cache, batch, rotary, k, v, q=None, out=None, positions=None, stream=None):
-    """kv_write of keys that are turned by their positions on the way (rotary: a Rotary,
-    None: not turned).  q [tokens, heads, head_dim], of the keys' type: the chunk's queries,
+    """kv_write of keys that are turned by their positions on the way (rotary: a Rotary, which
+    a captured graph needs kept; None: not turned).  q [tokens, heads, head_dim], of the keys' type: the chunk's queries,
     turned as well, into out (may be q; new when None), which is returned (None without q).
     positions: a contiguous int32 [tokens] where they are not those in the cache."""
     if k.requires_grad or v.requires_grad or q is not None and q.requires_grad:
@@ -269,6 +270,10 @@ def kv_append(cache, batch, rotary, k, v, q=None, out=None, positions=None, stre
         _bad("out belongs to q")
     if positions is not None and (positions.dtype != _torch().int32 or positions.shape != (n,) or not positions.is_contiguous() or not positions.is_cuda):
         _bad(f"positions must be a contiguous int32 [{n}] on the GPU")
+    here = k.get_device()
+    if cache._device != here or v.get_device() != here or rotary is not None and rotary._device != here or \
+            q is not None and (q.get_device() != here or out.get_device() != here):
+        _bad("the cache, the rotary and all tensors must be on one GPU")
     handle = _stream_of(stream, k)
     if rotary is not None and handle not in rotary._streams:
         _used_by(rotary, rotary.turns, handle, stream)
@@ -483,6 +488,7 @@ class Rotary:
         _check(lib().ckr_rotary_turns((ctypes.c_double * n)(*frequencies), n, host.data_ptr()))
         self.turns = host.to(device)   # complete when this returns
         _on_gpu(self.turns, "a rotary")
+        self._device = self.turns.get_device()
         self._streams = {torch.cuda.current_stream(self.turns.device).cuda_stream}   # whose work the table outlives
         self._c = _Rot(self.turns.data_ptr(), magnitude, n, self.interleaved)
         self._p = ctypes.byref(self._c)
@@ -523,6 +529,8 @@ def _rotate(rotary, positions, xs, outs, inverse, stream):
             places.append(st[:3] if four else (0, st[0], st[1]))
         if y.shape[-2] != x.shape[-2]:
             _bad(f"out of {'qk'[i]} must have its heads")
+        if x.get_device() != rotary._device or y.get_device() != rotary._device:
+            _bad(f"{'qk'[i]}, its output and the rotary must be on one GPU")
         x_ptr, y_ptr = x.data_ptr(), y.data_ptr()
         if x_ptr == y_ptr and places[0] != places[1]:
             _bad(f"{'qk'[i]} turned in place must have its own strides")
@@ -576,7 +584,9 @@ def rotary(rotary, positions, q, k=None, out=None, inverse=False, stream=None):
     [batch, tokens, heads, dim] with any strides but the last axis'; positions int32 [tokens] or
     [batch, tokens].  Returns the turned q, with k a pair; into out (a tensor, with k a pair; may
     be q and k themselves) when given.  inverse turns back, but for the magnitude: it is the transposed
-    matrix.  Gradients are recorded where q or k requires them (then without out and stream)."""
+    matrix.  Gradients are recorded where q or k requires them (then without out and stream);
+    a captured graph needs the Rotary kept, and a backward pass that is captured must not meet
+    leaves of an eager graph that is still alive (torch would run their sums on its stream)."""
     xs = (q,) if k is None else (q, k)
     if not 3 <= q.dim() <= 4 or any(x.dim() != q.dim() for x in xs):
         _bad("q and k must be [tokens, heads, dim] or [batch, tokens, heads, dim]")

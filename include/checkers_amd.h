@@ -589,7 +589,8 @@ typedef struct {
  * overlap, or be one: table_stride 0).  The arrays are on the
  * device and read when the call's kernels run.  A table entry outside
  * [0, n_pages), or a position beyond table_width pages, is an unmapped page:
- * it is not written, reads as zeros and is not attended to.  max_chunk and
+ * it is not written, reads as zeros and is not attended to.  Tokens that are written
+ * lie in slots of their own: of two in one slot, parts of either may stay.  max_chunk and
  * max_context (the longest chunk, the largest d_starts[s] + chunk) choose the
  * attention's kernel and how it splits the keys; the result is right whatever
  * they are. */
