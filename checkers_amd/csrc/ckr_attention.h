@@ -450,7 +450,13 @@ __device__ __forceinline__ uint32_t few_tiles(const FewSpan& f) {  // one at lea
 // below, with K's operand made of the 16 bytes (32 dimensions, one group) that a lane holds of a key,
 // V's of the 4 (8 dimensions) that it holds of each of 8 keys: widened by their groups' powers,
 // which the conversions take as they come.  Strides are in 16 bytes and fit 32 bits (the launch
-// has seen to it, and to the bytes of a page's head), so what a tile's page adds to an address is made in scalar registers.
+// has seen to it, and to the bytes of a page's head), so what a tile's page adds to an address is made in scalar
+// registers.
+// 64 sequences of 200 to 16000 tokens, 8 heads of 128 for 32 query heads: 536 MB in 111 us (4.8 TB/s; what a step's
+// later tiles add comes at 5.75, which is what a kernel that only reads such pages reaches).  Beside the bytes it
+// takes 14 us for the launch, the first tiles' way and the join, and each item more than its tiles (kItemPad).  With
+// branches around the loads the compiler waited for all of them before each tile (142 us); two tiles on their way
+// and two blocks a CU take 115.
 template <typename X, int DP>
 __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, uint32_t kvh, uint32_t token0, uint32_t row0, uint32_t rows,
                                               const FewSpan& span, int64_t lo, int n_tiles, float& m, float& l, f32x4 (&o)[DP / 16]) {
@@ -1672,6 +1678,9 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 // in float16, 64 query heads: 490 to 505 us, 0.69 PFLOP/s: a block is alone on its CU
 // and takes one tile of rows, so of the 50 us that one takes on average the 12 until
 // its first product runs beside nothing.
+// Over 4 bits no score and no weight meets a scale (FourShift), which leaves three and a half instructions: the
+// chunk 960 to 990 us, 1.07 PFLOP/s; the prompts of 150 to 3000 tokens with 64 query heads 648, 0.75.  A loop of its own
+// for the waves that stage keys spills 86 registers (1630 us).
 template <typename C, int DP> struct WideShape {
     static constexpr int TK = 64, BM = 256, RING = 4;
     static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 64;  // as ManyShape's

@@ -22,9 +22,13 @@ constexpr uint64_t kSplitMin = 128;   // keys of a split at least
 // Blocks of the few rows' kernel: two a CU.  (For heads of 256 its registers leave room
 // for one, so there a full launch runs in two rounds.)
 constexpr uint32_t kFewBlocks = 512;
-constexpr uint32_t kFourBlocks = 768;  // over a cache of 4 bits: three a CU (of heads of 256 two)
+// Over a cache of 4 bits three, with a tile on its way a wave (two, with two tiles: 64 sequences of 200 to 16000
+// tokens 112 / 118 us, 512 of 1000 133 / 144, 40 of 50 to 3000 24 / 25; float16 queries 126 / 123); of heads of 256 two.
+constexpr uint32_t kFourBlocks = 768;
 // There an item (its queries, the first tiles' way, the join) costs a block as much as so many tiles, so
-// that stretches with many short items are given fewer tiles; in stretches from kPadFrom tiles on.
+// that stretches with many short items are given fewer tiles (64 sequences of 200 to 16000 tokens: 126 us with
+// none, 124 with 8, 112 with 16, 116 with 24; 40 of 50 to 3000: 37, 25.5, 25 and 25); in stretches from kPadFrom
+// tiles on, below which a block has hardly more than one.
 constexpr uint32_t kItemPad = 16, kPadFrom = 32;
 uint32_t most_blocks(bool four, uint32_t dp) { return four && dp <= 128 ? kFourBlocks : kFewBlocks; }
 // Its tiles of 32 keys a block at least: one a wave (one token over a thousand: 9.5 us;

@@ -64,7 +64,7 @@ __device__ __forceinline__ float turned_second(float x, float y, float c, float 
 // ---- how tokens' rows are cut into blocks.  A thread keeps its row (a head) and its place in it
 // for all of its block's tokens, so that the products of strides are made once a thread or
 // once a token (whose share lies in LDS), not for each row: with all of them made for each,
-// integer multiplication took a third of their time.
+// their integer multiplications bounded these kernels.
 constexpr uint32_t kThreads = 512;                // of a block at most
 constexpr uint32_t kMostTokens = 64;              // of a block
 constexpr uint32_t kMostAngles = 32768;           // bytes of LDS for them
@@ -154,6 +154,10 @@ template <typename E, int N> __device__ __forceinline__ void store_some(uint8_t*
     }
 }
 
+// Bound by memory: queries and keys of 16384 tokens, 40 heads of 128 in bfloat16, 335 MB in 64 us (5.2 TB/s, a
+// copy's rate; 75 with one token's rows loaded at a time); 5997 tokens of 24 heads of 80 in float32, the first 20
+// turned, 92 MB in 31 us (3 TB/s: a row of 320 bytes takes six of its eight lanes).  Threads that took tokens side
+// by side and heads one after another measured the same or worse for heads that lie before tokens.
 template <typename E> __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArg a) {
     extern __shared__ __attribute__((aligned(16))) f32x2 s_cs[];
     __shared__ int64_t s_at[kMostTokens][4];  // a token's place in the inputs and outputs
@@ -299,6 +303,10 @@ __device__ __forceinline__ void find_places(const AppendArg& a, uint32_t token0,
 // of a turned row also load the values that they are paired with, which the row's other lanes bring
 // in anyway.  A row's lanes are of one wave, whose loads of a row come before its stores, so that queries
 // may be turned in place.
+// Bound by memory and by how many loads are on their way: 22448 tokens with 32 query heads over 8 of 128, bfloat16
+// to 4 bits, 484 MB in 120 us (4.0 TB/s; to e4m3 120, to bfloat16 121; 148 with one token's rows loaded at a
+// time, 108 without turning).  Blocks of one token take 400 us: eight share look-ups, angles and the lines of scales.
+// One token 4.6 us, a chain of dependent reads (chunk, table, rows).
 template <typename X, typename C> __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendArg a) {
     extern __shared__ __attribute__((aligned(16))) f32x2 s_cs[];
     __shared__ Places s_p;
@@ -427,7 +435,8 @@ template <typename X, typename C> __global__ void __launch_bounds__(kThreads) kv
     }
 }
 
-// A cache of 4 bits read back: the same rows (no queries), the other way round.
+// A cache of 4 bits read back: the same rows (no queries), the other way round.  Bound by memory: 124592 tokens of
+// 8 heads of 128 to bfloat16, 646 MB in 130 us (5.0 TB/s; 190 with 16 values a lane and a token a thread).
 template <typename X> __global__ void __launch_bounds__(kThreads) kv_read_four_kernel(AppendArg a) {
     __shared__ Places s_p;
     const RowCut& c = a.cut;

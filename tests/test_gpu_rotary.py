@@ -441,3 +441,54 @@ def test_refusals(gpu):
     bad("overlap", ck.kv_append, cache, b, r, kv, kv, q=q, out=q[:, :1].expand(2, 3, 64))
     bad("16-byte", ck.kv_append, cache, b, r, torch.zeros(2 * 64 + 1, device=gpu)[1:].view(2, 1, 64), kv)
     torch.cuda.synchronize()
+
+
+def test_example_over_four_bits(gpu):
+    """Tokens served over a parked and restored 4-bit cache."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "park_cache.py")
+    spec = importlib.util.spec_from_file_location("park_cache", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(["--tokens", "6", "--layers", "1", "--bits", "4"]) == 0
+
+
+def test_tensors_of_other_layouts(gpu):
+    """Heads before tokens, positions of every other token, a rotary for another dtype: strides are followed."""
+    r = ck.Rotary(64, interleaved=True)
+    base = torch.randn(2, 6, 40, 64, device=gpu)                       # batch, heads, tokens, dim
+    pos = _i32(np.arange(160).reshape(2, 80), gpu)[:, ::2]
+    got = ck.rotary(r, pos, base.transpose(1, 2))
+    want = ck.rotary(r, pos.contiguous(), base.transpose(1, 2).contiguous())
+    assert torch.equal(got, want) and got.shape == (2, 40, 6, 64)
+    shared = base[:, :1].expand(2, 6, 40, 64).transpose(1, 2)           # one head read by all
+    assert torch.equal(ck.rotary(r, pos, shared), ck.rotary(r, pos, shared.contiguous()))
+    x = base[:, :1].clone().requires_grad_()                            # the gradient of a broadcast input
+    y = ck.rotary(r, pos, x.expand(2, 6, 40, 64).transpose(1, 2))
+    g = torch.randn_like(y)
+    d, = torch.autograd.grad(y, x, g)
+    with torch.no_grad():
+        back = ck.rotary(r, pos, g, inverse=True).transpose(1, 2).sum(1, keepdim=True)
+    assert torch.allclose(d, back, rtol=0, atol=6 * 2 * ko.U32 * 6 * 8)   # six values of a few units, two orders of their sum
+    odd = torch.randn(33 * 3 * 50 + 1, device=gpu)[1:].view(33, 3, 50)  # rows on 4-byte boundaries
+    p = _i32(np.arange(33), gpu)
+    assert torch.equal(ck.rotary(ck.Rotary(46), p, odd), ck.rotary(ck.Rotary(46), p, odd.clone()))
+
+
+@pytest.mark.parametrize("rot,dim,inter", [(64, 128, False), (40, 80, False), (48, 64, True), (128, 128, False), (6, 32, False)])
+@pytest.mark.parametrize("n", [1, 700])
+def test_append_in_place_of_parts_of_heads(gpu, rot, dim, inter, n):
+    """Queries turned in place, whose lanes read values that other lanes write; many tokens a block."""
+    cache = ck.KvCache.empty(-(-n // 16), 16, 2, dim, ck.BF16)
+    b = ck.KvBatch(_i32([range(-(-n // 16))], gpu), _i32([0], gpu), _i32([0, n], gpu), n)
+    r = ck.Rotary(rot, interleaved=inter)
+    x = torch.randn(n, 9, dim, device=gpu).to(torch.bfloat16)
+    want = ck.rotary(r, _i32(range(n), gpu), x[:, :5].clone())
+    wk = ck.rotary(r, _i32(range(n), gpu), x[:, 5:7].clone())
+    v = x[:, 7:].clone()
+    q = x[:, :5]
+    assert ck.kv_append(cache, b, r, x[:, 5:7], x[:, 7:], q=q, out=q) is q
+    assert torch.equal(q, want) and torch.equal(x[:, 7:], v)
+    k2, v2 = ck.kv_read(cache, b)
+    assert torch.equal(k2, wk) and torch.equal(v2, v)
