@@ -63,8 +63,8 @@ __device__ __forceinline__ float turned_second(float x, float y, float c, float 
 
 // ---- how tokens' rows are cut into blocks.  A thread keeps its row (a head) and its place in it
 // for all of its block's tokens, so that the products of strides are made once a thread or
-// once a token (whose share lies in LDS), not for each row: with all of them made for each,
-// their integer multiplications bounded these kernels.
+// once a token (whose share lies in LDS), not for each row, and several tokens' rows can be
+// loaded before the first is used.
 constexpr uint32_t kThreads = 512;                // of a block at most
 constexpr uint32_t kMostTokens = 64;              // of a block
 constexpr uint32_t kMostAngles = 32768;           // bytes of LDS for them
@@ -635,6 +635,8 @@ int ckr_rotate(const ckr_rotary* rotary, const int32_t* d_positions, const int64
         y.copy = x.d_in != x.d_out && 2 * a.rot.pairs < head_dim;
         copy = copy || y.copy;
     }
+    if (n == 2 && a.x[0].heads && a.x[1].heads && (heads[0].d_out == heads[1].d_out || heads[0].d_out == heads[1].d_in || heads[1].d_out == heads[0].d_in))
+        return err(CKR_E_INVALID, "one tensor's output is the other tensor, or its output");
     a.n_tokens = (uint32_t)n_tokens, a.tokens = tokens, a.dim = head_dim, a.inverse = inverse != 0;
     a.chunks = (a.rot.pairs + 7) / 8 + (copy ? (head_dim - 2 * a.rot.pairs + 15) / 16 : 0);
     a.cut = row_cut(n_tokens, rows, a.chunks, a.rot.pairs, 4);
@@ -671,6 +673,7 @@ int ckr_kv_append(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const ck
     if (n_heads && ((rc = kv_check_rows(d_q, T, q_token_stride, n_heads, q_head_stride, D, es, false, "queries")) ||
                     (rc = kv_check_rows(d_out, T, out_token_stride, n_heads, out_head_stride, D, es, true, "output"))))
         return rc;
+    if (n_heads && (d_out == d_k || d_out == d_v)) return err(CKR_E_INVALID, "the queries' output is the keys or the values");
     if (n_heads && d_q == d_out && ((T > 1 && q_token_stride != out_token_stride) || (n_heads > 1 && q_head_stride != out_head_stride)))
         return err(CKR_E_INVALID, "queries turned in place have the output's strides");
     if (d_positions) {

@@ -158,6 +158,7 @@ class KvBatch:
         for t, what in ((page_table, "page_table"), (starts, "starts"), (offsets, "offsets")):
             _need(t.dtype == torch.int32 and (t.dim() == 2 or t.is_contiguous()), f"{what} must be int32, contiguous")
             _on_gpu(t, what)
+        self._device = page_table.get_device()
         _need(0 <= n_tokens < 1 << 31, "n_tokens out of range")
         self.page_table, self.starts, self.offsets, self.n_seqs, self.n_tokens = page_table, starts, offsets, n, int(n_tokens)
         self.max_chunk = int(n_tokens if max_chunk is None else max_chunk)
@@ -272,8 +273,9 @@ def kv_append(cache, batch, rotary, k, v, q=None, out=None, positions=None, stre
         _bad(f"positions must be a contiguous int32 [{n}] on the GPU")
     here = k.get_device()
     if cache._device != here or v.get_device() != here or rotary is not None and rotary._device != here or \
+            batch._device != here or positions is not None and positions.get_device() != here or \
             q is not None and (q.get_device() != here or out.get_device() != here):
-        _bad("the cache, the rotary and all tensors must be on one GPU")
+        _bad("the cache, the batch, the rotary and all tensors must be on one GPU")
     handle = _stream_of(stream, k)
     if rotary is not None and handle not in rotary._streams:
         _used_by(rotary, rotary.turns, handle, stream)
@@ -510,8 +512,8 @@ def _rotate(rotary, positions, xs, outs, inverse, stream):
         ps = positions.stride()
     else:
         ps = None
-    if ps is None or positions.dtype is not _torch().int32 or not positions.is_cuda:
-        _bad(f"positions must be int32 {list(shape[:-2])} or {[tokens]} on the GPU")
+    if ps is None or positions.dtype is not _torch().int32 or positions.get_device() != rotary._device:
+        _bad(f"positions must be int32 {list(shape[:-2])} or {[tokens]} on the rotary's GPU")
     handle = _stream_of(stream, q)
     if handle not in rotary._streams:
         _used_by(rotary, rotary.turns, handle, stream)
@@ -532,7 +534,7 @@ def _rotate(rotary, positions, xs, outs, inverse, stream):
         if x.get_device() != rotary._device or y.get_device() != rotary._device:
             _bad(f"{'qk'[i]}, its output and the rotary must be on one GPU")
         x_ptr, y_ptr = x.data_ptr(), y.data_ptr()
-        if x_ptr == y_ptr and places[0] != places[1]:
+        if x_ptr and x_ptr == y_ptr and places[0] != places[1]:
             _bad(f"{'qk'[i]} turned in place must have its own strides")
         flat += (x_ptr, y_ptr, *places[0], *places[1], x.shape[-2])
     rc = lib().ckr_rotate(rotary._p, positions.data_ptr(), _i64x2v(*ps), _i64x18(*flat), len(xs), batch, tokens, dim, _tag(dtype), inverse, handle)

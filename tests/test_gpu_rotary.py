@@ -443,6 +443,31 @@ def test_refusals(gpu):
     torch.cuda.synchronize()
 
 
+def test_outputs_that_other_rows_are_read_from(gpu):
+    """Two tensors swapped by their outputs, or written to one, would be read while they are written."""
+    r, pos = ck.Rotary(64), _i32([0, 1], gpu)
+    q, k, o = (torch.zeros(2, 3, 64, device=gpu) for _ in range(3))
+    cache = ck.KvCache.empty(2, 16, 3, 64, ck.F4)
+    b = ck.KvBatch(_i32([[0]], gpu), _i32([0], gpu), _i32([0, 2], gpu), 2)
+    for f, args, kw in ((ck.rotary, (r, pos, q, k), dict(out=(k, q))), (ck.rotary, (r, pos, q, k), dict(out=(o, o))),
+                        (ck.rotary, (r, pos, q, q), dict(out=(q, o))), (ck.rotary, (r, pos, q, q), dict(out=(o, q))),
+                        (ck.kv_append, (cache, b, r, k, o), dict(q=q, out=k)), (ck.kv_append, (cache, b, r, o, k), dict(q=q, out=k))):
+        with pytest.raises(ck.CkrError) as e:
+            f(*args, **kw)
+        assert e.value.code == ck.CKR_E_INVALID and "output" in str(e.value), str(e.value)
+    torch.cuda.synchronize()
+
+
+def test_no_heads_or_tokens_of_any_strides(gpu):
+    r, pos = ck.Rotary(64), _i32([0, 1], gpu)
+    q = torch.zeros(2, 2, 3, 64, device=gpu)
+    for x, p in ((q[:, :, :0], pos), (q.transpose(1, 2)[:, :, :0], pos.new_zeros(3)), (q[:, :0], pos[:0]), (q[:0], pos)):
+        assert ck.rotary(r, p, x).shape == x.shape
+        a, b = ck.rotary(r, p, x, x)
+        assert a.shape == b.shape == x.shape
+    torch.cuda.synchronize()
+
+
 def test_example_over_four_bits(gpu):
     """Tokens served over a parked and restored 4-bit cache."""
     import importlib.util
