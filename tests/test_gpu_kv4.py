@@ -302,6 +302,54 @@ def test_keys_later_than_a_block_expects(gpu, lens, typ):
     _check(sq, cache, q, out, lse, 4, 0)
 
 
+@pytest.mark.parametrize("typ,dim,lens", [("bf16", 128, [40]), ("f16", 256, [40]), ("bf16", 64, [100]), ("f16", 128, [100]), ("bf16", 128, [1])])
+@pytest.mark.parametrize("first", ["unmapped", "zeros"])
+@pytest.mark.parametrize("power", [0, -60, 60])
+def test_first_keys_without_a_scale(gpu, typ, dim, lens, first, power):
+    """A block whose first keys are not mapped, or zeros, has no scale to begin with; those after may be of any size."""
+    if typ == "f16" and power > 0:
+        pytest.skip("outputs of float16 end at 65504")
+    print(f"[case] first keys {typ} {dim} {lens} {first} {power}", flush=True)
+    sq = ko.Seqs([600], lens, 16, seed=2)
+
+    def change(sq, cache):
+        for t in (cache.k_scale, cache.v_scale):
+            _bytes(t)[:] += power if power > 0 else 0
+            _bytes(t)[:] -= -power if power < 0 else 0
+        if typ == "f16" or power > 0:
+            _bytes(cache.k_scale)[:] -= power if power > 0 else 0
+            _bytes(cache.k_scale)[:] += -power if power < 0 else 0
+        if first == "zeros":
+            for j in range(230):
+                p, slot = sq.place(0, j)
+                for t in (cache.k, cache.v):
+                    _bytes(t)[p, :, slot] = 0
+                for t in (cache.k_scale, cache.v_scale):
+                    _bytes(t)[p, :, :, slot] = 0
+
+    if first == "zeros":
+        sq, cache, b, q, plan, out, lse = _attend(gpu, typ, 2, 4, dim, 16, [600], lens, 0, sq=sq, change=change)
+    else:
+        cache = _cache(sq, 2, dim, gpu)
+        _fill(sq, cache, _batch(sq, gpu), 2, dim, gpu, 3)
+        change(sq, cache)
+        sq.table[0, :14] = -1
+        q = torch.randn(sq.tokens, 8, dim, device=gpu).to(TYPES[typ])
+        lse = torch.full((sq.tokens, 8), 9.0, device=gpu)
+        out = ck.KvAttention(8, 2, dim, 1, sq.tokens, max(lens), 700).run(cache, _batch(sq, gpu), q, lse=lse)
+        torch.cuda.synchronize()
+    if typ == "f16" and power < 0:      # outputs of 2^-60 are 0 in float16
+        assert out.abs().max() < 2.0 ** -24
+        return
+    D, (k, v) = dim, (k4.as_numpy(_values(cache, n)) for n in ("k", "v"))
+    ref = ko.attention(sq, k, v, q.cpu().double().numpy(), 4, D ** -0.5, 0)
+    bound, lbound = ko.attention_bounds(*ref, 2 * D, 2.0 ** -11, q.dtype, np.abs(v).max())
+    bound = bound - 2.0 ** -24 + 2.0 ** -24 * np.abs(v).max()   # the bound's absolute part, at the values' size
+    err = np.abs(out.cpu().double().numpy() - ref[0])
+    assert (err <= bound).all(), (err / bound).max()
+    assert (np.abs(lse.cpu().double().numpy() - ref[1]) <= np.broadcast_to(lbound, ref[1].shape)).all()
+
+
 @pytest.mark.parametrize("lens", [[1, 2], [70, 8]])
 @pytest.mark.parametrize("loud,scale", [(40.0, None), (0.0, None), (1.0, 0.0), (1.0, -0.3)])
 def test_peaked_and_flat_scores(gpu, lens, loud, scale):
