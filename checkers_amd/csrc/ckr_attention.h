@@ -1678,8 +1678,8 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 // in float16, 64 query heads: 490 to 505 us, 0.69 PFLOP/s: a block is alone on its CU
 // and takes one tile of rows, so of the 50 us that one takes on average the 12 until
 // its first product runs beside nothing.
-// Over 4 bits no score and no weight meets a scale (FourShift), which leaves three and a half instructions: the
-// chunk 960 to 990 us, 1.07 PFLOP/s; the prompts of 150 to 3000 tokens with 64 query heads 648, 0.75.  A loop of its own
+// Over 4 bits no score and no weight meets a scale (FourShift): the chunk 936 to 1060 us from card to card, 0.98 to
+// 1.11 PFLOP/s; the prompts of 150 to 3000 tokens with 64 query heads 641 to 712, 0.68 to 0.76.  A loop of its own
 // for the waves that stage keys spills 86 registers (1630 us).
 template <typename C, int DP> struct WideShape {
     static constexpr int TK = 64, BM = 256, RING = 4;
