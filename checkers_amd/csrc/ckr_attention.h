@@ -81,6 +81,12 @@ template <typename C> __device__ __forceinline__ u32x2 widen4_by(uint32_t v, flo
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// 2^(x y - ref) with the product rounded, as a maximum `ref` of such products is: of scores of 2^27
+// and more a bit of that rounding is worth all of a float16 weight's range.
+__device__ __forceinline__ float weight_apart(float x, float y, float ref) {
+#pragma clang fp contract(off)
+    return exp2_fast(x * y - ref);
+}
 // Maximum over the lanes l, l ^ 32 (and l ^ 16).
 __device__ __forceinline__ float max_half(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
@@ -2055,7 +2061,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 float p[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    p[i] = weight(k + i, g, f);
+                    p[i] = weight_apart(s[k + i], g[i], ref);
                     sum += p[i];
                 }
                 pf[sub][k / 8][k % 8 / 2] = pack16<P>(p[0] * gv[0], p[1] * gv[1]);
