@@ -463,7 +463,7 @@ __device__ __forceinline__ uint32_t few_tiles(const FewSpan& f) {  // one at lea
 // takes 14 us for the launch, the first tiles' way and the join, and each item more than its tiles (kItemPad).  With
 // branches around the loads the compiler waited for all of them before each tile (142 us); two tiles on their way
 // and two blocks a CU take 115.
-template <typename X, int DP>
+template <typename X, int DP, typename At = uint32_t>
 __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, uint32_t kvh, uint32_t token0, uint32_t row0, uint32_t rows,
                                               const FewSpan& span, int64_t lo, int n_tiles, float& m, float& l, f32x4 (&o)[DP / 16]) {
     typedef ElemBF16 P;
@@ -494,16 +494,16 @@ __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, ui
     const uint8_t* const cv = a.cv + (int64_t)kvh * a.vst[1];
     const uint8_t* const ckp = reinterpret_cast<const uint8_t*>(a.sk) + (int64_t)kvh * a.skst[1];
     const uint8_t* const cvp = reinterpret_cast<const uint8_t*>(a.sv) + (int64_t)kvh * a.svst[1];
-    const uint32_t kst0 = (uint32_t)(a.kst[0] >> 4), kst2 = (uint32_t)(a.kst[2] >> 4), vst0 = (uint32_t)(a.vst[0] >> 4), vst2 = (uint32_t)(a.vst[2] >> 4);
-    const uint32_t skst0 = (uint32_t)(a.skst[0] >> 4), svst0 = (uint32_t)(a.svst[0] >> 4);
+    const At kst0 = (At)(a.kst[0] >> 4), kst2 = (At)(a.kst[2] >> 4), vst0 = (At)(a.vst[0] >> 4), vst2 = (At)(a.vst[2] >> 4);
+    const At skst0 = (At)(a.skst[0] >> 4), svst0 = (At)(a.svst[0] >> 4);
     // the lane's places in the 16 keys that a page holds at least; past the head's size (where
     // queries are zero and outputs go nowhere) its last ones again
     const uint32_t k_piece = DP == 64 ? min(g, a.dim / 16 - 1) : min(g, a.dim / 32 - 1);
-    const uint32_t k_off = col * kst2 * 16 + k_piece * (DP == 64 ? 8 : 16), kp_off = ((DP == 64 ? k_piece / 2 : k_piece) << a.page_shift) + col;
+    const At k_off = col * kst2 * 16 + k_piece * (DP == 64 ? 8 : 16), kp_off = ((At)(DP == 64 ? k_piece / 2 : k_piece) << a.page_shift) + col;
     const uint32_t k_next = DP > 128 ? (min(4 + g, a.dim / 32 - 1) - k_piece) * 16 : 0;  // from a key's first piece to its second
     const uint32_t v_col = min(col, a.dim / NV - 1);
-    const uint32_t vp_off = (v_col * NV / kGroup << a.page_shift) + 4 * g;
-    uint32_t v_off[4];
+    const At vp_off = ((At)(v_col * NV / kGroup) << a.page_shift) + 4 * g;
+    At v_off[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) v_off[i] = (4 * g + i) * vst2 * 16 + v_col * (NV / 2);
     typedef __attribute__((address_space(1))) const int32_t* global_i32;
@@ -551,7 +551,7 @@ __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, ui
 #pragma unroll
                     for (int w = 0; w < 4; w++) r.k[h][j][w] = x[w];
                 }
-                r.kp[h][j] = kp[kp_off + (j * (k_next / 16) << a.page_shift)];
+                r.kp[h][j] = kp[kp_off + ((At)(j * (k_next / 16)) << a.page_shift)];
             }
         }
     };
@@ -1206,21 +1206,83 @@ __global__ void __launch_bounds__(64 * kFewWaves, few_waves<C>(DP)) attend_few_k
     }
 }
 
+// Which tile the n-th block takes.  Four bits: from the last one on, whose rows see the most keys, so that
+// short ones fill up the end (six prompts of 150 to 3000 tokens 648 us, 670 from the first on).
+template <typename C> __device__ __forceinline__ uint32_t nth_tile(const AttnArg& a, uint32_t n) {
+    return C::tag == CKR_F4 ? a.tiles - 1 - n : n;
+}
+
 // ---- four bits in float16.  A block's values are held against a power of two for each group of
 // 32 dimensions (keys of float16 queries against one for all groups): that of the
 // largest scale among its first keys.  float16 has 13 octaves above such a power and, with
 // all bits of a code, 23 below; where a later scale is above them, the block begins
 // again with the largest of all, so nothing is checked on the way but each staged
-// byte's maximum.  (A scale more than 23 octaves below the largest of its group over the
-// block's keys loses bits: its values are off by 2^-25 of that power at most.)
-constexpr int kRoom = 13;
+// byte's maximum and whether it is more than 23 octaves below, where codes would lose
+// bits.  Those may be all that a row sees (the power may be that of a key that it does
+// not see), so such a block's rows are taken by the few rows' products (attend_apart).
+constexpr int kRoom = 13, kBelow = 23;
 struct FourShift {
     uint32_t top[9], used[9];  // bytes: of the values' groups, [8]: of the keys
+    uint32_t apart;            // there are codes that float16 does not hold beside the others
     // what the conversion is given for a byte
     static __device__ __forceinline__ float power(uint32_t byte, uint32_t used) {
         return power_of((uint32_t)min(max((int)byte - (int)used + 127, 0), 127 + kRoom));
     }
+    // least: the smallest byte but 0 (no values), less 1
+    static __device__ __forceinline__ bool below(uint32_t least, uint32_t used) { return (int)(least + 1) < (int)used - kBelow; }
 };
+
+// A block whose scales are too far apart for float16: each wave's 32 rows in two tiles of
+// 16, over the block's range of keys (which starts at a multiple of TK), written as the kernels
+// of many rows do.  Where every block has one such scale, the chunk of 2048 behind 30000 takes 3.5 ms for
+// 0.96, the prompts of 150 to 3000 tokens 1.1 ms for 0.39, 16 times 128 rows a head 262 us for 102.
+template <typename X, int DP, uint32_t BM, int TK> __device__ __forceinline__ void attend_apart(const uint32_t* s_tmp) {
+    constexpr int NV = DP / 16;
+    constexpr float up = ProbMany<X, ElemF4>::up;
+    const AttnArg& a = args_here();
+    const Tile t = tile_found<BM, BM * 2>(a.group, s_tmp);
+    const auto scalar = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); };
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = nth_tile<ElemF4>(a, blockIdx.x / a.kv_heads), split = blockIdx.y;
+    const uint32_t seq = scalar(t.seq), token0 = scalar(t.token0), rows = scalar(t.rows), block_row = scalar(t.row0);
+    const int64_t start = (int32_t)scalar((uint32_t)t.start);
+    const int64_t pos_lo = start + block_row / a.group, pos_hi = start + min(block_row + BM - 1, rows - 1) / a.group;
+    const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
+    const int64_t first = a.window ? max((int64_t)0, pos_lo - (int64_t)a.window + 1) & ~(int64_t)(TK - 1) : 0;
+    const int64_t lo = first + (int64_t)split * a.split_len, hi = split + 1 == a.splits ? limit : min(limit, lo + (int64_t)a.split_len);
+    const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    for (uint32_t i = 0; i < 2; i++) {
+        const uint32_t row0 = scalar(block_row + threadIdx.x / 64 * 32 + i * kFewRows), row = row0 + col;
+        if (row0 >= rows) break;
+        FewSpan span = few_span(a, start, row0, rows);
+        span.limit = min(span.limit, hi);
+        const int64_t from = max(lo, span.first);
+        float m = -INFINITY, l = 0.f;
+        f32x4 o[NV];
+#pragma unroll
+        for (int c = 0; c < NV; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        few_item_four<X, DP, uint64_t>(a, seq, kvh, token0, row0, rows, span, from, span.limit > from ? (int)((span.limit - from + 31) / 32) : 0, m, l, o);
+        l = sum_quarters(l);
+        if (l != l && m == -INFINITY) m = 0.f;
+        if (row >= rows) continue;
+        const uint64_t p = (((uint64_t)tile * a.kv_heads + kvh) * a.splits + split) * BM + (row - block_row);
+        const uint32_t token = token0 + row / a.group, head = kvh * a.group + row % a.group;
+        uint8_t* const out = a.out + ((int64_t)token * a.o_tok + (int64_t)head * a.o_head) * 2;
+        const float inv = m == -INFINITY ? 0.f : 1.f / l;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int c = 0; c < NV; c += 4) {
+                const uint32_t d = (4 * g + k) * NV + c;
+                if (a.splits > 1)
+                    *reinterpret_cast<f32x4*>(a.part_o + p * DP + d) = f32x4{o[c][k], o[c + 1][k], o[c + 2][k], o[c + 3][k]};
+                else if (d < a.dim)
+                    *reinterpret_cast<u32x2*>(out + d * 2) = u32x2{pack16<X>(o[c][k] * inv, o[c + 1][k] * inv), pack16<X>(o[c + 2][k] * inv, o[c + 3][k] * inv)};
+            }
+        if (g) continue;
+        if (a.splits > 1) a.part_m[p * 2] = m + up, a.part_m[p * 2 + 1] = l;  // the kernels' sums are held against 2^(m - up)
+        else if (a.lse) a.lse[(int64_t)token * a.heads + head] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+    }
+}
 
 // The groups of 32 dimensions in which a row of the tile sees a value whose scale is NaN (64
 // keys a step, the whole wave; for tiles in which there is one).
@@ -1242,12 +1304,6 @@ __device__ __forceinline__ uint32_t sees_wild_groups(const AttnArg& a, const Til
         }
     }
     return hit;
-}
-
-// Which tile the n-th block takes.  Four bits: from the last one on, whose rows see the most keys, so that
-// short ones fill up the end (six prompts of 150 to 3000 tokens 648 us, 670 from the first on).
-template <typename C> __device__ __forceinline__ uint32_t nth_tile(const AttnArg& a, uint32_t n) {
-    return C::tag == CKR_F4 ? a.tiles - 1 - n : n;
 }
 
 // ------------------------------------------------------------ many rows
@@ -1295,7 +1351,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     const uint32_t kvh = blockIdx.x % a.kv_heads, tile = nth_tile<C>(a, blockIdx.x / a.kv_heads), split = blockIdx.y;
     Tile t;
     if (threadIdx.x == 0) s_wild = 0;
-    if (FOUR && threadIdx.x < 9) s_shift.top[threadIdx.x] = 0;
+    if (FOUR && threadIdx.x < 9) s_shift.top[threadIdx.x] = s_shift.apart = 0;
     if (!find_tile<128>(a.b, a.group, tile, s_tmp, t)) return;
     const uint32_t row = t.row0 + wave * 32 + col;
     const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + 127, t.rows - 1) / a.group;
@@ -1332,7 +1388,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
     const uint32_t my_group = FOUR ? piece * PIECE * 2 / kGroup : 0;  // that this thread's pieces lie in
     const uint8_t* const kp4 = reinterpret_cast<const uint8_t*>(a.sk) + (int64_t)kvh * a.skst[1] + ((int64_t)my_group << a.page_shift);
     const uint8_t* const vp4 = reinterpret_cast<const uint8_t*>(a.sv) + (int64_t)kvh * a.svst[1] + ((int64_t)my_group << a.page_shift);
-    uint32_t k_used = 127, v_used = 127, k_most = 0, v_most = 0;  // bytes: of the shifts, the largest so far
+    uint32_t k_used = 127, v_used = 127, k_most = 0, v_most = 0, k_least = 254, v_least = 254;  // bytes: of the shifts, the largest and the smallest so far
     const uint32_t slot_mask = (1u << a.page_shift) - 1;
     const int64_t c0 = lo >> a.page_shift;               // table column of lo, and lo's place in its page
     const uint32_t in0 = (uint32_t)lo & slot_mask;
@@ -1395,6 +1451,8 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                 if (!fine) s_wild = 1;
                 if (fine) v_most = max(v_most, vb[u]);
                 if (X::tag == CKR_F16 && kb[u] != 255) k_most = max(k_most, kb[u]);
+                if (X::tag == CKR_F16) k_least = min(k_least, kb[u] - 1);
+                v_least = min(v_least, vb[u] - 1);
                 const float kp = X::tag == CKR_BF16 || kb[u] == 255 ? power_of(kb[u]) : FourShift::power(kb[u], k_used);
                 const float vp = FourShift::power(fine ? vb[u] : 0, v_used);
 #pragma unroll
@@ -1598,7 +1656,9 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
         if constexpr (FOUR) {  // a scale above what float16 holds: begin again
             if (v_most) atomicMax(&s_shift.top[my_group], v_most);
             if (X::tag == CKR_F16 && k_most) atomicMax(&s_shift.top[8], k_most);
+            if (FourShift::below(v_least, v_used) || (X::tag == CKR_F16 && FourShift::below(k_least, k_used))) s_shift.apart = 1;
             __syncthreads();
+            if (__builtin_amdgcn_readfirstlane(s_shift.apart)) return attend_apart<X, DP, 128, TK>(s_tmp);
 #pragma unroll
             for (int i = 0; i < 9; i++) again |= (int)s_shift.top[i] > (int)s_shift.used[i] + kRoom;
             if (again) {
@@ -1718,7 +1778,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     const uint32_t kvh = blockIdx.x % a.kv_heads, tile = nth_tile<C>(a, blockIdx.x / a.kv_heads), split = blockIdx.y;
     Tile t;
     if (threadIdx.x == 0) s_wild = 0;
-    if (FOUR && threadIdx.x < 9) s_shift.top[threadIdx.x] = 0;
+    if (FOUR && threadIdx.x < 9) s_shift.top[threadIdx.x] = s_shift.apart = 0;
     if (!find_tile<Sh::BM, 512>(a.b, a.group, tile, s_tmp, t)) return;
     const int64_t pos_lo = t.start + t.row0 / a.group, pos_hi = t.start + min(t.row0 + Sh::BM - 1, t.rows - 1) / a.group;
     const int64_t limit = min(pos_hi + 1, (int64_t)a.b.width << a.page_shift);
@@ -1767,7 +1827,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     const int64_t st_b = stage_k ? a.skst[0] : a.svst[0];
     const uint8_t* const bytes4 = reinterpret_cast<const uint8_t*>(stage_k ? a.sk : a.sv) +
                                   (int64_t)kvh * (stage_k ? a.skst[1] : a.svst[1]) + ((int64_t)my_group << a.page_shift) + (row_of & 15);
-    uint32_t used = 127, most = 0;
+    uint32_t used = 127, most = 0, least = 254;
     float scale2 = a.scale2;
     uint8_t* const to = (stage_k ? s_k + row_of * KP : s_v + row_of * VP) + to_place;
     const uint32_t to_rows = ROWS * (stage_k ? KP : VP), to_slot = TK * (stage_k ? KP : VP);
@@ -1860,11 +1920,12 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 const bool in = held_valid >> row_of & 1, fine = held_b != 255;
                 if (stage_k) {
                     if (X::tag == CKR_F16 && in && fine) most = max(most, held_b);
+                    if (X::tag == CKR_F16 && in) least = min(least, held_b - 1);
                     held_p = X::tag == CKR_BF16 || !fine ? power_of(held_b) : FourShift::power(held_b, used);
                 } else {
                     if (in && !fine) s_wild = 1;
                     const uint32_t b = in && fine ? held_b : 0;
-                    most = max(most, b);
+                    most = max(most, b), least = min(least, b - 1);
                     held_p = FourShift::power(b, used);
                     if (!(in && fine)) held[0] = u32x4{0, 0, 0, 0};
                 }
@@ -2206,9 +2267,11 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         }
         if constexpr (FOUR) {  // a scale above what float16 holds: begin again
             if (most) atomicMax(&s_shift.top[stage_k ? 8 : my_group], most);
+            if (FourShift::below(least, used)) s_shift.apart = 1;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 9; i++) again |= (int)s_shift.top[i] > (int)s_shift.used[i] + kRoom;
+            again &= !s_shift.apart;
             if (again) {
                 __syncthreads();  // everybody has read
                 m = -INFINITY, l = 0.f, ref = 0.f;
@@ -2224,6 +2287,13 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                     for (int i = 0; i < 16; i++) o[dt][i] *= power;
                 }
             }
+        }
+    }
+    if constexpr (FOUR) {
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(s_shift.apart), 0)) {
+            asm volatile("" ::: "memory");
+            attend_apart<X, DP, Sh::BM, TK>(s_tmp);
+            __builtin_amdgcn_endpgm();  // a way out of its own: where both met, the loop above read its arguments again at each use (chunks 3 % slower)
         }
     }
     l = sum_half(l);
