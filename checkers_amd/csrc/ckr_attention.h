@@ -116,6 +116,9 @@ __device__ __forceinline__ float sum_quarters(float x) {
 //   error of 1.01: a chunk of 2048 behind 30000 1.12 ms, 1.06 with bfloat16 ones (the same
 //   instructions otherwise; with two products 1.41); 128 rows a head 109 us and 105.
 // - 128 rows, float16 over an 8-bit cache: two products, 132 us and 109.
+// - many rows over a 4-bit cache: float16 weights; of float16 queries in two products, an error of 1.00
+//   for 1.3 (128 rows a head 126 us and 109, prompts 820 and 647, a chunk of 2048 behind
+//   30000 1.21 ms and 0.92); of bfloat16 ones once, an error of 1.005 (two products: 1.20 ms for 0.92).
 // - many rows else: rounded once.  Two products are 630 us instead of 505 for prompts in
 //   float16, 750 instead of 560 for a chunk over bfloat16.
 // Their type is the queries' but for ProbMany: bfloat16 weights take the value's scale
@@ -146,8 +149,8 @@ template <> struct ProbMany<ElemBF16, ElemI8> : ProbScaled {};
 // Four bits: a value is its code times its group's power, exactly, so weights carry no
 // scale.  Few rows: bfloat16 values, which take any power, and bfloat16 weights in two
 // halves; float16 queries meet bfloat16 keys in two halves as well (11 bits in 16).  Many rows:
-// float16 weights and values, these against a power of their group that all of a
-// block's keys share (FourShift).
+// float16 weights (of float16 queries in two halves) and values, these against a power of
+// their group that all of a block's keys share (FourShift).
 template <typename X> struct Prob<X, ElemF4> {
     typedef ElemBF16 E;
     static constexpr bool split = false, scaled = false;
@@ -155,7 +158,7 @@ template <typename X> struct Prob<X, ElemF4> {
 };
 template <typename X> struct ProbMany<X, ElemF4> {
     typedef ElemF16 E;
-    static constexpr bool split = false, scaled = false;
+    static constexpr bool split = X::tag == CKR_F16, scaled = false;
     static constexpr float up = 7.f;
 };
 // e of the largest scale (at least kLeast: sums of weights without values stay in range;
@@ -1207,7 +1210,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, few_waves<C>(DP)) attend_few_k
 }
 
 // Which tile the n-th block takes.  Four bits: from the last one on, whose rows see the most keys, so that
-// short ones fill up the end (six prompts of 150 to 3000 tokens 648 us, 670 from the first on).
+// short ones fill up the end (six prompts of 150 to 3000 tokens, with one product a weight: 648 us, 670 from the first on).
 template <typename C> __device__ __forceinline__ uint32_t nth_tile(const AttnArg& a, uint32_t n) {
     return C::tag == CKR_F4 ? a.tiles - 1 - n : n;
 }
@@ -1592,7 +1595,7 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
                         for (int k = 0; k < 4; k++) p[i + k] *= f[k];
                     }
                 }
-                Halves<P> w;  // the second for float16 queries over 8 bits only
+                Halves<P> w;  // the second for float16 queries over 4 and 8 bits only
 #pragma unroll
                 for (int i = 0; i < 4; i++) w.add(i, p[2 * i], p[2 * i + 1]);
 #pragma unroll
@@ -1745,8 +1748,8 @@ __global__ void __launch_bounds__(256, (DP > 128 ? 1 : 2)) attend_many_kernel(At
 // and takes one tile of rows, so of the 50 us that one takes on average the 12 until
 // its first product runs beside nothing.
 // Over 4 bits no score and no weight meets a scale (FourShift): the chunk 936 to 1060 us from card to card, 0.98 to
-// 1.11 PFLOP/s; the prompts of 150 to 3000 tokens with 64 query heads 641 to 712, 0.68 to 0.76.  A loop of its own
-// for the waves that stage keys spills 86 registers (1630 us).
+// 1.11 PFLOP/s; the prompts of 150 to 3000 tokens in float16 with 64 query heads, whose weights take two products, 820 us,
+// 0.60 (one and a half times that in products).  A loop of its own for the waves that stage keys spills 86 registers (1630 us).
 template <typename C, int DP> struct WideShape {
     static constexpr int TK = 64, BM = 256, RING = 4;
     static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 64;  // as ManyShape's
@@ -1762,7 +1765,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     constexpr int TK = Sh::TK, KP = Sh::KP, VP = Sh::VP, LPR = Sh::LPR, LOADS = Sh::LOADS, RPW = Sh::RPW, ROWS = Sh::ROWS;
     constexpr int KS = DP / 16, DT = DP / 32, NM = 2 * KS;  // KS products for the scores, as many for the values
     static_assert(KS == 2 * DT && KS % 4 == 0, "pairs of products, operands in rings of four");
-    constexpr bool kScaled = ProbMany<X, C>::scaled, FOUR = C::tag == CKR_F4;
+    constexpr bool kScaled = ProbMany<X, C>::scaled, FOUR = C::tag == CKR_F4, kTwice = FOUR && ProbMany<X, C>::split;
     constexpr int PIECE = Sh::PIECE, WORDS = PIECE / 4;
     static_assert(!FOUR || (LOADS == 1 && RPW == 16), "four bits: a wave stages 16 rows of a tile, a lane one piece");
     constexpr float kMost = ProbMany<X, C>::up == 0.f ? 256.f : ProbMany<X, C>::up == 6.f ? 16384.f : 32768.f;  // 2^(kLag + up)
@@ -1980,6 +1983,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
     uint32_t flip = a.flip;
     f32x16 o[DT], s;
     u32x4 pf[2][2], kf[4], vf[4];  // weights of two turns; operands, read three pairs of steps ahead
+    u32x4 pf_lo[2][2];             // kTwice: what the weights' rounding leaves
     f32x4 fk[2], fv[2];            // the keys' scales, of keys 8 j + 4 half on
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
@@ -2065,6 +2069,11 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 p_even = C::bytes == 1 ? p_last * fv[k / 4 % 2][k % 4] : p_last;
             } else {
                 uint32_t w = pack16<P>(p_even, C::bytes == 1 ? p_last * fv[k / 4 % 2][k % 4] : p_last);
+                if constexpr (kTwice) {
+                    uint32_t x = pack16<P>(p_even - lo16<P>(w), p_last - hi16<P>(w));
+                    asm volatile("" : "+v"(x));
+                    pf_lo[sub][k / 8][k % 8 / 2] = x;
+                }
                 asm volatile("" : "+v"(w));
                 pf[sub][k / 8][k % 8 / 2] = w;
             }
@@ -2075,6 +2084,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 constexpr int j = S * NM / 16, e = j / 2;
                 if constexpr (j % 2 == 0) {
                     o[e % DT] = mfma32<P>(vf[e % 4], pf[1 - sub][e / DT], o[e % DT]);
+                    if constexpr (kTwice) o[e % DT] = mfma32<P>(vf[e % 4], pf_lo[1 - sub][e / DT], o[e % DT]);
                     if constexpr (e + 3 < KS) read_v(e + 3, now.v);
                     else read_v(e + 3 - KS, after.v);
                 } else {
@@ -2127,6 +2137,11 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
                 }
                 pf[sub][k / 8][k % 8 / 2] = pack16<P>(p[0] * gv[0], p[1] * gv[1]);
                 pf[sub][k / 8][k % 8 / 2 + 1] = pack16<P>(p[2] * gv[2], p[3] * gv[3]);
+                if constexpr (kTwice) {
+                    const uint32_t x = pf[sub][k / 8][k % 8 / 2], y = pf[sub][k / 8][k % 8 / 2 + 1];
+                    pf_lo[sub][k / 8][k % 8 / 2] = pack16<P>(p[0] - lo16<P>(x), p[1] - hi16<P>(x));
+                    pf_lo[sub][k / 8][k % 8 / 2 + 1] = pack16<P>(p[2] - lo16<P>(y), p[3] - hi16<P>(y));
+                }
             }
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
@@ -2210,6 +2225,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         }
         // turn 0 has no values before it: what it gathers is dropped after it
         pf[1][0] = pf[1][1] = u32x4{0, 0, 0, 0};
+        if constexpr (kTwice) pf_lo[1][0] = pf_lo[1][1] = u32x4{0, 0, 0, 0};
         Where now = {k_at(0, 1), v_at(0, 0), s_sk[full ? 0 : Sh::RING], s_sv[0]};
 #pragma unroll
         for (int e = 0; e < 3; e++) read_k(e, now.k), read_v(e, now.v);
@@ -2264,6 +2280,7 @@ __global__ void __launch_bounds__(512, 2) attend_wide_kernel(AttnArg a) {
         for (int e = 0; e < KS; e++) {
             if (e + 3 < KS) read_v(e + 3, now.v);
             o[e % DT] = mfma32<P>(vf[e % 4], pf[1][e / DT], o[e % DT]);
+            if constexpr (kTwice) o[e % DT] = mfma32<P>(vf[e % 4], pf_lo[1][e / DT], o[e % DT]);
         }
         if constexpr (FOUR) {  // a scale above what float16 holds: begin again
             if (most) atomicMax(&s_shift.top[stage_k ? 8 : my_group], most);
