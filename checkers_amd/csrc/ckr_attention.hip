@@ -40,10 +40,13 @@ constexpr uint32_t kFewTiles = 4;
 // over 4096 66 / 104.
 constexpr uint32_t kFewMost = 32;
 // Over 4 bits, whose tiles cost few rows half as much (e4m3's figures above; here 48 rows of 16 sequences over
-// 4096 tokens 48 / 101, of one over 32768 42 / 79, of 64 over 1024 47 / 59; 64 rows 60 / 100, 45 / 80 and 73 /
-// 59; 96 rows 70 / 102, 53 / 82 and 90 / 62; 128 rows 106 / 106, 60 / 86 and 127 / 64): more rows, and
-// more again over long contexts.
-constexpr uint32_t kFourMost = 48, kFourMostLong = 96, kFourLong = 2048;
+// 4096 tokens 52 / 101, of one over 32768 42 / 78, of 64 over 1024 44 / 56): more rows, and more again where
+// there is much to read and a tile of many rows for each sequence and head would not fill the card.  64 and 96 rows of
+// 16 sequences over 4096: 60 / 98 and 65 / 101, in a window of 1024 29 / 36 and 26 / 39, of 256 24 / 21 and 16 / 25;
+// of 48 over 4096 124 / 179 and 184 / 180; of one over 32768 46 / 81 and 54 / 84, over 2000 28 / 20 and 29 / 20; of 32
+// over 1024 42 / 43 and 45 / 44, over 512 36 / 25 and 32 / 27; of 64 over 4096 197 / 191 and 260 / 194, in a
+// window of 1024 70 / 57 and 87 / 59.
+constexpr uint32_t kFourMost = 48, kFourMostLong = 96, kFourLong = 1024, kFourKeys = 1 << 17;
 // Rows from which on a tile of 256 pays: 128 rows of 16 sequences over 4096 tokens 110
 // (many) / 144 (very many), 256 rows 158 / 148; 256 of one over 32768 102 / 100; float16
 // caches 129 / 111 and 184 / 115.
@@ -73,7 +76,14 @@ Cut cut(uint32_t n_heads, uint32_t n_kv, uint32_t dim, uint32_t n_seqs, uint32_t
     Cut c{};
     const uint64_t group = n_heads / n_kv, rows = (uint64_t)max_chunk * group;
     c.dp = padded_dim(dim);
-    const bool few = rows <= (!four ? kFewMost : max_context < kFourLong ? kFourMost : kFourMostLong) && (near_slots || !four) && most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1 + (four ? kItemPad : 0)) < (1ull << 31);
+    uint32_t few_most = kFewMost;
+    if (four) {
+        const uint64_t pairs = (uint64_t)std::min(n_seqs, n_tokens) * n_kv;  // of a sequence and a head
+        const uint64_t keys = window ? std::min<uint64_t>(max_context, (uint64_t)window + max_chunk) : max_context;
+        few_most = keys >= kFourLong && pairs * keys >= kFourKeys && pairs < blocks_wanted(kManyRows) ? kFourMostLong : kFourMost;
+    }
+    const bool few = rows <= few_most && (near_slots || !four) &&
+                     most_tiles(kFewRows, group, n_seqs, n_tokens) * n_kv * ((all_keys + 31) / 32 + 1 + (four ? kItemPad : 0)) < (1ull << 31);
     c.bm = few ? kFewRows : rows <= kManyMost || c.dp == 256 || !near_slots ? kManyRows : kWideRows;
     c.tiles = (uint32_t)most_tiles(c.bm, group, n_seqs, n_tokens);
     c.splits = 1;
