@@ -13,8 +13,9 @@ inputs, and keeps them (or records them on it) until it is done; outputs that
 a call makes belong to that stream and may be used on the current one once that
 waits for it.
 
-Only rotary has a backward pass: elsewhere tensors that require gradients are
-refused where gradients are recorded (not under torch.no_grad()).
+Only rotary has a backward pass, and a forward-mode derivative: elsewhere tensors that
+require gradients are refused where gradients are recorded (not under
+torch.no_grad()), and tensors with a tangent everywhere.
 """
 import ctypes
 import math
@@ -190,6 +191,22 @@ def _no_backward():
         _bad("these operators have no backward pass: call them under torch.no_grad(), or on detached tensors")
 
 
+_forward_ad = None
+
+
+def _tangents(*xs):
+    """Whether one of the tensors carries a forward-mode tangent (torch.no_grad() keeps them)."""
+    global _forward_ad
+    if _forward_ad is None:
+        _forward_ad = _torch().autograd.forward_ad
+    return _forward_ad._current_level >= 0 and any(x is not None and _forward_ad.unpack_dual(x).tangent is not None for x in xs)
+
+
+def _no_tangents(*xs):
+    if _tangents(*xs):
+        _bad("these operators have no forward-mode derivative: call them on detached tensors")
+
+
 def _rows(t, n_tokens, heads, dim, what):
     """(token stride, head stride) of a [tokens, heads, dim] tensor on a GPU."""
     shape = t.shape
@@ -233,6 +250,7 @@ def kv_write(cache, batch, k, v, stream=None):
     """Quantise the batch's keys and values [tokens, heads, head_dim] into the cache."""
     if k.requires_grad or v.requires_grad:
         _no_backward()
+    _no_tangents(k, v)
     dtype, n, h, d = k.dtype, batch.n_tokens, cache.n_heads, cache.head_dim
     if v.dtype != dtype:
         _bad("k and v must be of one type")
@@ -250,6 +268,7 @@ def kv_append(cache, batch, rotary, k, v, q=None, out=None, positions=None, stre
     positions: a contiguous int32 [tokens] where they are not those in the cache."""
     if k.requires_grad or v.requires_grad or q is not None and q.requires_grad:
         _no_backward()
+    _no_tangents(k, v, q)
     dtype, n, h, d = k.dtype, batch.n_tokens, cache.n_heads, cache.head_dim
     if v.dtype != dtype:
         _bad("k and v must be of one type")
@@ -332,6 +351,7 @@ class KvAttention:
         n_heads] that receives the logarithm of each row's sum of exponentials."""
         if q.requires_grad:
             _no_backward()
+        _no_tangents(q)
         n, h, d, dtype = batch.n_tokens, self.n_heads, cache.head_dim, q.dtype
         qt, qh = _rows(q, n, h, d, "q")
         if out is None:
@@ -365,6 +385,7 @@ def add_rms_norm(x, residual, weight, eps=1e-5, dtype=None, group=0, out=None, s
     backward pass."""
     if x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad:
         _no_backward()
+    _no_tangents(x, weight, residual)
     shape, x_dtype = x.shape, x.dtype
     if len(shape) != 2:
         _bad("x must be [rows, n]")
@@ -556,6 +577,7 @@ def _turn():
             def forward(ctx, rotary, positions, inverse, *xs):
                 ctx.rotary, ctx.inverse = rotary, inverse
                 ctx.save_for_backward(positions)
+                ctx.save_for_forward(positions)
                 ctx.set_materialize_grads(False)
                 outs = tuple(torch.empty_like(x) for x in xs)
                 _rotate(rotary, positions, xs, outs, inverse, None)
@@ -577,6 +599,11 @@ def _turn():
                         out[i] = g
                 return (None, None, None, *out)
 
+            @staticmethod
+            def jvp(ctx, _rotary, _positions, _inverse, *tangents):
+                positions, = ctx.saved_tensors
+                return Turn.apply(ctx.rotary, positions, ctx.inverse, *(t if t.stride(-1) == 1 else t.contiguous() for t in tangents))
+
         _Turn = Turn
     return _Turn
 
@@ -586,16 +613,21 @@ def rotary(rotary, positions, q, k=None, out=None, inverse=False, stream=None):
     [batch, tokens, heads, dim] with any strides but the last axis'; positions int32 [tokens] or
     [batch, tokens].  Returns the turned q, with k a pair; into out (a tensor, with k a pair; may
     be q and k themselves) when given.  inverse turns back, but for the magnitude: it is the transposed
-    matrix.  Gradients are recorded where q or k requires them (then without out and stream);
+    matrix.  Gradients are recorded where q or k requires them, and forward-mode tangents turned
+    where q or k has one (then without out and stream);
     a captured graph needs the Rotary kept, and a backward pass that is captured must not meet
     leaves of an eager graph that is still alive (torch would run their sums on its stream)."""
     xs = (q,) if k is None else (q, k)
     if not 3 <= q.dim() <= 4 or any(x.dim() != q.dim() for x in xs):
         _bad("q and k must be [tokens, heads, dim] or [batch, tokens, heads, dim]")
-    if _torch().is_grad_enabled() and any(x.requires_grad for x in xs):
+    tangents = _tangents(*xs)
+    if tangents or _torch().is_grad_enabled() and any(x.requires_grad for x in xs):
         if out is not None or stream is not None:
-            _bad("where gradients are recorded rotary takes neither out nor stream")
-        outs = _turn().apply(rotary, positions, bool(inverse), *xs)
+            _bad("where gradients are recorded, or tangents turned, rotary takes neither out nor stream")
+        if tangents:   # one of them may have none
+            outs = tuple(_turn().apply(rotary, positions, bool(inverse), x)[0] for x in xs)
+        else:
+            outs = _turn().apply(rotary, positions, bool(inverse), *xs)
     else:
         if out is None:
             outs = tuple(_new(x.shape, x.dtype, x.device, stream) for x in xs)
