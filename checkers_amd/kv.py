@@ -15,7 +15,8 @@ waits for it.
 
 Only rotary has a backward pass, and a forward-mode derivative: elsewhere tensors that
 require gradients are refused where gradients are recorded (not under
-torch.no_grad()), and tensors with a tangent everywhere.
+torch.no_grad()), and tensors with a tangent everywhere.  Calls are refused while
+torch.jit.trace, make_fx or torch.export record a program, which would not hold them.
 """
 import ctypes
 import math
@@ -172,13 +173,35 @@ class KvBatch:
         self._p = ctypes.byref(self._c)
 
 
+_accounts = _forward_ad = None   # torch's own of what is recorded, of the current stream, and of forward mode
+
+
+def _load_accounts():
+    global _accounts, _forward_ad
+    torch = _torch()
+    _forward_ad, c = torch.autograd.forward_ad, torch._C
+    _accounts = c._get_tracing_state, c._len_torch_dispatch_stack, c._len_torch_function_stack, c._cuda_getCurrentRawStream
+    return _accounts
+
+
+def _not_traced():
+    """Tracing (torch.jit.trace, make_fx, export) sees the output's allocation but not the call,
+    so what it records would return memory that nobody writes: refused.  Other modes look on."""
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    if _accounts[0]() is not None or get_proxy_mode() is not None:
+        _bad("the cache and norm operators cannot be recorded by tracing: call them outside of what is traced")
+
+
 def _stream_of(stream, tensor):
     """The stream's handle; None: the current stream of the tensor's GPU.  (A
     decoding step's calls last a few microseconds each, so neither this nor the
     checks below build objects that they do not need.)"""
+    traced, modes, functions, current = _accounts or _load_accounts()
+    if traced() is not None or modes() or functions():
+        _not_traced()
     if stream is not None:
         return stream.cuda_stream
-    return _torch()._C._cuda_getCurrentRawStream(tensor.get_device())
+    return current(tensor.get_device())
 
 
 def _bad(msg):
@@ -191,14 +214,10 @@ def _no_backward():
         _bad("these operators have no backward pass: call them under torch.no_grad(), or on detached tensors")
 
 
-_forward_ad = None
-
-
 def _tangents(*xs):
     """Whether one of the tensors carries a forward-mode tangent (torch.no_grad() keeps them)."""
-    global _forward_ad
     if _forward_ad is None:
-        _forward_ad = _torch().autograd.forward_ad
+        _load_accounts()
     return _forward_ad._current_level >= 0 and any(x is not None and _forward_ad.unpack_dual(x).tangent is not None for x in xs)
 
 
@@ -250,7 +269,8 @@ def kv_write(cache, batch, k, v, stream=None):
     """Quantise the batch's keys and values [tokens, heads, head_dim] into the cache."""
     if k.requires_grad or v.requires_grad:
         _no_backward()
-    _no_tangents(k, v)
+    if _forward_ad is None or _forward_ad._current_level >= 0:
+        _no_tangents(k, v)
     dtype, n, h, d = k.dtype, batch.n_tokens, cache.n_heads, cache.head_dim
     if v.dtype != dtype:
         _bad("k and v must be of one type")
@@ -268,7 +288,8 @@ def kv_append(cache, batch, rotary, k, v, q=None, out=None, positions=None, stre
     positions: a contiguous int32 [tokens] where they are not those in the cache."""
     if k.requires_grad or v.requires_grad or q is not None and q.requires_grad:
         _no_backward()
-    _no_tangents(k, v, q)
+    if _forward_ad is None or _forward_ad._current_level >= 0:
+        _no_tangents(k, v, q)
     dtype, n, h, d = k.dtype, batch.n_tokens, cache.n_heads, cache.head_dim
     if v.dtype != dtype:
         _bad("k and v must be of one type")
@@ -351,7 +372,8 @@ class KvAttention:
         n_heads] that receives the logarithm of each row's sum of exponentials."""
         if q.requires_grad:
             _no_backward()
-        _no_tangents(q)
+        if _forward_ad is None or _forward_ad._current_level >= 0:
+            _no_tangents(q)
         n, h, d, dtype = batch.n_tokens, self.n_heads, cache.head_dim, q.dtype
         qt, qh = _rows(q, n, h, d, "q")
         if out is None:
@@ -385,7 +407,8 @@ def add_rms_norm(x, residual, weight, eps=1e-5, dtype=None, group=0, out=None, s
     backward pass."""
     if x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad:
         _no_backward()
-    _no_tangents(x, weight, residual)
+    if _forward_ad is None or _forward_ad._current_level >= 0:
+        _no_tangents(x, weight, residual)
     shape, x_dtype = x.shape, x.dtype
     if len(shape) != 2:
         _bad("x must be [rows, n]")
@@ -620,7 +643,7 @@ def rotary(rotary, positions, q, k=None, out=None, inverse=False, stream=None):
     xs = (q,) if k is None else (q, k)
     if not 3 <= q.dim() <= 4 or any(x.dim() != q.dim() for x in xs):
         _bad("q and k must be [tokens, heads, dim] or [batch, tokens, heads, dim]")
-    tangents = _tangents(*xs)
+    tangents = (_forward_ad is None or _forward_ad._current_level >= 0) and _tangents(*xs)
     if tangents or _torch().is_grad_enabled() and any(x.requires_grad for x in xs):
         if out is not None or stream is not None:
             _bad("where gradients are recorded, or tangents turned, rotary takes neither out nor stream")
