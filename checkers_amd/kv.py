@@ -602,7 +602,7 @@ def _turn():
                 ctx.save_for_backward(positions)
                 ctx.save_for_forward(positions)
                 ctx.set_materialize_grads(False)
-                outs = tuple(torch.empty_like(x) for x in xs)
+                outs = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)   # contiguous, as without gradients
                 _rotate(rotary, positions, xs, outs, inverse, None)
                 return outs
 
@@ -634,8 +634,8 @@ def _turn():
 def rotary(rotary, positions, q, k=None, out=None, inverse=False, stream=None):
     """Heads turned by their tokens' positions (a Rotary): q, and k with it, [tokens, heads, dim] or
     [batch, tokens, heads, dim] with any strides but the last axis'; positions int32 [tokens] or
-    [batch, tokens].  Returns the turned q, with k a pair; into out (a tensor, with k a pair; may
-    be q and k themselves) when given.  inverse turns back, but for the magnitude: it is the transposed
+    [batch, tokens].  Returns the turned q, with k a pair: contiguous tensors, or into out (a tensor,
+    with k a pair; may be q and k themselves) when given.  inverse turns back, but for the magnitude: it is the transposed
     matrix.  Gradients are recorded where q or k requires them, and forward-mode tangents turned
     where q or k has one (then without out and stream);
     a captured graph needs the Rotary kept, and a backward pass that is captured must not meet

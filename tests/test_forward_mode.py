@@ -88,3 +88,17 @@ def test_refusals(plain):
         for call in calls:
             with pytest.raises(ck.CkrError, match="tangent|forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (1, 0, 2)])
+def test_one_layout_with_and_without_gradients(plain, order):
+    """Heads that lie before tokens: the output is contiguous whether a gradient is recorded, a
+    tangent turned, or neither."""
+    rot, at = plain
+    x = torch.randn(*(torch.empty(5, 3, 6).permute(order).shape)).permute(order)
+    with torch.no_grad():
+        want = ck.rotary(rot, at, x)
+    with fw.dual_level():
+        dual = fw.unpack_dual(ck.rotary(rot, at, fw.make_dual(x, torch.randn(5, 3, 6)))).primal
+    for y in (want, dual, ck.rotary(rot, at, x.detach().requires_grad_())):
+        assert y.is_contiguous() and y.stride() == want.stride() and torch.equal(y, want)
