@@ -577,10 +577,7 @@ def _rotate(rotary, positions, xs, outs, inverse, stream):
             _bad(f"out of {'qk'[i]} must have its heads")
         if x.get_device() != rotary._device or y.get_device() != rotary._device:
             _bad(f"{'qk'[i]}, its output and the rotary must be on one GPU")
-        x_ptr, y_ptr = x.data_ptr(), y.data_ptr()
-        if x_ptr and x_ptr == y_ptr and places[0] != places[1]:
-            _bad(f"{'qk'[i]} turned in place must have its own strides")
-        flat += (x_ptr, y_ptr, *places[0], *places[1], x.shape[-2])
+        flat += (x.data_ptr(), y.data_ptr(), *places[0], *places[1], x.shape[-2])
     rc = lib().ckr_rotate(rotary._p, positions.data_ptr(), _i64x2v(*ps), _i64x18(*flat), len(xs), batch, tokens, dim, _tag(dtype), inverse, handle)
     if rc:
         _check(rc)
