@@ -161,7 +161,7 @@ int ckr_kv_attention(const ckr_kv_cache* cache, const ckr_kv_batch* batch, const
     a.q = static_cast<const uint8_t*>(d_q), a.out = static_cast<uint8_t*>(d_out), a.lse = d_lse;
     a.q_tok = q_token_stride, a.q_head = q_head_stride, a.o_tok = out_token_stride, a.o_head = out_head_stride;
     a.ck = static_cast<const uint8_t*>(cache->d_k), a.cv = static_cast<const uint8_t*>(cache->d_v);
-    a.sk = static_cast<const float*>(cache->d_k_scale), a.sv = static_cast<const float*>(cache->d_v_scale);
+    a.sk = cache->d_k_scale, a.sv = cache->d_v_scale;
     const int ces = cache->dtype == CKR_F8 || cache->dtype == CKR_I8 || cache->dtype == CKR_F4 ? 1 : 2;  // of a stride's unit
     for (int i = 0; i < 3; i++) a.kst[i] = cache->k_stride[i] * ces, a.vst[i] = cache->v_stride[i] * ces;
     std::copy(cache->k_scale_stride, cache->k_scale_stride + 2, a.skst);

@@ -200,7 +200,7 @@ int rows_call(const ckr_kv_cache* c, const ckr_kv_batch* b, void* k, int64_t kt,
                      : kv_read_four(c, b, k, kt, kh, v, vt, vh, dtype, stream);
     RowsArg a{};
     a.k = k, a.v = v, a.k_tok = kt, a.k_head = kh, a.v_tok = vt, a.v_head = vh;
-    a.ck = static_cast<uint8_t*>(c->d_k), a.cv = static_cast<uint8_t*>(c->d_v), a.sk = static_cast<float*>(c->d_k_scale), a.sv = static_cast<float*>(c->d_v_scale);
+    a.ck = static_cast<uint8_t*>(c->d_k), a.cv = static_cast<uint8_t*>(c->d_v), a.sk = c->d_k_scale, a.sv = c->d_v_scale;
     std::copy(c->k_stride, c->k_stride + 3, a.kst);
     std::copy(c->v_stride, c->v_stride + 3, a.vst);
     std::copy(c->k_scale_stride, c->k_scale_stride + 2, a.skst);

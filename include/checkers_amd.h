@@ -570,8 +570,14 @@ CKR_API int ckr_make_contiguous(const void* d_src, int ndim, const int64_t* shap
 typedef struct {
     void* d_k;
     void* d_v;
-    void* d_k_scale;            /* fp32, of CKR_F4 bytes; NULL without scales   */
-    void* d_v_scale;
+    union {                     /* NULL without scales                          */
+        float* d_k_scale;       /* CKR_F8, CKR_I8                               */
+        uint8_t* d_k_power;     /* CKR_F4                                       */
+    };
+    union {
+        float* d_v_scale;
+        uint8_t* d_v_power;
+    };
     int64_t k_stride[3];        /* page, head, slot                             */
     int64_t v_stride[3];
     int64_t k_scale_stride[2];  /* page, head                                   */
