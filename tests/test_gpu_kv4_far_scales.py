@@ -155,3 +155,46 @@ def test_groups_without_values_are_no_scales(gpu):
         p, slot = sq.place(0, j)
         _bytes(cache.v_scale)[p, :, :, slot] = 0
     assert torch.equal(plan.run(cache, b, q), want)
+
+
+@pytest.mark.parametrize("typ,lens,window", [("bf16", [40, 3, 25, 0, 30], 0), ("f16", [30, 90, 1], 0), ("bf16", [70, 90], 60)])
+def test_several_sequences(gpu, typ, lens, window):
+    """Far scales in one sequence, on pages of its own, beside others without."""
+    print(f"[case] several {typ} {lens} {window}", flush=True)
+    starts = [60, 200, 17, 5, 130][:len(lens)]
+    sq = ko.Seqs(starts, lens, 16, seed=4)
+    cache = _cache(sq, 2, 128, gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 128, gpu, 3)
+    _shift(sq, cache, "v", range(0, starts[0] + lens[0] // 2), -13)
+    _shift(sq, cache, "v", range(starts[0] + lens[0] // 2, starts[0] + lens[0]), 13)
+    q = torch.randn(sq.tokens, 8, 128, generator=torch.Generator(device=gpu).manual_seed(4), device=gpu).to(TYPES[typ])
+    plan = ck.KvAttention(8, 2, 128, len(lens), sq.tokens, max(lens), 300)
+    lse = torch.full((sq.tokens, 8), 9.0, device=gpu)
+    out = plan.run(cache, b, q, window=window, lse=lse)
+    torch.cuda.synchronize()
+    _check_rows(sq, cache, q, out, lse, 4, window)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+def test_slots_far_apart(gpu, typ):
+    """Slots of a page 2^26 bytes apart, which the 128-row kernel alone takes: near and far scales."""
+    step, page = 1 << 26, 16
+    raw = [torch.zeros((page - 1) * step + 64, dtype=torch.uint8, device=gpu) for _ in range(2)]
+    k, v = (r.as_strided((1, 1, page, 64), (0, 0, step, 1)).view(torch.float4_e2m1fn_x2) for r in raw)
+    ks, vs = (torch.zeros(1, 1, 4, page, dtype=torch.uint8, device=gpu).view(torch.float8_e8m0fnu) for _ in range(2))
+    cache = ck.KvCache(k, v, ks, vs)
+    sq = ko.Seqs([0], [page], page, spare=0)
+    b = _batch(sq, gpu)
+    g = torch.Generator(device=gpu).manual_seed(2)
+    ck.kv_write(cache, b, *(torch.randn(page, 1, 128, generator=g, device=gpu) for _ in range(2)))
+    q = torch.randn(page, 12, 128, generator=g, device=gpu).to(TYPES[typ])
+    plan = ck.KvAttention(12, 1, 128, 1, page, page, page)
+    for far in (False, True):
+        if far:
+            _shift(sq, cache, "v", range(0, 8), -13)
+            _shift(sq, cache, "v", range(8, 16), 13)
+        lse = torch.full((page, 12), 9.0, device=gpu)
+        out = plan.run(cache, b, q, lse=lse)
+        torch.cuda.synchronize()
+        _check_rows(sq, cache, q, out, lse, 12, 0)
