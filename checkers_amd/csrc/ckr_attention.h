@@ -239,7 +239,9 @@ template <typename E> __device__ __forceinline__ u32x4 ones(uint32_t seen) {
 
 constexpr uint32_t kFewRows = 16, kManyRows = 128, kWideRows = 256;  // rows of a tile
 constexpr uint32_t kFewWaves = 4;                                    // waves of a block of few rows
-constexpr int kFourTiles = 1, kFourWaves = 3;                         // four bits: tiles on their way a wave, waves a SIMD
+// Four bits: tiles on their way a wave, waves a SIMD.  (Written for one tile, without the loops over kFourTiles, the
+// same code spills 41 registers.)
+constexpr int kFourTiles = 1, kFourWaves = 3;
 
 // f(0) .. f(N - 1) with constants.
 template <typename F, int... I> __device__ __forceinline__ void unroll_list(F f, std::integer_sequence<int, I...>) {
@@ -465,7 +467,7 @@ __device__ __forceinline__ uint32_t few_tiles(const FewSpan& f) {  // one at lea
 // later tiles add comes at 5.75, which is what a kernel that only reads such pages reaches).  Beside the bytes it
 // takes 14 us for the launch, the first tiles' way and the join, and each item more than its tiles (kItemPad).  With
 // branches around the loads the compiler waited for all of them before each tile (142 us); two tiles on their way
-// and two blocks a CU take 115.
+// and two blocks a CU take 118.
 template <typename X, int DP, typename At = uint32_t>
 __device__ __forceinline__ void few_item_four(const AttnArg& a, uint32_t seq, uint32_t kvh, uint32_t token0, uint32_t row0, uint32_t rows,
                                               const FewSpan& span, int64_t lo, int n_tiles, float& m, float& l, f32x4 (&o)[DP / 16]) {
