@@ -680,7 +680,8 @@ CKR_API int ckr_kv_append(const ckr_kv_cache* cache, const ckr_kv_batch* batch, 
  * must be of the same type; with CKR_F16 the values of an 8-bit cache reach at
  * most 65504) with token and head strides in elements, rows on
  * 16-byte boundaries.  d_lse (may be NULL): [n_tokens][n_heads] fp32, the
- * logarithm of the sum of exp(scale * q.k).  A token that attends to nothing
+ * logarithm of the sum of exp(scale * q.k).  Weighted values are summed in fp32 before
+ * they are divided: values beyond 2^100 may give infinities.  A token that attends to nothing
  * gives zeros and -infinity.  The workspace (256-byte aligned) must be all
  * zeros when it is first used and is left fit for the next call; calls that share one
  * must follow each other in stream order.  One sized for the largest n_seqs,
