@@ -186,9 +186,14 @@ def _load_accounts():
 
 def _not_traced():
     """Tracing (torch.jit.trace, make_fx, export) sees the output's allocation but not the call,
-    so what it records would return memory that nobody writes: refused.  Other modes look on."""
+    so what it records would return memory that nobody writes: refused.  Other modes look on
+    (and a default device, which is one as well, is told apart without asking further)."""
+    traced, modes, functions, _ = _accounts
+    at = _torch()._C._get_function_stack_at
+    if traced() is None and not modes() and all(type(at(i)).__module__ == "torch.utils._device" for i in range(functions())):
+        return
     from torch.fx.experimental.proxy_tensor import get_proxy_mode
-    if _accounts[0]() is not None or get_proxy_mode() is not None:
+    if traced() is not None or get_proxy_mode() is not None:
         _bad("the cache and norm operators cannot be recorded by tracing: call them outside of what is traced")
 
 

@@ -72,4 +72,6 @@ def test_modes_that_record_nothing_are_no_tracing(calls):
         assert kv._stream_of(Stream, None) == 7
     with torch.device("cpu"):
         assert kv._stream_of(Stream, None) == 7
+        with pytest.raises(ck.CkrError, match="tracing"):
+            make_fx(lambda x: kv._stream_of(Stream, None) + x, pre_dispatch=True)(torch.zeros(1))
     assert kv._stream_of(Stream, None) == 7
