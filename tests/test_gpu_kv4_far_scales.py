@@ -198,3 +198,30 @@ def test_slots_far_apart(gpu, typ):
         out = plan.run(cache, b, q, lse=lse)
         torch.cuda.synchronize()
         _check_rows(sq, cache, q, out, lse, 12, 0)
+
+
+@pytest.mark.parametrize("typ,chunk", [("bf16", 30), ("f16", 90)])
+def test_captured(gpu, typ, chunk):
+    """A captured call whose scales move apart and together between replays."""
+    sq = ko.Seqs([100], [chunk], 16, seed=2)
+    cache = _cache(sq, 2, 128, gpu)
+    b = _batch(sq, gpu)
+    _fill(sq, cache, b, 2, 128, gpu, 3)
+    q = torch.randn(sq.tokens, 8, 128, generator=torch.Generator(device=gpu).manual_seed(4), device=gpu).to(TYPES[typ])
+    plan = ck.KvAttention(8, 2, 128, 1, sq.tokens, chunk, 100 + chunk)
+    out, lse = torch.zeros_like(q), torch.zeros(sq.tokens, 8, device=gpu)
+    plan.run(cache, b, q, out=out, lse=lse)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run(cache, b, q, out=out, lse=lse)
+    for turn in range(4):
+        _shift(sq, cache, "v", range(0, 100 + chunk // 2), -26 if turn % 2 == 0 else 26)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), lse.clone()
+        _check_rows(sq, cache, q, *got, 4, 0)
+        plan.run(cache, b, q, out=out, lse=lse)
+        torch.cuda.synchronize()
+        assert torch.equal(out, got[0]) and torch.equal(lse, got[1])
